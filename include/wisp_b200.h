@@ -434,6 +434,149 @@ WispError wisp_b200_ep_combine_f16(const uint16_t* d_yback, const int* d_slot,
                                    int hidden, float* d_out, cudaStream_t stream,
                                    WispErrCtx* err);
 
+/* --------------------------------------------------------------------------
+ * 4-bit block-scaled operands ("fp4"): rows of e2m1 values (+-{0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6}), two per byte along the row (low nibble = even index), and one
+ * scale byte per block of consecutive values. No counterpart in the reference,
+ * whose 4-bit format is integer (wisp/converter/quantizer.py:1-17).
+ *   WISP_FP4_MX: blocks of 32, scale = 2^(byte - 127) (byte 255: NaN)
+ *   WISP_FP4_NV: blocks of 16, scale = e4m3(byte) * tensor_scale, where
+ *                tensor_scale is one positive fp32 on the device per matrix
+ * Rows are contiguous: cols/2 code bytes and cols/block scale bytes each.
+ * ------------------------------------------------------------------------ */
+enum { WISP_FP4_MX = 0, WISP_FP4_NV = 1 };
+enum { WISP_DT_F32 = 0, WISP_DT_BF16 = 1, WISP_DT_F16 = 2 };
+
+/* Quantises rows: row p of the result is row d_src[p] of d_x (d_src NULL:
+ * row p; an index outside [0, x_rows) gives a row of zeros). d_x has x_rows
+ * rows of cols values of x_type, ld elements apart. cols is a multiple of the
+ * block. Per block, with a = max|x|:
+ *   MX: scale = 2^(floor(log2 a) - 2), at least 2^-127
+ *   NV: scale byte = e4m3(a / (6 tensor_scale)) rounded to nearest even and
+ *       saturated at 448
+ * and each code is the e2m1 value nearest to x / scale (ties to the even
+ * code, saturated at 6), decided as if by exact arithmetic. A zero scale
+ * gives zero codes; a block holding an infinity or a NaN, or a tensor_scale
+ * that is not positive and finite, gives the NaN scale byte and zero codes.
+ * rows = 0 is allowed and launches nothing. */
+WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t ld, int x_rows,
+                                 const int* d_src, int rows, int cols, int format,
+                                 const float* d_tensor_scale, uint8_t* d_codes,
+                                 uint8_t* d_scales, cudaStream_t stream, WispErrCtx* err);
+
+/* The values of quantised rows, rounded once to out_type (ld elements
+ * between output rows). */
+WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int rows,
+                                   int cols, int format, const float* d_tensor_scale, void* d_out,
+                                   int out_type, int64_t ld, cudaStream_t stream,
+                                   WispErrCtx* err);
+
+/* A set of n_entries matrices [n x k] (one per expert), used by one product. */
+typedef struct {
+    int format;    /* WISP_FP4_* (weights and rows) */
+    int n_entries;
+    int n;         /* output features, any n >= 1 */
+    int k;         /* multiple of 32 */
+    int swiglu;    /* 1: silu(gate x) * up x over two sets, 0: one set */
+    int out_type;  /* WISP_DT_* */
+} WispFp4Config;
+
+/* codes: [n_entries x n x k/2] contiguous, 16-byte aligned, used where they
+ * lie. prepared: from wisp_b200_fp4_prepare over the set's scale bytes.
+ * tensor_scale: [n_entries] fp32 or NULL (all 1). */
+typedef struct {
+    const uint8_t* codes;
+    const void* prepared;
+    const float* tensor_scale;
+} WispFp4Mats;
+
+/* Activation rows from wisp_b200_fp4_quantize; tensor_scale: one fp32 or NULL
+ * (1). codes 16-byte aligned. */
+typedef struct {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const float* tensor_scale;
+    int rows;
+} WispFp4Rows;
+
+/* One-time layout of a set's scale bytes [n_entries x n x k/block] as the
+ * tensor cores take them (128 features x 256 k per run). d_prepared: 256-byte
+ * aligned, wisp_b200_fp4_prepared_bytes bytes. */
+size_t wisp_b200_fp4_prepared_bytes(const WispFp4Config* cfg);
+WispError wisp_b200_fp4_prepare(const WispFp4Config* cfg, const uint8_t* d_scales,
+                                void* d_prepared, size_t prepared_bytes, cudaStream_t stream,
+                                WispErrCtx* err);
+
+/* out[p, f] = sum_k x[p, k] w_e[f, k] (fp32 accumulation, rounded once to
+ * out_type; with swiglu silu(w x) * (up x)) for every row p of every segment,
+ * e = the segment's expert. d_segs: DEVICE array of n_segs <= 1025 segments
+ * over the rows, which must not overlap; NULL: all rows through entry 0. Rows
+ * in no segment are left as they are. A segment whose expert or rows lie
+ * outside the set or the rows is skipped and sets *d_error_flag to 2. ld: elements
+ * between output rows. up is NULL unless swiglu. d_error_flag as for
+ * wisp_b200_grouped_ffn (may be NULL; the call does not clear it).
+ * rows = 0 is allowed and launches nothing. */
+WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
+                                const WispFp4Mats* up, const WispFp4Rows* x,
+                                const WispSegment* d_segs, int n_segs, void* d_out, int64_t ld,
+                                int* d_error_flag, cudaStream_t stream, WispErrCtx* err);
+
+/* The MoE layer of wisp_b200_moe_forward over fp4 experts: route, dispatch
+ * plan, quantise the gathered rows, gate/up product with SwiGLU (bf16 rows),
+ * quantise, down product (fp32 rows), each token's rows summed in a fixed
+ * order with the routing weights. gate, up: sets of E (+1 shared) entries
+ * [inter x hidden], down: [hidden x inter], all prepared. cfg->group_size,
+ * cfg->deterministic are ignored (every run gives the same bits). x_scale,
+ * h_scale: the NV tensor scales of the layer's input and of the SwiGLU output
+ * (device, from calibration; NULL for MX). */
+typedef struct {
+    const uint16_t* router_w;  /* as in WispMoeWeights */
+    const float* router_bias;
+    WispFp4Mats gate, up, down;
+    const float* x_scale;
+    const float* h_scale;
+    int format;
+} WispFp4MoeWeights;
+
+size_t wisp_b200_fp4_moe_workspace_bytes(const WispMoeConfig* cfg, int format);
+WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const WispFp4MoeWeights* w,
+                                    const uint16_t* d_x, float* d_out, int* d_topk_idx,
+                                    float* d_topk_w, void* d_workspace, size_t workspace_bytes,
+                                    int* d_error_flag, cudaStream_t stream, WispErrCtx* err);
+
+/* --------------------------------------------------------------------------
+ * Norms around a block, with its gate and its residual (the reference runs
+ * them as op_rmsnorm, op_residual and op_rmsnorm over fp32,
+ * csrc/core/wisp_engine.c:1715-1722):
+ *   p  = post_norm ? y / rms(y) * (weight_offset + post_w) : y
+ *   x' = residual_scale * x + gate * p          (without y: x' = x)
+ *   n  = x' / rms(x') * (weight_offset + pre_w) (when d_n is not NULL)
+ * rms(v) = sqrt(mean(v^2) + eps). All in fp32; n is taken from x' before x'
+ * is rounded to x_type, so each output is rounded once.
+ * ------------------------------------------------------------------------ */
+enum { WISP_GATE_NONE = 0, WISP_GATE_CHANNEL = 1, WISP_GATE_TOKEN = 2, WISP_GATE_ELEMENT = 3 };
+
+typedef struct {
+    int tokens;            /* 0 allowed: launches nothing */
+    int hidden;            /* 1 .. 32768 */
+    int x_type, y_type;    /* WISP_DT_*: residual stream, block output */
+    int w_type, gate_type; /* norm weights, gate */
+    int n_type;            /* normalised output */
+    int post_norm;         /* 0: y enters without a norm */
+    int gate_kind;         /* WISP_GATE_*: [hidden], [tokens] or [tokens x hidden] */
+    float residual_scale;
+    float eps;             /* >= 0 */
+    float weight_offset;   /* 0, or 1 for weights stored around 0 */
+    int64_t ld_x, ld_y, ld_gate, ld_x_out, ld_n; /* elements between rows */
+} WispBlockNorm;
+
+/* d_y NULL: no block output (d_x_out, if given, is left as it is). d_post_w /
+ * d_pre_w NULL: ones. d_x_out NULL: x' is not stored; it may equal d_x. d_n
+ * NULL: no norm after. No other buffers may overlap. */
+WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* d_x, const void* d_y,
+                               const void* d_gate, const void* d_post_w, const void* d_pre_w,
+                               void* d_x_out, void* d_n, cudaStream_t stream, WispErrCtx* err);
+
 /* Between stacked layers: d_out[t] = bf16(d_in[t] / rms(d_in[t])), fp32 in. */
 WispError wisp_b200_rms_rescale(const float* d_in, uint16_t* d_out, int tokens, int hidden,
                                 float eps, cudaStream_t stream, WispErrCtx* err);

@@ -27,6 +27,16 @@ WISP_ERR_TIMEOUT = 7
 WISP_SCORE_SOFTMAX = 0
 WISP_SCORE_SIGMOID_GROUPED = 1
 
+WISP_FP4_MX = 0
+WISP_FP4_NV = 1
+WISP_DT_F32 = 0
+WISP_DT_BF16 = 1
+WISP_DT_F16 = 2
+WISP_GATE_NONE = 0
+WISP_GATE_CHANNEL = 1
+WISP_GATE_TOKEN = 2
+WISP_GATE_ELEMENT = 3
+
 
 class WispErrCtx(C.Structure):
     _fields_ = [("code", C.c_int), ("message", C.c_char * 512), ("file", C.c_char_p),
@@ -66,12 +76,42 @@ class WispSegment(C.Structure):
                 ("reserved", C.c_int32)]
 
 
+class WispFp4Config(C.Structure):
+    _fields_ = [("format", C.c_int), ("n_entries", C.c_int), ("n", C.c_int), ("k", C.c_int),
+                ("swiglu", C.c_int), ("out_type", C.c_int)]
+
+
+class WispFp4Mats(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("prepared", C.c_void_p), ("tensor_scale", C.c_void_p)]
+
+
+class WispFp4Rows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("tensor_scale", C.c_void_p),
+                ("rows", C.c_int)]
+
+
+class WispFp4MoeWeights(C.Structure):
+    _fields_ = [("router_w", C.c_void_p), ("router_bias", C.c_void_p), ("gate", WispFp4Mats),
+                ("up", WispFp4Mats), ("down", WispFp4Mats), ("x_scale", C.c_void_p),
+                ("h_scale", C.c_void_p), ("format", C.c_int)]
+
+
+class WispBlockNorm(C.Structure):
+    _fields_ = [("tokens", C.c_int), ("hidden", C.c_int), ("x_type", C.c_int), ("y_type", C.c_int),
+                ("w_type", C.c_int), ("gate_type", C.c_int), ("n_type", C.c_int),
+                ("post_norm", C.c_int), ("gate_kind", C.c_int), ("residual_scale", C.c_float),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("ld_x", C.c_int64),
+                ("ld_y", C.c_int64), ("ld_gate", C.c_int64), ("ld_x_out", C.c_int64),
+                ("ld_n", C.c_int64)]
+
+
 assert C.sizeof(WispInt4Expert) == 72 and C.sizeof(WispSegment) == 16
 
 _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
 _SZ = C.c_size_t
+_L = C.c_int64
 _E = C.POINTER(WispErrCtx)
 
 # name -> (restype, argtypes)
@@ -110,6 +150,17 @@ SIGNATURES = {
     "wisp_b200_dense_mlp": (_I, [C.POINTER(WispMoeConfig), _P, _P, _P, _P, _P, _SZ, _P, _P, _E]),
     "wisp_b200_pack_rows": (_I, [_P, _P, _I, _I, _P, _P, _E]),
     "wisp_b200_dispatch_plan": (_I, [C.POINTER(WispMoeConfig), _P, _P, _P, _P, _P, _P, _P, _E]),
+    "wisp_b200_fp4_quantize": (_I, [_P, _I, _L, _I, _P, _I, _I, _I, _P, _P, _P, _P, _E]),
+    "wisp_b200_fp4_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _P, _I, _L, _P, _E]),
+    "wisp_b200_fp4_prepared_bytes": (_SZ, [C.POINTER(WispFp4Config)]),
+    "wisp_b200_fp4_prepare": (_I, [C.POINTER(WispFp4Config), _P, _P, _SZ, _P, _E]),
+    "wisp_b200_fp4_product": (_I, [C.POINTER(WispFp4Config), C.POINTER(WispFp4Mats),
+                                   C.POINTER(WispFp4Mats), C.POINTER(WispFp4Rows), _P, _I, _P, _L,
+                                   _P, _P, _E]),
+    "wisp_b200_fp4_moe_workspace_bytes": (_SZ, [C.POINTER(WispMoeConfig), _I]),
+    "wisp_b200_fp4_moe_forward": (_I, [C.POINTER(WispMoeConfig), C.POINTER(WispFp4MoeWeights), _P,
+                                       _P, _P, _P, _P, _SZ, _P, _P, _E]),
+    "wisp_b200_block_norm": (_I, [C.POINTER(WispBlockNorm), _P, _P, _P, _P, _P, _P, _P, _P, _E]),
     "wisp_b200_rms_rescale": (_I, [_P, _P, _I, _I, _F, _P, _E]),
     "wisp_b200_combine_rows": (_I, [_P, _P, _P, _I, _I, _P, _P, _E]),
     "wisp_b200_ep_block_bytes": (_SZ, [_I, _I, _I, _I]),

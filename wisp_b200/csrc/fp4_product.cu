@@ -1,0 +1,560 @@
+// fp4_product.cu -- out[p, f] = sum_k x[p, k] w_e[f, k] over 4-bit
+// block-scaled rows and expert matrices (one expert per segment of rows), on
+// the tensor cores' block-scaled 4-bit instructions.
+//
+// The features are the MMA's M (128 per tile, so that a weight matrix streams
+// through shared memory once per token tile), the rows its N: any multiple of
+// 16 up to kMaxN, set per tile in the instruction descriptor, so one kernel
+// serves single tokens and prefill. An accumulator lane is then one feature
+// and a column one row: an epilogue warp stores 32 consecutive features of a
+// row at a time, and SwiGLU pairs the gate and up accumulators lane by lane.
+//
+// Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
+// scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 copy the rows'
+// scale bytes into the layout tcgen05.cp spreads over tensor memory, 1 issues
+// the scale copies and MMAs, 4-11 are the epilogue. tcgen05.mma after
+// tcgen05.cp of one thread are ordered; the reverse is not documented, so the
+// scales in tensor memory are double-buffered and a buffer is refilled only
+// when the MMAs of the stage before the last have completed.
+#include "common.cuh"
+#include "internal.h"
+#include "numeric.cuh"
+
+namespace {
+
+using namespace wb;
+
+constexpr int kThreads = 384;
+constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
+constexpr int kMaxSegs = 1025;
+constexpr int kABytes = 128 * 128;
+
+template <bool NV, bool SWIGLU>
+struct Shape {
+  static constexpr int kWords = NV ? 4 : 2;           // 4-scale words per row and stage
+  static constexpr int kMats = SWIGLU ? 2 : 1;
+  // Accumulators: two sets (gate and up, or two tiles of one) of kMaxN
+  // columns, beside two buffers of scales, in 512 columns.
+  static constexpr int kMaxN = NV ? 192 : 224;
+  static constexpr int kAccBufs = SWIGLU ? 1 : 2;
+  static constexpr int kSfA = 2 * kMaxN;              // first scale column
+  static constexpr int kSfCols = kWords * (4 * kMats + 8);
+  static_assert(2 * kMaxN + 2 * kSfCols <= 512, "tensor memory");
+  static constexpr int kSfaBytes = kWords * 512;
+  static constexpr int kSfbBytes = kWords * 2 * 512;
+  static constexpr int kBBytes = kMaxN * 128;
+  static constexpr int kStageBytes = kMats * (kABytes + kSfaBytes) + kBBytes + kSfbBytes;
+  static constexpr int kStages = SWIGLU ? 3 : 4;
+};
+
+template <int S>
+struct Bars {
+  uint64_t full[S];
+  uint64_t empty[S];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem;
+  int abort;
+  int bad;
+  int n_tiles;
+};
+
+struct alignas(64) Params {
+  CUtensorMap tm_w, tm_up, tm_x;
+  const uint8_t* sf_w;
+  const uint8_t* sf_up;
+  const float* ts_w;
+  const float* ts_up;
+  const float* ts_x;
+  const uint8_t* xs;      // row scales, xs_ld bytes per row
+  int xs_ld;
+  int xs_wide;            // whole stages may be read as one 8 or 16 byte word
+  int rows;
+  const WispSegment* segs;
+  int nseg;
+  int V, N, nk, ftiles;
+  void* out;
+  int64_t ld;
+  int out_type;
+  int* error_flag;
+};
+
+// Instruction descriptor of the block-scaled 4-bit MMAs: A and B e2m1, both
+// K-major, M = 128; scale type bit 23 (0: e4m3, 1: e8m0); the scale bytes
+// used within each 32-bit word at bits 29 (A) and 4 (B).
+template <bool NV>
+WB_DEV uint32_t idesc_fp4(int n) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((NV ? 0u : 1u) << 23) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+template <bool NV>
+WB_DEV void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                    uint32_t acc) {
+  if (NV)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+
+// 32 rows x 16 bytes of shared memory into 4 columns of every warp's lanes.
+WB_DEV void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+
+// Shared-memory descriptor of a 512-byte scale tile: no swizzle, 8-row groups
+// of 16-byte rows 128 bytes apart.
+WB_DEV uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) |
+         ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
+}
+
+struct Tile {
+  int expert, row0, cnt;   // rows row0 .. row0 + cnt - 1
+};
+
+// Rows per tile of a segment: as many tiles as kMaxN demands, of equal size
+// up to the MMA's granularity of 16.
+template <int MAXN>
+WB_DEV int tile_rows(int rows) {
+  const int t = (rows + MAXN - 1) / MAXN;
+  return ((rows + t - 1) / t + 15) & ~15;
+}
+
+WB_DEV WispSegment segment(const Params& p, int s) {
+  if (p.segs) return p.segs[s];
+  WispSegment v;
+  v.expert = 0;
+  v.row_begin = 0;
+  v.rows = p.rows;
+  v.reserved = 0;
+  return v;
+}
+
+WB_DEV bool segment_ok(const Params& p, const WispSegment& v) {
+  return v.rows >= 0 && v.row_begin >= 0 && (int64_t)v.row_begin + v.rows <= p.rows &&
+         (v.rows == 0 || (v.expert >= 0 && v.expert < p.V));
+}
+
+// pref[s] = token tiles of the segments before s.
+template <int MAXN>
+WB_DEV Tile find_tile(const Params& p, const int* pref, int nseg, int tt) {
+  int lo = 0, hi = nseg;       // the last s with pref[s] <= tt
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (pref[m] <= tt)
+      lo = m;
+    else
+      hi = m;
+  }
+  const WispSegment v = segment(p, lo);
+  const int per = tile_rows<MAXN>(v.rows);
+  const int r0 = (tt - pref[lo]) * per;
+  Tile t;
+  t.expert = v.expert;
+  t.row0 = v.row_begin + r0;
+  t.cnt = min(per, v.rows - r0);
+  return t;
+}
+
+template <bool NV, bool SWIGLU>
+__global__ void __launch_bounds__(kThreads, 1)
+fp4_product_kernel(const __grid_constant__ Params p) {
+  using C = Shape<NV, SWIGLU>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ Bars<S> bars;
+  __shared__ int pref[kMaxSegs + 1];
+  __shared__ int warp_tot[kThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort = &bars.abort;
+
+  if (tid == 0) {
+    for (int i = 0; i < S; i++) {
+      mbar_init(&bars.full[i], 3);      // producer, two scale warps
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&bars.acc_full[i], 1);
+      mbar_init(&bars.acc_empty[i], 8);
+    }
+    bars.abort = 0;
+    bars.bad = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&bars.tmem, 512);
+  // Token tiles before each segment: 3 segments per thread, then one scan.
+  const int nseg = p.segs ? p.nseg : 1;
+  {
+    int n[3], sum = 0;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+      const int s = tid * 3 + j;
+      n[j] = 0;
+      if (s < nseg) {
+        const WispSegment v = segment(p, s);
+        if (!segment_ok(p, v))
+          bad = true;
+        else if (v.rows > 0) {
+          const int per = tile_rows<C::kMaxN>(v.rows);
+          n[j] = (v.rows + per - 1) / per;
+        }
+      }
+      sum += n[j];
+    }
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_tot[warp] = x;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int base = x - sum;
+    for (int w = 0; w < warp; w++) base += warp_tot[w];
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+      const int s = tid * 3 + j;
+      if (s < nseg) pref[s] = base;
+      base += n[j];
+    }
+    if (tid == kThreads - 1) bars.n_tiles = base;
+    if (bad && p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
+  }
+  __syncthreads();
+  const uint32_t tmem = bars.tmem;
+  const int64_t items = (int64_t)bars.n_tiles * p.ftiles;
+  const int nk = p.nk;
+  auto stage = [&](int s) { return smem + s * C::kStageBytes; };
+  // a stage: weights (gate, up), their scales (gate, up), row codes, row scales
+  constexpr int kOffSfa = C::kMats * kABytes;
+  // the swizzle needs 1024-byte aligned operands, the scales 16
+  constexpr int kOffB = kOffSfa;
+  constexpr int kOffSf = kOffB + C::kBBytes;
+  constexpr int kOffSfb = kOffSf + C::kMats * C::kSfaBytes;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&p.tm_w);
+      tma_prefetch_desc(&p.tm_x);
+      if (SWIGLU) tma_prefetch_desc(&p.tm_up);
+      int i = 0;
+      int64_t uses = 0;
+      for (int64_t it = blockIdx.x; it < items && !*abort; it += gridDim.x) {
+        const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
+        const int ft = (int)(it % p.ftiles);
+        const int wrow = t.expert * p.N + ft * 128;
+        const int64_t sf = ((int64_t)t.expert * p.ftiles + ft) * nk;
+        const int nb = (t.cnt + 31) >> 5;
+        const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * 4096;
+        for (int kk = 0; kk < nk; kk++, uses++) {
+          const int s = (int)(uses % S);
+          if (uses >= S && !mbar_wait(&bars.empty[s], (uint32_t)(uses / S - 1) & 1, abort)) break;
+          uint8_t* st = stage(s);
+          mbar_arrive_expect_tx(&bars.full[s], bytes);
+          tma_load_2d(st, &p.tm_w, &bars.full[s], kk * 128, wrow);
+          bulk_load(st + kOffSf, p.sf_w + (sf + kk) * C::kSfaBytes, C::kSfaBytes, &bars.full[s]);
+          if (SWIGLU) {
+            tma_load_2d(st + kABytes, &p.tm_up, &bars.full[s], kk * 128, wrow);
+            bulk_load(st + kOffSf + C::kSfaBytes, p.sf_up + (sf + kk) * C::kSfaBytes, C::kSfaBytes,
+                      &bars.full[s]);
+          }
+          for (int b = 0; b < nb; b++)
+            tma_load_2d(st + kOffB + b * 4096, &p.tm_x, &bars.full[s], kk * 128, t.row0 + b * 32);
+        }
+        (void)i;
+      }
+      if (*abort) {
+        // let the copies in flight land before the CTA's memory goes away
+        for (int64_t u = uses > S ? uses - S : 0; u < uses; u++)
+          mbar_wait(&bars.full[u % S], (uint32_t)(u / S) & 1, abort, 20000000LL);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int64_t uses = 0;
+      int64_t nt = 0;
+      bool ok = true;
+      for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x, nt++) {
+        const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
+        const int n = (t.cnt + 15) & ~15;
+        const uint32_t idesc = idesc_fp4<NV>(n);
+        const int ab = (int)(nt % C::kAccBufs);
+        const int64_t au = nt / C::kAccBufs;
+        if (au >= 1 && !mbar_wait(&bars.acc_empty[ab], (uint32_t)(au - 1) & 1, abort)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + ab * C::kMaxN;
+        for (int kk = 0; kk < nk; kk++, uses++) {
+          const int s = (int)(uses % S);
+          if (!mbar_wait(&bars.full[s], (uint32_t)(uses / S) & 1, abort)) { ok = false; break; }
+          // the scale buffer's last readers: the MMAs of stage uses - 2
+          if (uses >= 2) {
+            const int64_t u = uses - 2;
+            if (!mbar_wait(&bars.empty[u % S], (uint32_t)(u / S) & 1, abort)) { ok = false; break; }
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(stage(s));
+          const uint32_t sfa = tmem + C::kSfA + (uint32_t)(uses & 1) * C::kSfCols;
+          const uint32_t sfb = sfa + C::kMats * C::kWords * 4;
+#pragma unroll
+          for (int w = 0; w < C::kMats * C::kWords; w++)
+            tmem_cp_scales(sfa + w * 4, scale_desc(st + kOffSf + w * 512));
+#pragma unroll
+          for (int w = 0; w < C::kWords; w++) {
+            tmem_cp_scales(sfb + w * 8, scale_desc(st + kOffSfb + w * 1024));
+            if (n > 128) tmem_cp_scales(sfb + w * 8 + 4, scale_desc(st + kOffSfb + w * 1024 + 512));
+          }
+          const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + kOffB);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {          // 64 k (32 bytes) each
+            const int w = NV ? j : j >> 1;
+            const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2;
+            const uint32_t ids = idesc | (id << 29) | (id << 4);
+            const uint32_t acc = (kk | j) ? 1u : 0u;
+            mma_fp4<NV>(d, da + j * 2, db + j * 2, ids, sfa + w * 4, sfb + w * 8, acc);
+            if (SWIGLU)
+              mma_fp4<NV>(d + C::kMaxN, da + (kABytes >> 4) + j * 2, db + j * 2, ids,
+                          sfa + (C::kWords + w) * 4, sfb + w * 8, acc);
+          }
+          mma_commit(&bars.empty[s]);
+        }
+        if (ok) mma_commit(&bars.acc_full[ab]);
+      }
+      if (*abort) {
+        for (int64_t u = uses > S ? uses - S : 0; u < uses; u++)
+          mbar_wait(&bars.empty[u % S], (uint32_t)(u / S) & 1, abort, 20000000LL);
+      }
+    }
+  } else if (warp < kEpiWarp) {
+    // Row scales: two warps, rows lid, lid + 64, ... of the tile; the words of
+    // the next stage are read before the wait for this stage's slot.
+    constexpr int R = (C::kMaxN + 63) / 64;
+    const int lid = tid - 64;
+    int64_t uses = 0;
+    auto fetch = [&](const Tile& t, int kk, uint32_t (&w)[R][C::kWords]) {
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int r = lid + 64 * i;
+#pragma unroll
+        for (int j = 0; j < C::kWords; j++) w[i][j] = 0;
+        if (r < t.cnt) {
+          const uint8_t* src = p.xs + (int64_t)(t.row0 + r) * p.xs_ld + kk * C::kWords * 4;
+          const int left = p.xs_ld - kk * C::kWords * 4;
+          if (p.xs_wide && left >= C::kWords * 4) {
+            if (NV) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+              w[i][C::kWords - 2] = v.z;
+              w[i][C::kWords - 1] = v.w;
+            } else {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+              w[i][0] = v.x;
+              w[i][1] = v.y;
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < C::kWords * 4; b++)
+              if (b < left) w[i][b >> 2] |= (uint32_t)__ldg(src + b) << (8 * (b & 3));
+          }
+        }
+      }
+    };
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
+      uint32_t cur[R][C::kWords];
+      fetch(t, 0, cur);
+      for (int kk = 0; kk < nk; kk++, uses++) {
+        uint32_t nxt[R][C::kWords];
+        fetch(t, min(kk + 1, nk - 1), nxt);
+        const int s = (int)(uses % S);
+        if (uses >= S) ok = mbar_wait(&bars.empty[s], (uint32_t)(uses / S - 1) & 1, abort);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        uint32_t* dst = reinterpret_cast<uint32_t*>(stage(s) + kOffSfb);
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+          const int r = lid + 64 * i;
+          if (r < C::kMaxN) {
+#pragma unroll
+            for (int w = 0; w < C::kWords; w++)
+              dst[w * 256 + (r >> 7) * 128 + (r & 31) * 4 + ((r >> 5) & 3)] = cur[i][w];
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.full[s]);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int w = 0; w < C::kWords; w++) cur[i][w] = nxt[i][w];
+      }
+    }
+  } else {
+    // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
+    // take alternate groups of 16 rows.
+    const int quad = warp & 3, half = (warp - kEpiWarp) >> 2;
+    const float tx = p.ts_x ? __ldg(p.ts_x) : 1.f;
+    int64_t nt = 0;
+    for (int64_t it = blockIdx.x; it < items; it += gridDim.x, nt++) {
+      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
+      const int f = (int)(it % p.ftiles) * 128 + quad * 32 + lane;
+      const int ab = (int)(nt % C::kAccBufs);
+      const int64_t au = nt / C::kAccBufs;
+      const float ag = tx * (p.ts_w ? __ldg(p.ts_w + t.expert) : 1.f);
+      const float au2 = SWIGLU ? tx * (p.ts_up ? __ldg(p.ts_up + t.expert) : 1.f) : 0.f;
+      const bool ok = mbar_wait(&bars.acc_full[ab], (uint32_t)au & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + ab * C::kMaxN + ((uint32_t)(quad * 32) << 16);
+      for (int c = half * 16; c < t.cnt; c += 32) {
+        uint32_t g[16], u[16];
+        tmem_ld16(d + c, g);
+        if (SWIGLU) tmem_ld16(d + C::kMaxN + c, u);
+        tmem_wait_ld();
+        if (f < p.N) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            if (c + i < t.cnt) {
+              float v = __uint_as_float(g[i]) * ag;
+              if (SWIGLU) v = v / (1.f + expf(-v)) * (__uint_as_float(u[i]) * au2);
+              store_one(p.out, p.out_type, (int64_t)(t.row0 + c + i) * p.ld + f, v);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.acc_empty[ab]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 512);
+  }
+  if (tid == 0 && bars.abort && p.error_flag) atomicMax(p.error_flag, 1);
+}
+
+// Code rows [rows x k/2 bytes] as a 2D tensor; one box = box_rows x 128 bytes
+// (256 k), 128-byte swizzle. Bytes past a row and rows past the end read 0.
+bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box_rows) {
+  wb::TensorMapEncodeFn fn = wb::tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)k / 2, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)k / 2};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool NV, bool SWIGLU>
+WispError launch_product(const Params& p, int64_t max_items, cudaStream_t stream,
+                         WispErrCtx* err) {
+  using C = Shape<NV, SWIGLU>;
+  const int smem = C::kStages * C::kStageBytes + 1024;
+  auto kernel = fp4_product_kernel<NV, SWIGLU>;
+  int dev = 0, sms = 0;
+  WB_CUDA_CHECK(cudaGetDevice(&dev));
+  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  WB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int grid = (int)(max_items < sms ? max_items : sms);
+  wb::launch_k(kernel, grid, kThreads, smem, stream, p);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
+WispError check_mats(const WispFp4Mats* m, const char* what, WispErrCtx* err) {
+  if (!m || !m->codes || !m->prepared)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: null pointer argument (%s)", what);
+  if (((uintptr_t)m->codes & 15) || ((uintptr_t)m->prepared & 255) ||
+      ((uintptr_t)m->tensor_scale & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp4_product: %s codes must be 16-byte, prepared 256-byte aligned", what);
+  return WISP_OK;
+}
+
+}  // namespace
+
+extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
+                                           const WispFp4Mats* up, const WispFp4Rows* x,
+                                           const WispSegment* d_segs, int n_segs, void* d_out,
+                                           int64_t ld, int* d_error_flag, cudaStream_t stream,
+                                           WispErrCtx* err) {
+  WispError e = wb::fp4_validate(cfg, "fp4_product", err);
+  if (e != WISP_OK) return e;
+  if ((e = check_mats(w, "weights", err)) != WISP_OK) return e;
+  if (cfg->swiglu && (e = check_mats(up, "up weights", err)) != WISP_OK) return e;
+  if (!cfg->swiglu && up)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: up weights without swiglu");
+  if (!x || x->rows < 0) return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: bad rows");
+  if (d_segs ? (n_segs < 0 || n_segs > kMaxSegs) : n_segs != 0)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: n_segs=%d (0..%d, 0 without segments)",
+                   n_segs, kMaxSegs);
+  if (ld < cfg->n)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: ld=%lld < n=%d", (long long)ld, cfg->n);
+  if (x->rows == 0 || (d_segs && n_segs == 0)) return WISP_OK;
+  if (!x->codes || !x->scales || !d_out)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: null pointer argument (rows, out)");
+  if (((uintptr_t)x->codes & 15) || ((uintptr_t)x->tensor_scale & 3) ||
+      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp4_product: row codes must be 16-byte aligned, out to its type");
+  const bool nv = cfg->format == WISP_FP4_NV;
+  Params p;
+  memset(&p, 0, sizeof p);
+  const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
+  if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
+      (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
+      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, 32))
+    return WB_FAIL(WISP_ERR_CUDA, "fp4_product: cuTensorMapEncodeTiled failed");
+  p.sf_w = static_cast<const uint8_t*>(w->prepared);
+  p.ts_w = w->tensor_scale;
+  if (cfg->swiglu) {
+    p.sf_up = static_cast<const uint8_t*>(up->prepared);
+    p.ts_up = up->tensor_scale;
+  }
+  p.ts_x = x->tensor_scale;
+  p.xs = x->scales;
+  p.xs_ld = cfg->k / (nv ? 16 : 32);
+  const int wide = nv ? 16 : 8;
+  p.xs_wide = p.xs_ld % wide == 0 && (uintptr_t)x->scales % wide == 0;
+  p.rows = x->rows;
+  p.segs = d_segs;
+  p.nseg = n_segs;
+  p.V = cfg->n_entries;
+  p.N = cfg->n;
+  p.nk = (cfg->k + 255) / 256;
+  p.ftiles = (cfg->n + 127) / 128;
+  p.out = d_out;
+  p.ld = ld;
+  p.out_type = cfg->out_type;
+  p.error_flag = d_error_flag;
+  // at most one token tile per row, and per segment one more than its rows fill
+  const int64_t tiles = d_segs ? (int64_t)x->rows / 192 + n_segs + x->rows / 192
+                               : ((int64_t)x->rows + 15) / 16;
+  const int64_t items = (tiles < x->rows ? tiles : x->rows) * p.ftiles;
+  if (nv)
+    return cfg->swiglu ? launch_product<true, true>(p, items, stream, err)
+                       : launch_product<true, false>(p, items, stream, err);
+  return cfg->swiglu ? launch_product<false, true>(p, items, stream, err)
+                     : launch_product<false, false>(p, items, stream, err);
+}

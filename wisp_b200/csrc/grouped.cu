@@ -983,6 +983,12 @@ EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+}  // namespace
+
+wb::TensorMapEncodeFn wb::tensor_map_encoder() { return get_encode_fn(); }
+
+namespace {
+
 // fp16 activation rows [rows x cols] as a 3D tensor {64 K, rows, K / 64} for
 // the tensor-core kernel: one box = box_rows rows x 128 K, stored as two [box_rows][128 B]
 // halves (one per 64 K) with the 128-byte swizzle -- the MMA's B operand of

@@ -1,6 +1,7 @@
 // internal.h -- host-side helpers shared by the wisp_b200 translation units.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdarg>
@@ -62,6 +63,17 @@ struct DecodeUnits {
   uint8_t* xq;   // q16 input rows in the same workspace
   int per_gu, per_dn, cols, sk_rows, ks_dn, nk_dn, target;
 };
+
+// cuTensorMapEncodeTiled from the loaded driver (nullptr without one).
+using TensorMapEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                       const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                       const cuuint32_t*, CUtensorMapInterleave,
+                                       CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                       CUtensorMapFloatOOBfill);
+TensorMapEncodeFn tensor_map_encoder();
+
+// Checks shared by the fp4 weight-set entry points (fp4.cu).
+WispError fp4_validate(const WispFp4Config* c, const char* who, WispErrCtx* err);
 
 // Fill a WispErrCtx the way the reference's WISP_ERR_SET does
 // (csrc/core/wisp_engine.h:66-72) and return the code.

@@ -410,6 +410,131 @@ extern "C" WispError wisp_b200_dense_mlp(const WispMoeConfig* cfg, const void* d
                               stream, err);
 }
 
+// ---------------------------------------------------------------------------
+// The same layer over fp4 experts: route and dispatch plan as above, then the
+// products of fp4_product.cu with the rows quantised before each, and the
+// fixed-order combine.
+// ---------------------------------------------------------------------------
+namespace {
+
+struct Fp4Ws {
+  Workspace base;      // routing, plan, y, token lists
+  float* part;
+  uint8_t* xc;
+  uint8_t* xs;
+  uint16_t* h;
+  uint8_t* hc;
+  uint8_t* hs;
+  size_t bytes;
+};
+
+Fp4Ws carve_fp4(const WispMoeConfig* c, int format, void* base) {
+  Fp4Ws ws;
+  Carve cv;
+  const int T = c->tokens, E = c->n_experts, k = c->top_k, M = c->hidden, I = c->inter;
+  const int V = E + (c->has_shared ? 1 : 0);
+  const int block = format == WISP_FP4_NV ? 16 : 32;
+  Workspace& b = ws.base;
+  b.lanes = k + (c->has_shared ? 1 : 0);
+  b.rows = T * b.lanes;
+  b.splits = wb::router_splits(T, E, M);
+  ws.part = cv.take<float>(base, b.splits * (size_t)T * E);
+  b.plan_scratch = cv.take<int>(base, std::max<size_t>(1, wb::plan_scratch_ints(c)));
+  b.idx = cv.take<int>(base, (size_t)T * k);
+  b.w = cv.take<float>(base, (size_t)T * k);
+  b.counts = cv.take<int>(base, V);
+  b.segs = cv.take<WispSegment>(base, V);
+  b.row_token = cv.take<int>(base, b.rows);
+  b.row_weight = cv.take<float>(base, b.rows);
+  b.y = cv.take<float>(base, (size_t)b.rows * M);
+  b.tok_cnt = cv.take<int>(base, T);
+  b.tok_list = cv.take<int>(base, (size_t)T * b.lanes);
+  ws.xc = cv.take<uint8_t>(base, (size_t)b.rows * (M / 2));
+  ws.xs = cv.take<uint8_t>(base, (size_t)b.rows * (M / block));
+  ws.h = cv.take<uint16_t>(base, (size_t)b.rows * I);
+  ws.hc = cv.take<uint8_t>(base, (size_t)b.rows * (I / 2));
+  ws.hs = cv.take<uint8_t>(base, (size_t)b.rows * (I / block));
+  ws.bytes = (cv.off + 255) & ~(size_t)255;
+  return ws;
+}
+
+// group_size is the int4 layer's; any valid value passes its check.
+WispError validate_fp4(const WispMoeConfig* c, int format, WispErrCtx* err) {
+  if (!c) return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_moe: null config");
+  if (format != WISP_FP4_MX && format != WISP_FP4_NV)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_moe: unknown format %d", format);
+  WispMoeConfig v = *c;
+  v.group_size = 128;
+  return validate(&v, err);
+}
+
+}  // namespace
+
+extern "C" size_t wisp_b200_fp4_moe_workspace_bytes(const WispMoeConfig* cfg, int format) {
+  if (validate_fp4(cfg, format, nullptr) != WISP_OK) return 0;
+  return carve_fp4(cfg, format, nullptr).bytes;
+}
+
+extern "C" WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const WispFp4MoeWeights* w,
+                                               const uint16_t* d_x, float* d_out, int* d_topk_idx,
+                                               float* d_topk_w, void* d_workspace,
+                                               size_t workspace_bytes, int* d_error_flag,
+                                               cudaStream_t stream, WispErrCtx* err) {
+  if (!w) return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_moe_forward: null weights");
+  WispError e = validate_fp4(cfg, w->format, err);
+  if (e != WISP_OK) return e;
+  if (!w->router_w || !d_x || !d_out || !d_workspace)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp4_moe_forward: null pointer argument (router_w, x, out, workspace)");
+  if (((uintptr_t)d_x | (uintptr_t)w->router_w) & 15 || (uintptr_t)d_workspace & 255)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp4_moe_forward: x and router_w must be 16-byte, workspace 256-byte aligned");
+  if (w->format == WISP_FP4_NV && (!w->x_scale || !w->h_scale))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_moe_forward: NV needs x_scale and h_scale");
+  const Fp4Ws ws = carve_fp4(cfg, w->format, d_workspace);
+  if (workspace_bytes < ws.bytes)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_moe_forward: workspace %zu < required %zu",
+                   workspace_bytes, ws.bytes);
+  const Workspace& b = ws.base;
+  const int T = cfg->tokens, M = cfg->hidden, I = cfg->inter;
+  const int V = cfg->n_experts + (cfg->has_shared ? 1 : 0);
+  int* idx = d_topk_idx ? d_topk_idx : b.idx;
+  float* wt = d_topk_w ? d_topk_w : b.w;
+  const bool nv = w->format == WISP_FP4_NV;
+  const float* xsc = nv ? w->x_scale : nullptr;
+  const float* hsc = nv ? w->h_scale : nullptr;
+
+  e = wb::launch_route(cfg, d_x, w->router_w, w->router_bias, ws.part, b.splits, nullptr, idx, wt,
+                       stream, err);
+  if (e != WISP_OK) return e;
+  e = wb::launch_plan(cfg, idx, wt, b.counts, b.segs, b.row_token, b.row_weight, stream, err,
+                      b.plan_scratch);
+  if (e != WISP_OK) return e;
+  e = wisp_b200_fp4_quantize(d_x, WISP_DT_BF16, M, T, b.row_token, b.rows, M, w->format, xsc, ws.xc,
+                             ws.xs, stream, err);
+  if (e != WISP_OK) return e;
+  WispFp4Config gu = {w->format, V, I, M, 1, WISP_DT_BF16};
+  const WispFp4Rows xr = {ws.xc, ws.xs, xsc, b.rows};
+  e = wisp_b200_fp4_product(&gu, &w->gate, &w->up, &xr, b.segs, V, ws.h, I, d_error_flag, stream,
+                            err);
+  if (e != WISP_OK) return e;
+  e = wisp_b200_fp4_quantize(ws.h, WISP_DT_BF16, I, b.rows, nullptr, b.rows, I, w->format, hsc,
+                             ws.hc, ws.hs, stream, err);
+  if (e != WISP_OK) return e;
+  WispFp4Config dn = {w->format, V, M, I, 0, WISP_DT_F32};
+  const WispFp4Rows hr = {ws.hc, ws.hs, hsc, b.rows};
+  e = wisp_b200_fp4_product(&dn, &w->down, nullptr, &hr, b.segs, V, b.y, M, d_error_flag, stream,
+                            err);
+  if (e != WISP_OK) return e;
+  WB_CUDA_CHECK(cudaMemsetAsync(b.tok_cnt, 0, (size_t)T * sizeof(int), stream));
+  wb::launch_k(token_rows_kernel, (b.rows + 255) / 256, 256, 0, stream, b.row_token, b.segs, V,
+               b.rows, b.lanes, b.tok_cnt, b.tok_list);
+  wb::launch_k(combine_ordered_kernel, dim3(T, (M + 1023) / 1024), 256, 0, stream, b.y,
+               b.row_weight, b.tok_cnt, b.tok_list, b.lanes, M, d_out);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
 // Pointers into a reference blob (header at offset 0) from its parsed meta.
 extern "C" WispError wisp_b200_blob_expert(const WispExpertMeta* meta, const void* d_blob,
                                            WispInt4Expert* out, WispErrCtx* err) {

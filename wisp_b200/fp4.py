@@ -1,0 +1,317 @@
+"""4-bit block-scaled (MXFP4 / NVFP4) rows, expert matrices and MoE layer.
+
+Thin wrappers over the C ABI (include/wisp_b200.h): tensors are PyTorch CUDA
+tensors used as device memory; every launch goes on the current torch stream
+of the tensors' device. The work itself runs in libwisp_b200.so.
+
+    q = quantize(x, abi.WISP_FP4_MX)                # rows -> codes and scales
+    w = Fp4Weights(abi.WISP_FP4_MX, codes, scales)  # [V, n, k/2], [V, n, k/32]
+    y = product(q, w, segments)                     # rows by their experts' matrices
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from . import abi
+
+BLOCK = {abi.WISP_FP4_MX: 32, abi.WISP_FP4_NV: 16}
+DTYPES = {torch.float32: abi.WISP_DT_F32, torch.bfloat16: abi.WISP_DT_BF16,
+          torch.float16: abi.WISP_DT_F16}
+
+
+def invalid(msg: str) -> RuntimeError:
+    return RuntimeError(f"wisp engine error [{abi.WISP_ERR_INVALID_ARG}]: {msg}")
+
+
+def on_device(t: torch.Tensor):
+    """Context in which launches go to t's device (nothing to do on the current one)."""
+    if t.device.type != "cuda":
+        raise invalid(f"tensor on {t.device}: the kernels have no CPU path")
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def dtype_code(dtype: torch.dtype, what: str) -> int:
+    code = DTYPES.get(dtype)
+    if code is None:
+        raise invalid(f"{what}: {dtype} (float32, bfloat16 or float16)")
+    return code
+
+
+def row_stride(t: torch.Tensor, what: str) -> int:
+    """Elements between the rows of a 2D tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise invalid(f"{what}: a 2D tensor with contiguous rows is needed")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def same_device(ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise invalid(f"{name} is on {t.device}, not on {ref.device}")
+
+
+def _check_scale(ts: torch.Tensor | None, n: int, what: str) -> None:
+    if ts is not None and (ts.dtype != torch.float32 or ts.numel() != n or not ts.is_contiguous()):
+        raise invalid(f"{what}: {n} contiguous float32 needed")
+
+
+def _check_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor) -> int:
+    """Checks a codes/scales pair; returns the row length."""
+    if fmt not in BLOCK:
+        raise invalid(f"unknown format {fmt}")
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise invalid("codes and scales are uint8")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise invalid("codes and scales must be contiguous")
+    k = codes.shape[-1] * 2
+    if codes.shape[:-1] != scales.shape[:-1] or k % BLOCK[fmt] or \
+            scales.shape[-1] != k // BLOCK[fmt]:
+        raise invalid(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} disagree "
+                      f"(blocks of {BLOCK[fmt]})")
+    same_device(codes, scales=scales)
+    return k
+
+
+@dataclass
+class Fp4Rows:
+    """Quantised rows: codes [R, K/2], scales [R, K/block], one tensor scale (NV)."""
+    fmt: int
+    codes: torch.Tensor
+    scales: torch.Tensor
+    tensor_scale: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        if self.codes.dim() != 2:
+            raise invalid("rows are 2D")
+        self.cols = _check_codes(self.fmt, self.codes, self.scales)
+        _check_scale(self.tensor_scale, 1, "tensor_scale")
+        same_device(self.codes, tensor_scale=self.tensor_scale)
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+
+def tensor_scale(x: torch.Tensor) -> torch.Tensor:
+    """The NV tensor scale that lets the largest block scale reach 448: max|x| / 2688
+    (1 for an all-zero tensor)."""
+    s = x.detach().abs().amax().float() / (6.0 * 448.0)
+    return torch.where(s > 0, s, torch.ones_like(s)).reshape(1)
+
+
+def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None,
+             rows: torch.Tensor | None = None) -> Fp4Rows:
+    """Rows of x (float32, bfloat16 or float16) as 4-bit codes; rows (int32): row p of the
+    result is row rows[p] of x, a row of zeros where rows[p] is outside x."""
+    if fmt not in BLOCK:
+        raise invalid(f"unknown format {fmt}")
+    ld = row_stride(x, "x")
+    n, cols = x.shape
+    if cols % BLOCK[fmt] or cols == 0:
+        raise invalid(f"row length {cols} is no multiple of {BLOCK[fmt]}")
+    if fmt == abi.WISP_FP4_NV and tensor_scale is None:
+        raise invalid("NV rows need a tensor scale")
+    _check_scale(tensor_scale, 1, "tensor_scale")
+    if rows is not None:
+        if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+            raise invalid("rows: a contiguous 1D int32 tensor")
+    same_device(x, tensor_scale=tensor_scale, rows=rows)
+    dt = dtype_code(x.dtype, "x")
+    r = n if rows is None else rows.shape[0]
+    with on_device(x):
+        codes = torch.empty((r, cols // 2), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((r, cols // BLOCK[fmt]), dtype=torch.uint8, device=x.device)
+        abi.call("wisp_b200_fp4_quantize", x.data_ptr(), dt, ld, n,
+                 None if rows is None else rows.data_ptr(), r, cols, fmt,
+                 None if tensor_scale is None else tensor_scale.data_ptr(), codes.data_ptr(),
+                 scales.data_ptr(), stream_of(x))
+    return Fp4Rows(fmt, codes, scales, tensor_scale if fmt == abi.WISP_FP4_NV else None)
+
+
+def dequantize(q: Fp4Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of quantised rows."""
+    dt = dtype_code(dtype, "dtype")
+    with on_device(q.codes):
+        out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.codes.device)
+        abi.call("wisp_b200_fp4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows,
+                 q.cols, q.fmt, None if q.tensor_scale is None else q.tensor_scale.data_ptr(),
+                 out.data_ptr(), dt, q.cols, stream_of(q.codes))
+    return out
+
+
+class Fp4Weights:
+    """V matrices [n, k] (one per expert) laid out once for the product; with ``up``, V pairs
+    for silu(gate x) * up x. codes [V, n, k/2] stay in use where they are; scales
+    [V, n, k/block] are laid out into a buffer of the object and no longer needed; scale: fp32
+    [V] tensor scales or None."""
+
+    def __init__(self, fmt: int, codes: torch.Tensor, scales: torch.Tensor,
+                 scale: torch.Tensor | None = None, up: tuple | None = None):
+        if codes.dim() != 3:
+            raise invalid("weight codes are [entries, n, k/2]")
+        self.fmt = fmt
+        self.k = _check_codes(fmt, codes, scales)
+        self.entries, self.n = codes.shape[:2]
+        if self.k % 32:
+            raise invalid(f"k={self.k} is no multiple of 32")
+        mats = [(codes, scales, scale)] + ([tuple(up)] if up is not None else [])
+        self.cfg = abi.WispFp4Config(fmt, self.entries, self.n, self.k, len(mats) - 1,
+                                     abi.WISP_DT_F32)
+        self._keep, structs = [], []
+        with on_device(codes):
+            nbytes = abi.lib().wisp_b200_fp4_prepared_bytes(C.byref(self.cfg))
+            if nbytes == 0:
+                raise invalid(f"weights [{self.entries}, {self.n}, {self.k}] are not supported")
+            for c, s, ts in mats:
+                if c.shape != codes.shape:
+                    raise invalid("gate and up differ in shape")
+                _check_codes(fmt, c, s)
+                _check_scale(ts, self.entries, "scale")
+                same_device(codes, codes=c, scales=s, scale=ts)
+                prepared = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+                abi.call("wisp_b200_fp4_prepare", C.byref(self.cfg), s.data_ptr(),
+                         prepared.data_ptr(), nbytes, stream_of(codes))
+                self._keep.append((c, prepared, ts))
+                structs.append(abi.WispFp4Mats(c.data_ptr(), prepared.data_ptr(),
+                                               None if ts is None else ts.data_ptr()))
+            self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
+            # laid out once: any stream may use the object from here on
+            torch.cuda.current_stream(codes.device).synchronize()
+        self.mats = structs[0]
+        self.up_mats = structs[1] if len(structs) == 2 else None
+
+    @classmethod
+    def from_values(cls, fmt: int, w: torch.Tensor, up: torch.Tensor | None = None) -> "Fp4Weights":
+        """Quantises matrices w [V, n, k] (and up), one tensor scale per matrix for NV."""
+        sets = []
+        for m in [w] if up is None else [w, up]:
+            if m.dim() != 3:
+                raise invalid("weights are [entries, n, k]")
+            ts = None
+            if fmt == abi.WISP_FP4_NV:
+                ts = torch.cat([tensor_scale(e) for e in m])
+            qs = [quantize(e, fmt, None if ts is None else ts[i:i + 1]) for i, e in enumerate(m)]
+            sets.append((torch.stack([q.codes for q in qs]), torch.stack([q.scales for q in qs]),
+                         ts))
+        return cls(fmt, *sets[0], up=sets[1] if len(sets) == 2 else None)
+
+    @property
+    def device(self) -> torch.device:
+        return self.error_word.device
+
+    def check(self) -> None:
+        """Raise if a product with these weights gave up waiting or met a bad segment."""
+        with on_device(self.error_word):
+            abi.call("wisp_b200_check_error_flag", self.error_word.data_ptr(),
+                     stream_of(self.error_word))
+
+
+def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """out[p] = w_e q[p] (silu(gate q) * up q for paired weights) for the rows p of each
+    segment. segments: int32 [S, 4] (expert, first row, rows, 0) on the device, as
+    wisp_b200_dispatch_plan writes them; None: all rows through entry 0. Rows in no segment are
+    left as they are (out given) or undefined (out allocated here)."""
+    if q.fmt != w.fmt or q.cols != w.k:
+        raise invalid(f"rows (format {q.fmt}, k={q.cols}) do not fit the weights (format "
+                      f"{w.fmt}, k={w.k})")
+    if segments is not None:
+        if segments.dtype != torch.int32 or segments.dim() != 2 or segments.shape[1] != 4 or \
+                not segments.is_contiguous():
+            raise invalid("segments: a contiguous int32 [S, 4] tensor")
+    same_device(q.codes, weights=w.error_word, segments=segments, out=out)
+    with on_device(q.codes):
+        if out is None:
+            out = torch.empty((q.rows, w.n), dtype=dtype, device=q.codes.device)
+        elif out.shape != (q.rows, w.n):
+            raise invalid(f"out {tuple(out.shape)}, not {(q.rows, w.n)}")
+        ld = row_stride(out, "out")
+        cfg = abi.WispFp4Config(w.fmt, w.entries, w.n, w.k, w.cfg.swiglu,
+                                dtype_code(out.dtype, "out"))
+        x = abi.WispFp4Rows(q.codes.data_ptr(), q.scales.data_ptr(),
+                            None if q.tensor_scale is None else q.tensor_scale.data_ptr(), q.rows)
+        abi.call("wisp_b200_fp4_product", C.byref(cfg), C.byref(w.mats),
+                 None if w.up_mats is None else C.byref(w.up_mats), C.byref(x),
+                 None if segments is None else segments.data_ptr(),
+                 0 if segments is None else segments.shape[0], out.data_ptr(), ld,
+                 w.error_word.data_ptr(), stream_of(q.codes))
+    return out
+
+
+class Fp4MoeLayer:
+    """One routed-expert MoE layer over fp4 weights (the counterpart of moe.MoeLayer): router,
+    dispatch, quantised rows, gate/up + SwiGLU, quantised rows, down, fixed-order combine."""
+
+    def __init__(self, spec, router_w: torch.Tensor, router_bias: torch.Tensor | None,
+                 gate_up: Fp4Weights, down: Fp4Weights, tokens: int,
+                 x_scale: torch.Tensor | None = None, h_scale: torch.Tensor | None = None):
+        """spec: a synth.MoeSpec (its group_size is not used). x_scale, h_scale: the NV tensor
+        scales of the layer's input and of the SwiGLU output."""
+        V = spec.n_virtual
+        if (gate_up.entries, gate_up.n, gate_up.k) != (V, spec.inter, spec.hidden) or \
+                gate_up.up_mats is None:
+            raise invalid("gate_up does not fit the layer")
+        if (down.entries, down.n, down.k) != (V, spec.hidden, spec.inter) or \
+                down.up_mats is not None or down.fmt != gate_up.fmt:
+            raise invalid("down does not fit the layer")
+        if gate_up.fmt == abi.WISP_FP4_NV and (x_scale is None or h_scale is None):
+            raise invalid("NV layers need x_scale and h_scale")
+        if router_w.dtype not in (torch.bfloat16, torch.float16) or \
+                router_w.shape != (spec.n_experts, spec.hidden) or not router_w.is_contiguous():
+            raise invalid("router_w: contiguous bfloat16 or float16 [experts, hidden]")
+        if router_bias is not None and (router_bias.dtype != torch.float32 or
+                                        router_bias.shape != (spec.n_experts,) or
+                                        not router_bias.is_contiguous()):
+            raise invalid("router_bias: contiguous float32 [experts]")
+        _check_scale(x_scale, 1, "x_scale")
+        _check_scale(h_scale, 1, "h_scale")
+        same_device(gate_up.error_word, router_w=router_w, router_bias=router_bias,
+                    down=down.error_word, x_scale=x_scale, h_scale=h_scale)
+        self.spec, self.gate_up, self.down = spec, gate_up, down
+        self.cfg = spec.cfg(tokens)
+        self.cfg.router_fp16 = 1 if router_w.dtype == torch.float16 else 0
+        self._keep = (router_w, router_bias, x_scale, h_scale)
+        w = self._w = abi.WispFp4MoeWeights()
+        w.router_w = router_w.data_ptr()
+        w.router_bias = None if router_bias is None else router_bias.data_ptr()
+        w.gate, w.up, w.down = gate_up.mats, gate_up.up_mats, down.mats
+        w.x_scale = None if x_scale is None else x_scale.data_ptr()
+        w.h_scale = None if h_scale is None else h_scale.data_ptr()
+        w.format = gate_up.fmt
+        nbytes = abi.lib().wisp_b200_fp4_moe_workspace_bytes(C.byref(self.cfg), gate_up.fmt)
+        if nbytes == 0:
+            raise invalid("invalid MoE config")
+        dev = gate_up.device
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self.idx = torch.empty((tokens, spec.top_k), dtype=torch.int32, device=dev)
+        self.wt = torch.empty((tokens, spec.top_k), dtype=torch.float32, device=dev)
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """x bf16 [tokens, hidden] -> fp32 [tokens, hidden]. One call at a time per layer."""
+        shape = (self.cfg.tokens, self.spec.hidden)
+        if x.dtype != torch.bfloat16 or not x.is_contiguous() or x.shape != shape:
+            raise invalid(f"x: contiguous bfloat16 {shape}")
+        same_device(self.workspace, x=x, out=out)
+        with on_device(x):
+            if out is None:
+                out = torch.empty(shape, dtype=torch.float32, device=x.device)
+            elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
+                raise invalid(f"out: contiguous float32 {shape}")
+            abi.call("wisp_b200_fp4_moe_forward", C.byref(self.cfg), C.byref(self._w),
+                     x.data_ptr(), out.data_ptr(), self.idx.data_ptr(), self.wt.data_ptr(),
+                     self.workspace.data_ptr(), self.workspace.numel(),
+                     self.gate_up.error_word.data_ptr(), stream_of(x))
+        return out
+
+    def check(self) -> None:
+        self.gate_up.check()
