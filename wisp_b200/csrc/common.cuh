@@ -408,6 +408,18 @@ WB_DEV void red_add_f32(float* addr, float v) {
   asm volatile("red.global.add.f32 [%0], %1;" ::"l"(addr), "f"(v) : "memory");
 }
 
+// One lane of a converged warp, the same at every call. Code that issues tcgen05
+// or TMA instructions under it, from warp-uniform values, keeps their operands
+// in uniform registers (a thread-index test makes the compiler move each one
+// there: measured ~70 cycles per tcgen05.cp and ~80 per tcgen05.mma against 8
+// and the MMA's own time).
+WB_DEV bool elect_sync() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(p));
+  return p != 0;
+}
+
 WB_DEV bool elect_one() { return (threadIdx.x & 31) == 0; }
 
 }  // namespace wb

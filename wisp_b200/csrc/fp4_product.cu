@@ -28,6 +28,8 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
 constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
+constexpr int kMaxStages = 8;
+constexpr int kRingBytes = 220 * 1024;
 
 template <bool NV, bool SWIGLU>
 struct Shape {
@@ -36,27 +38,28 @@ struct Shape {
   // Accumulators: two sets (gate and up, or two tiles of one) of kMaxN
   // columns, beside two buffers of scales, in 512 columns.
   static constexpr int kMaxN = NV ? 192 : 224;
-  static constexpr int kAccBufs = SWIGLU ? 1 : 2;
   static constexpr int kSfA = 2 * kMaxN;              // first scale column
   static constexpr int kSfCols = kWords * (4 * kMats + 8);
   static_assert(2 * kMaxN + 2 * kSfCols <= 512, "tensor memory");
   static constexpr int kSfaBytes = kWords * 512;
   static constexpr int kSfbBytes = kWords * 2 * 512;
-  static constexpr int kBBytes = kMaxN * 128;
-  static constexpr int kStageBytes = kMats * (kABytes + kSfaBytes) + kBBytes + kSfbBytes;
-  static constexpr int kStages = SWIGLU ? 3 : 4;
+  // A stage: weights (gate, up), their scales, the row scales, then as many
+  // 32-row boxes of row codes as the launch's largest tile has.
+  static constexpr int kOffSfa = kMats * kABytes;
+  static constexpr int kOffSfb = kOffSfa + kMats * kSfaBytes;
+  static constexpr int kOffB = kOffSfb + kSfbBytes;
+  static_assert(kOffB % 1024 == 0, "128-byte swizzle atoms");
 };
 
-template <int S>
 struct Bars {
-  uint64_t full[S];
-  uint64_t empty[S];
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint32_t tmem;
   int abort;
-  int bad;
   int n_tiles;
+  int max_cnt;
 };
 
 struct alignas(64) Params {
@@ -166,22 +169,58 @@ WB_DEV Tile find_tile(const Params& p, const int* pref, int nseg, int tt) {
   return t;
 }
 
+// A position in the ring of stages.
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;     // parity of the slot's current use
+  WB_DEV void next(int S) {
+    if (++s == S) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+// The accumulators: two halves of kMaxN columns. A tile of one matrix, or a
+// gate/up tile of at most kMaxN / 2 rows (up kMaxN / 2 columns after gate),
+// takes one half, so its epilogue overlaps the next tile's MMAs; a larger
+// gate/up tile takes both (gate, up). MMA and epilogue warps walk the tiles in
+// the same order and so agree on the halves and their phases.
+template <int MAXN, bool SWIGLU>
+struct Acc {
+  int h = 0;                       // the tile's (first) half
+  bool both = false;
+  int nxt = 0;
+  uint32_t uses0 = 0, uses1 = 0;   // of each half, before this tile
+  WB_DEV void take(int cnt) {
+    both = SWIGLU && cnt > MAXN / 2;
+    h = both ? 0 : nxt;
+  }
+  WB_DEV uint32_t uses() const { return h ? uses1 : uses0; }
+  WB_DEV uint32_t up_offset() const { return both ? MAXN : MAXN / 2; }
+  WB_DEV void done() {
+    if (both || h == 0) uses0++;
+    if (both || h == 1) uses1++;
+    if (!both) nxt ^= 1;
+  }
+};
+
 template <bool NV, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
   using C = Shape<NV, SWIGLU>;
-  constexpr int S = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ Bars<S> bars;
+  __shared__ Bars bars;
   __shared__ int pref[kMaxSegs + 1];
   __shared__ int warp_tot[kThreads / 32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   volatile int* abort = &bars.abort;
 
   if (tid == 0) {
-    for (int i = 0; i < S; i++) {
-      mbar_init(&bars.full[i], 3);      // producer, two scale warps
+    for (int i = 0; i < kMaxStages; i++) {
+      mbar_init(&bars.full[i], 2);      // the copies, one scale warp
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -189,14 +228,14 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       mbar_init(&bars.acc_empty[i], 8);
     }
     bars.abort = 0;
-    bars.bad = 0;
+    bars.max_cnt = 0;
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(&bars.tmem, 512);
   // Token tiles before each segment: 3 segments per thread, then one scan.
   const int nseg = p.segs ? p.nseg : 1;
   {
-    int n[3], sum = 0;
+    int n[3], sum = 0, most = 0;
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < 3; j++) {
@@ -204,11 +243,12 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       n[j] = 0;
       if (s < nseg) {
         const WispSegment v = segment(p, s);
-        if (!segment_ok(p, v))
+        if (!segment_ok(p, v)) {
           bad = true;
-        else if (v.rows > 0) {
+        } else if (v.rows > 0) {
           const int per = tile_rows<C::kMaxN>(v.rows);
           n[j] = (v.rows + per - 1) / per;
+          most = max(most, min(per, v.rows));
         }
       }
       sum += n[j];
@@ -223,6 +263,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (most > 0) atomicMax(&bars.max_cnt, most);
     int base = x - sum;
     for (int w = 0; w < warp; w++) base += warp_tot[w];
 #pragma unroll
@@ -236,201 +277,244 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   }
   __syncthreads();
   const uint32_t tmem = bars.tmem;
-  const int64_t items = (int64_t)bars.n_tiles * p.ftiles;
+  const int items = bars.n_tiles * p.ftiles;
   const int nk = p.nk;
-  auto stage = [&](int s) { return smem + s * C::kStageBytes; };
-  // a stage: weights (gate, up), their scales (gate, up), row codes, row scales
-  constexpr int kOffSfa = C::kMats * kABytes;
-  // the swizzle needs 1024-byte aligned operands, the scales 16
-  constexpr int kOffB = kOffSfa;
-  constexpr int kOffSf = kOffB + C::kBBytes;
-  constexpr int kOffSfb = kOffSf + C::kMats * C::kSfaBytes;
+  // Few rows leave room for more stages in flight, which is what hides the
+  // memory's latency when the weights are most of the traffic.
+  const int stage_bytes = C::kOffB + ((bars.max_cnt + 31) >> 5) * 4096;
+  const int S = min(kMaxStages, kRingBytes / max(stage_bytes, 1));
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_sync()) {
       tma_prefetch_desc(&p.tm_w);
       tma_prefetch_desc(&p.tm_x);
       if (SWIGLU) tma_prefetch_desc(&p.tm_up);
-      int i = 0;
-      int64_t uses = 0;
-      for (int64_t it = blockIdx.x; it < items && !*abort; it += gridDim.x) {
-        const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
-        const int ft = (int)(it % p.ftiles);
-        const int wrow = t.expert * p.N + ft * 128;
-        const int64_t sf = ((int64_t)t.expert * p.ftiles + ft) * nk;
-        const int nb = (t.cnt + 31) >> 5;
-        const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * 4096;
-        for (int kk = 0; kk < nk; kk++, uses++) {
-          const int s = (int)(uses % S);
-          if (uses >= S && !mbar_wait(&bars.empty[s], (uint32_t)(uses / S - 1) & 1, abort)) break;
-          uint8_t* st = stage(s);
-          mbar_arrive_expect_tx(&bars.full[s], bytes);
-          tma_load_2d(st, &p.tm_w, &bars.full[s], kk * 128, wrow);
-          bulk_load(st + kOffSf, p.sf_w + (sf + kk) * C::kSfaBytes, C::kSfaBytes, &bars.full[s]);
-          if (SWIGLU) {
-            tma_load_2d(st + kABytes, &p.tm_up, &bars.full[s], kk * 128, wrow);
-            bulk_load(st + kOffSf + C::kSfaBytes, p.sf_up + (sf + kk) * C::kSfaBytes, C::kSfaBytes,
-                      &bars.full[s]);
-          }
+    }
+    __syncwarp();
+    Ring r;
+    bool first = true, ok = true;
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
+      const int ft = it % p.ftiles;
+      const int wrow = t.expert * p.N + ft * 128;
+      const int64_t sf = ((int64_t)t.expert * p.ftiles + ft) * nk * C::kSfaBytes;
+      const uint8_t* sfw = p.sf_w + sf;
+      const uint8_t* sfu = p.sf_up + sf;
+      const int nb = (t.cnt + 31) >> 5;
+      const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * 4096;
+      for (int kk = 0; kk < nk; kk++) {
+        if (!first && !mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort)) { ok = false; break; }
+        uint8_t* st = smem + r.s * stage_bytes;
+        uint64_t* full = &bars.full[r.s];
+        if (elect_sync()) {
+          mbar_arrive_expect_tx(full, bytes);
+          tma_load_2d(st, &p.tm_w, full, kk * 128, wrow);
+          if (SWIGLU) tma_load_2d(st + kABytes, &p.tm_up, full, kk * 128, wrow);
+          bulk_load(st + C::kOffSfa, sfw + kk * C::kSfaBytes, C::kSfaBytes, full);
+          if (SWIGLU)
+            bulk_load(st + C::kOffSfa + C::kSfaBytes, sfu + kk * C::kSfaBytes, C::kSfaBytes, full);
           for (int b = 0; b < nb; b++)
-            tma_load_2d(st + kOffB + b * 4096, &p.tm_x, &bars.full[s], kk * 128, t.row0 + b * 32);
+            tma_load_2d(st + C::kOffB + b * 4096, &p.tm_x, full, kk * 128, t.row0 + b * 32);
         }
-        (void)i;
+        __syncwarp();
+        r.next(S);
+        if (r.s == 0) first = false;
       }
-      if (*abort) {
-        // let the copies in flight land before the CTA's memory goes away
-        for (int64_t u = uses > S ? uses - S : 0; u < uses; u++)
-          mbar_wait(&bars.full[u % S], (uint32_t)(u / S) & 1, abort, 20000000LL);
+    }
+    if (*abort) {
+      // let the copies in flight land before the CTA's memory goes away
+      for (int i = 0; i < S; i++) {
+        const int s = (r.s + i) % S;
+        const bool wrapped = s >= r.s;
+        if (first && wrapped) continue;      // never used
+        mbar_wait(&bars.full[s], wrapped ? r.ph ^ 1 : r.ph, abort, 20000000LL);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int64_t uses = 0;
-      int64_t nt = 0;
-      bool ok = true;
-      for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x, nt++) {
-        const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
-        const int n = (t.cnt + 15) & ~15;
-        const uint32_t idesc = idesc_fp4<NV>(n);
-        const int ab = (int)(nt % C::kAccBufs);
-        const int64_t au = nt / C::kAccBufs;
-        if (au >= 1 && !mbar_wait(&bars.acc_empty[ab], (uint32_t)(au - 1) & 1, abort)) break;
+    Ring r;
+    Acc<C::kMaxN, SWIGLU> acc;
+    int uses = 0;       // stages so far, up to 2
+    uint32_t buf = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
+      const int n = (t.cnt + 15) & ~15;
+      const uint32_t idesc = idesc_fp4<NV>(n);
+      acc.take(t.cnt);
+      if (acc.uses() && !mbar_wait(&bars.acc_empty[acc.h], (acc.uses() - 1) & 1, abort)) break;
+      if (acc.both && acc.uses1 && !mbar_wait(&bars.acc_empty[1], (acc.uses1 - 1) & 1, abort)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + acc.h * C::kMaxN, du = d + acc.up_offset();
+      for (int kk = 0; kk < nk; kk++) {
+        if (!mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        // the scale buffer's last readers: the MMAs of the stage before the last
+        if (uses >= 2) {
+          const int s2 = r.s >= 2 ? r.s - 2 : r.s - 2 + S;
+          if (!mbar_wait(&bars.empty[s2], r.s >= 2 ? r.ph : r.ph ^ 1, abort)) { ok = false; break; }
+        } else {
+          uses++;
+        }
         tc_fence_after();
-        const uint32_t d = tmem + ab * C::kMaxN;
-        for (int kk = 0; kk < nk; kk++, uses++) {
-          const int s = (int)(uses % S);
-          if (!mbar_wait(&bars.full[s], (uint32_t)(uses / S) & 1, abort)) { ok = false; break; }
-          // the scale buffer's last readers: the MMAs of stage uses - 2
-          if (uses >= 2) {
-            const int64_t u = uses - 2;
-            if (!mbar_wait(&bars.empty[u % S], (uint32_t)(u / S) & 1, abort)) { ok = false; break; }
-          }
-          tc_fence_after();
-          const uint32_t st = smem_u32(stage(s));
-          const uint32_t sfa = tmem + C::kSfA + (uint32_t)(uses & 1) * C::kSfCols;
-          const uint32_t sfb = sfa + C::kMats * C::kWords * 4;
+        const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
+        const uint32_t sfa = tmem + C::kSfA + buf * C::kSfCols;
+        const uint32_t sfb = sfa + C::kMats * C::kWords * 4;
+        if (elect_sync()) {
+          const uint64_t dsa = scale_desc(st + C::kOffSfa), dsb = scale_desc(st + C::kOffSfb);
 #pragma unroll
-          for (int w = 0; w < C::kMats * C::kWords; w++)
-            tmem_cp_scales(sfa + w * 4, scale_desc(st + kOffSf + w * 512));
+          for (int w = 0; w < C::kMats * C::kWords; w++) tmem_cp_scales(sfa + w * 4, dsa + w * 32);
 #pragma unroll
-          for (int w = 0; w < C::kWords; w++) {
-            tmem_cp_scales(sfb + w * 8, scale_desc(st + kOffSfb + w * 1024));
-            if (n > 128) tmem_cp_scales(sfb + w * 8 + 4, scale_desc(st + kOffSfb + w * 1024 + 512));
+          for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8, dsb + w * 64);
+          if (n > 128) {
+#pragma unroll
+            for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8 + 4, dsb + w * 64 + 32);
           }
-          const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + kOffB);
+          const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + C::kOffB);
 #pragma unroll
           for (int j = 0; j < 4; j++) {          // 64 k (32 bytes) each
             const int w = NV ? j : j >> 1;
             const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2;
             const uint32_t ids = idesc | (id << 29) | (id << 4);
-            const uint32_t acc = (kk | j) ? 1u : 0u;
-            mma_fp4<NV>(d, da + j * 2, db + j * 2, ids, sfa + w * 4, sfb + w * 8, acc);
+            const uint32_t add = (kk | j) ? 1u : 0u;
+            mma_fp4<NV>(d, da + j * 2, db + j * 2, ids, sfa + w * 4, sfb + w * 8, add);
             if (SWIGLU)
-              mma_fp4<NV>(d + C::kMaxN, da + (kABytes >> 4) + j * 2, db + j * 2, ids,
-                          sfa + (C::kWords + w) * 4, sfb + w * 8, acc);
+              mma_fp4<NV>(du, da + (kABytes >> 4) + j * 2, db + j * 2, ids,
+                          sfa + (C::kWords + w) * 4, sfb + w * 8, add);
           }
-          mma_commit(&bars.empty[s]);
+          mma_commit(&bars.empty[r.s]);
+          if (kk == nk - 1) {
+            mma_commit(&bars.acc_full[acc.h]);
+            if (acc.both) mma_commit(&bars.acc_full[1]);
+          }
         }
-        if (ok) mma_commit(&bars.acc_full[ab]);
+        __syncwarp();
+        r.next(S);
+        buf ^= 1;
       }
-      if (*abort) {
-        for (int64_t u = uses > S ? uses - S : 0; u < uses; u++)
-          mbar_wait(&bars.empty[u % S], (uint32_t)(u / S) & 1, abort, 20000000LL);
+      acc.done();
+    }
+    if (*abort) {
+      // MMAs in flight read shared memory: wait for the last stages issued
+      for (int i = 0; i < uses; i++) {
+        const int s = (r.s + 2 * S - 1 - i) % S;
+        mbar_wait(&bars.empty[s], s < r.s ? r.ph : r.ph ^ 1, abort, 20000000LL);
       }
     }
   } else if (warp < kEpiWarp) {
-    // Row scales: two warps, rows lid, lid + 64, ... of the tile; the words of
-    // the next stage are read before the wait for this stage's slot.
-    constexpr int R = (C::kMaxN + 63) / 64;
-    const int lid = tid - 64;
-    int64_t uses = 0;
-    auto fetch = [&](const Tile& t, int kk, uint32_t (&w)[R][C::kWords]) {
+    // Row scales: the two warps take alternate stages. A lane copies rows
+    // lane + 32 i, whose words lie side by side in the layout; the words of
+    // the warp's next stage are on their way while it waits for a slot.
+    constexpr int R = C::kMaxN / 32, W = C::kWords;
+    struct Pos {
+      int it, kk;
+      Tile t;
+    };
+    auto advance = [&](Pos& q, int by) {
+      q.kk += by;
+      while (q.it < items && q.kk >= nk) {
+        q.kk -= nk;
+        q.it += gridDim.x;
+        if (q.it < items) q.t = find_tile<C::kMaxN>(p, pref, nseg, q.it / p.ftiles);
+      }
+    };
+    auto fetch = [&](const Pos& q, uint32_t (&w)[W][8]) {
+#pragma unroll
+      for (int j = 0; j < W; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[j][i] = 0;
+      if (q.it >= items) return;
+      const int left = p.xs_ld - q.kk * W * 4;
+      const uint8_t* src = p.xs + (int64_t)(q.t.row0 + lane) * p.xs_ld + q.kk * W * 4;
 #pragma unroll
       for (int i = 0; i < R; i++) {
-        const int r = lid + 64 * i;
-#pragma unroll
-        for (int j = 0; j < C::kWords; j++) w[i][j] = 0;
-        if (r < t.cnt) {
-          const uint8_t* src = p.xs + (int64_t)(t.row0 + r) * p.xs_ld + kk * C::kWords * 4;
-          const int left = p.xs_ld - kk * C::kWords * 4;
-          if (p.xs_wide && left >= C::kWords * 4) {
+        if (lane + 32 * i < q.t.cnt) {
+          const uint8_t* g = src + (int64_t)(32 * i) * p.xs_ld;
+          if (p.xs_wide && left >= W * 4) {
             if (NV) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-              w[i][0] = v.x;
-              w[i][1] = v.y;
-              w[i][C::kWords - 2] = v.z;
-              w[i][C::kWords - 1] = v.w;
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(g));
+              w[0][i] = v.x;
+              w[1][i] = v.y;
+              w[W - 2][i] = v.z;
+              w[W - 1][i] = v.w;
             } else {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-              w[i][0] = v.x;
-              w[i][1] = v.y;
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(g));
+              w[0][i] = v.x;
+              w[1][i] = v.y;
             }
           } else {
 #pragma unroll
-            for (int b = 0; b < C::kWords * 4; b++)
-              if (b < left) w[i][b >> 2] |= (uint32_t)__ldg(src + b) << (8 * (b & 3));
+            for (int b = 0; b < W * 4; b++)
+              if (b < left) w[b >> 2][i] |= (uint32_t)__ldg(g + b) << (8 * (b & 3));
           }
         }
       }
     };
-    bool ok = true;
-    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
-      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
-      uint32_t cur[R][C::kWords];
-      fetch(t, 0, cur);
-      for (int kk = 0; kk < nk; kk++, uses++) {
-        uint32_t nxt[R][C::kWords];
-        fetch(t, min(kk + 1, nk - 1), nxt);
-        const int s = (int)(uses % S);
-        if (uses >= S) ok = mbar_wait(&bars.empty[s], (uint32_t)(uses / S - 1) & 1, abort);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        uint32_t* dst = reinterpret_cast<uint32_t*>(stage(s) + kOffSfb);
+    Ring r;
+    int use = 0;
+    auto put = [&](const uint32_t (&w)[W][8]) {
+      bool ok = use < S || mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      uint4* dst = reinterpret_cast<uint4*>(smem + r.s * stage_bytes + C::kOffSfb) + lane;
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-          const int r = lid + 64 * i;
-          if (r < C::kMaxN) {
-#pragma unroll
-            for (int w = 0; w < C::kWords; w++)
-              dst[w * 256 + (r >> 7) * 128 + (r & 31) * 4 + ((r >> 5) & 3)] = cur[i][w];
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.full[s]);
-#pragma unroll
-        for (int i = 0; i < R; i++)
-#pragma unroll
-          for (int w = 0; w < C::kWords; w++) cur[i][w] = nxt[i][w];
+      for (int j = 0; j < W; j++) {
+        dst[j * 64] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+        dst[j * 64 + 32] = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.full[r.s]);
+      r.next(S);
+      r.next(S);
+      use = min(use + 2, 1 << 20);
+      return true;
+    };
+    Pos q;
+    q.it = blockIdx.x;
+    q.kk = 0;
+    if (q.it < items) q.t = find_tile<C::kMaxN>(p, pref, nseg, q.it / p.ftiles);
+    if (warp == 3) {
+      advance(q, 1);
+      r.next(S);
+      use = 1;
+    }
+    uint32_t a[W][8], b[W][8];
+    fetch(q, a);
+    while (q.it < items) {
+      advance(q, 2);
+      fetch(q, b);
+      if (!put(a) || q.it >= items) break;
+      advance(q, 2);
+      fetch(q, a);
+      if (!put(b)) break;
     }
   } else {
     // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
     // take alternate groups of 16 rows.
     const int quad = warp & 3, half = (warp - kEpiWarp) >> 2;
     const float tx = p.ts_x ? __ldg(p.ts_x) : 1.f;
-    int64_t nt = 0;
-    for (int64_t it = blockIdx.x; it < items; it += gridDim.x, nt++) {
-      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, (int)(it / p.ftiles));
-      const int f = (int)(it % p.ftiles) * 128 + quad * 32 + lane;
-      const int ab = (int)(nt % C::kAccBufs);
-      const int64_t au = nt / C::kAccBufs;
+    Acc<C::kMaxN, SWIGLU> acc;
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
+      const int f = (it % p.ftiles) * 128 + quad * 32 + lane;
       const float ag = tx * (p.ts_w ? __ldg(p.ts_w + t.expert) : 1.f);
-      const float au2 = SWIGLU ? tx * (p.ts_up ? __ldg(p.ts_up + t.expert) : 1.f) : 0.f;
-      const bool ok = mbar_wait(&bars.acc_full[ab], (uint32_t)au & 1, abort);
+      const float au = SWIGLU ? tx * (p.ts_up ? __ldg(p.ts_up + t.expert) : 1.f) : 0.f;
+      acc.take(t.cnt);
+      bool ok = mbar_wait(&bars.acc_full[acc.h], acc.uses() & 1, abort);
+      if (acc.both) ok = ok && mbar_wait(&bars.acc_full[1], acc.uses1 & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t d = tmem + ab * C::kMaxN + ((uint32_t)(quad * 32) << 16);
+      const uint32_t d = tmem + acc.h * C::kMaxN + ((uint32_t)(quad * 32) << 16);
+      const uint32_t du = d + acc.up_offset();
       for (int c = half * 16; c < t.cnt; c += 32) {
         uint32_t g[16], u[16];
         tmem_ld16(d + c, g);
-        if (SWIGLU) tmem_ld16(d + C::kMaxN + c, u);
+        if (SWIGLU) tmem_ld16(du + c, u);
         tmem_wait_ld();
         if (f < p.N) {
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             if (c + i < t.cnt) {
               float v = __uint_as_float(g[i]) * ag;
-              if (SWIGLU) v = v / (1.f + expf(-v)) * (__uint_as_float(u[i]) * au2);
+              if (SWIGLU) v = v / (1.f + expf(-v)) * (__uint_as_float(u[i]) * au);
               store_one(p.out, p.out_type, (int64_t)(t.row0 + c + i) * p.ld + f, v);
             }
           }
@@ -439,7 +523,11 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.acc_empty[ab]);
+      if (lane == 0) {
+        mbar_arrive(&bars.acc_empty[acc.h]);
+        if (acc.both) mbar_arrive(&bars.acc_empty[1]);
+      }
+      acc.done();
     }
   }
   tc_fence_before();
@@ -469,8 +557,7 @@ bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box
 template <bool NV, bool SWIGLU>
 WispError launch_product(const Params& p, int64_t max_items, cudaStream_t stream,
                          WispErrCtx* err) {
-  using C = Shape<NV, SWIGLU>;
-  const int smem = C::kStages * C::kStageBytes + 1024;
+  const int smem = kRingBytes + 1024;
   auto kernel = fp4_product_kernel<NV, SWIGLU>;
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(cudaGetDevice(&dev));
