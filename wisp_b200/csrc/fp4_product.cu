@@ -205,6 +205,37 @@ struct Acc {
   }
 };
 
+WB_DEV void put_out(float* q, float v) { *q = v; }
+WB_DEV void put_out(__nv_bfloat16* q, float v) { *q = __float2bfloat16_rn(v); }
+WB_DEV void put_out(__half* q, float v) { *q = __float2half_rn(v); }
+
+// One warp's part of a tile: its lane's feature f, rows 16 half + 32 i ...
+// The quotient of the sigmoid is the 2-ulp one; everything else is rounded
+// once, and the result once to the output type.
+template <bool SWIGLU, typename T>
+WB_DEV void store_tile(const Params& p, const Tile& t, uint32_t d, uint32_t du, int half, int f,
+                       float ag, float au) {
+  const int64_t ld = p.ld;
+  T* out = static_cast<T*>(p.out) + (t.row0 + half * 16) * ld + f;
+  for (int c = half * 16; c < t.cnt; c += 32, out += 32 * ld) {
+    uint32_t g[16], u[16];
+    tmem_ld16(d + c, g);
+    if (SWIGLU) tmem_ld16(du + c, u);
+    tmem_wait_ld();
+    const int left = t.cnt - c;
+    if (f < p.N) {
+      T* q = out;
+#pragma unroll
+      for (int i = 0; i < 16; i++, q += ld) {
+        float v = __uint_as_float(g[i]) * ag;
+        if (SWIGLU) v = __fdividef(v, 1.f + expf(-v)) * (__uint_as_float(u[i]) * au);
+        if (i < left) put_out(q, v);
+      }
+    }
+    __syncwarp();
+  }
+}
+
 template <bool NV, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
@@ -504,23 +535,12 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       tc_fence_after();
       const uint32_t d = tmem + acc.h * C::kMaxN + ((uint32_t)(quad * 32) << 16);
       const uint32_t du = d + acc.up_offset();
-      for (int c = half * 16; c < t.cnt; c += 32) {
-        uint32_t g[16], u[16];
-        tmem_ld16(d + c, g);
-        if (SWIGLU) tmem_ld16(du + c, u);
-        tmem_wait_ld();
-        if (f < p.N) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            if (c + i < t.cnt) {
-              float v = __uint_as_float(g[i]) * ag;
-              if (SWIGLU) v = v / (1.f + expf(-v)) * (__uint_as_float(u[i]) * au);
-              store_one(p.out, p.out_type, (int64_t)(t.row0 + c + i) * p.ld + f, v);
-            }
-          }
-        }
-        __syncwarp();
-      }
+      if (p.out_type == WISP_DT_F32)
+        store_tile<SWIGLU, float>(p, t, d, du, half, f, ag, au);
+      else if (p.out_type == WISP_DT_BF16)
+        store_tile<SWIGLU, __nv_bfloat16>(p, t, d, du, half, f, ag, au);
+      else
+        store_tile<SWIGLU, __half>(p, t, d, du, half, f, ag, au);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
