@@ -6,13 +6,18 @@
 // the one exact arithmetic gives, so that codes do not depend on how a scale
 // was divided out:
 //   MX: the scale is a power of two; x / scale is exact in fp32.
-//   NV: the scale is e4m3 * tensor_scale (4 + 24 significant bits). q = x times
-//       the fp32 reciprocal is within 3 roundings (2^-22.4 relative) of the
-//       quotient, so the code is certain unless 4 q is within 2^-16 of an
-//       integer (every border is a multiple of 0.25, and q <= 6.5 wherever
-//       the border matters); those few values are decided by comparing |x|
-//       with border * scale in fp64, where both are exact (31 bits).
+//   NV: the scale is e4m3 * tensor_scale (4 + 24 significant bits). x times
+//       the fp32 reciprocal of that product is within 3 roundings (2^-22.4
+//       relative) of the quotient, so the codes of the products with the
+//       reciprocal made 2^-21 smaller and larger enclose the right one. Where
+//       they differ (one value in about 800 for bf16 rows under the tensor
+//       scale of their own maximum), |x| is compared with border * scale by
+//       the sign of one fused multiply-add: border * e4m3 has 7 bits, so the
+//       difference is rounded once and its sign is right. The scale byte
+//       itself is found in the same way.
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -24,12 +29,20 @@ using namespace wb;
 
 constexpr int kUnit = 16;   // values per thread: one NV block, half an MX block
 
-// Codes of (a, b): a in the low nibble. Round to nearest even, saturating.
-WB_DEV uint32_t e2m1x2(float a, float b) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}"
-      : "=r"(r) : "f"(a), "f"(b));
-  return r;
+// Codes of eight values, the first in the low nibble. Round to nearest even,
+// saturating.
+WB_DEV uint32_t e2m1x8(const float* v, float r) {
+  uint32_t o;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(o)
+      : "f"(v[0] * r), "f"(v[1] * r), "f"(v[2] * r), "f"(v[3] * r), "f"(v[4] * r), "f"(v[5] * r),
+        "f"(v[6] * r), "f"(v[7] * r));
+  return o;
 }
 
 // Exact code (sign excluded) of |x| over the scale s * g.
@@ -45,11 +58,15 @@ __device__ __noinline__ uint32_t e2m1_exact(float ax, float s, float g) {
   return c;
 }
 
-// e4m3 of a / (6 g), nearest even, saturating; exact like the codes. The
-// quotient goes to fp32 by rounding to odd (truncate, then set the last bit
-// when anything was cut off), so that the rounding to 4 significant bits
-// decides as it would on the exact quotient.
-WB_DEV uint32_t nv_scale_byte(float a, float g) {
+WB_DEV float e4m3_value(uint32_t b) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+}
+
+// e4m3 of a / (6 g), nearest even, saturating. The quotient goes to fp32 by
+// rounding to odd (truncate, then set the last bit when anything was cut
+// off), so that the rounding to 4 significant bits decides as it would on the
+// exact quotient.
+__device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
   const double d = 6.0 * (double)g;
   float t = __double2float_rz((double)a / d);
   if (t < 512.f) {
@@ -60,13 +77,28 @@ WB_DEV uint32_t nv_scale_byte(float a, float g) {
   return __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
 }
 
-WB_DEV float e4m3_value(uint32_t b) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+// Tensor scales for which nothing in the fp32 decisions overflows or drops
+// below fp32's last subnormal bit (the least product compared is 2^-111, of 31
+// significant bits).
+WB_DEV bool nv_plain_range(float g) { return g >= 1e-30f && g <= 1e30f; }
+
+constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
+
+// The same for a plain g: the byte of the scaled-down and scaled-up fp32
+// quotient, or where those differ by the sign of border * 6 g - a.
+WB_DEV uint32_t nv_scale_byte(float a, float g) {
+  const float t = a * __frcp_rn(6.f * g);
+  const uint32_t both =
+      __nv_cvt_float2_to_fp8x2(make_float2(t * kBelow, t * kAbove), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = both & 255u, hi = both >> 8;
+  if (lo == hi) return lo;
+  const float border = 0.5f * (e4m3_value(lo) + e4m3_value(hi));
+  const float d = fmaf(6.f * border, g, -a);
+  return d < 0.f || (d == 0.f && !(hi & 1)) ? hi : lo;
 }
 
 struct QuantParams {
   const void* x;
-  int type;
   int64_t ld;
   int x_rows;
   const int* src;
@@ -77,9 +109,113 @@ struct QuantParams {
   int wide;   // rows of x start on 16-byte boundaries
 };
 
-// grid (rows, ceil(cols / 16 / blockDim)): one thread per 16 values, 32 (bf16)
-// or 64 (fp32) bytes read and 8 written.
-template <bool NV>
+// 16 values of one thread as floats, and the largest magnitude's bits (as an
+// integer, so that a NaN is the largest of all).
+template <typename T>
+WB_DEV uint32_t load16(const T* x, bool wide, float (&v)[16]) {
+  uint32_t top = 0;
+  if (sizeof(T) == 4) {
+    const float* q = reinterpret_cast<const float*>(x);
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(q) + j);
+        v[4 * j] = f.x;
+        v[4 * j + 1] = f.y;
+        v[4 * j + 2] = f.z;
+        v[4 * j + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++) v[j] = __ldg(q + j);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    return top;
+  }
+  constexpr int type = sizeof(T) == 2 && std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16;
+  uint32_t u[8];
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(x);
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const uint4 f = __ldg(reinterpret_cast<const uint4*>(q) + j);
+      u[4 * j] = f.x;
+      u[4 * j + 1] = f.y;
+      u[4 * j + 2] = f.z;
+      u[4 * j + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) u[j] = __ldg(q + 2 * j) | (uint32_t)__ldg(q + 2 * j + 1) << 16;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float2 f = unpack2(u[j], type);
+    v[2 * j] = f.x;
+    v[2 * j + 1] = f.y;
+    top = __vmaxu2(top, u[j] & 0x7fff7fffu);
+  }
+  const float2 f = unpack2(max(top & 0xffffu, top >> 16), type);
+  return __float_as_uint(f.x);
+}
+
+// Codes and scale byte of one NV block for any g and x: every decision in
+// fp64.
+__device__ __noinline__ uint32_t nv_block_exact(const float (&v)[16], uint32_t top, float g,
+                                                uint32_t (&code)[2]) {
+  const uint32_t sb = nv_scale_exact(__uint_as_float(top), g);
+  const float s = e4m3_value(sb);
+  for (int j = 0; j < 16; j++) {
+    const uint32_t c = (s > 0.f ? e2m1_exact(fabsf(v[j]), s, g) : 0u) |
+                       (__float_as_uint(v[j]) >> 28 & 8u);
+    code[j >> 3] |= c << (4 * (j & 7));
+  }
+  return sb;
+}
+
+// Decides the values among eight whose two candidate codes differ.
+WB_DEV uint32_t nv_settle(const float* v, uint32_t lo, uint32_t hi, float r, float s, float g) {
+  const uint32_t diff = lo ^ hi;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    if (diff >> (4 * j) & 15u) {
+      const float ax = fabsf(v[j]);
+      const float border = 0.25f * rintf(4.f * ax * r);   // borders are multiples of 1/4
+      const float d = fmaf(border * s, g, -ax);
+      const uint32_t even = !(hi >> (4 * j) & 1u);
+      if (d < 0.f || (d == 0.f && even)) lo = (lo & ~(15u << (4 * j))) | (hi & 15u << (4 * j));
+    }
+  }
+  return lo;
+}
+
+WB_DEV uint32_t nv_block(const float (&v)[16], uint32_t top, float g, uint32_t (&code)[2]) {
+  code[0] = code[1] = 0u;
+  if (top >= 0x7f800000u || !(g > 0.f && g <= 3.402823466e38f)) return 0x7f;
+  if (!nv_plain_range(g)) {
+    float w[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) w[j] = v[j];
+    return nv_block_exact(w, top, g, code);
+  }
+  const uint32_t sb = nv_scale_byte(__uint_as_float(top), g);
+  const float s = e4m3_value(sb);
+  // a zero scale: zero codes with the values' signs
+  const float r = sb ? __frcp_rn(s * g) : 0.f;
+  const float rl = r * kBelow, rh = r * kAbove;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    code[i] = e2m1x8(v + 8 * i, rl);
+    const uint32_t hi = e2m1x8(v + 8 * i, rh);
+    if (code[i] != hi) code[i] = nv_settle(v + 8 * i, code[i], hi, r, s, g);
+  }
+  return sb;
+}
+
+// grid (rows, ceil(cols / 16 / blockDim)): one thread per 16 values, 32
+// (16-bit types) or 64 (fp32) bytes read and 8 written.
+template <bool NV, typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   const int64_t row = blockIdx.x;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
@@ -87,89 +223,46 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   const bool in = u < units;
   const int64_t sr = p.src ? (int64_t)p.src[row] : row;
   float v[16];
-#pragma unroll
-  for (int j = 0; j < 16; j++) v[j] = 0.f;
-  if (in && sr >= 0 && sr < p.x_rows) {
-    const int64_t i = sr * p.ld + (int64_t)u * kUnit;
-    float a[8], b[8];
-    load8(p.x, p.type, i, p.wide, 8, a);
-    load8(p.x, p.type, i + 8, p.wide, 8, b);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      v[j] = a[j];
-      v[8 + j] = b[j];
-    }
-  }
-  // as integers, so that a NaN is the largest of all
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < 16; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  for (int j = 0; j < 16; j++) v[j] = 0.f;
+  if (in && sr >= 0 && sr < p.x_rows)
+    top = load16(static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit, p.wide, v);
   uint32_t code[2] = {0u, 0u};
+  const int64_t o = row * units + u;
   if (NV) {
     if (!in) return;
-    const float g = *p.ts;
-    const int64_t o = row * units + u;
-    const bool bad = top >= 0x7f800000u || !(g > 0.f && g <= 3.402823466e38f);
-    uint32_t sb = 0x7f;
-    if (!bad) {
-      sb = nv_scale_byte(__uint_as_float(top), g);
-      const float s = e4m3_value(sb);
-      const float t = s * g;
-      if (t >= 1.1754943508e-38f) {
-        const float r = __frcp_rn(t);
-        float near = 1.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float q0 = v[2 * j] * r, q1 = v[2 * j + 1] * r;
-          const float f0 = 4.f * q0, f1 = 4.f * q1;
-          // distance to the nearest integer (the sum rounds to one); values
-          // near 0 are code 0 whatever they are
-          const float d0 = fabsf(f0) < 0.5f ? 1.f : fabsf(f0 - ((f0 + 12582912.f) - 12582912.f));
-          const float d1 = fabsf(f1) < 0.5f ? 1.f : fabsf(f1 - ((f1 + 12582912.f) - 12582912.f));
-          near = fminf(near, fminf(d0, d1));
-          code[j >> 2] |= e2m1x2(q0, q1) << (8 * (j & 3));
-        }
-        // r itself overflows for the very smallest scales: 1 / t of a t below
-        // 2^-126 never gets here, above it r <= 2^126
-        if (near < 1.52587890625e-5f) {
-          code[0] = code[1] = 0u;
-#pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const uint32_t c = e2m1_exact(fabsf(v[j]), s, g) |
-                               (__float_as_uint(v[j]) >> 28 & 8u);
-            code[j >> 3] |= c << (4 * (j & 7));
-          }
-        }
-      } else if (s > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-          const uint32_t c = e2m1_exact(fabsf(v[j]), s, g) | (__float_as_uint(v[j]) >> 28 & 8u);
-          code[j >> 3] |= c << (4 * (j & 7));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-          code[j >> 3] |= (__float_as_uint(v[j]) >> 28 & 8u) << (4 * (j & 7));
-      }
-    }
-    p.scales[o] = (uint8_t)sb;
-    *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
+    p.scales[o] = (uint8_t)nv_block(v, top, *p.ts, code);
   } else {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     if (!in) return;
-    const int64_t o = row * units + u;
     uint32_t sb = 255;
     if (top < 0x7f800000u) {
       const uint32_t e = top >> 23;
       sb = e > 2 ? e - 2 : 0;
       const float inv = __uint_as_float((254u - sb) << 23);   // 2^(127 - sb)
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        code[j >> 2] |= e2m1x2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * (j & 3));
+      code[0] = e2m1x8(v, inv);
+      code[1] = e2m1x8(v + 8, inv);
     }
     if (!(u & 1)) p.scales[o >> 1] = (uint8_t)sb;
-    *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
   }
+  *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
+}
+
+template <bool NV>
+void launch_quantize(const QuantParams& p, int type, dim3 grid, int threads, cudaStream_t st) {
+  if (type == WISP_DT_F32)
+    wb::launch_k(quantize_kernel<NV, float>, grid, threads, 0, st, p);
+  else if (type == WISP_DT_BF16)
+    wb::launch_k(quantize_kernel<NV, __nv_bfloat16>, grid, threads, 0, st, p);
+  else
+    wb::launch_k(quantize_kernel<NV, __half>, grid, threads, 0, st, p);
+}
+
+// A row of `units` threads split over equal blocks of at most 256.
+int row_threads(int units) {
+  const int blocks = (units + 255) / 256;
+  return ((units + blocks - 1) / blocks + 31) / 32 * 32;
 }
 
 struct DequantParams {
@@ -178,7 +271,6 @@ struct DequantParams {
   int cols;
   const float* ts;
   void* out;
-  int type;
   int64_t ld;
   int wide;
 };
@@ -189,18 +281,19 @@ WB_DEV float2 e2m1_values(uint32_t byte) {
   return __half22float2(u2h2(h));
 }
 
-// grid (rows, ceil(cols / 8 / blockDim)): one thread per 8 values. code *
-// scale is exact in fp32 (2 x 4 significant bits); the tensor scale and the
-// output type round once each.
-template <bool NV>
+// grid (rows, ceil(cols / 16 / blockDim)): one thread per 16 values, 8 bytes
+// read and 32 (16-bit types) or 64 written. code * scale is exact in fp32 (2 x
+// 4 significant bits); the tensor scale and the output type round once each.
+template <bool NV, int TYPE>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
   const int64_t row = blockIdx.x;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
-  const int units = p.cols / 8;
+  const int units = p.cols / kUnit;
   if (u >= units) return;
   const int64_t o = row * units + u;
-  const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(p.codes) + o);
-  const uint32_t sb = __ldg(p.scales + (NV ? o >> 1 : o >> 2));
+  const uint32_t c[2] = {__ldg(reinterpret_cast<const uint32_t*>(p.codes) + o * 2),
+                         __ldg(reinterpret_cast<const uint32_t*>(p.codes) + o * 2 + 1)};
+  const uint32_t sb = __ldg(p.scales + (NV ? o : o >> 1));
   float s, g = 1.f;
   if (NV) {
     s = e4m3_value(sb);
@@ -209,14 +302,27 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) 
     // 2^(sb - 127): 2^-127 is subnormal, 255 is NaN
     s = __uint_as_float(sb == 255 ? 0x7fffffffu : sb == 0 ? 0x00400000u : sb << 23);
   }
-  float v[8];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const float2 f = e2m1_values((c >> (8 * j)) & 255u);
-    v[2 * j] = f.x * s * g;
-    v[2 * j + 1] = f.y * s * g;
+  for (int h = 0; h < 2; h++) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float2 f = e2m1_values((c[h] >> (8 * j)) & 255u);
+      v[2 * j] = NV ? f.x * s * g : f.x * s;
+      v[2 * j + 1] = NV ? f.y * s * g : f.y * s;
+    }
+    store8(p.out, TYPE, row * p.ld + (int64_t)u * kUnit + 8 * h, p.wide, 8, v);
   }
-  store8(p.out, p.type, row * p.ld + (int64_t)u * 8, p.wide, 8, v);
+}
+
+template <bool NV>
+void launch_dequantize(const DequantParams& p, int type, dim3 grid, int threads, cudaStream_t st) {
+  if (type == WISP_DT_F32)
+    wb::launch_k(dequantize_kernel<NV, WISP_DT_F32>, grid, threads, 0, st, p);
+  else if (type == WISP_DT_BF16)
+    wb::launch_k(dequantize_kernel<NV, WISP_DT_BF16>, grid, threads, 0, st, p);
+  else
+    wb::launch_k(dequantize_kernel<NV, WISP_DT_F16>, grid, threads, 0, st, p);
 }
 
 // Scale bytes [entries x n x kb] to runs of one 128-feature x 256-k stage:
@@ -281,7 +387,6 @@ extern "C" WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_quantize: x not aligned to its type");
   QuantParams p;
   p.x = d_x;
-  p.type = x_type;
   p.ld = ld;
   p.x_rows = x_rows;
   p.src = d_src;
@@ -291,12 +396,12 @@ extern "C" WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t
   p.scales = d_scales;
   p.wide = !((uintptr_t)d_x & 15) && (ld * dt_size(x_type)) % 16 == 0;
   const int units = cols / kUnit;
-  const int threads = units >= 256 ? 256 : (units + 31) / 32 * 32;
+  const int threads = row_threads(units);
   const dim3 grid(rows, (units + threads - 1) / threads);
   if (format == WISP_FP4_NV)
-    wb::launch_k(quantize_kernel<true>, grid, threads, 0, stream, p);
+    launch_quantize<true>(p, x_type, grid, threads, stream);
   else
-    wb::launch_k(quantize_kernel<false>, grid, threads, 0, stream, p);
+    launch_quantize<false>(p, x_type, grid, threads, stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
 }
@@ -327,16 +432,15 @@ extern "C" WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint
   p.cols = cols;
   p.ts = d_tensor_scale;
   p.out = d_out;
-  p.type = out_type;
   p.ld = ld;
   p.wide = !((uintptr_t)d_out & 15) && (ld * dt_size(out_type)) % 16 == 0;
-  const int units = cols / 8;
-  const int threads = units >= 256 ? 256 : (units + 31) / 32 * 32;
+  const int units = cols / kUnit;
+  const int threads = row_threads(units);
   const dim3 grid(rows, (units + threads - 1) / threads);
   if (format == WISP_FP4_NV)
-    wb::launch_k(dequantize_kernel<true>, grid, threads, 0, stream, p);
+    launch_dequantize<true>(p, out_type, grid, threads, stream);
   else
-    wb::launch_k(dequantize_kernel<false>, grid, threads, 0, stream, p);
+    launch_dequantize<false>(p, out_type, grid, threads, stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
 }

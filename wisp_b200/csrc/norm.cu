@@ -1,10 +1,9 @@
 // norm.cu -- the norms after and before a block with its gate and residual:
 //   p = y / rms(y) * (o + w_post),  x' = rs * x + gate * p,
 //   n = x' / rms(x') * (o + w_pre)
-// One CTA per row; a row's x and y stay in registers (8 values per vector, at
-// most V vectors per thread), so each input is read once and each output
-// written once and the bound is HBM (and, for a few rows, the latency of one
-// load, two block sums and one store). n is taken from the fp32 x'.
+// A row's x and y are held by one CTA, so each input is read once and each
+// output written once and the bound is HBM (and, for a few rows, the latency
+// of one load, two block sums and one store). n is taken from the fp32 x'.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -22,8 +21,6 @@ struct NormParams {
   const void* pre_w;
   void* x_out;
   void* n;
-  // whether rows start on 16-byte boundaries and hold whole vectors
-  int wide_x, wide_y, wide_g, wide_post, wide_pre, wide_xo, wide_n;
 };
 
 // Sum over the block, the same bits in every thread.
@@ -39,8 +36,45 @@ WB_DEV float block_sum(float v, float* buf) {
   return v;
 }
 
-template <int V>
-__global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant__ NormParams p) {
+// Vectors of 8: thread i of `VEC` kernels holds elements 8 (k blockDim + i) ..
+// + 7; otherwise (a row that does not start on 16 bytes) elements
+// (8 k + j) blockDim + i, so that a warp's single loads are consecutive.
+template <bool VEC>
+WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, float (&v)[8]) {
+  if (VEC) {
+    const int i = (k * blockDim.x + threadIdx.x) * 8;
+    if (i < M) {
+      load8(q, type, base + i, true, 8, v);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = (8 * k + j) * blockDim.x + threadIdx.x;
+      v[j] = i < M ? load_one(q, type, base + i) : 0.f;
+    }
+  }
+}
+
+template <bool VEC>
+WB_DEV void store_row(void* q, int type, int64_t base, int k, int M, const float (&v)[8]) {
+  if (VEC) {
+    const int i = (k * blockDim.x + threadIdx.x) * 8;
+    if (i < M) store8(q, type, base + i, true, 8, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = (8 * k + j) * blockDim.x + threadIdx.x;
+      if (i < M) store_one(q, type, base + i, v[j]);
+    }
+  }
+}
+
+// One row per CTA.
+template <int V, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float buf[2][32];
   const WispBlockNorm& c = p.c;
   const int64_t t = blockIdx.x;
@@ -48,14 +82,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant_
   float x[V][8], y[V][8];
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    const int i = (k * blockDim.x + threadIdx.x) * 8, n = M - i;
-    if (n > 0) {
-      if (p.y) load8(p.y, c.y_type, t * c.ld_y + i, p.wide_y && n >= 8, n, y[k]);
-      load8(p.x, c.x_type, t * c.ld_x + i, p.wide_x && n >= 8, n, x[k]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[k][j] = y[k][j] = 0.f;
-    }
+    if (p.y) load_row<VEC>(p.y, c.y_type, t * c.ld_y, k, M, y[k]);
+    load_row<VEC>(p.x, c.x_type, t * c.ld_x, k, M, x[k]);
   }
   if (p.y) {
     float r = 1.f;
@@ -67,61 +95,170 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant_
         for (int j = 0; j < 8; j++) s = fmaf(y[k][j], y[k][j], s);
       r = 1.f / sqrtf(block_sum(s, buf[0]) / (float)M + c.eps);
     }
-    const float gt = c.gate_kind == WISP_GATE_TOKEN ? load_one(p.gate, c.gate_type, t) : 1.f;
+    if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
     for (int k = 0; k < V; k++) {
-      const int i = (k * blockDim.x + threadIdx.x) * 8, n = M - i;
-      if (n <= 0) continue;
       float w[8];
-      if (c.post_norm) {
-        if (p.post_w) {
-          load8(p.post_w, c.w_type, i, p.wide_post && n >= 8, n, w);
 #pragma unroll
-          for (int j = 0; j < 8; j++) y[k][j] = y[k][j] * r * (c.weight_offset + w[j]);
-        } else {
+      for (int j = 0; j < 8; j++) y[k][j] *= r;
+      if (p.post_w) {
+        load_row<VEC>(p.post_w, c.w_type, 0, k, M, w);
 #pragma unroll
-          for (int j = 0; j < 8; j++) y[k][j] *= r;
-        }
+        for (int j = 0; j < 8; j++) y[k][j] *= c.weight_offset + w[j];
       }
       if (c.gate_kind == WISP_GATE_CHANNEL || c.gate_kind == WISP_GATE_ELEMENT) {
-        const int64_t g0 = c.gate_kind == WISP_GATE_ELEMENT ? t * c.ld_gate : 0;
-        load8(p.gate, c.gate_type, g0 + i, p.wide_g && n >= 8, n, w);
+        load_row<VEC>(p.gate, c.gate_type, c.gate_kind == WISP_GATE_ELEMENT ? t * c.ld_gate : 0, k,
+                      M, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) y[k][j] *= w[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[k][j] *= gt;
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) x[k][j] = fmaf(c.residual_scale, x[k][j], y[k][j]);
-      if (p.x_out)
-        store8(p.x_out, c.x_type, t * c.ld_x_out + i, p.wide_xo && n >= 8, n, x[k]);
+      if (p.x_out) store_row<VEC>(p.x_out, c.x_type, t * c.ld_x_out, k, M, x[k]);
     }
   }
   if (p.n) {
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-      const int n = M - (int)(k * blockDim.x + threadIdx.x) * 8;
+    for (int k = 0; k < V; k++)
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j < n) s = fmaf(x[k][j], x[k][j], s);
-    }
+      for (int j = 0; j < 8; j++) s = fmaf(x[k][j], x[k][j], s);
     const float r = 1.f / sqrtf(block_sum(s, buf[1]) / (float)M + c.eps);
 #pragma unroll
     for (int k = 0; k < V; k++) {
-      const int i = (k * blockDim.x + threadIdx.x) * 8, n = M - i;
-      if (n <= 0) continue;
       float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[k][j] *= r;
       if (p.pre_w) {
-        load8(p.pre_w, c.w_type, i, p.wide_pre && n >= 8, n, w);
+        load_row<VEC>(p.pre_w, c.w_type, 0, k, M, w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = x[k][j] * r * (c.weight_offset + w[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = x[k][j] * r;
+        for (int j = 0; j < 8; j++) x[k][j] *= c.weight_offset + w[j];
       }
-      store8(p.n, c.n_type, t * c.ld_n + i, p.wide_n && n >= 8, n, w);
+      store_row<VEC>(p.n, c.n_type, t * c.ld_n, k, M, x[k]);
+    }
+  }
+}
+
+// Many rows: persistent CTAs that take rows blockIdx.x, + gridDim.x, ..., whose
+// x and y arrive through a ring of bulk copies, so that the memory stays busy
+// while a row's sums go round the CTA. A thread holds 8 columns, and their
+// weights and channel gate for good. (One row per CTA measured 2.4 TB/s of
+// 10-byte-per-value traffic at 4096 x 7168: its loads, sums and stores follow
+// one another, and two CTAs fit an SM.)
+constexpr int kNormStages = 8;
+struct RingShape {
+  int stages, x_bytes, y_bytes;
+};
+
+__global__ void __launch_bounds__(1024, 1)
+block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape rs) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kNormStages];
+  __shared__ float buf[2][2][32];
+  __shared__ int abort;
+  const WispBlockNorm& c = p.c;
+  const int M = c.hidden, tid = threadIdx.x, T = c.tokens;
+  const int stage = rs.x_bytes + rs.y_bytes;
+  const uint8_t* gx = static_cast<const uint8_t*>(p.x);
+  const uint8_t* gy = static_cast<const uint8_t*>(p.y);
+  const int64_t sx = c.ld_x * dt_size(c.x_type), sy = c.ld_y * dt_size(c.y_type);
+  auto issue = [&](int s, int64_t t) {
+    mbar_arrive_expect_tx(&full[s], rs.x_bytes + rs.y_bytes);
+    bulk_load(ring + s * stage, gx + t * sx, rs.x_bytes, &full[s]);
+    if (rs.y_bytes) bulk_load(ring + s * stage + rs.x_bytes, gy + t * sy, rs.y_bytes, &full[s]);
+  };
+  if (tid == 0) {
+    abort = 0;
+    for (int i = 0; i < rs.stages; i++) mbar_init(&full[i], 1);
+    fence_barrier_init();
+    for (int i = 0; i < rs.stages; i++) {
+      const int64_t t = blockIdx.x + (int64_t)i * gridDim.x;
+      if (t < T) issue(i, t);
+    }
+  }
+  const int i0 = tid * 8;
+  const bool in = i0 < M;
+  // columns' factors: a of y / rms(y), b of x' / rms(x')
+  float a[8], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) a[j] = b[j] = 1.f;
+  if (in) {
+    float w[8];
+    if (p.post_w) {
+      load8(p.post_w, c.w_type, i0, true, 8, w);
+#pragma unroll
+      for (int j = 0; j < 8; j++) a[j] = c.weight_offset + w[j];
+    }
+    if (c.gate_kind == WISP_GATE_CHANNEL) {
+      load8(p.gate, c.gate_type, i0, true, 8, w);
+#pragma unroll
+      for (int j = 0; j < 8; j++) a[j] *= w[j];
+    }
+    if (p.pre_w) {
+      load8(p.pre_w, c.w_type, i0, true, 8, w);
+#pragma unroll
+      for (int j = 0; j < 8; j++) b[j] = c.weight_offset + w[j];
+    }
+  }
+  __syncthreads();
+  int s = 0, flip = 0;
+  uint32_t ph = 0;
+  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
+    // a copy that never lands (bounded wait) makes the row NaN
+    const bool ok = mbar_wait(&full[s], ph, &abort);
+    const float none = ok ? 0.f : __uint_as_float(0x7fffffffu);
+    float x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = y[j] = none;
+    const uint8_t* st = ring + s * stage;
+    if (in && ok) {
+      load8(st, c.x_type, i0, true, 8, x);
+      if (p.y) load8(st + rs.x_bytes, c.y_type, i0, true, 8, y);
+    }
+    if (p.y) {
+      float r = 1.f;
+      if (c.post_norm) {
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q = fmaf(y[j], y[j], q);
+        r = 1.f / sqrtf(block_sum(q, buf[flip][0]) / (float)M + c.eps);
+      }
+      if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] *= r * a[j];
+      if (c.gate_kind == WISP_GATE_ELEMENT && in) {
+        float w[8];
+        load8(p.gate, c.gate_type, t * c.ld_gate + i0, true, 8, w);
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] *= w[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = fmaf(c.residual_scale, x[j], y[j]);
+      if (p.x_out && in) store8(p.x_out, c.x_type, t * c.ld_x_out + i0, true, 8, x);
+    }
+    float r = 0.f;
+    if (p.n) {
+      float q = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) q = fmaf(x[j], x[j], q);
+      r = 1.f / sqrtf(block_sum(q, buf[flip][1]) / (float)M + c.eps);
+    } else if (!c.post_norm) {
+      __syncthreads();
+    }
+    // every thread has read this stage (a block sum or the barrier lies between)
+    if (tid == 0) {
+      const int64_t next = t + (int64_t)rs.stages * gridDim.x;
+      if (next < T) issue(s, next);
+    }
+    if (p.n && in) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] *= r * b[j];
+      store8(p.n, c.n_type, t * c.ld_n + i0, true, 8, x);
+    }
+    flip ^= 1;
+    if (++s == rs.stages) {
+      s = 0;
+      ph ^= 1;
     }
   }
 }
@@ -173,21 +310,39 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   p.x_out = d_x_out;
   p.n = d_n;
   auto wide = [](const void* q, int type, int64_t ld) {
-    return (int)(!((uintptr_t)q & 15) && ld * dt_size(type) % 16 == 0);
+    return !((uintptr_t)q & 15) && ld * dt_size(type) % 16 == 0;
   };
-  p.wide_x = wide(d_x, c.x_type, c.ld_x);
-  p.wide_y = wide(d_y, c.y_type, c.ld_y);
-  p.wide_g = wide(d_gate, c.gate_type, c.gate_kind == WISP_GATE_ELEMENT ? c.ld_gate : 0);
-  p.wide_post = wide(d_post_w, c.w_type, 0);
-  p.wide_pre = wide(d_pre_w, c.w_type, 0);
-  p.wide_xo = wide(d_x_out, c.x_type, c.ld_x_out);
-  p.wide_n = wide(d_n, c.n_type, c.ld_n);
-  const int vecs = (c.hidden + 7) / 8;
-  if (vecs <= 1024 && c.tokens <= 296) {
-    wb::launch_k(block_norm_kernel<1>, c.tokens, (vecs + 31) / 32 * 32, 0, stream, p);
+  const bool vec =
+      c.hidden % 8 == 0 && wide(d_x, c.x_type, c.ld_x) && (!d_y || wide(d_y, c.y_type, c.ld_y)) &&
+      wide(d_gate, c.gate_type, c.gate_kind == WISP_GATE_ELEMENT ? c.ld_gate : 0) &&
+      wide(d_post_w, c.w_type, 0) && wide(d_pre_w, c.w_type, 0) &&
+      (!p.x_out || wide(d_x_out, c.x_type, c.ld_x_out)) && (!d_n || wide(d_n, c.n_type, c.ld_n));
+  const int vecs = (c.hidden + 7) / 8, T = c.tokens;
+  const int threads1 = (vecs + 31) / 32 * 32, threads4 = ((vecs + 3) / 4 + 31) / 32 * 32;
+  int dev = 0, sms = 0;
+  WB_CUDA_CHECK(cudaGetDevice(&dev));
+  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (vec && threads1 <= 1024 && T > 2 * sms) {
+    RingShape rs;
+    rs.x_bytes = c.hidden * dt_size(c.x_type);
+    rs.y_bytes = d_y ? c.hidden * dt_size(c.y_type) : 0;
+    // as many CTAs per SM as make 1024 threads, which share its memory
+    const int ctas = threads1 >= 512 ? 1 : 1024 / threads1 < 8 ? 1024 / threads1 : 8;
+    const int budget = 200 * 1024 / ctas, stage = rs.x_bytes + rs.y_bytes;
+    rs.stages = budget / stage < kNormStages ? budget / stage : kNormStages;
+    WB_CUDA_CHECK(cudaFuncSetAttribute(block_norm_stream_kernel,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    const int grid = ctas * sms < T ? ctas * sms : T;
+    wb::launch_k(block_norm_stream_kernel, grid, threads1, (size_t)rs.stages * stage, stream, p, rs);
+  } else if (threads1 <= 1024) {
+    if (vec)
+      wb::launch_k(block_norm_kernel<1, 1024, true>, T, threads1, 0, stream, p);
+    else
+      wb::launch_k(block_norm_kernel<1, 1024, false>, T, threads1, 0, stream, p);
+  } else if (vec) {
+    wb::launch_k(block_norm_kernel<4, 1024, true>, T, threads4, 0, stream, p);
   } else {
-    const int threads = ((vecs + 3) / 4 + 31) / 32 * 32;
-    wb::launch_k(block_norm_kernel<4>, c.tokens, threads, 0, stream, p);
+    wb::launch_k(block_norm_kernel<4, 1024, false>, T, threads4, 0, stream, p);
   }
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
