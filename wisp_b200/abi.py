@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import re
+import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libwisp_b200.so"
@@ -221,9 +222,18 @@ def check(code: int, err: WispErrCtx) -> None:
         raise RuntimeError(msg)
 
 
+_tls = threading.local()
+
+
 def call(name: str, *args) -> None:
-    """Call a WispError-returning entry point with a fresh error context as
+    """Call a WispError-returning entry point with this thread's error context as
     its last argument; raise RuntimeError on failure."""
-    err = WispErrCtx()
-    code = getattr(lib(), name)(*args, C.byref(err))
-    check(code, err)
+    try:
+        err, ref = _tls.err
+    except AttributeError:
+        err = WispErrCtx()
+        ref = C.byref(err)
+        _tls.err = (err, ref)
+    code = getattr(_lib or lib(), name)(*args, ref)
+    if code != WISP_OK:
+        check(code, err)

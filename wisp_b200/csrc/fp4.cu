@@ -29,10 +29,23 @@ using namespace wb;
 
 constexpr int kUnit = 16;   // values per thread: one NV block, half an MX block
 
+// A row of `units` threads split over equal blocks of at most 256.
+int row_threads(int units) {
+  const int blocks = (units + 255) / 256;
+  return ((units + blocks - 1) / blocks + 31) / 32 * 32;
+}
+
 // Codes of eight values, the first in the low nibble. Round to nearest even,
 // saturating.
 WB_DEV uint32_t e2m1x8(const float* v, float r) {
   uint32_t o;
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 4; j++)     // two products per instruction
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(q[2 * j]), "=f"(q[2 * j + 1])
+        : "f"(v[2 * j]), "f"(v[2 * j + 1]), "f"(r));
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -40,8 +53,7 @@ WB_DEV uint32_t e2m1x8(const float* v, float r) {
       "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
       "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(o)
-      : "f"(v[0] * r), "f"(v[1] * r), "f"(v[2] * r), "f"(v[3] * r), "f"(v[4] * r), "f"(v[5] * r),
-        "f"(v[6] * r), "f"(v[7] * r));
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
   return o;
 }
 
@@ -82,12 +94,19 @@ __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
 // significant bits).
 WB_DEV bool nv_plain_range(float g) { return g >= 1e-30f && g <= 1e30f; }
 
+// 1 / x to 1 ulp, for normal x and 1 / x.
+WB_DEV float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
 
 // The same for a plain g: the byte of the scaled-down and scaled-up fp32
 // quotient, or where those differ by the sign of border * 6 g - a.
 WB_DEV uint32_t nv_scale_byte(float a, float g) {
-  const float t = a * __frcp_rn(6.f * g);
+  const float t = a * rcp_approx(6.f * g);
   const uint32_t both =
       __nv_cvt_float2_to_fp8x2(make_float2(t * kBelow, t * kAbove), __NV_SATFINITE, __NV_E4M3);
   const uint32_t lo = both & 255u, hi = both >> 8;
@@ -102,62 +121,58 @@ struct QuantParams {
   int64_t ld;
   int x_rows;
   const int* src;
-  int cols;
+  int rows, cols;
   const float* ts;
   uint8_t* codes;
   uint8_t* scales;
-  int wide;   // rows of x start on 16-byte boundaries
+  int wide;   // rows of x start on 32-byte boundaries
 };
 
-// 16 values of one thread as floats, and the largest magnitude's bits (as an
-// integer, so that a NaN is the largest of all).
+// 16 values of one thread as they lie in memory.
 template <typename T>
-WB_DEV uint32_t load16(const T* x, bool wide, float (&v)[16]) {
-  uint32_t top = 0;
-  if (sizeof(T) == 4) {
-    const float* q = reinterpret_cast<const float*>(x);
-    if (wide) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(q) + j);
-        v[4 * j] = f.x;
-        v[4 * j + 1] = f.y;
-        v[4 * j + 2] = f.z;
-        v[4 * j + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; j++) v[j] = __ldg(q + j);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; j++) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-    return top;
-  }
-  constexpr int type = sizeof(T) == 2 && std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16;
-  uint32_t u[8];
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(x);
+struct Raw {
+  uint32_t u[4 * sizeof(T)];
+};
+
+template <typename T>
+WB_DEV void load_raw(const T* x, bool wide, Raw<T>& r) {
+  constexpr int W = 4 * sizeof(T);
   if (wide) {
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const uint4 f = __ldg(reinterpret_cast<const uint4*>(q) + j);
-      u[4 * j] = f.x;
-      u[4 * j + 1] = f.y;
-      u[4 * j + 2] = f.z;
-      u[4 * j + 3] = f.w;
-    }
+    for (int j = 0; j < W / 8; j++) load32(reinterpret_cast<const uint8_t*>(x) + 32 * j, r.u + 8 * j);
+  } else if (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < W; j++) r.u[j] = __ldg(reinterpret_cast<const uint32_t*>(x) + j);
   } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(x);
 #pragma unroll
-    for (int j = 0; j < 8; j++) u[j] = __ldg(q + 2 * j) | (uint32_t)__ldg(q + 2 * j + 1) << 16;
+    for (int j = 0; j < W; j++) r.u[j] = __ldg(q + 2 * j) | (uint32_t)__ldg(q + 2 * j + 1) << 16;
   }
+}
+
+// Their values, and the largest magnitude's bits in fp32 (found on integers,
+// so that a NaN is the largest of all).
+template <typename T>
+WB_DEV uint32_t unpack_raw(const Raw<T>& r, float (&v)[16]) {
+  uint32_t top = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float2 f = unpack2(u[j], type);
-    v[2 * j] = f.x;
-    v[2 * j + 1] = f.y;
-    top = __vmaxu2(top, u[j] & 0x7fff7fffu);
+    for (int j = 0; j < 16; j++) {
+      v[j] = __uint_as_float(r.u[j]);
+      top = max(top, r.u[j] & 0x7fffffffu);
+    }
+    return top;
+  } else {
+    constexpr int type = std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float2 f = unpack2(r.u[j], type);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+      top = __vmaxu2(top, r.u[j] & 0x7fff7fffu);
+    }
+    return __float_as_uint(unpack2(max(top & 0xffffu, top >> 16), type).x);
   }
-  const float2 f = unpack2(max(top & 0xffffu, top >> 16), type);
-  return __float_as_uint(f.x);
 }
 
 // Codes and scale byte of one NV block for any g and x: every decision in
@@ -202,7 +217,7 @@ WB_DEV uint32_t nv_block(const float (&v)[16], uint32_t top, float g, uint32_t (
   const uint32_t sb = nv_scale_byte(__uint_as_float(top), g);
   const float s = e4m3_value(sb);
   // a zero scale: zero codes with the values' signs
-  const float r = sb ? __frcp_rn(s * g) : 0.f;
+  const float r = sb ? rcp_approx(s * g) : 0.f;
   const float rl = r * kBelow, rh = r * kAbove;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -213,62 +228,83 @@ WB_DEV uint32_t nv_block(const float (&v)[16], uint32_t top, float g, uint32_t (
   return sb;
 }
 
-// grid (rows, ceil(cols / 16 / blockDim)): one thread per 16 values, 32
-// (16-bit types) or 64 (fp32) bytes read and 8 written.
-template <bool NV, typename T>
+// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): one thread per 16 values
+// of R rows, 32 (16-bit types) or 64 (fp32) bytes read and 8 written for each;
+// the R rows' loads are issued together.
+template <bool NV, typename T, int R>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
-  const int64_t row = blockIdx.x;
+  const int64_t row0 = (int64_t)blockIdx.x * R;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
   const int units = p.cols / kUnit;
   const bool in = u < units;
-  const int64_t sr = p.src ? (int64_t)p.src[row] : row;
-  float v[16];
-  uint32_t top = 0;
+  const float g = NV ? __ldg(p.ts) : 1.f;
+  Raw<T> raw[R];
 #pragma unroll
-  for (int j = 0; j < 16; j++) v[j] = 0.f;
-  if (in && sr >= 0 && sr < p.x_rows)
-    top = load16(static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit, p.wide, v);
-  uint32_t code[2] = {0u, 0u};
-  const int64_t o = row * units + u;
-  if (NV) {
-    if (!in) return;
-    p.scales[o] = (uint8_t)nv_block(v, top, *p.ts, code);
-  } else {
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    if (!in) return;
-    uint32_t sb = 255;
-    if (top < 0x7f800000u) {
-      const uint32_t e = top >> 23;
-      sb = e > 2 ? e - 2 : 0;
-      const float inv = __uint_as_float((254u - sb) << 23);   // 2^(127 - sb)
-      code[0] = e2m1x8(v, inv);
-      code[1] = e2m1x8(v + 8, inv);
-    }
-    if (!(u & 1)) p.scales[o >> 1] = (uint8_t)sb;
+  for (int i = 0; i < R; i++) {
+    const int64_t row = row0 + i;
+    int64_t sr = -1;
+    if (row < p.rows) sr = p.src ? (int64_t)__ldg(p.src + row) : row;
+#pragma unroll
+    for (int j = 0; j < 4 * (int)sizeof(T); j++) raw[i].u[j] = 0;
+    if (in && sr >= 0 && sr < p.x_rows)
+      load_raw(static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit, p.wide, raw[i]);
   }
-  *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int64_t row = row0 + i, o = row * units + u;
+    float v[16];
+    uint32_t top = unpack_raw(raw[i], v);
+    uint32_t code[2] = {0u, 0u};
+    if (NV) {
+      const uint32_t sb = nv_block(v, top, g, code);
+      if (in && row < p.rows) {
+        p.scales[o] = (uint8_t)sb;
+        *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
+      }
+    } else {
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      uint32_t sb = 255;
+      if (top < 0x7f800000u) {
+        const uint32_t e = top >> 23;
+        sb = e > 2 ? e - 2 : 0;
+        const float inv = __uint_as_float((254u - sb) << 23);   // 2^(127 - sb)
+        code[0] = e2m1x8(v, inv);
+        code[1] = e2m1x8(v + 8, inv);
+      }
+      if (in && row < p.rows) {
+        if (!(u & 1)) p.scales[o >> 1] = (uint8_t)sb;
+        *reinterpret_cast<uint2*>(p.codes + o * 8) = make_uint2(code[0], code[1]);
+      }
+    }
+  }
+}
+
+template <bool NV, typename T>
+void launch_quantize_t(const QuantParams& p, cudaStream_t st) {
+  const int units = p.cols / kUnit, threads = row_threads(units);
+  const int gy = (units + threads - 1) / threads;
+  constexpr int R = NV || sizeof(T) == 4 ? 2 : 4;
+  // Several rows per thread once there are enough to fill the GPU all the same.
+  if ((int64_t)p.rows * gy >= 148 * 8 * R)
+    wb::launch_k(quantize_kernel<NV, T, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
+  else
+    wb::launch_k(quantize_kernel<NV, T, 1>, dim3(p.rows, gy), threads, 0, st, p);
 }
 
 template <bool NV>
-void launch_quantize(const QuantParams& p, int type, dim3 grid, int threads, cudaStream_t st) {
+void launch_quantize(const QuantParams& p, int type, cudaStream_t st) {
   if (type == WISP_DT_F32)
-    wb::launch_k(quantize_kernel<NV, float>, grid, threads, 0, st, p);
+    launch_quantize_t<NV, float>(p, st);
   else if (type == WISP_DT_BF16)
-    wb::launch_k(quantize_kernel<NV, __nv_bfloat16>, grid, threads, 0, st, p);
+    launch_quantize_t<NV, __nv_bfloat16>(p, st);
   else
-    wb::launch_k(quantize_kernel<NV, __half>, grid, threads, 0, st, p);
-}
-
-// A row of `units` threads split over equal blocks of at most 256.
-int row_threads(int units) {
-  const int blocks = (units + 255) / 256;
-  return ((units + blocks - 1) / blocks + 31) / 32 * 32;
+    launch_quantize_t<NV, __half>(p, st);
 }
 
 struct DequantParams {
   const uint8_t* codes;
   const uint8_t* scales;
-  int cols;
+  int rows, cols;
   const float* ts;
   void* out;
   int64_t ld;
@@ -281,48 +317,115 @@ WB_DEV float2 e2m1_values(uint32_t byte) {
   return __half22float2(u2h2(h));
 }
 
-// grid (rows, ceil(cols / 16 / blockDim)): one thread per 16 values, 8 bytes
-// read and 32 (16-bit types) or 64 written. code * scale is exact in fp32 (2 x
-// 4 significant bits); the tensor scale and the output type round once each.
-template <bool NV, int TYPE>
+WB_DEV float scale_value(uint32_t sb, bool nv) {
+  // MX 2^(sb - 127): 2^-127 is subnormal, 255 is NaN
+  return nv ? e4m3_value(sb)
+            : __uint_as_float(sb == 255 ? 0x7fffffffu : sb == 0 ? 0x00400000u : sb << 23);
+}
+
+// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 values of R rows per
+// thread. fp32: in four chunks of 16 bytes blockDim apart, so that a warp's
+// stores are 512 consecutive bytes (14336 x 4096: 63 -> 45 us); 16-bit types:
+// 16 neighbours, read with one load and written as one sector. code * scale is
+// exact in fp32 (2 x 4 significant bits); the tensor scale and the output type
+// round once each.
+template <bool NV, int TYPE, int R>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
-  const int64_t row = blockIdx.x;
-  const int u = blockIdx.y * blockDim.x + threadIdx.x;
-  const int units = p.cols / kUnit;
-  if (u >= units) return;
-  const int64_t o = row * units + u;
-  const uint32_t c[2] = {__ldg(reinterpret_cast<const uint32_t*>(p.codes) + o * 2),
-                         __ldg(reinterpret_cast<const uint32_t*>(p.codes) + o * 2 + 1)};
-  const uint32_t sb = __ldg(p.scales + (NV ? o : o >> 1));
-  float s, g = 1.f;
-  if (NV) {
-    s = e4m3_value(sb);
-    if (p.ts) g = __ldg(p.ts);
-  } else {
-    // 2^(sb - 127): 2^-127 is subnormal, 255 is NaN
-    s = __uint_as_float(sb == 255 ? 0x7fffffffu : sb == 0 ? 0x00400000u : sb << 23);
-  }
+  const int64_t row = (int64_t)blockIdx.x * R;
+  const int tid = threadIdx.x;
+  const float g = NV && p.ts ? __ldg(p.ts) : 1.f;
+  const uint8_t* codes = p.codes + row * (p.cols / 2);
+  const uint8_t* scales = p.scales + row * (p.cols / (NV ? 16 : 32));
+  if (TYPE == WISP_DT_F32) {
+    const int first = blockIdx.y * blockDim.x * 4 + tid, chunks = p.cols / 4;
+    uint32_t c[4];
+    float s[4];
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float2 f = e2m1_values((c[h] >> (8 * j)) & 255u);
-      v[2 * j] = NV ? f.x * s * g : f.x * s;
-      v[2 * j + 1] = NV ? f.y * s * g : f.y * s;
+    for (int i = 0; i < 4; i++) {
+      const int u = first + i * blockDim.x;
+      if (u < chunks) {
+        c[i] = __ldg(reinterpret_cast<const uint16_t*>(codes) + u);
+        s[i] = scale_value(__ldg(scales + (NV ? u >> 2 : u >> 3)), NV);
+      }
     }
-    store8(p.out, TYPE, row * p.ld + (int64_t)u * kUnit + 8 * h, p.wide, 8, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int u = first + i * blockDim.x;
+      if (u < chunks) {
+        float* q = static_cast<float*>(p.out) + row * p.ld + (int64_t)u * 4;
+        const float2 f0 = e2m1_values(c[i] & 255u), f1 = e2m1_values(c[i] >> 8);
+        const float4 v = make_float4(f0.x * s[i] * g, f0.y * s[i] * g, f1.x * s[i] * g, f1.y * s[i] * g);
+        if (p.wide) {
+          *reinterpret_cast<float4*>(q) = v;
+        } else {
+          q[0] = v.x;
+          q[1] = v.y;
+          q[2] = v.z;
+          q[3] = v.w;
+        }
+      }
+    }
+  } else {
+    const int u = blockIdx.y * blockDim.x + tid;
+    if (u >= p.cols / kUnit) return;
+    uint32_t c[R][2];
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (row + r < p.rows) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(codes + (int64_t)r * (p.cols / 2));
+        c[r][0] = __ldg(q + 2 * u);
+        c[r][1] = __ldg(q + 2 * u + 1);
+        s[r] = scale_value(__ldg(scales + (int64_t)r * (p.cols / (NV ? 16 : 32)) + (NV ? u : u >> 1)), NV);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (row + r < p.rows) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float2 f = e2m1_values((c[r][j >> 2] >> (8 * (j & 3))) & 255u);
+          v[2 * j] = f.x * s[r] * g;
+          v[2 * j + 1] = f.y * s[r] * g;
+        }
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] = pack2(v[2 * j], v[2 * j + 1], TYPE);
+        uint16_t* q = static_cast<uint16_t*>(p.out) + (row + r) * p.ld + (int64_t)u * kUnit;
+        if (p.wide) {
+          store32(q, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            q[2 * j] = (uint16_t)o[j];
+            q[2 * j + 1] = (uint16_t)(o[j] >> 16);
+          }
+        }
+      }
+    }
   }
 }
 
-template <bool NV>
-void launch_dequantize(const DequantParams& p, int type, dim3 grid, int threads, cudaStream_t st) {
-  if (type == WISP_DT_F32)
-    wb::launch_k(dequantize_kernel<NV, WISP_DT_F32>, grid, threads, 0, st, p);
-  else if (type == WISP_DT_BF16)
-    wb::launch_k(dequantize_kernel<NV, WISP_DT_BF16>, grid, threads, 0, st, p);
+template <bool NV, int TYPE>
+void launch_dequantize_t(const DequantParams& p, cudaStream_t st) {
+  const int units = p.cols / kUnit, threads = row_threads(units);
+  const int gy = (units + threads - 1) / threads;
+  constexpr int R = TYPE == WISP_DT_F32 ? 1 : 2;
+  if ((int64_t)p.rows * gy >= 148 * 8 * R)
+    wb::launch_k(dequantize_kernel<NV, TYPE, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
   else
-    wb::launch_k(dequantize_kernel<NV, WISP_DT_F16>, grid, threads, 0, st, p);
+    wb::launch_k(dequantize_kernel<NV, TYPE, 1>, dim3(p.rows, gy), threads, 0, st, p);
+}
+
+template <bool NV>
+void launch_dequantize(const DequantParams& p, int type, cudaStream_t st) {
+  if (type == WISP_DT_F32)
+    launch_dequantize_t<NV, WISP_DT_F32>(p, st);
+  else if (type == WISP_DT_BF16)
+    launch_dequantize_t<NV, WISP_DT_BF16>(p, st);
+  else
+    launch_dequantize_t<NV, WISP_DT_F16>(p, st);
 }
 
 // Scale bytes [entries x n x kb] to runs of one 128-feature x 256-k stage:
@@ -390,18 +493,16 @@ extern "C" WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t
   p.ld = ld;
   p.x_rows = x_rows;
   p.src = d_src;
+  p.rows = rows;
   p.cols = cols;
   p.ts = d_tensor_scale;
   p.codes = d_codes;
   p.scales = d_scales;
-  p.wide = !((uintptr_t)d_x & 15) && (ld * dt_size(x_type)) % 16 == 0;
-  const int units = cols / kUnit;
-  const int threads = row_threads(units);
-  const dim3 grid(rows, (units + threads - 1) / threads);
+  p.wide = !((uintptr_t)d_x & 31) && (ld * dt_size(x_type)) % 32 == 0;
   if (format == WISP_FP4_NV)
-    launch_quantize<true>(p, x_type, grid, threads, stream);
+    launch_quantize<true>(p, x_type, stream);
   else
-    launch_quantize<false>(p, x_type, grid, threads, stream);
+    launch_quantize<false>(p, x_type, stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
 }
@@ -429,18 +530,17 @@ extern "C" WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint
   DequantParams p;
   p.codes = d_codes;
   p.scales = d_scales;
+  p.rows = rows;
   p.cols = cols;
   p.ts = d_tensor_scale;
   p.out = d_out;
   p.ld = ld;
-  p.wide = !((uintptr_t)d_out & 15) && (ld * dt_size(out_type)) % 16 == 0;
-  const int units = cols / kUnit;
-  const int threads = row_threads(units);
-  const dim3 grid(rows, (units + threads - 1) / threads);
+  const int align = out_type == WISP_DT_F32 ? 16 : 32;
+  p.wide = (uintptr_t)d_out % align == 0 && ld * dt_size(out_type) % align == 0;
   if (format == WISP_FP4_NV)
-    launch_dequantize<true>(p, out_type, grid, threads, stream);
+    launch_dequantize<true>(p, out_type, stream);
   else
-    launch_dequantize<false>(p, out_type, grid, threads, stream);
+    launch_dequantize<false>(p, out_type, stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
 }

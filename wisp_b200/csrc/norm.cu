@@ -21,19 +21,37 @@ struct NormParams {
   const void* pre_w;
   void* x_out;
   void* n;
+  float inv_m;     // 1 / hidden
 };
 
-// Sum over the block, the same bits in every thread.
-WB_DEV float block_sum(float v, float* buf) {
+// 1 / rms from the mean square (rsqrt: 2 ulp at most, under the sum's own error).
+WB_DEV float inv_rms(float mean_sq, float eps) { return rsqrtf(mean_sq + eps); }
+
+// Sums of N values over the block, the same bits in every thread.
+template <int N>
+WB_DEV void block_sum(float (&v)[N], float (*buf)[32]) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   const int warps = (blockDim.x + 31) >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = lane < warps ? buf[lane] : 0.f;
+  if (lane == 0) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+    for (int i = 0; i < N; i++) buf[i][threadIdx.x >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = lane < warps ? buf[i][lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+}
+
+WB_DEV float square_sum(const float (&v)[8], float s) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
+  return s;
 }
 
 // Vectors of 8: thread i of `VEC` kernels holds elements 8 (k blockDim + i) ..
@@ -75,7 +93,7 @@ WB_DEV void store_row(void* q, int type, int64_t base, int k, int M, const float
 // One row per CTA.
 template <int V, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float buf[2][32];
+  __shared__ float buf[2][1][32];
   const WispBlockNorm& c = p.c;
   const int64_t t = blockIdx.x;
   const int M = c.hidden;
@@ -88,12 +106,11 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_consta
   if (p.y) {
     float r = 1.f;
     if (c.post_norm) {
-      float s = 0.f;
+      float s[1] = {0.f};
 #pragma unroll
-      for (int k = 0; k < V; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) s = fmaf(y[k][j], y[k][j], s);
-      r = 1.f / sqrtf(block_sum(s, buf[0]) / (float)M + c.eps);
+      for (int k = 0; k < V; k++) s[0] = square_sum(y[k], s[0]);
+      block_sum(s, buf[0]);
+      r = inv_rms(s[0] * p.inv_m, c.eps);
     }
     if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
@@ -118,12 +135,11 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_consta
     }
   }
   if (p.n) {
-    float s = 0.f;
+    float s[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < V; k++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) s = fmaf(x[k][j], x[k][j], s);
-    const float r = 1.f / sqrtf(block_sum(s, buf[1]) / (float)M + c.eps);
+    for (int k = 0; k < V; k++) s[0] = square_sum(x[k], s[0]);
+    block_sum(s, buf[1]);
+    const float r = inv_rms(s[0] * p.inv_m, c.eps);
 #pragma unroll
     for (int k = 0; k < V; k++) {
       float w[8];
@@ -142,9 +158,10 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_consta
 // Many rows: persistent CTAs that take rows blockIdx.x, + gridDim.x, ..., whose
 // x and y arrive through a ring of bulk copies, so that the memory stays busy
 // while a row's sums go round the CTA. A thread holds 8 columns, and their
-// weights and channel gate for good. (One row per CTA measured 2.4 TB/s of
-// 10-byte-per-value traffic at 4096 x 7168: its loads, sums and stores follow
-// one another, and two CTAs fit an SM.)
+// weights and channel gate for good. The sum of a row's x'^2 goes round
+// together with the sum of the next row's y^2: one barrier per row. (At 4096 x
+// 7168, 10 bytes a value, one row per CTA took 117 us, this ring with two
+// sums after one another 64, with one 51; 45 us are the copy rate.)
 constexpr int kNormStages = 8;
 struct RingShape {
   int stages, x_bytes, y_bytes;
@@ -200,29 +217,43 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       for (int j = 0; j < 8; j++) b[j] = c.weight_offset + w[j];
     }
   }
-  __syncthreads();
   int s = 0, flip = 0;
   uint32_t ph = 0;
-  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
-    // a copy that never lands (bounded wait) makes the row NaN
+  float x[8], y[8];
+  // The ring's next row into x and y; a copy that never lands (the wait is
+  // bounded) makes the row NaN. The slot may be refilled after the next
+  // barrier.
+  auto take = [&](int64_t t) {
     const bool ok = mbar_wait(&full[s], ph, &abort);
+    const uint8_t* st = ring + s * stage;
     const float none = ok ? 0.f : __uint_as_float(0x7fffffffu);
-    float x[8], y[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = y[j] = none;
-    const uint8_t* st = ring + s * stage;
     if (in && ok) {
       load8(st, c.x_type, i0, true, 8, x);
       if (p.y) load8(st + rs.x_bytes, c.y_type, i0, true, 8, y);
     }
+  };
+  auto refill = [&](int64_t t) {      // the slot row t was taken from
+    if (tid == 0) {
+      const int64_t next = t + (int64_t)rs.stages * gridDim.x;
+      if (next < T) issue(s, next);
+    }
+    if (++s == rs.stages) {
+      s = 0;
+      ph ^= 1;
+    }
+  };
+  __syncthreads();
+  int64_t t = blockIdx.x;
+  take(t);
+  float q[2] = {0.f, square_sum(y, 0.f)};
+  block_sum(q, buf[flip]);
+  refill(t);
+  for (; t < T; t += gridDim.x) {
+    flip ^= 1;
     if (p.y) {
-      float r = 1.f;
-      if (c.post_norm) {
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) q = fmaf(y[j], y[j], q);
-        r = 1.f / sqrtf(block_sum(q, buf[flip][0]) / (float)M + c.eps);
-      }
+      float r = c.post_norm ? inv_rms(q[1] * p.inv_m, c.eps) : 1.f;
       if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] *= r * a[j];
@@ -236,29 +267,20 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       for (int j = 0; j < 8; j++) x[j] = fmaf(c.residual_scale, x[j], y[j]);
       if (p.x_out && in) store8(p.x_out, c.x_type, t * c.ld_x_out + i0, true, 8, x);
     }
-    float r = 0.f;
-    if (p.n) {
-      float q = 0.f;
+    float xp[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) q = fmaf(x[j], x[j], q);
-      r = 1.f / sqrtf(block_sum(q, buf[flip][1]) / (float)M + c.eps);
-    } else if (!c.post_norm) {
-      __syncthreads();
-    }
-    // every thread has read this stage (a block sum or the barrier lies between)
-    if (tid == 0) {
-      const int64_t next = t + (int64_t)rs.stages * gridDim.x;
-      if (next < T) issue(s, next);
-    }
+    for (int j = 0; j < 8; j++) xp[j] = x[j];
+    q[0] = square_sum(x, 0.f);
+    const int64_t tn = t + gridDim.x;
+    if (tn < T) take(tn);
+    q[1] = square_sum(y, 0.f);
+    block_sum(q, buf[flip]);
+    if (tn < T) refill(tn);
     if (p.n && in) {
+      const float r = inv_rms(q[0] * p.inv_m, c.eps);
 #pragma unroll
-      for (int j = 0; j < 8; j++) x[j] *= r * b[j];
-      store8(p.n, c.n_type, t * c.ld_n + i0, true, 8, x);
-    }
-    flip ^= 1;
-    if (++s == rs.stages) {
-      s = 0;
-      ph ^= 1;
+      for (int j = 0; j < 8; j++) xp[j] *= r * b[j];
+      store8(p.n, c.n_type, t * c.ld_n + i0, true, 8, xp);
     }
   }
 }
@@ -309,6 +331,7 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   p.pre_w = d_pre_w;
   p.x_out = d_x_out;
   p.n = d_n;
+  p.inv_m = 1.f / (float)c.hidden;
   auto wide = [](const void* q, int type, int64_t ld) {
     return !((uintptr_t)q & 15) && ld * dt_size(type) % 16 == 0;
   };
@@ -327,7 +350,7 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
     rs.x_bytes = c.hidden * dt_size(c.x_type);
     rs.y_bytes = d_y ? c.hidden * dt_size(c.y_type) : 0;
     // as many CTAs per SM as make 1024 threads, which share its memory
-    const int ctas = threads1 >= 512 ? 1 : 1024 / threads1 < 8 ? 1024 / threads1 : 8;
+    const int ctas = 1024 / threads1 < 8 ? 1024 / threads1 : 8;
     const int budget = 200 * 1024 / ctas, stage = rs.x_bytes + rs.y_bytes;
     rs.stages = budget / stage < kNormStages ? budget / stage : kNormStages;
     WB_CUDA_CHECK(cudaFuncSetAttribute(block_norm_stream_kernel,

@@ -45,6 +45,21 @@ WB_DEV uint32_t pack2(float a, float b, int type) {
   return h22u(__floats2half2_rn(a, b));
 }
 
+// 32 bytes per thread in one instruction (32-byte aligned): a warp's access is
+// then 1 KB of whole sectors, where two 16-byte accesses each touch half of
+// every sector.
+WB_DEV void load32(const void* p, uint32_t* u) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
+                 "=r"(u[6]), "=r"(u[7])
+               : "l"(p));
+}
+WB_DEV void store32(void* p, const uint32_t* u) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]),
+               "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
+
 // Eight consecutive values from element i. `wide`: p + i is 16-byte aligned
 // (32-byte runs for fp32 are two 16-byte loads) and all eight exist; else the
 // first n are read one by one and the rest are 0.

@@ -27,17 +27,23 @@ def invalid(msg: str) -> RuntimeError:
     return RuntimeError(f"wisp engine error [{abi.WISP_ERR_INVALID_ARG}]: {msg}")
 
 
-def on_device(t: torch.Tensor):
-    """Context in which launches go to t's device (nothing to do on the current one)."""
-    if t.device.type != "cuda":
+def elsewhere(t: torch.Tensor):
+    """None when t is on the current CUDA device (the usual case, kept cheap), else the context
+    in which launches go to t's device."""
+    dev = t.get_device()
+    if dev < 0:
         raise invalid(f"tensor on {t.device}: the kernels have no CPU path")
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    if dev == torch._C._cuda_getDevice():
+        return None
+    return torch.cuda.device(dev)
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def dtype_code(dtype: torch.dtype, what: str) -> int:
@@ -55,8 +61,9 @@ def row_stride(t: torch.Tensor, what: str) -> int:
 
 
 def same_device(ref: torch.Tensor, **tensors) -> None:
+    dev = ref.get_device()
     for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != dev:
             raise invalid(f"{name} is on {t.device}, not on {ref.device}")
 
 
@@ -101,6 +108,13 @@ class Fp4Rows:
     def rows(self) -> int:
         return self.codes.shape[0]
 
+    @classmethod
+    def _made(cls, fmt, codes, scales, tensor_scale, cols) -> "Fp4Rows":
+        """Rows whose parts this module allocated itself (nothing left to check)."""
+        q = cls.__new__(cls)
+        q.fmt, q.codes, q.scales, q.tensor_scale, q.cols = fmt, codes, scales, tensor_scale, cols
+        return q
+
 
 def tensor_scale(x: torch.Tensor) -> torch.Tensor:
     """The NV tensor scale that lets the largest block scale reach 448: max|x| / 2688
@@ -113,39 +127,50 @@ def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None
              rows: torch.Tensor | None = None) -> Fp4Rows:
     """Rows of x (float32, bfloat16 or float16) as 4-bit codes; rows (int32): row p of the
     result is row rows[p] of x, a row of zeros where rows[p] is outside x."""
-    if fmt not in BLOCK:
+    block = BLOCK.get(fmt)
+    if block is None:
         raise invalid(f"unknown format {fmt}")
     ld = row_stride(x, "x")
     n, cols = x.shape
-    if cols % BLOCK[fmt] or cols == 0:
-        raise invalid(f"row length {cols} is no multiple of {BLOCK[fmt]}")
-    if fmt == abi.WISP_FP4_NV and tensor_scale is None:
-        raise invalid("NV rows need a tensor scale")
-    _check_scale(tensor_scale, 1, "tensor_scale")
+    if cols % block or cols == 0:
+        raise invalid(f"row length {cols} is no multiple of {block}")
+    nv = fmt == abi.WISP_FP4_NV
+    if nv:
+        if tensor_scale is None:
+            raise invalid("NV rows need a tensor scale")
+        _check_scale(tensor_scale, 1, "tensor_scale")
+    else:
+        tensor_scale = None
+    r = n
     if rows is not None:
         if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
             raise invalid("rows: a contiguous 1D int32 tensor")
-    same_device(x, tensor_scale=tensor_scale, rows=rows)
+        r = rows.shape[0]
     dt = dtype_code(x.dtype, "x")
-    r = n if rows is None else rows.shape[0]
-    with on_device(x):
-        codes = torch.empty((r, cols // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((r, cols // BLOCK[fmt]), dtype=torch.uint8, device=x.device)
-        abi.call("wisp_b200_fp4_quantize", x.data_ptr(), dt, ld, n,
-                 None if rows is None else rows.data_ptr(), r, cols, fmt,
-                 None if tensor_scale is None else tensor_scale.data_ptr(), codes.data_ptr(),
-                 scales.data_ptr(), stream_of(x))
-    return Fp4Rows(fmt, codes, scales, tensor_scale if fmt == abi.WISP_FP4_NV else None)
+    other = elsewhere(x)
+    if other is not None:
+        with other:
+            return quantize(x, fmt, tensor_scale, rows)
+    if nv or rows is not None:
+        same_device(x, tensor_scale=tensor_scale, rows=rows)
+    codes = x.new_empty((r, cols // 2), dtype=torch.uint8)
+    scales = x.new_empty((r, cols // block), dtype=torch.uint8)
+    abi.call("wisp_b200_fp4_quantize", x.data_ptr(), dt, ld, n, ptr(rows), r, cols, fmt,
+             ptr(tensor_scale), codes.data_ptr(), scales.data_ptr(), stream_of(x))
+    return Fp4Rows._made(fmt, codes, scales, tensor_scale, cols)
 
 
 def dequantize(q: Fp4Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of quantised rows."""
     dt = dtype_code(dtype, "dtype")
-    with on_device(q.codes):
-        out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.codes.device)
-        abi.call("wisp_b200_fp4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows,
-                 q.cols, q.fmt, None if q.tensor_scale is None else q.tensor_scale.data_ptr(),
-                 out.data_ptr(), dt, q.cols, stream_of(q.codes))
+    codes = q.codes
+    other = elsewhere(codes)
+    if other is not None:
+        with other:
+            return dequantize(q, dtype)
+    out = codes.new_empty((q.rows, q.cols), dtype=dtype)
+    abi.call("wisp_b200_fp4_dequantize", codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols,
+             q.fmt, ptr(q.tensor_scale), out.data_ptr(), dt, q.cols, stream_of(codes))
     return out
 
 
@@ -168,7 +193,7 @@ class Fp4Weights:
         self.cfg = abi.WispFp4Config(fmt, self.entries, self.n, self.k, len(mats) - 1,
                                      abi.WISP_DT_F32)
         self._keep, structs = [], []
-        with on_device(codes):
+        with elsewhere(codes) or contextlib.nullcontext():
             nbytes = abi.lib().wisp_b200_fp4_prepared_bytes(C.byref(self.cfg))
             if nbytes == 0:
                 raise invalid(f"weights [{self.entries}, {self.n}, {self.k}] are not supported")
@@ -182,13 +207,18 @@ class Fp4Weights:
                 abi.call("wisp_b200_fp4_prepare", C.byref(self.cfg), s.data_ptr(),
                          prepared.data_ptr(), nbytes, stream_of(codes))
                 self._keep.append((c, prepared, ts))
-                structs.append(abi.WispFp4Mats(c.data_ptr(), prepared.data_ptr(),
-                                               None if ts is None else ts.data_ptr()))
+                structs.append(abi.WispFp4Mats(c.data_ptr(), prepared.data_ptr(), ptr(ts)))
             self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
             # laid out once: any stream may use the object from here on
             torch.cuda.current_stream(codes.device).synchronize()
         self.mats = structs[0]
         self.up_mats = structs[1] if len(structs) == 2 else None
+        # what a product passes, by output type
+        self._cfgs = {dt: C.byref(abi.WispFp4Config(fmt, self.entries, self.n, self.k,
+                                                    len(mats) - 1, code))
+                      for dt, code in DTYPES.items()}
+        self._mats = C.byref(self.mats)
+        self._up_mats = None if self.up_mats is None else C.byref(self.up_mats)
 
     @classmethod
     def from_values(cls, fmt: int, w: torch.Tensor, up: torch.Tensor | None = None) -> "Fp4Weights":
@@ -211,7 +241,7 @@ class Fp4Weights:
 
     def check(self) -> None:
         """Raise if a product with these weights gave up waiting or met a bad segment."""
-        with on_device(self.error_word):
+        with elsewhere(self.error_word) or contextlib.nullcontext():
             abi.call("wisp_b200_check_error_flag", self.error_word.data_ptr(),
                      stream_of(self.error_word))
 
@@ -225,26 +255,31 @@ def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
     if q.fmt != w.fmt or q.cols != w.k:
         raise invalid(f"rows (format {q.fmt}, k={q.cols}) do not fit the weights (format "
                       f"{w.fmt}, k={w.k})")
+    n_segs = 0
     if segments is not None:
         if segments.dtype != torch.int32 or segments.dim() != 2 or segments.shape[1] != 4 or \
                 not segments.is_contiguous():
             raise invalid("segments: a contiguous int32 [S, 4] tensor")
-    same_device(q.codes, weights=w.error_word, segments=segments, out=out)
-    with on_device(q.codes):
-        if out is None:
-            out = torch.empty((q.rows, w.n), dtype=dtype, device=q.codes.device)
-        elif out.shape != (q.rows, w.n):
-            raise invalid(f"out {tuple(out.shape)}, not {(q.rows, w.n)}")
+        n_segs = segments.shape[0]
+    codes = q.codes
+    other = elsewhere(codes)
+    if other is not None:
+        with other:
+            return product(q, w, segments, out, dtype)
+    same_device(codes, weights=w.error_word, segments=segments, out=out)
+    rows = codes.shape[0]
+    if out is None:
+        dtype_code(dtype, "dtype")
+        out = codes.new_empty((rows, w.n), dtype=dtype)
+        ld = w.n
+    else:
+        if out.shape != (rows, w.n):
+            raise invalid(f"out {tuple(out.shape)}, not {(rows, w.n)}")
+        dtype_code(out.dtype, "out")
         ld = row_stride(out, "out")
-        cfg = abi.WispFp4Config(w.fmt, w.entries, w.n, w.k, w.cfg.swiglu,
-                                dtype_code(out.dtype, "out"))
-        x = abi.WispFp4Rows(q.codes.data_ptr(), q.scales.data_ptr(),
-                            None if q.tensor_scale is None else q.tensor_scale.data_ptr(), q.rows)
-        abi.call("wisp_b200_fp4_product", C.byref(cfg), C.byref(w.mats),
-                 None if w.up_mats is None else C.byref(w.up_mats), C.byref(x),
-                 None if segments is None else segments.data_ptr(),
-                 0 if segments is None else segments.shape[0], out.data_ptr(), ld,
-                 w.error_word.data_ptr(), stream_of(q.codes))
+    x = abi.WispFp4Rows(codes.data_ptr(), q.scales.data_ptr(), ptr(q.tensor_scale), rows)
+    abi.call("wisp_b200_fp4_product", w._cfgs[out.dtype], w._mats, w._up_mats, C.byref(x),
+             ptr(segments), n_segs, out.data_ptr(), ld, w.error_word.data_ptr(), stream_of(codes))
     return out
 
 
@@ -302,15 +337,18 @@ class Fp4MoeLayer:
         if x.dtype != torch.bfloat16 or not x.is_contiguous() or x.shape != shape:
             raise invalid(f"x: contiguous bfloat16 {shape}")
         same_device(self.workspace, x=x, out=out)
-        with on_device(x):
-            if out is None:
-                out = torch.empty(shape, dtype=torch.float32, device=x.device)
-            elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
-                raise invalid(f"out: contiguous float32 {shape}")
-            abi.call("wisp_b200_fp4_moe_forward", C.byref(self.cfg), C.byref(self._w),
-                     x.data_ptr(), out.data_ptr(), self.idx.data_ptr(), self.wt.data_ptr(),
-                     self.workspace.data_ptr(), self.workspace.numel(),
-                     self.gate_up.error_word.data_ptr(), stream_of(x))
+        other = elsewhere(x)
+        if other is not None:
+            with other:
+                return self.forward(x, out)
+        if out is None:
+            out = torch.empty(shape, dtype=torch.float32, device=x.device)
+        elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
+            raise invalid(f"out: contiguous float32 {shape}")
+        abi.call("wisp_b200_fp4_moe_forward", C.byref(self.cfg), C.byref(self._w), x.data_ptr(),
+                 out.data_ptr(), self.idx.data_ptr(), self.wt.data_ptr(),
+                 self.workspace.data_ptr(), self.workspace.numel(),
+                 self.gate_up.error_word.data_ptr(), stream_of(x))
         return out
 
     def check(self) -> None:

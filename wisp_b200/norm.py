@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import abi
-from .fp4 import dtype_code, invalid, on_device, row_stride, same_device, stream_of
+from .fp4 import dtype_code, elsewhere, invalid, ptr, row_stride, same_device, stream_of
 
 
 def _weight(w: torch.Tensor | None, hidden: int, what: str) -> None:
@@ -30,69 +30,73 @@ def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     post=False) and pre_norm alike. gate: [hidden], [tokens, 1] or [tokens, hidden]; the two
     weights share a dtype. x' has x's dtype (x_out may be x itself), n has ``dtype``; n is None
     with pre=False."""
-    T, M = x.shape if x.dim() == 2 else (0, 0)
-    c = abi.WispBlockNorm()
-    c.tokens, c.hidden = T, M
-    c.ld_x = row_stride(x, "x")
-    c.x_type = dtype_code(x.dtype, "x")
-    c.eps, c.residual_scale, c.weight_offset = eps, residual_scale, weight_offset
+    ld_x = row_stride(x, "x")
+    T, M = x.shape
+    x_type = dtype_code(x.dtype, "x")
+    ld_y = y_type = ld_gate = gate_type = gate_kind = w_type = 0
     if y is None:
         if gate is not None or post_weight is not None or x_out is not None:
             raise invalid("gate, post_weight and x_out need y")
         if not pre:
             raise invalid("nothing to compute")
+        post = False
     else:
         if y.shape != x.shape:
             raise invalid(f"y {tuple(y.shape)}, x {tuple(x.shape)}")
-        c.ld_y = row_stride(y, "y")
-        c.y_type = dtype_code(y.dtype, "y")
-        c.post_norm = 1 if post else 0
+        ld_y = row_stride(y, "y")
+        y_type = dtype_code(y.dtype, "y")
         if post_weight is not None and not post:
             raise invalid("post_weight without post")
-    if pre_weight is not None and not pre:
-        raise invalid("pre_weight without pre")
-    if n_out is not None and not pre:
-        raise invalid("n_out without pre")
+    if not pre and (pre_weight is not None or n_out is not None):
+        raise invalid("pre_weight or n_out without pre")
     _weight(post_weight, M, "post_weight")
     _weight(pre_weight, M, "pre_weight")
     w = pre_weight if pre_weight is not None else post_weight
     if w is not None:
-        c.w_type = dtype_code(w.dtype, "weight")
+        w_type = dtype_code(w.dtype, "weight")
         if post_weight is not None and post_weight.dtype != w.dtype:
             raise invalid("post_weight and pre_weight differ in dtype")
     if gate is not None:
-        c.gate_type = dtype_code(gate.dtype, "gate")
+        gate_type = dtype_code(gate.dtype, "gate")
         if gate.shape == (M,) and gate.is_contiguous():
-            c.gate_kind = abi.WISP_GATE_CHANNEL
+            gate_kind = abi.WISP_GATE_CHANNEL
         elif gate.shape == (T, 1) and gate.is_contiguous():
-            c.gate_kind = abi.WISP_GATE_TOKEN
+            gate_kind = abi.WISP_GATE_TOKEN
         elif gate.shape == (T, M):
-            c.gate_kind = abi.WISP_GATE_ELEMENT
-            c.ld_gate = row_stride(gate, "gate")
+            gate_kind = abi.WISP_GATE_ELEMENT
+            ld_gate = row_stride(gate, "gate")
         else:
             raise invalid(f"gate {tuple(gate.shape)}: [{M}], [{T}, 1] or [{T}, {M}]")
+    other = elsewhere(x)
+    if other is not None:
+        with other:
+            return block_norm(x, y, gate=gate, residual_scale=residual_scale,
+                              post_weight=post_weight, pre_weight=pre_weight, post=post, pre=pre,
+                              eps=eps, weight_offset=weight_offset, dtype=dtype, x_out=x_out,
+                              n_out=n_out)
     same_device(x, y=y, gate=gate, post_weight=post_weight, pre_weight=pre_weight, x_out=x_out,
                 n_out=n_out)
-    with on_device(x):
-        if y is None:
-            x_new, xo = x, None
+    x_new, ld_xo = x, 0
+    if y is not None:
+        if x_out is None:
+            x_out, ld_xo = x.new_empty((T, M)), M
         else:
-            if x_out is None:
-                x_out = torch.empty((T, M), dtype=x.dtype, device=x.device)
-            elif x_out.shape != x.shape or x_out.dtype != x.dtype:
+            if x_out.shape != x.shape or x_out.dtype != x.dtype:
                 raise invalid("x_out differs from x in shape or dtype")
-            c.ld_x_out = row_stride(x_out, "x_out")
-            x_new, xo = x_out, x_out.data_ptr()
-        if pre:
-            if n_out is None:
-                n_out = torch.empty((T, M), dtype=dtype, device=x.device)
-            elif n_out.shape != x.shape:
+            ld_xo = row_stride(x_out, "x_out")
+        x_new = x_out
+    n_type = ld_n = 0
+    if pre:
+        if n_out is None:
+            n_out, ld_n = x.new_empty((T, M), dtype=dtype), M
+        else:
+            if n_out.shape != x.shape:
                 raise invalid("n_out differs from x in shape")
-            c.n_type = dtype_code(n_out.dtype, "n")
-            c.ld_n = row_stride(n_out, "n_out")
-        abi.call("wisp_b200_block_norm", C.byref(c), x.data_ptr(),
-                 None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
-                 None if post_weight is None else post_weight.data_ptr(),
-                 None if pre_weight is None else pre_weight.data_ptr(), xo,
-                 n_out.data_ptr() if pre else None, stream_of(x))
-    return x_new, n_out if pre else None
+            ld_n = row_stride(n_out, "n_out")
+        n_type = dtype_code(n_out.dtype, "n")
+    c = abi.WispBlockNorm(T, M, x_type, y_type, w_type, gate_type, n_type, 1 if post else 0,
+                          gate_kind, residual_scale, eps, weight_offset, ld_x, ld_y, ld_gate,
+                          ld_xo, ld_n)
+    abi.call("wisp_b200_block_norm", C.byref(c), x.data_ptr(), ptr(y), ptr(gate),
+             ptr(post_weight), ptr(pre_weight), ptr(x_out), ptr(n_out), stream_of(x))
+    return x_new, n_out
