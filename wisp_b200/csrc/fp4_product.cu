@@ -24,12 +24,14 @@ namespace {
 
 using namespace wb;
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 416;
 constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
+constexpr int kSchedWarp = 12;
 constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
 constexpr int kMaxStages = 8;
-constexpr int kRingBytes = 220 * 1024;
+constexpr int kRingBytes = 218 * 1024;
+constexpr int kTileRing = 8;
 
 template <bool NV, bool SWIGLU>
 struct Shape {
@@ -42,13 +44,12 @@ struct Shape {
   static constexpr int kSfCols = kWords * (4 * kMats + 8);
   static_assert(2 * kMaxN + 2 * kSfCols <= 512, "tensor memory");
   static constexpr int kSfaBytes = kWords * 512;
-  static constexpr int kSfbBytes = kWords * 2 * 512;
-  // A stage: weights (gate, up), their scales, the row scales, then as many
-  // 32-row boxes of row codes as the launch's largest tile has.
+  // A stage: weights (gate, up), their scales, the row scales (a 512-byte
+  // tile per word and 128 rows), then as many 32-row boxes of row codes as
+  // the launch's largest tile has.
   static constexpr int kOffSfa = kMats * kABytes;
   static constexpr int kOffSfb = kOffSfa + kMats * kSfaBytes;
-  static constexpr int kOffB = kOffSfb + kSfbBytes;
-  static_assert(kOffB % 1024 == 0, "128-byte swizzle atoms");
+  static_assert((kOffSfb + kWords * 512) % 1024 == 0, "128-byte swizzle atoms");
 };
 
 struct Bars {
@@ -56,9 +57,12 @@ struct Bars {
   uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
+  uint64_t tile_full[kTileRing];
+  uint64_t tile_empty[kTileRing];
+  int4 tile[kTileRing];     // expert (-1: no more), first row, rows, feature tile
   uint32_t tmem;
   int abort;
-  int n_tiles;
+  int n_tiles, n_single, n_used;   // token tiles, of them single, segments with rows
   int max_cnt;
 };
 
@@ -123,6 +127,7 @@ WB_DEV uint64_t scale_desc(uint32_t saddr) {
 
 struct Tile {
   int expert, row0, cnt;   // rows row0 .. row0 + cnt - 1
+  int ft;                  // features 128 ft ..
 };
 
 // Rows per tile of a segment: as many tiles as kMaxN demands, of equal size
@@ -148,10 +153,20 @@ WB_DEV bool segment_ok(const Params& p, const WispSegment& v) {
          (v.rows == 0 || (v.expert >= 0 && v.expert < p.V));
 }
 
-// pref[s] = token tiles of the segments before s.
+// The order of the work: token tiles tt of the segments in `order` (those of a
+// single tile first, then the others), pref[i] tiles before the i-th; each has
+// ftiles items. A single tile's weights come from memory while the tiles after
+// the first of a larger segment find theirs in the L2 cache, so the items of
+// the two kinds are dealt out evenly over the launch, each kind in its order.
 template <int MAXN>
-WB_DEV Tile find_tile(const Params& p, const int* pref, int nseg, int tt) {
-  int lo = 0, hi = nseg;       // the last s with pref[s] <= tt
+WB_DEV Tile find_tile(const Params& p, const int* pref, const uint16_t* order, int nseg, int n_tiles,
+                      int n_single, int it) {
+  const int items = n_tiles * p.ftiles, single = n_single * p.ftiles;
+  const int before = (int)((int64_t)it * single / items);     // singles among the items before
+  const int after = (int)((int64_t)(it + 1) * single / items);
+  const int i = after > before ? before : single + it - before;
+  const int tt = i / p.ftiles;
+  int lo = 0, hi = nseg;       // the last entry with pref <= tt
   while (hi - lo > 1) {
     const int m = (lo + hi) >> 1;
     if (pref[m] <= tt)
@@ -159,13 +174,14 @@ WB_DEV Tile find_tile(const Params& p, const int* pref, int nseg, int tt) {
     else
       hi = m;
   }
-  const WispSegment v = segment(p, lo);
+  const WispSegment v = segment(p, order[lo]);
   const int per = tile_rows<MAXN>(v.rows);
   const int r0 = (tt - pref[lo]) * per;
   Tile t;
   t.expert = v.expert;
   t.row0 = v.row_begin + r0;
   t.cnt = min(per, v.rows - r0);
+  t.ft = i - tt * p.ftiles;
   return t;
 }
 
@@ -236,6 +252,30 @@ WB_DEV void store_tile(const Params& p, const Tile& t, uint32_t d, uint32_t du, 
   }
 }
 
+// A role's walk through the tiles that the scheduler warp puts into the ring.
+struct Tiles {
+  int s = 0;
+  uint32_t ph = 0;
+  // Every lane gets the tile; false: no more, or the wait was given up.
+  WB_DEV bool next(Bars& bars, Tile& t, volatile int* abort) {
+    const bool ok = mbar_wait(&bars.tile_full[s], ph, abort);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    const int4 v = bars.tile[s];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars.tile_empty[s]);
+    if (++s == kTileRing) {
+      s = 0;
+      ph ^= 1;
+    }
+    t.expert = __shfl_sync(0xffffffffu, v.x, 0);
+    t.row0 = __shfl_sync(0xffffffffu, v.y, 0);
+    t.cnt = __shfl_sync(0xffffffffu, v.z, 0);
+    t.ft = __shfl_sync(0xffffffffu, v.w, 0);
+    return t.expert >= 0;
+  }
+};
+constexpr int kTileReaders = 12;   // producer, MMA, two scale, eight epilogue warps
+
 template <bool NV, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
@@ -244,7 +284,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
   __shared__ int pref[kMaxSegs + 1];
-  __shared__ int warp_tot[kThreads / 32];
+  __shared__ uint16_t order[kMaxSegs];
+  __shared__ int4 warp_tot[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   volatile int* abort = &bars.abort;
@@ -258,15 +299,22 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       mbar_init(&bars.acc_full[i], 1);
       mbar_init(&bars.acc_empty[i], 8);
     }
+    for (int i = 0; i < kTileRing; i++) {
+      mbar_init(&bars.tile_full[i], 1);
+      mbar_init(&bars.tile_empty[i], kTileReaders);
+    }
     bars.abort = 0;
     bars.max_cnt = 0;
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(&bars.tmem, 512);
-  // Token tiles before each segment: 3 segments per thread, then one scan.
+  // Token tiles of each segment, segments of one tile ordered before the
+  // others: 3 segments per thread, then one scan of (single segments, other
+  // segments, tiles of the others).
   const int nseg = p.segs ? p.nseg : 1;
   {
-    int n[3], sum = 0, most = 0;
+    int n[3], most = 0;
+    int3 sum = make_int3(0, 0, 0);
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < 3; j++) {
@@ -282,38 +330,70 @@ fp4_product_kernel(const __grid_constant__ Params p) {
           most = max(most, min(per, v.rows));
         }
       }
-      sum += n[j];
+      sum.x += n[j] == 1;
+      sum.y += n[j] > 1;
+      sum.z += n[j] > 1 ? n[j] : 0;
     }
-    int x = sum;
+    int3 x = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const int y0 = __shfl_up_sync(0xffffffffu, x.x, o);
+      const int y1 = __shfl_up_sync(0xffffffffu, x.y, o);
+      const int y2 = __shfl_up_sync(0xffffffffu, x.z, o);
+      if (lane >= o) {
+        x.x += y0;
+        x.y += y1;
+        x.z += y2;
+      }
     }
-    if (lane == 31) warp_tot[warp] = x;
+    if (lane == 31) warp_tot[warp] = make_int4(x.x, x.y, x.z, 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (most > 0) atomicMax(&bars.max_cnt, most);
-    int base = x - sum;
-    for (int w = 0; w < warp; w++) base += warp_tot[w];
+    int3 base = make_int3(x.x - sum.x, x.y - sum.y, x.z - sum.z);
+    int3 tot = make_int3(0, 0, 0);
+    for (int w = 0; w < kThreads / 32; w++) {
+      const int4 t = warp_tot[w];
+      if (w < warp) {
+        base.x += t.x;
+        base.y += t.y;
+        base.z += t.z;
+      }
+      tot.x += t.x;
+      tot.y += t.y;
+      tot.z += t.z;
+    }
 #pragma unroll
     for (int j = 0; j < 3; j++) {
       const int s = tid * 3 + j;
-      if (s < nseg) pref[s] = base;
-      base += n[j];
+      if (n[j] == 1) {
+        pref[base.x] = base.x;
+        order[base.x++] = (uint16_t)s;
+      } else if (n[j] > 1) {
+        pref[tot.x + base.y] = tot.x + base.z;
+        order[tot.x + base.y++] = (uint16_t)s;
+        base.z += n[j];
+      }
     }
-    if (tid == kThreads - 1) bars.n_tiles = base;
+    if (tid == 0) {
+      bars.n_single = tot.x;
+      bars.n_tiles = tot.x + tot.z;
+      bars.n_used = tot.x + tot.y;
+    }
     if (bad && p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
   }
   __syncthreads();
   const uint32_t tmem = bars.tmem;
-  const int items = bars.n_tiles * p.ftiles;
   const int nk = p.nk;
   // Few rows leave room for more stages in flight, which is what hides the
   // memory's latency when the weights are most of the traffic.
-  const int stage_bytes = C::kOffB + ((bars.max_cnt + 31) >> 5) * 4096;
-  const int S = min(kMaxStages, kRingBytes / max(stage_bytes, 1));
+  const int row_tiles = bars.max_cnt > 128 ? 2 : 1;     // of 128 rows' scales
+  const int off_b = C::kOffSfb + C::kWords * 512 * row_tiles;
+  const int stage_bytes = off_b + ((bars.max_cnt + 31) >> 5) * 4096;
+  const int S = min(kMaxStages, kRingBytes / stage_bytes);
+  Tiles tiles;
+  Tile t;
 
   if (warp == 0) {
     if (elect_sync()) {
@@ -324,11 +404,9 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     __syncwarp();
     Ring r;
     bool first = true, ok = true;
-    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
-      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
-      const int ft = it % p.ftiles;
-      const int wrow = t.expert * p.N + ft * 128;
-      const int64_t sf = ((int64_t)t.expert * p.ftiles + ft) * nk * C::kSfaBytes;
+    while (ok && tiles.next(bars, t, abort)) {
+      const int wrow = t.expert * p.N + t.ft * 128;
+      const int64_t sf = ((int64_t)t.expert * p.ftiles + t.ft) * nk * C::kSfaBytes;
       const uint8_t* sfw = p.sf_w + sf;
       const uint8_t* sfu = p.sf_up + sf;
       const int nb = (t.cnt + 31) >> 5;
@@ -345,7 +423,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
           if (SWIGLU)
             bulk_load(st + C::kOffSfa + C::kSfaBytes, sfu + kk * C::kSfaBytes, C::kSfaBytes, full);
           for (int b = 0; b < nb; b++)
-            tma_load_2d(st + C::kOffB + b * 4096, &p.tm_x, full, kk * 128, t.row0 + b * 32);
+            tma_load_2d(st + off_b + b * 4096, &p.tm_x, full, kk * 128, t.row0 + b * 32);
         }
         __syncwarp();
         r.next(S);
@@ -367,8 +445,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     int uses = 0;       // stages so far, up to 2
     uint32_t buf = 0;
     bool ok = true;
-    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
-      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
+    const int dsb_word = 32 * row_tiles;       // descriptor units of 16 bytes
+    while (ok && tiles.next(bars, t, abort)) {
       const int n = (t.cnt + 15) & ~15;
       const uint32_t idesc = idesc_fp4<NV>(n);
       acc.take(t.cnt);
@@ -394,12 +472,12 @@ fp4_product_kernel(const __grid_constant__ Params p) {
 #pragma unroll
           for (int w = 0; w < C::kMats * C::kWords; w++) tmem_cp_scales(sfa + w * 4, dsa + w * 32);
 #pragma unroll
-          for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8, dsb + w * 64);
+          for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8, dsb + w * dsb_word);
           if (n > 128) {
 #pragma unroll
-            for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8 + 4, dsb + w * 64 + 32);
+            for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8 + 4, dsb + w * dsb_word + 32);
           }
-          const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + C::kOffB);
+          const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + off_b);
 #pragma unroll
           for (int j = 0; j < 4; j++) {          // 64 k (32 bytes) each
             const int w = NV ? j : j >> 1;
@@ -436,15 +514,15 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     // the warp's next stage are on their way while it waits for a slot.
     constexpr int R = C::kMaxN / 32, W = C::kWords;
     struct Pos {
-      int it, kk;
+      int kk;
+      bool more;
       Tile t;
     };
     auto advance = [&](Pos& q, int by) {
       q.kk += by;
-      while (q.it < items && q.kk >= nk) {
+      while (q.more && q.kk >= nk) {
         q.kk -= nk;
-        q.it += gridDim.x;
-        if (q.it < items) q.t = find_tile<C::kMaxN>(p, pref, nseg, q.it / p.ftiles);
+        q.more = tiles.next(bars, q.t, abort);
       }
     };
     auto fetch = [&](const Pos& q, uint32_t (&w)[W][8]) {
@@ -452,7 +530,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       for (int j = 0; j < W; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) w[j][i] = 0;
-      if (q.it >= items) return;
+      if (!q.more) return;
       const int left = p.xs_ld - q.kk * W * 4;
       const uint8_t* src = p.xs + (int64_t)(q.t.row0 + lane) * p.xs_ld + q.kk * W * 4;
 #pragma unroll
@@ -487,8 +565,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       uint4* dst = reinterpret_cast<uint4*>(smem + r.s * stage_bytes + C::kOffSfb) + lane;
 #pragma unroll
       for (int j = 0; j < W; j++) {
-        dst[j * 64] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
-        dst[j * 64 + 32] = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
+        dst[j * 32 * row_tiles] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+        if (row_tiles == 2) dst[j * 64 + 32] = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -499,9 +577,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       return true;
     };
     Pos q;
-    q.it = blockIdx.x;
     q.kk = 0;
-    if (q.it < items) q.t = find_tile<C::kMaxN>(p, pref, nseg, q.it / p.ftiles);
+    q.more = tiles.next(bars, q.t, abort);
     if (warp == 3) {
       advance(q, 1);
       r.next(S);
@@ -509,23 +586,22 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     }
     uint32_t a[W][8], b[W][8];
     fetch(q, a);
-    while (q.it < items) {
+    while (q.more) {
       advance(q, 2);
       fetch(q, b);
-      if (!put(a) || q.it >= items) break;
+      if (!put(a) || !q.more) break;
       advance(q, 2);
       fetch(q, a);
       if (!put(b)) break;
     }
-  } else {
+  } else if (warp < kSchedWarp) {
     // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
     // take alternate groups of 16 rows.
     const int quad = warp & 3, half = (warp - kEpiWarp) >> 2;
     const float tx = p.ts_x ? __ldg(p.ts_x) : 1.f;
     Acc<C::kMaxN, SWIGLU> acc;
-    for (int it = blockIdx.x; it < items; it += gridDim.x) {
-      const Tile t = find_tile<C::kMaxN>(p, pref, nseg, it / p.ftiles);
-      const int f = (it % p.ftiles) * 128 + quad * 32 + lane;
+    while (tiles.next(bars, t, abort)) {
+      const int f = t.ft * 128 + quad * 32 + lane;
       const float ag = tx * (p.ts_w ? __ldg(p.ts_w + t.expert) : 1.f);
       const float au = SWIGLU ? tx * (p.ts_up ? __ldg(p.ts_up + t.expert) : 1.f) : 0.f;
       acc.take(t.cnt);
@@ -548,6 +624,29 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         if (acc.both) mbar_arrive(&bars.acc_empty[1]);
       }
       acc.done();
+    }
+  } else if (lane == 0) {
+    // Scheduler: finding a tile (a search, a segment read from memory, a
+    // division) takes ~1 us, which cost the MMA warp 5 to 24 % of its time.
+    const int items = bars.n_tiles * p.ftiles;
+    int s = 0;
+    uint32_t ph = 0;
+    bool first = true;
+    for (int it = blockIdx.x;; it += gridDim.x) {
+      Tile v;
+      v.expert = -1;
+      v.row0 = v.cnt = v.ft = 0;
+      if (it < items)
+        v = find_tile<C::kMaxN>(p, pref, order, bars.n_used, bars.n_tiles, bars.n_single, it);
+      if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) break;
+      bars.tile[s] = make_int4(v.expert, v.row0, v.cnt, v.ft);
+      mbar_arrive(&bars.tile_full[s]);
+      if (++s == kTileRing) {
+        s = 0;
+        ph ^= 1;
+        first = false;
+      }
+      if (it >= items) break;
     }
   }
   tc_fence_before();
