@@ -193,6 +193,28 @@ WB_DEV void mbar_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// The same with cluster-scope release: what this thread has seen or written
+// before is visible to the thread of the other CTA that waits (with
+// mbar_wait_cluster) for the phase. Costs about as much as a fence.
+WB_DEV void mbar_arrive_remote_release(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
+// Four floats of another CTA's shared memory (or this one's).
+WB_DEV float4 ld_cluster_f4(uint32_t cluster_ptr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_ptr) : "memory");
+  return v;
+}
+
+WB_DEV uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
 // All threads of every CTA of the cluster.
 WB_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"

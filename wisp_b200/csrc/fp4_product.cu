@@ -9,13 +9,23 @@
 // and a column one row: an epilogue warp stores 32 consecutive features of a
 // row at a time, and SwiGLU pairs the gate and up accumulators lane by lane.
 //
+// Two forms. CTA pairs (cta_group::2, M = 256) take two feature tiles of one
+// token tile, and each loads its own weights but only half of the row codes,
+// which halves what the rows cost in L2 traffic, shared memory and power; the
+// even CTA issues all MMAs, the odd CTA's MMA warp only passes on that its
+// stages are full. (At 4096 tokens over 257 experts 3 % faster than single
+// CTAs, at 40 tokens 2 %.) When there are so few tiles that they would leave
+// more than half of the SMs idle, clusters of 2, 4 or 8 single CTAs take one
+// tile each and split K; their partial sums meet in shared memory in the order
+// of K.
+//
 // Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
 // scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 copy the rows'
 // scale bytes into the layout tcgen05.cp spreads over tensor memory, 1 issues
 // the scale copies and MMAs, 4-11 are the epilogue. tcgen05.mma after
 // tcgen05.cp of one thread are ordered; the reverse is not documented, so the
-// scales in tensor memory are double-buffered and a buffer is refilled only
-// when the MMAs of the stage before the last have completed.
+// scales in tensor memory have several buffers, and one is refilled only when
+// the MMAs that read it have completed.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -37,10 +47,10 @@ template <bool NV, bool SWIGLU>
 struct Shape {
   static constexpr int kWords = NV ? 4 : 2;           // 4-scale words per row and stage
   static constexpr int kMats = SWIGLU ? 2 : 1;
-  // Accumulators: two sets (gate and up, or two tiles of one) of kMaxN
-  // columns, beside two buffers of scales, in 512 columns.
+  // Tensor memory: accumulators in two halves of as many columns as the
+  // launch's largest tile has rows (gate and up, or two tiles of one matrix),
+  // then two buffers of scales or more.
   static constexpr int kMaxN = NV ? 192 : 224;
-  static constexpr int kSfA = 2 * kMaxN;              // first scale column
   static constexpr int kSfCols = kWords * (4 * kMats + 8);
   static_assert(2 * kMaxN + 2 * kSfCols <= 512, "tensor memory");
   static constexpr int kSfaBytes = kWords * 512;
@@ -57,6 +67,7 @@ struct Bars {
   uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
+  uint64_t red_full, red_empty;     // partial sums of a cluster's CTAs
   uint64_t tile_full[kTileRing];
   uint64_t tile_empty[kTileRing];
   int4 tile[kTileRing];     // expert (-1: no more), first row, rows, feature tile
@@ -87,35 +98,54 @@ struct alignas(64) Params {
 };
 
 // Instruction descriptor of the block-scaled 4-bit MMAs: A and B e2m1, both
-// K-major, M = 128; scale type bit 23 (0: e4m3, 1: e8m0); the scale bytes
+// K-major, M = 128 (256 for a pair); scale type bit 23 (0: e4m3, 1: e8m0); the scale bytes
 // used within each 32-bit word at bits 29 (A) and 4 (B).
-template <bool NV>
+template <bool NV, bool PAIR>
 WB_DEV uint32_t idesc_fp4(int n) {
   return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((NV ? 0u : 1u) << 23) |
-         ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
 }
 
-template <bool NV>
+#define WB_MMA_FP4(GROUP, KIND)                                                              \
+  asm volatile(                                                                              \
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                        \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" \
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory")
+
+template <bool NV, bool PAIR>
 WB_DEV void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                     uint32_t acc) {
-  if (NV)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], "
-        "[%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
-        : "memory");
+  if constexpr (NV && PAIR)
+    WB_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (NV)
+    WB_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (PAIR)
+    WB_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
   else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
-        "[%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
-        : "memory");
+    WB_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+}
+#undef WB_MMA_FP4
+
+// 32 rows x 16 bytes of shared memory into 4 columns of every warp's lanes (in
+// a pair, each CTA's shared memory into its own tensor memory).
+template <bool PAIR>
+WB_DEV void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
 }
 
-// 32 rows x 16 bytes of shared memory into 4 columns of every warp's lanes.
-WB_DEV void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-               : "memory");
+// Arrive on a barrier (of both CTAs of a pair) when the MMAs and copies issued
+// so far have completed.
+template <bool PAIR>
+WB_DEV void commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    mma_commit_pair(bar);
+  else
+    mma_commit(bar);
 }
 
 // Shared-memory descriptor of a 512-byte scale tile: no swizzle, 8-row groups
@@ -131,11 +161,11 @@ struct Tile {
 };
 
 // Rows per tile of a segment: as many tiles as kMaxN demands, of equal size
-// up to the MMA's granularity of 16.
-template <int MAXN>
+// up to the MMA's granularity UNIT (16; 32 in a pair, 16 rows per CTA).
+template <int MAXN, int UNIT>
 WB_DEV int tile_rows(int rows) {
   const int t = (rows + MAXN - 1) / MAXN;
-  return ((rows + t - 1) / t + 15) & ~15;
+  return ((rows + t - 1) / t + UNIT - 1) / UNIT * UNIT;
 }
 
 WB_DEV WispSegment segment(const Params& p, int s) {
@@ -155,17 +185,17 @@ WB_DEV bool segment_ok(const Params& p, const WispSegment& v) {
 
 // The order of the work: token tiles tt of the segments in `order` (those of a
 // single tile first, then the others), pref[i] tiles before the i-th; each has
-// ftiles items. A single tile's weights come from memory while the tiles after
+// `fitems` items (feature tiles, or pairs of them). A single tile's weights come from memory while the tiles after
 // the first of a larger segment find theirs in the L2 cache, so the items of
 // the two kinds are dealt out evenly over the launch, each kind in its order.
-template <int MAXN>
+template <int MAXN, int UNIT>
 WB_DEV Tile find_tile(const Params& p, const int* pref, const uint16_t* order, int nseg, int n_tiles,
-                      int n_single, int it) {
-  const int items = n_tiles * p.ftiles, single = n_single * p.ftiles;
+                      int n_single, int fitems, int it) {
+  const int items = n_tiles * fitems, single = n_single * fitems;
   const int before = (int)((int64_t)it * single / items);     // singles among the items before
   const int after = (int)((int64_t)(it + 1) * single / items);
   const int i = after > before ? before : single + it - before;
-  const int tt = i / p.ftiles;
+  const int tt = i / fitems;
   int lo = 0, hi = nseg;       // the last entry with pref <= tt
   while (hi - lo > 1) {
     const int m = (lo + hi) >> 1;
@@ -175,13 +205,13 @@ WB_DEV Tile find_tile(const Params& p, const int* pref, const uint16_t* order, i
       hi = m;
   }
   const WispSegment v = segment(p, order[lo]);
-  const int per = tile_rows<MAXN>(v.rows);
+  const int per = tile_rows<MAXN, UNIT>(v.rows);
   const int r0 = (tt - pref[lo]) * per;
   Tile t;
   t.expert = v.expert;
   t.row0 = v.row_begin + r0;
   t.cnt = min(per, v.rows - r0);
-  t.ft = i - tt * p.ftiles;
+  t.ft = i - tt * fitems;
   return t;
 }
 
@@ -197,23 +227,24 @@ struct Ring {
   }
 };
 
-// The accumulators: two halves of kMaxN columns. A tile of one matrix, or a
-// gate/up tile of at most kMaxN / 2 rows (up kMaxN / 2 columns after gate),
-// takes one half, so its epilogue overlaps the next tile's MMAs; a larger
+// The accumulators: two halves of `cols` columns. A tile of one matrix, or a
+// gate/up tile of at most cols / 2 rows (up cols / 2 columns after gate), takes
+// one half, so its epilogue overlaps the next tile's MMAs; a larger
 // gate/up tile takes both (gate, up). MMA and epilogue warps walk the tiles in
 // the same order and so agree on the halves and their phases.
-template <int MAXN, bool SWIGLU>
+template <bool SWIGLU>
 struct Acc {
+  int cols;
   int h = 0;                       // the tile's (first) half
   bool both = false;
   int nxt = 0;
   uint32_t uses0 = 0, uses1 = 0;   // of each half, before this tile
-  WB_DEV void take(int cnt) {
-    both = SWIGLU && cnt > MAXN / 2;
+  WB_DEV void take(int n) {      // n: the MMA's columns
+    both = SWIGLU && n > cols / 2;
     h = both ? 0 : nxt;
   }
   WB_DEV uint32_t uses() const { return h ? uses1 : uses0; }
-  WB_DEV uint32_t up_offset() const { return both ? MAXN : MAXN / 2; }
+  WB_DEV uint32_t up_offset() const { return both ? cols : cols / 2; }
   WB_DEV void done() {
     if (both || h == 0) uses0++;
     if (both || h == 1) uses1++;
@@ -225,9 +256,16 @@ WB_DEV void put_out(float* q, float v) { *q = v; }
 WB_DEV void put_out(__nv_bfloat16* q, float v) { *q = __float2bfloat16_rn(v); }
 WB_DEV void put_out(__half* q, float v) { *q = __float2half_rn(v); }
 
+// silu(g) * u. The quotient is the 2-ulp one; 16-bit outputs take the fast
+// exponential too (its error, about |g| 2^-23 relative, is far below theirs).
+template <typename T>
+WB_DEV float swiglu(float g, float u) {
+  const float e = sizeof(T) == 4 ? expf(-g) : __expf(-g);
+  return __fdividef(g, 1.f + e) * u;
+}
+
 // One warp's part of a tile: its lane's feature f, rows 16 half + 32 i ...
-// The quotient of the sigmoid is the 2-ulp one; everything else is rounded
-// once, and the result once to the output type.
+// Everything is fp32 until the one rounding to the output type.
 template <bool SWIGLU, typename T>
 WB_DEV void store_tile(const Params& p, const Tile& t, uint32_t d, uint32_t du, int half, int f,
                        float ag, float au) {
@@ -241,16 +279,99 @@ WB_DEV void store_tile(const Params& p, const Tile& t, uint32_t d, uint32_t du, 
     const int left = t.cnt - c;
     if (f < p.N) {
       T* q = out;
+      if (left >= 16) {
 #pragma unroll
-      for (int i = 0; i < 16; i++, q += ld) {
-        float v = __uint_as_float(g[i]) * ag;
-        if (SWIGLU) v = __fdividef(v, 1.f + expf(-v)) * (__uint_as_float(u[i]) * au);
-        if (i < left) put_out(q, v);
+        for (int i = 0; i < 16; i++, q += ld) {
+          float v = __uint_as_float(g[i]) * ag;
+          if (SWIGLU) v = swiglu<T>(v, __uint_as_float(u[i]) * au);
+          put_out(q, v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++, q += ld) {
+          if (i < left) {
+            float v = __uint_as_float(g[i]) * ag;
+            if (SWIGLU) v = swiglu<T>(v, __uint_as_float(u[i]) * au);
+            put_out(q, v);
+          }
+        }
       }
     }
     __syncwarp();
   }
 }
+
+// The epilogue of a cluster that splits K. 32 rows at a time, every CTA puts its
+// partial sums into its shared memory, and CTA kp adds those of all, in the
+// order of K, for the rows kp, kp + ks, ... (a warp per row, 4 features per
+// lane).
+template <bool SWIGLU>
+struct Reduce {
+  float* buf;        // [gate, up][32 rows][128 features]
+  Bars* bars;
+  int ks, kp;
+  uint32_t uses = 0;
+
+  WB_DEV void arrive_all(uint64_t* bar) const {
+    __syncwarp();
+    const int j = threadIdx.x & 31;
+    if (j < ks) mbar_arrive_remote_release(cluster_addr(bar, j));
+  }
+
+  // w: 0..7, the warp's place among the epilogue's
+  template <typename T>
+  WB_DEV bool store(const Params& p, const Tile& t, uint32_t d, uint32_t du, int w, float ag,
+                    float au, volatile int* abort) {
+    const int lane = threadIdx.x & 31, half = w >> 2, quad = threadIdx.x >> 5 & 3;
+    for (int c = 0; c < t.cnt; c += 32, uses++) {
+      bool ok = uses == 0 || mbar_wait_cluster(&bars->red_empty, (uses - 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (c + half * 16 < t.cnt) {
+        uint32_t g[16], u[16];
+        tmem_ld16(d + c + half * 16, g);
+        if (SWIGLU) tmem_ld16(du + c + half * 16, u);
+        tmem_wait_ld();
+        float* q = buf + half * 16 * 128 + quad * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          q[i * 128] = __uint_as_float(g[i]);
+          if (SWIGLU) q[(32 + i) * 128] = __uint_as_float(u[i]);
+        }
+      }
+      arrive_all(&bars->red_full);
+      ok = mbar_wait_cluster(&bars->red_full, uses & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      for (int r = kp + ks * w; r < min(32, t.cnt - c); r += ks * 8) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < ks; j++) {
+          const uint32_t a = cluster_addr(buf + r * 128 + lane * 4, j);
+          const float4 y = ld_cluster_f4(a);
+          v[0] += y.x;
+          v[1] += y.y;
+          v[2] += y.z;
+          v[3] += y.w;
+          if (SWIGLU) {
+            const float4 z = ld_cluster_f4(a + 32 * 128 * 4);
+            x[0] += z.x;
+            x[1] += z.y;
+            x[2] += z.z;
+            x[3] += z.w;
+          }
+        }
+        const int f = t.ft * 128 + lane * 4;
+        T* out = static_cast<T*>(p.out) + (int64_t)(t.row0 + c + r) * p.ld + f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float o = v[i] * ag;
+          if (SWIGLU) o = swiglu<T>(o, x[i] * au);
+          if (f + i < p.N) put_out(out + i, o);
+        }
+      }
+      arrive_all(&bars->red_empty);
+    }
+    return true;
+  }
+};
 
 // A role's walk through the tiles that the scheduler warp puts into the ring.
 struct Tiles {
@@ -276,7 +397,7 @@ struct Tiles {
 };
 constexpr int kTileReaders = 12;   // producer, MMA, two scale, eight epilogue warps
 
-template <bool NV, bool SWIGLU>
+template <bool NV, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
   using C = Shape<NV, SWIGLU>;
@@ -289,16 +410,25 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   volatile int* abort = &bars.abort;
+  constexpr int kUnit = PAIR ? 32 : 16;
+  constexpr int kBox = PAIR ? 16 : 32;            // rows per copy of row codes
+  // pair: this CTA's place in it; else the K split: kp of ks
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int ks = PAIR ? 1 : (int)cluster_size(), kp = PAIR ? 0 : (int)cluster_rank();
+  const int fitems = PAIR ? (p.ftiles + 1) / 2 : p.ftiles;
 
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; i++) {
-      mbar_init(&bars.full[i], 2);      // the copies, one scale warp
+      // the copies, one scale warp; in a pair's even CTA also the odd one's word
+      mbar_init(&bars.full[i], PAIR && rank == 0 ? 3 : 2);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.acc_full[i], 1);
-      mbar_init(&bars.acc_empty[i], 8);
+      mbar_init(&bars.acc_empty[i], PAIR ? 16 : 8);
     }
+    mbar_init(&bars.red_full, 8 * ks);
+    mbar_init(&bars.red_empty, 8 * ks);
     for (int i = 0; i < kTileRing; i++) {
       mbar_init(&bars.tile_full[i], 1);
       mbar_init(&bars.tile_empty[i], kTileReaders);
@@ -307,7 +437,12 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     bars.max_cnt = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&bars.tmem, 512);
+  if (warp == 1) {
+    if (PAIR)
+      tmem_alloc_pair(&bars.tmem, 512);
+    else
+      tmem_alloc(&bars.tmem, 512);
+  }
   // Token tiles of each segment, segments of one tile ordered before the
   // others: 3 segments per thread, then one scan of (single segments, other
   // segments, tiles of the others).
@@ -325,7 +460,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         if (!segment_ok(p, v)) {
           bad = true;
         } else if (v.rows > 0) {
-          const int per = tile_rows<C::kMaxN>(v.rows);
+          const int per = tile_rows<C::kMaxN, kUnit>(v.rows);
           n[j] = (v.rows + per - 1) / per;
           most = max(most, min(per, v.rows));
         }
@@ -383,15 +518,21 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     }
     if (bad && p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
   }
-  __syncthreads();
+  cluster_sync();      // the other CTAs' barriers are initialised too
   const uint32_t tmem = bars.tmem;
-  const int nk = p.nk;
+  const int k0 = p.nk * kp / ks, k1 = p.nk * (kp + 1) / ks;     // this CTA's stages
   // Few rows leave room for more stages in flight, which is what hides the
   // memory's latency when the weights are most of the traffic.
   const int row_tiles = bars.max_cnt > 128 ? 2 : 1;     // of 128 rows' scales
   const int off_b = C::kOffSfb + C::kWords * 512 * row_tiles;
-  const int stage_bytes = off_b + ((bars.max_cnt + 31) >> 5) * 4096;
-  const int S = min(kMaxStages, kRingBytes / stage_bytes);
+  // a pair's CTA holds half of the tile's rows, in boxes of 16
+  const int stage_bytes = off_b + ((bars.max_cnt + 31) >> 5) * (PAIR ? 2048 : 4096);
+  constexpr int kRedBytes = C::kMats * 32 * 128 * 4;     // partial sums of 32 rows
+  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
+  // columns of an accumulator half (two sets of the largest tile's, where a
+  // half can hold gate and up), buffers of scales
+  const int cols = min(max((bars.max_cnt + 31) & ~31, 32) * C::kMats, C::kMaxN);
+  const int sf_bufs = min(S, (512 - 2 * cols) / C::kSfCols);
   Tiles tiles;
   Tile t;
 
@@ -406,12 +547,15 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     bool first = true, ok = true;
     while (ok && tiles.next(bars, t, abort)) {
       const int wrow = t.expert * p.N + t.ft * 128;
-      const int64_t sf = ((int64_t)t.expert * p.ftiles + t.ft) * nk * C::kSfaBytes;
+      // (an odd number of feature tiles leaves a pair's second without one)
+      const int64_t sf =
+          ((int64_t)t.expert * p.ftiles + min(t.ft, p.ftiles - 1)) * p.nk * C::kSfaBytes;
       const uint8_t* sfw = p.sf_w + sf;
       const uint8_t* sfu = p.sf_up + sf;
-      const int nb = (t.cnt + 31) >> 5;
-      const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * 4096;
-      for (int kk = 0; kk < nk; kk++) {
+      const int nb = (t.cnt + 31) >> 5;           // (in a pair: half of the rows each)
+      const int xrow = t.row0 + rank * nb * 16;
+      const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * kBox * 128;
+      for (int kk = k0; kk < k1; kk++) {
         if (!first && !mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort)) { ok = false; break; }
         uint8_t* st = smem + r.s * stage_bytes;
         uint64_t* full = &bars.full[r.s];
@@ -423,7 +567,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
           if (SWIGLU)
             bulk_load(st + C::kOffSfa + C::kSfaBytes, sfu + kk * C::kSfaBytes, C::kSfaBytes, full);
           for (int b = 0; b < nb; b++)
-            tma_load_2d(st + off_b + b * 4096, &p.tm_x, full, kk * 128, t.row0 + b * 32);
+            tma_load_2d(st + off_b + b * kBox * 128, &p.tm_x, full, kk * 128, xrow + b * kBox);
         }
         __syncwarp();
         r.next(S);
@@ -439,43 +583,60 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         mbar_wait(&bars.full[s], wrapped ? r.ph ^ 1 : r.ph, abort, 20000000LL);
       }
     }
+  } else if (warp == 1 && rank == 1) {
+    Ring r;
+    bool ok = true;
+    while (ok && tiles.next(bars, t, abort)) {
+      for (int kk = k0; kk < k1; kk++) {
+        if (!mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        if (lane == 0) mbar_arrive_remote(cluster_addr(&bars.full[r.s], 0));
+        __syncwarp();
+        r.next(S);
+      }
+    }
   } else if (warp == 1) {
     Ring r;
-    Acc<C::kMaxN, SWIGLU> acc;
-    int uses = 0;       // stages so far, up to 2
-    uint32_t buf = 0;
+    Acc<SWIGLU> acc;
+    acc.cols = cols;
+    int uses = 0;       // stages so far, up to sf_bufs
+    int buf = 0;
     bool ok = true;
     const int dsb_word = 32 * row_tiles;       // descriptor units of 16 bytes
     while (ok && tiles.next(bars, t, abort)) {
-      const int n = (t.cnt + 15) & ~15;
-      const uint32_t idesc = idesc_fp4<NV>(n);
-      acc.take(t.cnt);
+      const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
+      const uint32_t idesc = idesc_fp4<NV, PAIR>(n);
+      acc.take(n);
       if (acc.uses() && !mbar_wait(&bars.acc_empty[acc.h], (acc.uses() - 1) & 1, abort)) break;
       if (acc.both && acc.uses1 && !mbar_wait(&bars.acc_empty[1], (acc.uses1 - 1) & 1, abort)) break;
       tc_fence_after();
-      const uint32_t d = tmem + acc.h * C::kMaxN, du = d + acc.up_offset();
-      for (int kk = 0; kk < nk; kk++) {
+      const uint32_t d = tmem + acc.h * cols, du = d + acc.up_offset();
+      for (int kk = k0; kk < k1; kk++) {
         if (!mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
-        // the scale buffer's last readers: the MMAs of the stage before the last
-        if (uses >= 2) {
-          const int s2 = r.s >= 2 ? r.s - 2 : r.s - 2 + S;
-          if (!mbar_wait(&bars.empty[s2], r.s >= 2 ? r.ph : r.ph ^ 1, abort)) { ok = false; break; }
-        } else {
+        // The scale buffer's last readers are the MMAs of the stage sf_bufs
+        // before. (With as many buffers as stages they have completed: their
+        // slot has been filled again.)
+        if (uses < sf_bufs) {
           uses++;
+        } else if (sf_bufs < S) {
+          const int s2 = r.s - sf_bufs;
+          if (!mbar_wait(&bars.empty[s2 < 0 ? s2 + S : s2], s2 < 0 ? r.ph ^ 1 : r.ph, abort)) {
+            ok = false;
+            break;
+          }
         }
         tc_fence_after();
         const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
-        const uint32_t sfa = tmem + C::kSfA + buf * C::kSfCols;
+        const uint32_t sfa = tmem + 2 * cols + buf * C::kSfCols;
         const uint32_t sfb = sfa + C::kMats * C::kWords * 4;
         if (elect_sync()) {
           const uint64_t dsa = scale_desc(st + C::kOffSfa), dsb = scale_desc(st + C::kOffSfb);
 #pragma unroll
-          for (int w = 0; w < C::kMats * C::kWords; w++) tmem_cp_scales(sfa + w * 4, dsa + w * 32);
+          for (int w = 0; w < C::kMats * C::kWords; w++) tmem_cp_scales<PAIR>(sfa + w * 4, dsa + w * 32);
 #pragma unroll
-          for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8, dsb + w * dsb_word);
+          for (int w = 0; w < C::kWords; w++) tmem_cp_scales<PAIR>(sfb + w * 8, dsb + w * dsb_word);
           if (n > 128) {
 #pragma unroll
-            for (int w = 0; w < C::kWords; w++) tmem_cp_scales(sfb + w * 8 + 4, dsb + w * dsb_word + 32);
+            for (int w = 0; w < C::kWords; w++) tmem_cp_scales<PAIR>(sfb + w * 8 + 4, dsb + w * dsb_word + 32);
           }
           const uint64_t da = smem_desc_sw128(st), db = smem_desc_sw128(st + off_b);
 #pragma unroll
@@ -483,21 +644,21 @@ fp4_product_kernel(const __grid_constant__ Params p) {
             const int w = NV ? j : j >> 1;
             const uint32_t id = NV ? 0u : (uint32_t)(j & 1) * 2;
             const uint32_t ids = idesc | (id << 29) | (id << 4);
-            const uint32_t add = (kk | j) ? 1u : 0u;
-            mma_fp4<NV>(d, da + j * 2, db + j * 2, ids, sfa + w * 4, sfb + w * 8, add);
+            const uint32_t add = kk > k0 || j ? 1u : 0u;
+            mma_fp4<NV, PAIR>(d, da + j * 2, db + j * 2, ids, sfa + w * 4, sfb + w * 8, add);
             if (SWIGLU)
-              mma_fp4<NV>(du, da + (kABytes >> 4) + j * 2, db + j * 2, ids,
+              mma_fp4<NV, PAIR>(du, da + (kABytes >> 4) + j * 2, db + j * 2, ids,
                           sfa + (C::kWords + w) * 4, sfb + w * 8, add);
           }
-          mma_commit(&bars.empty[r.s]);
-          if (kk == nk - 1) {
-            mma_commit(&bars.acc_full[acc.h]);
-            if (acc.both) mma_commit(&bars.acc_full[1]);
+          commit<PAIR>(&bars.empty[r.s]);
+          if (kk == k1 - 1) {
+            commit<PAIR>(&bars.acc_full[acc.h]);
+            if (acc.both) commit<PAIR>(&bars.acc_full[1]);
           }
         }
         __syncwarp();
         r.next(S);
-        buf ^= 1;
+        if (++buf == sf_bufs) buf = 0;
       }
       acc.done();
     }
@@ -520,8 +681,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     };
     auto advance = [&](Pos& q, int by) {
       q.kk += by;
-      while (q.more && q.kk >= nk) {
-        q.kk -= nk;
+      while (q.more && q.kk >= k1) {
+        q.kk -= k1 - k0;
         q.more = tiles.next(bars, q.t, abort);
       }
     };
@@ -550,9 +711,21 @@ fp4_product_kernel(const __grid_constant__ Params p) {
               w[1][i] = v.y;
             }
           } else {
+// rows that start anywhere: aligned words around the bytes, none
+            // of them without a byte of the row, shifted into place; bytes
+            // past the row are 0
+            const int nb = min(left, W * 4);
+            const uint32_t* a = reinterpret_cast<const uint32_t*>((uintptr_t)g & ~(uintptr_t)3);
+            const int off = (int)((uintptr_t)g & 3);
+            uint32_t v[W + 1];
 #pragma unroll
-            for (int b = 0; b < W * 4; b++)
-              if (b < left) w[b >> 2][i] |= (uint32_t)__ldg(g + b) << (8 * (b & 3));
+            for (int j = 0; j <= W; j++) v[j] = 4 * j < off + nb ? __ldg(a + j) : 0u;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+              const uint32_t x = __funnelshift_r(v[j], v[j + 1], 8 * off);
+              const int valid = nb - 4 * j;
+              w[j][i] = valid >= 4 ? x : valid > 0 ? x & ((1u << (8 * valid)) - 1u) : 0u;
+            }
           }
         }
       }
@@ -577,7 +750,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       return true;
     };
     Pos q;
-    q.kk = 0;
+    q.kk = k0;
     q.more = tiles.next(bars, q.t, abort);
     if (warp == 3) {
       advance(q, 1);
@@ -598,46 +771,71 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
     // take alternate groups of 16 rows.
     const int quad = warp & 3, half = (warp - kEpiWarp) >> 2;
+    Reduce<SWIGLU> red;
+    red.buf = reinterpret_cast<float*>(smem + kRingBytes - kRedBytes);
+    red.bars = &bars;
+    red.ks = ks;
+    red.kp = kp;
     const float tx = p.ts_x ? __ldg(p.ts_x) : 1.f;
-    Acc<C::kMaxN, SWIGLU> acc;
+    Acc<SWIGLU> acc;
+    acc.cols = cols;
     while (tiles.next(bars, t, abort)) {
+      const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
       const int f = t.ft * 128 + quad * 32 + lane;
       const float ag = tx * (p.ts_w ? __ldg(p.ts_w + t.expert) : 1.f);
       const float au = SWIGLU ? tx * (p.ts_up ? __ldg(p.ts_up + t.expert) : 1.f) : 0.f;
-      acc.take(t.cnt);
+      acc.take(n);
       bool ok = mbar_wait(&bars.acc_full[acc.h], acc.uses() & 1, abort);
       if (acc.both) ok = ok && mbar_wait(&bars.acc_full[1], acc.uses1 & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const uint32_t d = tmem + acc.h * C::kMaxN + ((uint32_t)(quad * 32) << 16);
+      const uint32_t d = tmem + acc.h * cols + ((uint32_t)(quad * 32) << 16);
       const uint32_t du = d + acc.up_offset();
-      if (p.out_type == WISP_DT_F32)
+      if (!PAIR && ks > 1) {
+        if (p.out_type == WISP_DT_F32)
+          ok = red.template store<float>(p, t, d, du, warp - kEpiWarp, ag, au, abort);
+        else if (p.out_type == WISP_DT_BF16)
+          ok = red.template store<__nv_bfloat16>(p, t, d, du, warp - kEpiWarp, ag, au, abort);
+        else
+          ok = red.template store<__half>(p, t, d, du, warp - kEpiWarp, ag, au, abort);
+        if (!ok) break;
+      } else if (p.out_type == WISP_DT_F32) {
         store_tile<SWIGLU, float>(p, t, d, du, half, f, ag, au);
-      else if (p.out_type == WISP_DT_BF16)
+      } else if (p.out_type == WISP_DT_BF16) {
         store_tile<SWIGLU, __nv_bfloat16>(p, t, d, du, half, f, ag, au);
-      else
+      } else {
         store_tile<SWIGLU, __half>(p, t, d, du, half, f, ag, au);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&bars.acc_empty[acc.h]);
-        if (acc.both) mbar_arrive(&bars.acc_empty[1]);
+        if (PAIR) {
+          mbar_arrive_remote(cluster_addr(&bars.acc_empty[acc.h], 0));
+          if (acc.both) mbar_arrive_remote(cluster_addr(&bars.acc_empty[1], 0));
+        } else {
+          mbar_arrive(&bars.acc_empty[acc.h]);
+          if (acc.both) mbar_arrive(&bars.acc_empty[1]);
+        }
       }
       acc.done();
     }
   } else if (lane == 0) {
     // Scheduler: finding a tile (a search, a segment read from memory, a
     // division) takes ~1 us, which cost the MMA warp 5 to 24 % of its time.
-    const int items = bars.n_tiles * p.ftiles;
+    const int items = bars.n_tiles * fitems;
     int s = 0;
     uint32_t ph = 0;
     bool first = true;
-    for (int it = blockIdx.x;; it += gridDim.x) {
+    const int group = PAIR ? 2 : ks;       // CTAs that share a tile
+    for (int it = blockIdx.x / group;; it += gridDim.x / group) {
       Tile v;
       v.expert = -1;
       v.row0 = v.cnt = v.ft = 0;
-      if (it < items)
-        v = find_tile<C::kMaxN>(p, pref, order, bars.n_used, bars.n_tiles, bars.n_single, it);
+      if (it < items) {
+        v = find_tile<C::kMaxN, kUnit>(p, pref, order, bars.n_used, bars.n_tiles, bars.n_single,
+                                       fitems, it);
+        if (PAIR) v.ft = 2 * v.ft + rank;
+      }
       if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) break;
       bars.tile[s] = make_int4(v.expert, v.row0, v.cnt, v.ft);
       mbar_arrive(&bars.tile_full[s]);
@@ -649,12 +847,18 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       if (it >= items) break;
     }
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();      // no CTA's memory goes away while another uses it
   tc_fence_after();
   if (warp == 1) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, 512);
+    if (PAIR) {
+      tmem_relinquish_pair();
+      tmem_dealloc_pair(tmem, 512);
+    } else {
+      tmem_relinquish();
+      tmem_dealloc(tmem, 512);
+    }
   }
   if (tid == 0 && bars.abort && p.error_flag) atomicMax(p.error_flag, 1);
 }
@@ -673,19 +877,36 @@ bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool NV, bool SWIGLU>
-WispError launch_product(const Params& p, int64_t max_items, cudaStream_t stream,
+// grid CTAs in clusters of `cluster`.
+template <bool NV, bool SWIGLU, bool PAIR>
+WispError launch_product(const Params& p, unsigned grid, int cluster, cudaStream_t stream,
                          WispErrCtx* err) {
   const int smem = kRingBytes + 1024;
-  auto kernel = fp4_product_kernel<NV, SWIGLU>;
-  int dev = 0, sms = 0;
-  WB_CUDA_CHECK(cudaGetDevice(&dev));
-  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  auto kernel = fp4_product_kernel<NV, SWIGLU, PAIR>;
   WB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int grid = (int)(max_items < sms ? max_items : sms);
-  wb::launch_k(kernel, grid, kThreads, smem, stream, p);
-  WB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  WB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
   return WISP_OK;
+}
+
+template <bool PAIR>
+WispError launch_product(bool nv, bool swiglu, const Params& p, unsigned grid, int cluster,
+                         cudaStream_t stream, WispErrCtx* err) {
+  if (nv)
+    return swiglu ? launch_product<true, true, PAIR>(p, grid, cluster, stream, err)
+                  : launch_product<true, false, PAIR>(p, grid, cluster, stream, err);
+  return swiglu ? launch_product<false, true, PAIR>(p, grid, cluster, stream, err)
+                : launch_product<false, false, PAIR>(p, grid, cluster, stream, err);
 }
 
 WispError check_mats(const WispFp4Mats* m, const char* what, WispErrCtx* err) {
@@ -725,12 +946,25 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
     return WB_FAIL(WISP_ERR_INVALID_ARG,
                    "fp4_product: row codes must be 16-byte aligned, out to its type");
   const bool nv = cfg->format == WISP_FP4_NV;
+  int dev = 0, sms = 0;
+  WB_CUDA_CHECK(cudaGetDevice(&dev));
+  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  // Token tiles, an upper bound: at most one per row, and per segment one more
+  // than its rows fill.
+  const int64_t most = d_segs ? (int64_t)x->rows / 96 + n_segs : ((int64_t)x->rows + 95) / 96;
+  const int64_t tiles = most < x->rows ? most : x->rows;
+  const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 255) / 256;
+  // Pairs, unless all tiles together could use less than half of the SMs:
+  // then a tile's K over 2, 4 or 8 CTAs.
+  const bool pair = tiles * ftiles * 2 > sms || nk < 2;
+  int split = 2;
+  while (split < 8 && tiles * ftiles * split * 2 <= sms && split * 2 <= nk) split *= 2;
   Params p;
   memset(&p, 0, sizeof p);
   const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
   if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
       (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
-      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, 32))
+      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, pair ? 16 : 32))
     return WB_FAIL(WISP_ERR_CUDA, "fp4_product: cuTensorMapEncodeTiled failed");
   p.sf_w = static_cast<const uint8_t*>(w->prepared);
   p.ts_w = w->tensor_scale;
@@ -748,19 +982,17 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   p.nseg = n_segs;
   p.V = cfg->n_entries;
   p.N = cfg->n;
-  p.nk = (cfg->k + 255) / 256;
-  p.ftiles = (cfg->n + 127) / 128;
+  p.nk = nk;
+  p.ftiles = ftiles;
   p.out = d_out;
   p.ld = ld;
   p.out_type = cfg->out_type;
   p.error_flag = d_error_flag;
-  // at most one token tile per row, and per segment one more than its rows fill
-  const int64_t tiles = d_segs ? (int64_t)x->rows / 192 + n_segs + x->rows / 192
-                               : ((int64_t)x->rows + 15) / 16;
-  const int64_t items = (tiles < x->rows ? tiles : x->rows) * p.ftiles;
-  if (nv)
-    return cfg->swiglu ? launch_product<true, true>(p, items, stream, err)
-                       : launch_product<true, false>(p, items, stream, err);
-  return cfg->swiglu ? launch_product<false, true>(p, items, stream, err)
-                     : launch_product<false, false>(p, items, stream, err);
+  if (pair) {
+    const int64_t want = tiles * ((p.ftiles + 1) / 2) * 2;
+    return launch_product<true>(nv, cfg->swiglu, p, (unsigned)(want < (sms & ~1) ? want : sms & ~1),
+                                2, stream, err);
+  }
+  return launch_product<false>(nv, cfg->swiglu, p, (unsigned)(tiles * ftiles * split), split, stream,
+                               err);
 }
