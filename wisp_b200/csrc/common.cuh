@@ -215,6 +215,11 @@ WB_DEV uint32_t cluster_size() {
   return r;
 }
 
+// The two halves of a cluster barrier: a thread that has arrived must wait
+// before it arrives again.
+WB_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+WB_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // All threads of every CTA of the cluster.
 WB_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"

@@ -26,6 +26,7 @@
 // tcgen05.cp of one thread are ordered; the reverse is not documented, so the
 // scales in tensor memory have several buffers, and one is refilled only when
 // the MMAs that read it have completed.
+#include <cstdlib>
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -41,7 +42,7 @@ constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 218 * 1024;
-constexpr int kTileRing = 8;
+constexpr int kTileRing = kMaxStages;
 
 template <bool NV, bool SWIGLU>
 struct Shape {
@@ -73,8 +74,6 @@ struct Bars {
   int4 tile[kTileRing];     // expert (-1: no more), first row, rows, feature tile
   uint32_t tmem;
   int abort;
-  int n_tiles, n_single, n_used;   // token tiles, of them single, segments with rows
-  int max_cnt;
 };
 
 struct alignas(64) Params {
@@ -164,8 +163,12 @@ struct Tile {
 // up to the MMA's granularity UNIT (16; 32 in a pair, 16 rows per CTA).
 template <int MAXN, int UNIT>
 WB_DEV int tile_rows(int rows) {
-  const int t = (rows + MAXN - 1) / MAXN;
-  return ((rows + t - 1) / t + UNIT - 1) / UNIT * UNIT;
+  int per = rows;
+  if (rows > MAXN) {
+    const int t = (rows + MAXN - 1) / MAXN;
+    per = (rows + t - 1) / t;
+  }
+  return (per + UNIT - 1) & ~(UNIT - 1);
 }
 
 WB_DEV WispSegment segment(const Params& p, int s) {
@@ -183,35 +186,55 @@ WB_DEV bool segment_ok(const Params& p, const WispSegment& v) {
          (v.rows == 0 || (v.expert >= 0 && v.expert < p.V));
 }
 
-// The order of the work: token tiles tt of the segments in `order` (those of a
-// single tile first, then the others), pref[i] tiles before the i-th; each has
-// `fitems` items (feature tiles, or pairs of them). A single tile's weights come from memory while the tiles after
-// the first of a larger segment find theirs in the L2 cache, so the items of
-// the two kinds are dealt out evenly over the launch, each kind in its order.
+// The work: each token tile has `fitems` items (feature tiles, or pairs of
+// them). Segments of one token tile and those of several are listed apart, in
+// order (the second list from the end of the arrays); pref holds the tiles
+// before a segment within its list. A single tile's weights come from memory
+// while the tiles after the first of a larger segment find theirs in the L2
+// cache, so the items of the two lists are dealt out evenly over the launch,
+// each list in its order.
+struct Plan {
+  const int* pref;
+  const uint16_t* order;
+  int singles, multis, multi_tiles;     // segments of one, of several tiles; tiles of these
+  int fitems;
+};
+
 template <int MAXN, int UNIT>
-WB_DEV Tile find_tile(const Params& p, const int* pref, const uint16_t* order, int nseg, int n_tiles,
-                      int n_single, int fitems, int it) {
-  const int items = n_tiles * fitems, single = n_single * fitems;
-  const int before = (int)((int64_t)it * single / items);     // singles among the items before
-  const int after = (int)((int64_t)(it + 1) * single / items);
-  const int i = after > before ? before : single + it - before;
-  const int tt = i / fitems;
-  int lo = 0, hi = nseg;       // the last entry with pref <= tt
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (pref[m] <= tt)
-      lo = m;
-    else
-      hi = m;
+__device__ __noinline__ Tile find_tile(const Params& p, const Plan& q, int it) {
+  const int fitems = q.fitems, single = q.singles * fitems;
+  const int items = single + q.multi_tiles * fitems;
+  int i = it;
+  bool one = q.multi_tiles == 0;
+  if (q.multi_tiles > 0 && single > 0) {
+    const int before = (int)((int64_t)it * single / items);     // singles among the items before
+    const int after = (int)((int64_t)(it + 1) * single / items);
+    one = after > before;
+    i = one ? before : it - before;
   }
-  const WispSegment v = segment(p, order[lo]);
-  const int per = tile_rows<MAXN, UNIT>(v.rows);
-  const int r0 = (tt - pref[lo]) * per;
+  int tt = i / fitems;
   Tile t;
-  t.expert = v.expert;
-  t.row0 = v.row_begin + r0;
-  t.cnt = min(per, v.rows - r0);
   t.ft = i - tt * fitems;
+  int at = tt;                  // its place in the list
+  if (!one) {
+    int lo = 0, hi = q.multis;       // the last segment with pref <= tt
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (q.pref[kMaxSegs - 1 - m] <= tt)
+        lo = m;
+      else
+        hi = m;
+    }
+    at = kMaxSegs - 1 - lo;
+    tt -= q.pref[at];
+  } else {
+    tt = 0;
+  }
+  const WispSegment v = segment(p, q.order[at]);
+  const int per = tile_rows<MAXN, UNIT>(v.rows);
+  t.expert = v.expert;
+  t.row0 = v.row_begin + tt * per;
+  t.cnt = min(per, v.rows - tt * per);
   return t;
 }
 
@@ -404,7 +427,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
-  __shared__ int pref[kMaxSegs + 1];
+  __shared__ int pref[kMaxSegs];
   __shared__ uint16_t order[kMaxSegs];
   __shared__ int4 warp_tot[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -417,24 +440,30 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   const int ks = PAIR ? 1 : (int)cluster_size(), kp = PAIR ? 0 : (int)cluster_rank();
   const int fitems = PAIR ? (p.ftiles + 1) / 2 : p.ftiles;
 
-  if (tid == 0) {
-    for (int i = 0; i < kMaxStages; i++) {
-      // the copies, one scale warp; in a pair's even CTA also the odd one's word
-      mbar_init(&bars.full[i], PAIR && rank == 0 ? 3 : 2);
-      mbar_init(&bars.empty[i], 1);
+  if (warp == 0 && elect_sync()) {
+    tma_prefetch_desc(&p.tm_w);
+    tma_prefetch_desc(&p.tm_x);
+    if (SWIGLU) tma_prefetch_desc(&p.tm_up);
+  }
+  __syncwarp();
+  // The prologue is most of a single token's time, so its parts overlap: the
+  // barriers are initialised by as many threads, the cluster barrier is waited
+  // for only where another CTA's barriers are used, and the thread that holds
+  // the first tile's segment hands that tile out itself.
+  if (tid < kMaxStages) {
+    // the copies, one scale warp; in a pair's even CTA also the odd one's word
+    mbar_init(&bars.full[tid], PAIR && rank == 0 ? 3 : 2);
+    mbar_init(&bars.empty[tid], 1);
+    mbar_init(&bars.tile_full[tid], 1);
+    mbar_init(&bars.tile_empty[tid], kTileReaders);
+    if (tid < 2) {
+      mbar_init(&bars.acc_full[tid], 1);
+      mbar_init(&bars.acc_empty[tid], PAIR ? 16 : 8);
+    } else if (tid == 2) {
+      mbar_init(&bars.red_full, 8 * ks);
+      mbar_init(&bars.red_empty, 8 * ks);
+      bars.abort = 0;
     }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&bars.acc_full[i], 1);
-      mbar_init(&bars.acc_empty[i], PAIR ? 16 : 8);
-    }
-    mbar_init(&bars.red_full, 8 * ks);
-    mbar_init(&bars.red_empty, 8 * ks);
-    for (int i = 0; i < kTileRing; i++) {
-      mbar_init(&bars.tile_full[i], 1);
-      mbar_init(&bars.tile_empty[i], kTileReaders);
-    }
-    bars.abort = 0;
-    bars.max_cnt = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -443,106 +472,109 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     else
       tmem_alloc(&bars.tmem, 512);
   }
-  // Token tiles of each segment, segments of one tile ordered before the
-  // others: 3 segments per thread, then one scan of (single segments, other
-  // segments, tiles of the others).
+  const int group = PAIR ? 2 : ks;                   // CTAs that share a tile
+  const int it0 = blockIdx.x / group, it_step = gridDim.x / group;
+  // The lists of segments and the largest tile: a scan over (segments of one
+  // tile | segments of several << 16, tiles of these), kThreads segments at a
+  // time. (Loops are not unrolled: this runs once, from cold instructions.)
+  Plan plan;
+  plan.pref = pref;
+  plan.order = order;
+  plan.singles = plan.multis = plan.multi_tiles = 0;
+  plan.fitems = fitems;
+  int max_cnt = 0;
+  bool first_done = false;
   const int nseg = p.segs ? p.nseg : 1;
-  {
-    int n[3], most = 0;
-    int3 sum = make_int3(0, 0, 0);
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < 3; j++) {
-      const int s = tid * 3 + j;
-      n[j] = 0;
-      if (s < nseg) {
-        const WispSegment v = segment(p, s);
-        if (!segment_ok(p, v)) {
-          bad = true;
-        } else if (v.rows > 0) {
-          const int per = tile_rows<C::kMaxN, kUnit>(v.rows);
-          n[j] = (v.rows + per - 1) / per;
-          most = max(most, min(per, v.rows));
-        }
+#pragma unroll 1
+  for (int s0 = 0; s0 < nseg; s0 += kThreads) {
+    WispSegment v;
+    v.rows = 0;
+    int n = 0, per = 0;
+    if (s0 + tid < nseg) {
+      v = segment(p, s0 + tid);
+      if (!segment_ok(p, v)) {
+        if (p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
+      } else if (v.rows > 0) {
+        per = tile_rows<C::kMaxN, kUnit>(v.rows);
+        n = v.rows <= C::kMaxN ? 1 : (v.rows + per - 1) / per;
       }
-      sum.x += n[j] == 1;
-      sum.y += n[j] > 1;
-      sum.z += n[j] > 1 ? n[j] : 0;
     }
-    int3 x = sum;
-#pragma unroll
+    const int most = __reduce_max_sync(0xffffffffu, min(per, v.rows));
+    const int kind = n == 0 ? 0 : n == 1 ? 1 : 1 << 16, many = n > 1 ? n : 0;
+    int x = kind, z = many;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-      const int y0 = __shfl_up_sync(0xffffffffu, x.x, o);
-      const int y1 = __shfl_up_sync(0xffffffffu, x.y, o);
-      const int y2 = __shfl_up_sync(0xffffffffu, x.z, o);
+      const int y0 = __shfl_up_sync(0xffffffffu, x, o), y1 = __shfl_up_sync(0xffffffffu, z, o);
       if (lane >= o) {
-        x.x += y0;
-        x.y += y1;
-        x.z += y2;
+        x += y0;
+        z += y1;
       }
     }
-    if (lane == 31) warp_tot[warp] = make_int4(x.x, x.y, x.z, 0);
+    if (s0 > 0) __syncthreads();          // the last round's totals have been read
+    if (lane == 31) warp_tot[warp] = make_int4(x, z, most, 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (most > 0) atomicMax(&bars.max_cnt, most);
-    int3 base = make_int3(x.x - sum.x, x.y - sum.y, x.z - sum.z);
-    int3 tot = make_int3(0, 0, 0);
-    for (int w = 0; w < kThreads / 32; w++) {
-      const int4 t = warp_tot[w];
-      if (w < warp) {
-        base.x += t.x;
-        base.y += t.y;
-        base.z += t.z;
-      }
-      tot.x += t.x;
-      tot.y += t.y;
-      tot.z += t.z;
-    }
-#pragma unroll
-    for (int j = 0; j < 3; j++) {
-      const int s = tid * 3 + j;
-      if (n[j] == 1) {
-        pref[base.x] = base.x;
-        order[base.x++] = (uint16_t)s;
-      } else if (n[j] > 1) {
-        pref[tot.x + base.y] = tot.x + base.z;
-        order[tot.x + base.y++] = (uint16_t)s;
-        base.z += n[j];
+    if (s0 == 0) cluster_arrive();
+    // every warp scans the warps' totals
+    const int4 w = lane < kThreads / 32 ? warp_tot[lane] : make_int4(0, 0, 0, 0);
+    int wx = w.x, wz = w.y;
+#pragma unroll 1
+    for (int o = 1; o < 16; o <<= 1) {
+      const int y0 = __shfl_up_sync(0xffffffffu, wx, o), y1 = __shfl_up_sync(0xffffffffu, wz, o);
+      if (lane >= o) {
+        wx += y0;
+        wz += y1;
       }
     }
-    if (tid == 0) {
-      bars.n_single = tot.x;
-      bars.n_tiles = tot.x + tot.z;
-      bars.n_used = tot.x + tot.y;
+    max_cnt = max(max_cnt, __reduce_max_sync(0xffffffffu, w.z));
+    const int bx = __shfl_sync(0xffffffffu, wx - w.x, warp) + x - kind;
+    const int bz = __shfl_sync(0xffffffffu, wz - w.y, warp) + z - many;
+    if (n == 1) {
+      const int at = plan.singles + (bx & 0xffff);
+      order[at] = (uint16_t)(s0 + tid);
+    } else if (n > 1) {
+      const int at = kMaxSegs - 1 - (plan.multis + (bx >> 16));
+      order[at] = (uint16_t)(s0 + tid);
+      pref[at] = plan.multi_tiles + bz;
     }
-    if (bad && p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
+    // The first tile, when every segment is one tile and this thread has it.
+    const int tx = __shfl_sync(0xffffffffu, wx, 15);
+    first_done = nseg <= kThreads && tx > 0 && tx < (1 << 16) && it0 < tx * fitems;
+    if (first_done && n == 1) {
+      const int ft = it0 - (bx & 0xffff) * fitems;
+      if (ft >= 0 && ft < fitems) {
+        bars.tile[0] = make_int4(v.expert, v.row_begin, v.rows, PAIR ? 2 * ft + rank : ft);
+        mbar_arrive(&bars.tile_full[0]);
+      }
+    }
+    plan.singles += tx & 0xffff;
+    plan.multis += tx >> 16;
+    plan.multi_tiles += __shfl_sync(0xffffffffu, wz, 15);
   }
-  cluster_sync();      // the other CTAs' barriers are initialised too
+  // the scheduler warp reads pref and order
+  if (warp == kSchedWarp)
+    asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kThreads) : "memory");
+  else
+    asm volatile("barrier.cta.arrive.aligned 1, %0;" ::"n"(kThreads) : "memory");
   const uint32_t tmem = bars.tmem;
   const int k0 = p.nk * kp / ks, k1 = p.nk * (kp + 1) / ks;     // this CTA's stages
   // Few rows leave room for more stages in flight, which is what hides the
   // memory's latency when the weights are most of the traffic.
-  const int row_tiles = bars.max_cnt > 128 ? 2 : 1;     // of 128 rows' scales
+  const int row_tiles = max_cnt > 128 ? 2 : 1;     // of 128 rows' scales
   const int off_b = C::kOffSfb + C::kWords * 512 * row_tiles;
   // a pair's CTA holds half of the tile's rows, in boxes of 16
-  const int stage_bytes = off_b + ((bars.max_cnt + 31) >> 5) * (PAIR ? 2048 : 4096);
+  const int stage_bytes = off_b + ((max_cnt + 31) >> 5) * (PAIR ? 2048 : 4096);
   constexpr int kRedBytes = C::kMats * 32 * 128 * 4;     // partial sums of 32 rows
   const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
   // columns of an accumulator half (two sets of the largest tile's, where a
   // half can hold gate and up), buffers of scales
-  const int cols = min(max((bars.max_cnt + 31) & ~31, 32) * C::kMats, C::kMaxN);
+  const int cols = min(max((max_cnt + 31) & ~31, 32) * C::kMats, C::kMaxN);
   const int sf_bufs = min(S, (512 - 2 * cols) / C::kSfCols);
   Tiles tiles;
   Tile t;
 
   if (warp == 0) {
-    if (elect_sync()) {
-      tma_prefetch_desc(&p.tm_w);
-      tma_prefetch_desc(&p.tm_x);
-      if (SWIGLU) tma_prefetch_desc(&p.tm_up);
-    }
-    __syncwarp();
     Ring r;
     bool first = true, ok = true;
     while (ok && tiles.next(bars, t, abort)) {
@@ -584,6 +616,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       }
     }
   } else if (warp == 1 && rank == 1) {
+    cluster_wait();
     Ring r;
     bool ok = true;
     while (ok && tiles.next(bars, t, abort)) {
@@ -595,6 +628,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       }
     }
   } else if (warp == 1) {
+    cluster_wait();
     Ring r;
     Acc<SWIGLU> acc;
     acc.cols = cols;
@@ -768,6 +802,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       if (!put(b)) break;
     }
   } else if (warp < kSchedWarp) {
+    cluster_wait();
     // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
     // take alternate groups of 16 rows.
     const int quad = warp & 3, half = (warp - kEpiWarp) >> 2;
@@ -822,18 +857,16 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   } else if (lane == 0) {
     // Scheduler: finding a tile (a search, a segment read from memory, a
     // division) takes ~1 us, which cost the MMA warp 5 to 24 % of its time.
-    const int items = bars.n_tiles * fitems;
-    int s = 0;
+    const int items = (plan.singles + plan.multi_tiles) * fitems;
+    int s = first_done ? 1 : 0;
     uint32_t ph = 0;
     bool first = true;
-    const int group = PAIR ? 2 : ks;       // CTAs that share a tile
-    for (int it = blockIdx.x / group;; it += gridDim.x / group) {
+    for (int it = first_done ? it0 + it_step : it0;; it += it_step) {
       Tile v;
       v.expert = -1;
       v.row0 = v.cnt = v.ft = 0;
       if (it < items) {
-        v = find_tile<C::kMaxN, kUnit>(p, pref, order, bars.n_used, bars.n_tiles, bars.n_single,
-                                       fitems, it);
+        v = find_tile<C::kMaxN, kUnit>(p, plan, it);
         if (PAIR) v.ft = 2 * v.ft + rank;
       }
       if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) break;
@@ -848,6 +881,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     }
   }
   __syncwarp();
+  if (warp != 1 && (warp < kEpiWarp || warp == kSchedWarp)) cluster_wait();
   tc_fence_before();
   cluster_sync();      // no CTA's memory goes away while another uses it
   tc_fence_after();
@@ -956,9 +990,10 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 255) / 256;
   // Pairs, unless all tiles together could use less than half of the SMs:
   // then a tile's K over 2, 4 or 8 CTAs.
-  const bool pair = tiles * ftiles * 2 > sms || nk < 2;
+  bool pair = tiles * ftiles * 2 > sms || nk < 2;
   int split = 2;
   while (split < 8 && tiles * ftiles * split * 2 <= sms && split * 2 <= nk) split *= 2;
+  if (const char* e = getenv("WB_SPLIT")) { pair = e[0] == 'p'; split = atoi(e); if (split > nk) split = 1; }
   Params p;
   memset(&p, 0, sizeof p);
   const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
