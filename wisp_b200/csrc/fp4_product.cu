@@ -14,19 +14,17 @@
 // which halves what the rows cost in L2 traffic, shared memory and power; the
 // even CTA issues all MMAs, the odd CTA's MMA warp only passes on that its
 // stages are full. (At 4096 tokens over 257 experts 3 % faster than single
-// CTAs, at 40 tokens 2 %.) When there are so few tiles that they would leave
-// more than half of the SMs idle, clusters of 2, 4 or 8 single CTAs take one
-// tile each and split K; their partial sums meet in shared memory in the order
-// of K.
+// CTAs, at 40 tokens 2 %.) When there are few tiles, clusters of 2 or 4 single
+// CTAs take one tile each and split K; their partial sums meet in shared memory
+// and are added in the order of K.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
-// scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 copy the rows'
+// scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 and 13-14 copy the rows'
 // scale bytes into the layout tcgen05.cp spreads over tensor memory, 1 issues
 // the scale copies and MMAs, 4-11 are the epilogue. tcgen05.mma after
 // tcgen05.cp of one thread are ordered; the reverse is not documented, so the
 // scales in tensor memory have several buffers, and one is refilled only when
 // the MMAs that read it have completed.
-#include <cstdlib>
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -35,9 +33,10 @@ namespace {
 
 using namespace wb;
 
-constexpr int kThreads = 416;
+constexpr int kThreads = 480;
 constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
 constexpr int kSchedWarp = 12;
+constexpr int kScaleWarps = 4;    // warps 2, 3, 13, 14
 constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
 constexpr int kMaxStages = 8;
@@ -418,7 +417,7 @@ struct Tiles {
     return t.expert >= 0;
   }
 };
-constexpr int kTileReaders = 12;   // producer, MMA, two scale, eight epilogue warps
+constexpr int kTileReaders = 10 + kScaleWarps;   // producer, MMA, scale, eight epilogue warps
 
 template <bool NV, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -703,10 +702,13 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         mbar_wait(&bars.empty[s], s < r.s ? r.ph : r.ph ^ 1, abort, 20000000LL);
       }
     }
-  } else if (warp < kEpiWarp) {
-    // Row scales: the two warps take alternate stages. A lane copies rows
-    // lane + 32 i, whose words lie side by side in the layout; the words of
-    // the warp's next stage are on their way while it waits for a slot.
+  } else if (warp < kEpiWarp || warp > kSchedWarp) {
+    // Row scales: the warps take stages in turn. A lane copies rows lane + 32
+    // i, whose words lie side by side in the layout; the words of the warp's
+    // next stage are on their way while it waits for a slot. (A round trip to
+    // L2 every other stage, with two warps, bounded the stages at ~400
+    // cycles.)
+    const int first = warp < kEpiWarp ? warp - 2 : warp - kSchedWarp + 1;
     constexpr int R = C::kMaxN / 32, W = C::kWords;
     struct Pos {
       int kk;
@@ -778,26 +780,24 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.full[r.s]);
-      r.next(S);
-      r.next(S);
-      use = min(use + 2, 1 << 20);
+#pragma unroll
+      for (int i = 0; i < kScaleWarps; i++) r.next(S);
+      use = min(use + kScaleWarps, 1 << 20);
       return true;
     };
     Pos q;
     q.kk = k0;
     q.more = tiles.next(bars, q.t, abort);
-    if (warp == 3) {
-      advance(q, 1);
-      r.next(S);
-      use = 1;
-    }
+    advance(q, first);
+    for (int i = 0; i < first; i++) r.next(S);
+    use = first;
     uint32_t a[W][8], b[W][8];
     fetch(q, a);
     while (q.more) {
-      advance(q, 2);
+      advance(q, kScaleWarps);
       fetch(q, b);
       if (!put(a) || !q.more) break;
-      advance(q, 2);
+      advance(q, kScaleWarps);
       fetch(q, a);
       if (!put(b)) break;
     }
@@ -881,7 +881,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     }
   }
   __syncwarp();
-  if (warp != 1 && (warp < kEpiWarp || warp == kSchedWarp)) cluster_wait();
+  if (warp != 1 && (warp < kEpiWarp || warp >= kSchedWarp)) cluster_wait();
   tc_fence_before();
   cluster_sync();      // no CTA's memory goes away while another uses it
   tc_fence_after();
@@ -988,18 +988,20 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   const int64_t most = d_segs ? (int64_t)x->rows / 96 + n_segs : ((int64_t)x->rows + 95) / 96;
   const int64_t tiles = most < x->rows ? most : x->rows;
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 255) / 256;
-  // Pairs, unless all tiles together could use less than half of the SMs:
-  // then a tile's K over 2, 4 or 8 CTAs.
-  bool pair = tiles * ftiles * 2 > sms || nk < 2;
-  int split = 2;
-  while (split < 8 && tiles * ftiles * split * 2 <= sms && split * 2 <= nk) split *= 2;
-  if (const char* e = getenv("WB_SPLIT")) { pair = e[0] == 'p'; split = atoi(e); if (split > nk) split = 1; }
+  // Pairs, unless all tiles together could use at most 3/8 of the SMs as
+  // single CTAs: then clusters of 4 (2) of these split K, as long as they fill
+  // at most 3/4 of the SMs (GPCs of an odd number of SMs hold fewer clusters)
+  // and have two stages of K each. One row, warm L2, us a call, as pairs / split
+  // by 2 / by 4: 2048 x 7168 11.6 / 10.4 / 8.6, with gate and up 13.1 / 11.9 /
+  // 9.6, 2048 x 2048 7.3 / 7.5 / 7.0, 7168 x 2048 7.6 / 7.8 / 14.0 (two waves).
+  const int64_t items = tiles * ftiles;
+  const int split = nk < 8 ? 1 : items * 16 <= 3 * (int64_t)sms ? 4 : items * 8 <= 3 * (int64_t)sms ? 2 : 1;
   Params p;
   memset(&p, 0, sizeof p);
   const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
   if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
       (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
-      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, pair ? 16 : 32))
+      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, split > 1 ? 32 : 16))
     return WB_FAIL(WISP_ERR_CUDA, "fp4_product: cuTensorMapEncodeTiled failed");
   p.sf_w = static_cast<const uint8_t*>(w->prepared);
   p.ts_w = w->tensor_scale;
@@ -1023,11 +1025,9 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   p.ld = ld;
   p.out_type = cfg->out_type;
   p.error_flag = d_error_flag;
-  if (pair) {
-    const int64_t want = tiles * ((p.ftiles + 1) / 2) * 2;
-    return launch_product<true>(nv, cfg->swiglu, p, (unsigned)(want < (sms & ~1) ? want : sms & ~1),
-                                2, stream, err);
-  }
-  return launch_product<false>(nv, cfg->swiglu, p, (unsigned)(tiles * ftiles * split), split, stream,
-                               err);
+  if (split > 1)
+    return launch_product<false>(nv, cfg->swiglu, p, (unsigned)(items * split), split, stream, err);
+  const int64_t want = tiles * ((ftiles + 1) / 2) * 2;
+  return launch_product<true>(nv, cfg->swiglu, p, (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2,
+                              stream, err);
 }
