@@ -913,11 +913,12 @@ bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box
 
 // grid CTAs in clusters of `cluster`.
 template <bool NV, bool SWIGLU, bool PAIR>
-WispError launch_product(const Params& p, unsigned grid, int cluster, cudaStream_t stream,
+WispError launch_product(const Params& p, int dev, unsigned grid, int cluster, cudaStream_t stream,
                          WispErrCtx* err) {
   const int smem = kRingBytes + 1024;
   auto kernel = fp4_product_kernel<NV, SWIGLU, PAIR>;
-  WB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> raised{0};
+  WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
@@ -934,13 +935,13 @@ WispError launch_product(const Params& p, unsigned grid, int cluster, cudaStream
 }
 
 template <bool PAIR>
-WispError launch_product(bool nv, bool swiglu, const Params& p, unsigned grid, int cluster,
-                         cudaStream_t stream, WispErrCtx* err) {
+WispError launch_product(bool nv, bool swiglu, const Params& p, int dev, unsigned grid,
+                         int cluster, cudaStream_t stream, WispErrCtx* err) {
   if (nv)
-    return swiglu ? launch_product<true, true, PAIR>(p, grid, cluster, stream, err)
-                  : launch_product<true, false, PAIR>(p, grid, cluster, stream, err);
-  return swiglu ? launch_product<false, true, PAIR>(p, grid, cluster, stream, err)
-                : launch_product<false, false, PAIR>(p, grid, cluster, stream, err);
+    return swiglu ? launch_product<true, true, PAIR>(p, dev, grid, cluster, stream, err)
+                  : launch_product<true, false, PAIR>(p, dev, grid, cluster, stream, err);
+  return swiglu ? launch_product<false, true, PAIR>(p, dev, grid, cluster, stream, err)
+                : launch_product<false, false, PAIR>(p, dev, grid, cluster, stream, err);
 }
 
 WispError check_mats(const WispFp4Mats* m, const char* what, WispErrCtx* err) {
@@ -981,8 +982,7 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
                    "fp4_product: row codes must be 16-byte aligned, out to its type");
   const bool nv = cfg->format == WISP_FP4_NV;
   int dev = 0, sms = 0;
-  WB_CUDA_CHECK(cudaGetDevice(&dev));
-  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
   // Token tiles, an upper bound: at most one per row, and per segment one more
   // than its rows fill.
   const int64_t most = d_segs ? (int64_t)x->rows / 96 + n_segs : ((int64_t)x->rows + 95) / 96;
@@ -1026,8 +1026,9 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   p.out_type = cfg->out_type;
   p.error_flag = d_error_flag;
   if (split > 1)
-    return launch_product<false>(nv, cfg->swiglu, p, (unsigned)(items * split), split, stream, err);
+    return launch_product<false>(nv, cfg->swiglu, p, dev, (unsigned)(items * split), split, stream,
+                                 err);
   const int64_t want = tiles * ((ftiles + 1) / 2) * 2;
-  return launch_product<true>(nv, cfg->swiglu, p, (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2,
-                              stream, err);
+  return launch_product<true>(nv, cfg->swiglu, p, dev,
+                              (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2, stream, err);
 }

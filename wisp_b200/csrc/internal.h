@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -71,6 +72,31 @@ using TensorMapEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint
                                        CUtensorMapSwizzle, CUtensorMapL2promotion,
                                        CUtensorMapFloatOOBfill);
 TensorMapEncodeFn tensor_map_encoder();
+
+// SMs of the current device, and a kernel's dynamic shared memory raised to
+// `bytes` (both asked of the driver once per device: a call costs as much as a
+// small kernel's launch).
+inline cudaError_t device_sms(int* dev, int* sms) {
+  static std::atomic<int> known[64];
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return e;
+  const bool keep = *dev >= 0 && *dev < 64;
+  if (keep && (*sms = known[*dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev);
+  if (e == cudaSuccess && keep) known[*dev].store(*sms, std::memory_order_relaxed);
+  return e;
+}
+
+// `raised`: the kernel's own record, one bit per device.
+template <typename K>
+inline cudaError_t raise_smem(K* kernel, int bytes, int dev, std::atomic<uint64_t>& raised) {
+  const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
+  if (raised.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) raised.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Checks shared by the fp4 weight-set entry points (fp4.cu).
 WispError fp4_validate(const WispFp4Config* c, const char* who, WispErrCtx* err);

@@ -343,8 +343,7 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   const int vecs = (c.hidden + 7) / 8, T = c.tokens;
   const int threads1 = (vecs + 31) / 32 * 32, threads4 = ((vecs + 3) / 4 + 31) / 32 * 32;
   int dev = 0, sms = 0;
-  WB_CUDA_CHECK(cudaGetDevice(&dev));
-  WB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
   if (vec && threads1 <= 1024 && T > 2 * sms) {
     RingShape rs;
     rs.x_bytes = c.hidden * dt_size(c.x_type);
@@ -353,8 +352,8 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
     const int ctas = 1024 / threads1 < 8 ? 1024 / threads1 : 8;
     const int budget = 200 * 1024 / ctas, stage = rs.x_bytes + rs.y_bytes;
     rs.stages = budget / stage < kNormStages ? budget / stage : kNormStages;
-    WB_CUDA_CHECK(cudaFuncSetAttribute(block_norm_stream_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    static std::atomic<uint64_t> raised{0};
+    WB_CUDA_CHECK(wb::raise_smem(block_norm_stream_kernel, 200 * 1024, dev, raised));
     const int grid = ctas * sms < T ? ctas * sms : T;
     wb::launch_k(block_norm_stream_kernel, grid, threads1, (size_t)rs.stages * stage, stream, p, rs);
   } else if (threads1 <= 1024) {

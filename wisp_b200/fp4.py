@@ -12,7 +12,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
-from dataclasses import dataclass
 
 import torch
 
@@ -55,9 +54,10 @@ def dtype_code(dtype: torch.dtype, what: str) -> int:
 
 def row_stride(t: torch.Tensor, what: str) -> int:
     """Elements between the rows of a 2D tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise invalid(f"{what}: a 2D tensor with contiguous rows is needed")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def same_device(ref: torch.Tensor, **tensors) -> None:
@@ -89,31 +89,52 @@ def _check_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor) -> int:
     return k
 
 
-@dataclass
 class Fp4Rows:
-    """Quantised rows: codes [R, K/2], scales [R, K/block], one tensor scale (NV)."""
-    fmt: int
-    codes: torch.Tensor
-    scales: torch.Tensor
-    tensor_scale: torch.Tensor | None = None
+    """Quantised rows: codes [rows, cols/2], scales [rows, cols/block], one tensor scale (NV)."""
 
-    def __post_init__(self) -> None:
-        if self.codes.dim() != 2:
+    def __init__(self, fmt: int, codes: torch.Tensor, scales: torch.Tensor,
+                 tensor_scale: torch.Tensor | None = None):
+        if codes.dim() != 2:
             raise invalid("rows are 2D")
-        self.cols = _check_codes(self.fmt, self.codes, self.scales)
-        _check_scale(self.tensor_scale, 1, "tensor_scale")
-        same_device(self.codes, tensor_scale=self.tensor_scale)
-
-    @property
-    def rows(self) -> int:
-        return self.codes.shape[0]
+        self.cols = _check_codes(fmt, codes, scales)
+        _check_scale(tensor_scale, 1, "tensor_scale")
+        same_device(codes, tensor_scale=tensor_scale)
+        self.fmt, self.tensor_scale, self.rows = fmt, tensor_scale, codes.shape[0]
+        self._views = (codes, scales)
+        self._buf = codes
+        self._codes, self._scales = codes.data_ptr(), scales.data_ptr()
+        self._ts = ptr(tensor_scale)
 
     @classmethod
-    def _made(cls, fmt, codes, scales, tensor_scale, cols) -> "Fp4Rows":
-        """Rows whose parts this module allocated itself (nothing left to check)."""
+    def _empty(cls, x: torch.Tensor, fmt: int, rows: int, cols: int,
+               tensor_scale: torch.Tensor | None) -> "Fp4Rows":
+        """Rows to be written, in one allocation on x's device; the codes and scales tensors
+        are made when someone asks for them (they cost more than the launch)."""
         q = cls.__new__(cls)
-        q.fmt, q.codes, q.scales, q.tensor_scale, q.cols = fmt, codes, scales, tensor_scale, cols
+        split = (rows * cols // 2 + 31) & ~31
+        q._buf = buf = x.new_empty(split + rows * cols // BLOCK[fmt], dtype=torch.uint8)
+        q._views = None
+        q._codes = buf.data_ptr()
+        q._scales = q._codes + split
+        q.fmt, q.tensor_scale, q.rows, q.cols = fmt, tensor_scale, rows, cols
+        q._ts = None if tensor_scale is None else tensor_scale.data_ptr()
         return q
+
+    def _split(self) -> tuple[torch.Tensor, torch.Tensor]:
+        if self._views is None:
+            n, m = self.rows * self.cols // 2, self.rows * self.cols // BLOCK[self.fmt]
+            at = self._scales - self._codes
+            self._views = (self._buf[:n].view(self.rows, self.cols // 2),
+                           self._buf[at:at + m].view(self.rows, self.cols // BLOCK[self.fmt]))
+        return self._views
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._split()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._split()[1]
 
 
 def tensor_scale(x: torch.Tensor) -> torch.Tensor:
@@ -134,8 +155,7 @@ def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None
     n, cols = x.shape
     if cols % block or cols == 0:
         raise invalid(f"row length {cols} is no multiple of {block}")
-    nv = fmt == abi.WISP_FP4_NV
-    if nv:
+    if fmt == abi.WISP_FP4_NV:
         if tensor_scale is None:
             raise invalid("NV rows need a tensor scale")
         _check_scale(tensor_scale, 1, "tensor_scale")
@@ -151,26 +171,27 @@ def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None
     if other is not None:
         with other:
             return quantize(x, fmt, tensor_scale, rows)
-    if nv or rows is not None:
+    if tensor_scale is not None or rows is not None:
         same_device(x, tensor_scale=tensor_scale, rows=rows)
-    codes = x.new_empty((r, cols // 2), dtype=torch.uint8)
-    scales = x.new_empty((r, cols // block), dtype=torch.uint8)
-    abi.call("wisp_b200_fp4_quantize", x.data_ptr(), dt, ld, n, ptr(rows), r, cols, fmt,
-             ptr(tensor_scale), codes.data_ptr(), scales.data_ptr(), stream_of(x))
-    return Fp4Rows._made(fmt, codes, scales, tensor_scale, cols)
+    q = Fp4Rows._empty(x, fmt, r, cols, tensor_scale)
+    abi.call("wisp_b200_fp4_quantize", x.data_ptr(), dt, ld, n,
+             None if rows is None else rows.data_ptr(), r, cols, fmt, q._ts, q._codes, q._scales,
+             stream_of(x))
+    return q
 
 
 def dequantize(q: Fp4Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of quantised rows."""
     dt = dtype_code(dtype, "dtype")
-    codes = q.codes
-    other = elsewhere(codes)
+    buf = q._buf
+    other = elsewhere(buf)
     if other is not None:
         with other:
             return dequantize(q, dtype)
-    out = codes.new_empty((q.rows, q.cols), dtype=dtype)
-    abi.call("wisp_b200_fp4_dequantize", codes.data_ptr(), q.scales.data_ptr(), q.rows, q.cols,
-             q.fmt, ptr(q.tensor_scale), out.data_ptr(), dt, q.cols, stream_of(codes))
+    cols = q.cols
+    out = buf.new_empty((q.rows, cols), dtype=dtype)
+    abi.call("wisp_b200_fp4_dequantize", q._codes, q._scales, q.rows, cols, q.fmt, q._ts,
+             out.data_ptr(), dt, cols, stream_of(buf))
     return out
 
 
@@ -219,6 +240,7 @@ class Fp4Weights:
                       for dt, code in DTYPES.items()}
         self._mats = C.byref(self.mats)
         self._up_mats = None if self.up_mats is None else C.byref(self.up_mats)
+        self._error = self.error_word.data_ptr()
 
     @classmethod
     def from_values(cls, fmt: int, w: torch.Tensor, up: torch.Tensor | None = None) -> "Fp4Weights":
@@ -261,25 +283,27 @@ def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
                 not segments.is_contiguous():
             raise invalid("segments: a contiguous int32 [S, 4] tensor")
         n_segs = segments.shape[0]
-    codes = q.codes
-    other = elsewhere(codes)
+    buf = q._buf
+    other = elsewhere(buf)
     if other is not None:
         with other:
             return product(q, w, segments, out, dtype)
-    same_device(codes, weights=w.error_word, segments=segments, out=out)
-    rows = codes.shape[0]
+    same_device(buf, weights=w.error_word, segments=segments, out=out)
+    rows = q.rows
     if out is None:
         dtype_code(dtype, "dtype")
-        out = codes.new_empty((rows, w.n), dtype=dtype)
+        out = buf.new_empty((rows, w.n), dtype=dtype)
         ld = w.n
     else:
         if out.shape != (rows, w.n):
             raise invalid(f"out {tuple(out.shape)}, not {(rows, w.n)}")
-        dtype_code(out.dtype, "out")
+        dtype = out.dtype
+        dtype_code(dtype, "out")
         ld = row_stride(out, "out")
-    x = abi.WispFp4Rows(codes.data_ptr(), q.scales.data_ptr(), ptr(q.tensor_scale), rows)
-    abi.call("wisp_b200_fp4_product", w._cfgs[out.dtype], w._mats, w._up_mats, C.byref(x),
-             ptr(segments), n_segs, out.data_ptr(), ld, w.error_word.data_ptr(), stream_of(codes))
+    x = abi.WispFp4Rows(q._codes, q._scales, q._ts, rows)
+    abi.call("wisp_b200_fp4_product", w._cfgs[dtype], w._mats, w._up_mats, C.byref(x),
+             None if segments is None else segments.data_ptr(), n_segs, out.data_ptr(), ld,
+             w._error, stream_of(buf))
     return out
 
 
