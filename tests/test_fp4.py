@@ -337,6 +337,19 @@ def test_product_more_tiles_than_ctas(fmt):
 
 @pytest.mark.gpu
 @FMTS
+@pytest.mark.parametrize("k", [2080, 4128, 7168])
+def test_product_long_rows_in_short_rings(fmt, k):
+    """Tiles of many rows leave room for few stages of K, so that a warp's next turn at the row
+    scales may lie two rounds of the ring ahead; repeated runs give the same bits."""
+    for swiglu, n, counts in ((True, 1000, [510, 8, 0, 79, 333]), (False, 300, [450]), (True, 64, [190])):
+        q, w, mats, segs, dev, out = _run_product(fmt, swiglu, torch.float32, n, k, counts)
+        for _ in range(10):
+            assert torch.equal(fp4.product(q, w, dev, dtype=torch.float32), out)
+        w.check()
+
+
+@pytest.mark.gpu
+@FMTS
 def test_product_many_segments_same_expert(fmt):
     """1025 segments, experts out of order and repeated."""
     counts = [(i * 7) % 4 for i in range(1025)]

@@ -33,10 +33,8 @@ namespace {
 
 using namespace wb;
 
-constexpr int kThreads = 480;
 constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
-constexpr int kSchedWarp = 12;
-constexpr int kScaleWarps = 4;    // warps 2, 3, 13, 14
+constexpr int kSchedWarp = 12;    // then the scale warps after 2 and 3
 constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
 constexpr int kMaxStages = 8;
@@ -47,6 +45,12 @@ template <bool NV, bool SWIGLU>
 struct Shape {
   static constexpr int kWords = NV ? 4 : 2;           // 4-scale words per row and stage
   static constexpr int kMats = SWIGLU ? 2 : 1;
+  // The row scales' warps take turns at 16 bytes a row; from the last stage
+  // of a warp's turn to the first of its next are kTurn stages at most, and
+  // the ring must hold as many (see there).
+  static constexpr int kUnitStages = 4 / kWords, kScaleWarps = NV ? 3 : 2;
+  static constexpr int kTurn = (kScaleWarps - 1) * kUnitStages + 1;
+  static constexpr int kThreads = 32 * (kSchedWarp + 1 + kScaleWarps - 2);
   // Tensor memory: accumulators in two halves of as many columns as the
   // launch's largest tile has rows (gate and up, or two tiles of one matrix),
   // then two buffers of scales or more.
@@ -84,7 +88,6 @@ struct alignas(64) Params {
   const float* ts_x;
   const uint8_t* xs;      // row scales, xs_ld bytes per row
   int xs_ld;
-  int xs_wide;            // whole stages may be read as one 8 or 16 byte word
   int rows;
   const WispSegment* segs;
   int nseg;
@@ -323,13 +326,14 @@ WB_DEV void store_tile(const Params& p, const Tile& t, uint32_t d, uint32_t du, 
   }
 }
 
-// The epilogue of a cluster that splits K. 32 rows at a time, every CTA puts its
-// partial sums into its shared memory, and CTA kp adds those of all, in the
-// order of K, for the rows kp, kp + ks, ... (a warp per row, 4 features per
-// lane).
+// The epilogue of a cluster that splits K. 16 rows at a time, every CTA puts its
+// partial sums into its shared memory (four warps the gate's or the only ones,
+// four the up's), and CTA kp adds those of all, in the order of K, for the rows
+// kp, kp + ks, ... (a warp per row, 4 features per lane).
+constexpr int kRedRows = 16;
 template <bool SWIGLU>
 struct Reduce {
-  float* buf;        // [gate, up][32 rows][128 features]
+  float* buf;        // [gate, up][kRedRows][128 features]
   Bars* bars;
   int ks, kp;
   uint32_t uses = 0;
@@ -345,25 +349,21 @@ struct Reduce {
   WB_DEV bool store(const Params& p, const Tile& t, uint32_t d, uint32_t du, int w, float ag,
                     float au, volatile int* abort) {
     const int lane = threadIdx.x & 31, half = w >> 2, quad = threadIdx.x >> 5 & 3;
-    for (int c = 0; c < t.cnt; c += 32, uses++) {
+    for (int c = 0; c < t.cnt; c += kRedRows, uses++) {
       bool ok = uses == 0 || mbar_wait_cluster(&bars->red_empty, (uses - 1) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) return false;
-      if (c + half * 16 < t.cnt) {
-        uint32_t g[16], u[16];
-        tmem_ld16(d + c + half * 16, g);
-        if (SWIGLU) tmem_ld16(du + c + half * 16, u);
+      if (half == 0 || SWIGLU) {
+        uint32_t g[16];
+        tmem_ld16((half ? du : d) + c, g);
         tmem_wait_ld();
-        float* q = buf + half * 16 * 128 + quad * 32 + lane;
+        float* q = buf + half * kRedRows * 128 + quad * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          q[i * 128] = __uint_as_float(g[i]);
-          if (SWIGLU) q[(32 + i) * 128] = __uint_as_float(u[i]);
-        }
+        for (int i = 0; i < 16; i++) q[i * 128] = __uint_as_float(g[i]);
       }
       arrive_all(&bars->red_full);
       ok = mbar_wait_cluster(&bars->red_full, uses & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) return false;
-      for (int r = kp + ks * w; r < min(32, t.cnt - c); r += ks * 8) {
+      for (int r = kp + ks * w; r < min(kRedRows, t.cnt - c); r += ks * 8) {
         float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
         for (int j = 0; j < ks; j++) {
           const uint32_t a = cluster_addr(buf + r * 128 + lane * 4, j);
@@ -373,7 +373,7 @@ struct Reduce {
           v[2] += y.z;
           v[3] += y.w;
           if (SWIGLU) {
-            const float4 z = ld_cluster_f4(a + 32 * 128 * 4);
+            const float4 z = ld_cluster_f4(a + kRedRows * 128 * 4);
             x[0] += z.x;
             x[1] += z.y;
             x[2] += z.z;
@@ -417,12 +417,12 @@ struct Tiles {
     return t.expert >= 0;
   }
 };
-constexpr int kTileReaders = 10 + kScaleWarps;   // producer, MMA, scale, eight epilogue warps
 
 template <bool NV, bool SWIGLU, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<NV, SWIGLU>::kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
   using C = Shape<NV, SWIGLU>;
+  constexpr int kThreads = C::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
@@ -450,11 +450,11 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   // for only where another CTA's barriers are used, and the thread that holds
   // the first tile's segment hands that tile out itself.
   if (tid < kMaxStages) {
-    // the copies, one scale warp; in a pair's even CTA also the odd one's word
+    // the copies, a scale warp; in a pair's even CTA also the odd one's word
     mbar_init(&bars.full[tid], PAIR && rank == 0 ? 3 : 2);
     mbar_init(&bars.empty[tid], 1);
     mbar_init(&bars.tile_full[tid], 1);
-    mbar_init(&bars.tile_empty[tid], kTileReaders);
+    mbar_init(&bars.tile_empty[tid], 10 + C::kScaleWarps);   // all warps but the scheduler
     if (tid < 2) {
       mbar_init(&bars.acc_full[tid], 1);
       mbar_init(&bars.acc_empty[tid], PAIR ? 16 : 8);
@@ -552,6 +552,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     plan.multi_tiles += __shfl_sync(0xffffffffu, wz, 15);
   }
   // the scheduler warp reads pref and order
+  __syncwarp();
   if (warp == kSchedWarp)
     asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kThreads) : "memory");
   else
@@ -564,7 +565,10 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   const int off_b = C::kOffSfb + C::kWords * 512 * row_tiles;
   // a pair's CTA holds half of the tile's rows, in boxes of 16
   const int stage_bytes = off_b + ((max_cnt + 31) >> 5) * (PAIR ? 2048 : 4096);
-  constexpr int kRedBytes = C::kMats * 32 * 128 * 4;     // partial sums of 32 rows
+  constexpr int kRedBytes = C::kMats * kRedRows * 128 * 4;     // a cluster's partial sums
+  // S >= kTurn even for the largest stages (kMaxN rows in one CTA)
+  static_assert(kRingBytes - kRedBytes >= C::kTurn * (C::kOffSfb + C::kWords * 1024 + C::kMaxN * 128),
+                "ring");
   const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
   // columns of an accumulator half (two sets of the largest tile's, where a
   // half can hold gate and up), buffers of scales
@@ -703,103 +707,120 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       }
     }
   } else if (warp < kEpiWarp || warp > kSchedWarp) {
-    // Row scales: the warps take stages in turn. A lane copies rows lane + 32
-    // i, whose words lie side by side in the layout; the words of the warp's
-    // next stage are on their way while it waits for a slot. (A round trip to
-    // L2 every other stage, with two warps, bounded the stages at ~400
-    // cycles.)
-    const int first = warp < kEpiWarp ? warp - 2 : warp - kSchedWarp + 1;
-    constexpr int R = C::kMaxN / 32, W = C::kWords;
+    // Row scales. The warps take turns at units of 16 scale bytes per row (two
+    // stages of MX, one of NV). A lane reads the one or two 16-byte words
+    // around the bytes of rows lane + 32 i (rows may start anywhere), while the
+    // warp's last unit waits for its slots, and puts the four rows whose words
+    // lie side by side in the layout down at once. (Measured and dropped: every
+    // warp at every stage with 32 rows each, where four proxy fences a stage
+    // made dense NV products 28 % slower; narrower reads, whose sectors bound a
+    // stage of 224 unaligned rows at ~2000 cycles.)
+    constexpr int R = (C::kMaxN + 31) / 32, W = C::kWords, U = C::kUnitStages;
+    const int wi = warp < kEpiWarp ? warp - 2 : warp - kSchedWarp + 1;
     struct Pos {
       int kk;
       bool more;
       Tile t;
     };
-    auto advance = [&](Pos& q, int by) {
-      q.kk += by;
-      while (q.more && q.kk >= k1) {
-        q.kk -= k1 - k0;
+    Pos q;
+    q.kk = k0;
+    q.more = tiles.next(bars, q.t, abort);
+    auto step = [&]() {      // one unit on; the stages of the one left behind
+      const int n = min(U, k1 - q.kk);
+      q.kk += U;
+      if (q.kk >= k1) {
+        q.kk = k0;
         q.more = tiles.next(bars, q.t, abort);
       }
+      return n;
     };
-    auto fetch = [&](const Pos& q, uint32_t (&w)[W][8]) {
-#pragma unroll
-      for (int j = 0; j < W; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[j][i] = 0;
-      if (!q.more) return;
-      const int left = p.xs_ld - q.kk * W * 4;
-      const uint8_t* src = p.xs + (int64_t)(q.t.row0 + lane) * p.xs_ld + q.kk * W * 4;
+    auto skip = [&](int units) {
+      int n = 0;
+      for (int i = 0; i < units && q.more; i++) n += step();
+      return n;
+    };
+    uint4 v[R][2];
+    auto fetch = [&]() {
+      const int at = q.kk * W * 4, nb = min(p.xs_ld - at, 16);
 #pragma unroll
       for (int i = 0; i < R; i++) {
-        if (lane + 32 * i < q.t.cnt) {
-          const uint8_t* g = src + (int64_t)(32 * i) * p.xs_ld;
-          if (p.xs_wide && left >= W * 4) {
-            if (NV) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(g));
-              w[0][i] = v.x;
-              w[1][i] = v.y;
-              w[W - 2][i] = v.z;
-              w[W - 1][i] = v.w;
-            } else {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(g));
-              w[0][i] = v.x;
-              w[1][i] = v.y;
-            }
-          } else {
-// rows that start anywhere: aligned words around the bytes, none
-            // of them without a byte of the row, shifted into place; bytes
-            // past the row are 0
-            const int nb = min(left, W * 4);
-            const uint32_t* a = reinterpret_cast<const uint32_t*>((uintptr_t)g & ~(uintptr_t)3);
-            const int off = (int)((uintptr_t)g & 3);
-            uint32_t v[W + 1];
-#pragma unroll
-            for (int j = 0; j <= W; j++) v[j] = 4 * j < off + nb ? __ldg(a + j) : 0u;
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-              const uint32_t x = __funnelshift_r(v[j], v[j + 1], 8 * off);
-              const int valid = nb - 4 * j;
-              w[j][i] = valid >= 4 ? x : valid > 0 ? x & ((1u << (8 * valid)) - 1u) : 0u;
-            }
-          }
+        v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (q.more && lane + 32 * i < q.t.cnt) {
+          const uint8_t* g = p.xs + (int64_t)(q.t.row0 + lane + 32 * i) * p.xs_ld + at;
+          const int off = (int)((uintptr_t)g & 15);
+          const uint4* a = reinterpret_cast<const uint4*>(g - off);
+          v[i][0] = __ldg(a);
+          if (16 < off + nb) v[i][1] = __ldg(a + 1);     // never without a byte of the row
         }
       }
     };
     Ring r;
-    int use = 0;
-    auto put = [&](const uint32_t (&w)[W][8]) {
-      bool ok = use < S || mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort);
-      if (!__all_sync(0xffffffffu, ok)) return false;
-      uint4* dst = reinterpret_cast<uint4*>(smem + r.s * stage_bytes + C::kOffSfb) + lane;
-#pragma unroll
-      for (int j = 0; j < W; j++) {
-        dst[j * 32 * row_tiles] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
-        if (row_tiles == 2) dst[j * 64 + 32] = make_uint4(w[j][4], w[j][5], w[j][6], w[j][7]);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.full[r.s]);
-#pragma unroll
-      for (int i = 0; i < kScaleWarps; i++) r.next(S);
-      use = min(use + kScaleWarps, 1 << 20);
-      return true;
+    int use = 0;            // stages so far, up to S
+    bool ok = true;
+    // Waits for the slot of the next stage, i, in the ring: for the MMAs of
+    // stage i - S. The parity would take those of i - 3 S for them, were i - 2 S
+    // not complete. But this warp has put down stage i - kTurn, or a later one,
+    // and so seen stage i - kTurn - S complete, which is i - 2 S or later as
+    // long as S >= kTurn.
+    auto slot = [&]() {
+      ok = use < S || mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort);
+      ok = __all_sync(0xffffffffu, ok);
     };
-    Pos q;
-    q.kk = k0;
-    q.more = tiles.next(bars, q.t, abort);
-    advance(q, first);
-    for (int i = 0; i < first; i++) r.next(S);
-    use = first;
-    uint32_t a[W][8], b[W][8];
-    fetch(q, a);
-    while (q.more) {
-      advance(q, kScaleWarps);
-      fetch(q, b);
-      if (!put(a) || !q.more) break;
-      advance(q, kScaleWarps);
-      fetch(q, a);
-      if (!put(b)) break;
+    auto leave = [&]() {
+      r.next(S);
+      use = min(use + 1, S);
+    };
+    int ahead = skip(wi);   // stages of the other warps before this one's next
+    fetch();
+    while (q.more && ok) {
+      const int n = min(U, k1 - q.kk), at = q.kk * W * 4, nb = min(p.xs_ld - at, 16);
+      uint32_t w[4][8];     // [word][row / 32]
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (i < R) {
+          const uint32_t off =
+              (uint32_t)((uintptr_t)p.xs + (q.t.row0 + lane + 32 * i) * (int64_t)p.xs_ld + at) & 15u;
+          uint32_t u[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w,
+                           v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+#pragma unroll
+          for (int j = 0; j < 7; j++) u[j] = off & 4u ? u[j + 1] : u[j];
+#pragma unroll
+          for (int j = 0; j < 5; j++) u[j] = off & 8u ? u[j + 2] : u[j];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int valid = nb - 4 * j;       // bytes past the row count as 0
+            const uint32_t x = __funnelshift_r(u[j], u[j + 1], 8 * (off & 3u));
+            w[j][i] = valid >= 4 ? x : valid > 0 ? x & ((1u << (8 * valid)) - 1u) : 0u;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; j++) w[j][i] = 0u;
+        }
+      }
+      step();
+      const int others = skip(C::kScaleWarps - 1);
+      fetch();
+      for (int i = 0; i < ahead; i++) leave();
+      ahead = others;
+#pragma unroll
+      for (int st = 0; st < U; st++) {
+        if (st < n && ok) {
+          slot();
+          if (ok) {
+            uint4* dst = reinterpret_cast<uint4*>(smem + r.s * stage_bytes + C::kOffSfb) + lane;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+              const uint32_t* x = w[st * W + j];
+              dst[j * 32 * row_tiles] = make_uint4(x[0], x[1], x[2], x[3]);
+              if (row_tiles == 2) dst[j * 64 + 32] = make_uint4(x[4], x[5], x[6], x[7]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.full[r.s]);
+            leave();
+          }
+        }
+      }
     }
   } else if (warp < kSchedWarp) {
     cluster_wait();
@@ -921,7 +942,7 @@ WispError launch_product(const Params& p, int dev, unsigned grid, int cluster, c
   WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(Shape<NV, SWIGLU>::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -1012,8 +1033,6 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   p.ts_x = x->tensor_scale;
   p.xs = x->scales;
   p.xs_ld = cfg->k / (nv ? 16 : 32);
-  const int wide = nv ? 16 : 8;
-  p.xs_wide = p.xs_ld % wide == 0 && (uintptr_t)x->scales % wide == 0;
   p.rows = x->rows;
   p.segs = d_segs;
   p.nseg = n_segs;
