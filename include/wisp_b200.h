@@ -587,7 +587,9 @@ WispError wisp_b200_pack_rows(const uint16_t* d_x, const int* d_src, int n_rows,
                               uint16_t* d_xp, cudaStream_t stream, WispErrCtx* err);
 
 /* Device error word written by the tcgen05 kernels when a bounded wait gave
- * up (nonzero = the results of that launch are invalid). */
+ * up (nonzero = the results of that launch are invalid): WISP_ERR_TIMEOUT. 2,
+ * from wisp_b200_fp4_product alone: a segment was skipped,
+ * WISP_ERR_INVALID_ARG. */
 WispError wisp_b200_check_error_flag(const int* d_error_flag, cudaStream_t stream,
                                      WispErrCtx* err);
 

@@ -67,7 +67,7 @@ def _run(T, M, x="bf16", y="fp32", w="bf16", gate="channel", n="bf16", post=True
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 5, 297])
-@pytest.mark.parametrize("M", [1, 7, 8, 64, 1000, 2077, 7168, 8193, 32761, 32768])
+@pytest.mark.parametrize("M", [1, 7, 8, 64, 248, 264, 520, 1000, 1024, 1032, 2077, 7168, 8193, 32761, 32768])
 def test_sizes(T, M):
     _run(T, M)
     _run(T, M, y=None, gate="none", post=False, n="fp32")

@@ -392,6 +392,19 @@ def test_product_leaves_other_rows_and_columns(fmt):
 
 @pytest.mark.gpu
 @FMTS
+def test_product_of_no_segments(fmt):
+    g = torch.Generator(device=DEV).manual_seed(14)
+    w = fp4.Fp4Weights(fmt, *_mats(g, fmt, 2, 64, 64))
+    out = torch.full((20, 64), 7.0, device=DEV)
+    none = torch.empty((0, 4), dtype=torch.int32, device=DEV)
+    for segs in (none, torch.zeros((3, 4), dtype=torch.int32, device=DEV)):
+        fp4.product(_rows(g, fmt, 20, 64), w, segs, out=out)
+        assert (out == 7.0).all()
+    w.check()
+
+
+@pytest.mark.gpu
+@FMTS
 def test_product_skips_bad_segments(fmt):
     g = torch.Generator(device=DEV).manual_seed(5)
     mats = _mats(g, fmt, 2, 64, 64)
@@ -403,7 +416,7 @@ def test_product_skips_bad_segments(fmt):
         fp4.product(q, w, segs, out=out)
         ref.check_product(out, q, [mats], [(1, 8, 5)], 64)
         assert (out[:8] == 7.0).all() and (out[13:] == 7.0).all()
-        with pytest.raises(RuntimeError, match=r"wisp engine error \[7\]"):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*segment"):
             w.check()
         w.error_word.zero_()
 

@@ -54,15 +54,17 @@ WB_DEV float square_sum(const float (&v)[8], float s) {
   return s;
 }
 
-// Vectors of 8: thread i of `VEC` kernels holds elements 8 (k blockDim + i) ..
-// + 7; otherwise (a row that does not start on 16 bytes) elements
-// (8 k + j) blockDim + i, so that a warp's single loads are consecutive.
+// A row's values over nt threads, vectors of 8: thread i of `VEC` kernels holds
+// elements 8 (k nt + i) .. + 7; otherwise (a row that does not start on 16
+// bytes) elements (8 k + j) nt + i, so that a warp's single loads are
+// consecutive.
 template <bool VEC>
-WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, float (&v)[8]) {
+WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, int i, int nt,
+                     float (&v)[8]) {
   if (VEC) {
-    const int i = (k * blockDim.x + threadIdx.x) * 8;
-    if (i < M) {
-      load8(q, type, base + i, true, 8, v);
+    const int e = (k * nt + i) * 8;
+    if (e < M) {
+      load8(q, type, base + e, true, 8, v);
       return;
     }
 #pragma unroll
@@ -70,47 +72,45 @@ WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, float 
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const int i = (8 * k + j) * blockDim.x + threadIdx.x;
-      v[j] = i < M ? load_one(q, type, base + i) : 0.f;
+      const int e = (8 * k + j) * nt + i;
+      v[j] = e < M ? load_one(q, type, base + e) : 0.f;
     }
   }
 }
 
 template <bool VEC>
-WB_DEV void store_row(void* q, int type, int64_t base, int k, int M, const float (&v)[8]) {
+WB_DEV void store_row(void* q, int type, int64_t base, int k, int M, int i, int nt,
+                      const float (&v)[8]) {
   if (VEC) {
-    const int i = (k * blockDim.x + threadIdx.x) * 8;
-    if (i < M) store8(q, type, base + i, true, 8, v);
+    const int e = (k * nt + i) * 8;
+    if (e < M) store8(q, type, base + e, true, 8, v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const int i = (8 * k + j) * blockDim.x + threadIdx.x;
-      if (i < M) store_one(q, type, base + i, v[j]);
+      const int e = (8 * k + j) * nt + i;
+      if (e < M) store_one(q, type, base + e, v[j]);
     }
   }
 }
 
-// One row per CTA.
-template <int V, int THREADS, bool VEC>
-__global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float buf[2][1][32];
+// One row over nt threads; `sum` adds a value over them (round: 0, then 1).
+template <int V, bool VEC, typename Sum>
+WB_DEV void norm_row(const NormParams& p, int64_t t, int i, int nt, Sum sum) {
   const WispBlockNorm& c = p.c;
-  const int64_t t = blockIdx.x;
   const int M = c.hidden;
   float x[V][8], y[V][8];
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    if (p.y) load_row<VEC>(p.y, c.y_type, t * c.ld_y, k, M, y[k]);
-    load_row<VEC>(p.x, c.x_type, t * c.ld_x, k, M, x[k]);
+    if (p.y) load_row<VEC>(p.y, c.y_type, t * c.ld_y, k, M, i, nt, y[k]);
+    load_row<VEC>(p.x, c.x_type, t * c.ld_x, k, M, i, nt, x[k]);
   }
   if (p.y) {
     float r = 1.f;
     if (c.post_norm) {
-      float s[1] = {0.f};
+      float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < V; k++) s[0] = square_sum(y[k], s[0]);
-      block_sum(s, buf[0]);
-      r = inv_rms(s[0] * p.inv_m, c.eps);
+      for (int k = 0; k < V; k++) s = square_sum(y[k], s);
+      r = inv_rms(sum(s, 0) * p.inv_m, c.eps);
     }
     if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
@@ -119,40 +119,79 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 8; j++) y[k][j] *= r;
       if (p.post_w) {
-        load_row<VEC>(p.post_w, c.w_type, 0, k, M, w);
+        load_row<VEC>(p.post_w, c.w_type, 0, k, M, i, nt, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) y[k][j] *= c.weight_offset + w[j];
       }
       if (c.gate_kind == WISP_GATE_CHANNEL || c.gate_kind == WISP_GATE_ELEMENT) {
         load_row<VEC>(p.gate, c.gate_type, c.gate_kind == WISP_GATE_ELEMENT ? t * c.ld_gate : 0, k,
-                      M, w);
+                      M, i, nt, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) y[k][j] *= w[j];
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) x[k][j] = fmaf(c.residual_scale, x[k][j], y[k][j]);
-      if (p.x_out) store_row<VEC>(p.x_out, c.x_type, t * c.ld_x_out, k, M, x[k]);
+      if (p.x_out) store_row<VEC>(p.x_out, c.x_type, t * c.ld_x_out, k, M, i, nt, x[k]);
     }
   }
   if (p.n) {
-    float s[1] = {0.f};
+    float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < V; k++) s[0] = square_sum(x[k], s[0]);
-    block_sum(s, buf[1]);
-    const float r = inv_rms(s[0] * p.inv_m, c.eps);
+    for (int k = 0; k < V; k++) s = square_sum(x[k], s);
+    const float r = inv_rms(sum(s, 1) * p.inv_m, c.eps);
 #pragma unroll
     for (int k = 0; k < V; k++) {
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) x[k][j] *= r;
       if (p.pre_w) {
-        load_row<VEC>(p.pre_w, c.w_type, 0, k, M, w);
+        load_row<VEC>(p.pre_w, c.w_type, 0, k, M, i, nt, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) x[k][j] *= c.weight_offset + w[j];
       }
-      store_row<VEC>(p.n, c.n_type, t * c.ld_n, k, M, x[k]);
+      store_row<VEC>(p.n, c.n_type, t * c.ld_n, k, M, i, nt, x[k]);
     }
   }
+}
+
+// Rows of at most 512: one per warp, no barrier (65,536 rows of 64: 59 us with
+// the ring below, 27 so; 16,384 of 1024 the other way round, 31 and 47).
+constexpr int kNormWarps = 8;
+template <int V, bool VEC>
+__global__ void __launch_bounds__(32 * kNormWarps)
+block_norm_warp_kernel(const __grid_constant__ NormParams p) {
+  const int64_t t = (int64_t)blockIdx.x * kNormWarps + (threadIdx.x >> 5);
+  if (t >= p.c.tokens) return;
+  norm_row<V, VEC>(p, t, threadIdx.x & 31, 32, [](float s, int) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  });
+}
+
+// One row per CTA.
+template <int V, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float buf[2][1][32];
+  norm_row<V, VEC>(p, blockIdx.x, threadIdx.x, blockDim.x, [&](float s, int round) {
+    float v[1] = {s};
+    block_sum(v, buf[round]);
+    return v[0];
+  });
+}
+
+template <bool VEC>
+void launch_rows(const NormParams& p, cudaStream_t st) {
+  const int T = p.c.tokens, vecs = (p.c.hidden + 7) / 8;
+  const int blocks = (T + kNormWarps - 1) / kNormWarps;
+  if (vecs <= 32)
+    wb::launch_k(block_norm_warp_kernel<1, VEC>, blocks, 32 * kNormWarps, 0, st, p);
+  else if (vecs <= 64)
+    wb::launch_k(block_norm_warp_kernel<2, VEC>, blocks, 32 * kNormWarps, 0, st, p);
+  else if (vecs <= 1024)
+    wb::launch_k(block_norm_kernel<1, 1024, VEC>, T, (vecs + 31) / 32 * 32, 0, st, p);
+  else
+    wb::launch_k(block_norm_kernel<4, 1024, VEC>, T, ((vecs + 3) / 4 + 31) / 32 * 32, 0, st, p);
 }
 
 // Many rows: persistent CTAs that take rows blockIdx.x, + gridDim.x, ..., whose
@@ -160,8 +199,9 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_consta
 // while a row's sums go round the CTA. A thread holds 8 columns, and their
 // weights and channel gate for good. The sum of a row's x'^2 goes round
 // together with the sum of the next row's y^2: one barrier per row. (At 4096 x
-// 7168, 10 bytes a value, one row per CTA took 117 us, this ring with two
-// sums after one another 64, with one 51; 45 us are the copy rate.)
+// 7168, 10 bytes a value, one row per CTA took 117 us, this ring with two sums
+// after one another 64, with one 53 = 5.5 TB/s; 45 us are the copy rate. What
+// is left is the issue of 28 warps' arithmetic between two barriers.)
 constexpr int kNormStages = 8;
 struct RingShape {
   int stages, x_bytes, y_bytes;
@@ -340,11 +380,10 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
       wide(d_gate, c.gate_type, c.gate_kind == WISP_GATE_ELEMENT ? c.ld_gate : 0) &&
       wide(d_post_w, c.w_type, 0) && wide(d_pre_w, c.w_type, 0) &&
       (!p.x_out || wide(d_x_out, c.x_type, c.ld_x_out)) && (!d_n || wide(d_n, c.n_type, c.ld_n));
-  const int vecs = (c.hidden + 7) / 8, T = c.tokens;
-  const int threads1 = (vecs + 31) / 32 * 32, threads4 = ((vecs + 3) / 4 + 31) / 32 * 32;
+  const int threads1 = (c.hidden + 255) / 256 * 32, T = c.tokens;    // a vector of 8 each
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
-  if (vec && threads1 <= 1024 && T > 2 * sms) {
+  if (vec && threads1 > 64 && threads1 <= 1024 && T > 2 * sms) {
     RingShape rs;
     rs.x_bytes = c.hidden * dt_size(c.x_type);
     rs.y_bytes = d_y ? c.hidden * dt_size(c.y_type) : 0;
@@ -356,15 +395,10 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
     WB_CUDA_CHECK(wb::raise_smem(block_norm_stream_kernel, 200 * 1024, dev, raised));
     const int grid = ctas * sms < T ? ctas * sms : T;
     wb::launch_k(block_norm_stream_kernel, grid, threads1, (size_t)rs.stages * stage, stream, p, rs);
-  } else if (threads1 <= 1024) {
-    if (vec)
-      wb::launch_k(block_norm_kernel<1, 1024, true>, T, threads1, 0, stream, p);
-    else
-      wb::launch_k(block_norm_kernel<1, 1024, false>, T, threads1, 0, stream, p);
   } else if (vec) {
-    wb::launch_k(block_norm_kernel<4, 1024, true>, T, threads4, 0, stream, p);
+    launch_rows<true>(p, stream);
   } else {
-    wb::launch_k(block_norm_kernel<4, 1024, false>, T, threads4, 0, stream, p);
+    launch_rows<false>(p, stream);
   }
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;

@@ -262,7 +262,7 @@ class Fp4Weights:
         return self.error_word.device
 
     def check(self) -> None:
-        """Raise if a product with these weights gave up waiting or met a bad segment."""
+        """Raise if a product with these weights gave up waiting or skipped a bad segment."""
         with elsewhere(self.error_word) or contextlib.nullcontext():
             abi.call("wisp_b200_check_error_flag", self.error_word.data_ptr(),
                      stream_of(self.error_word))
@@ -300,6 +300,8 @@ def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
         dtype = out.dtype
         dtype_code(dtype, "out")
         ld = row_stride(out, "out")
+    if segments is not None and n_segs == 0:
+        return out          # (an empty tensor has no address, which would mean "all rows")
     x = abi.WispFp4Rows(q._codes, q._scales, q._ts, rows)
     abi.call("wisp_b200_fp4_product", w._cfgs[dtype], w._mats, w._up_mats, C.byref(x),
              None if segments is None else segments.data_ptr(), n_segs, out.data_ptr(), ld,

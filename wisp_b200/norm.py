@@ -7,12 +7,7 @@ import ctypes as C
 import torch
 
 from . import abi
-from .fp4 import dtype_code, elsewhere, invalid, row_stride, stream_of
-
-
-def _weight(w: torch.Tensor | None, hidden: int, what: str) -> None:
-    if w is not None and (w.shape != (hidden,) or not w.is_contiguous()):
-        raise invalid(f"{what}: a contiguous vector of {hidden}")
+from .fp4 import DTYPES, elsewhere, invalid, row_stride, stream_of
 
 
 def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
@@ -30,63 +25,75 @@ def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     post=False) and pre_norm alike. gate: [hidden], [tokens, 1] or [tokens, hidden]; the two
     weights share a dtype. x' has x's dtype (x_out may be x itself), n has ``dtype``; n is None
     with pre=False."""
+    # (One pass over the arguments: at a few rows this function takes longer than its kernel.)
     ld_x = row_stride(x, "x")
-    T, M = x.shape
-    x_type = dtype_code(x.dtype, "x")
-    ld_y = y_type = ld_gate = gate_type = gate_kind = w_type = ld_xo = n_type = ld_n = 0
-    xp, yp, gp, pp, qp, xop, nop = x.data_ptr(), None, None, None, None, None, None
+    shape = x.shape
+    T, M = shape
+    vector = (M,)
     dev = x.get_device()
     same = True       # all tensors on x's device
-    if y is None:
-        if gate is not None or post_weight is not None or x_out is not None:
+    ld_y = y_type = ld_gate = gate_type = gate_kind = w_type = ld_xo = n_type = ld_n = 0
+    yp = gp = pp = qp = xop = nop = None
+    try:
+        x_type = DTYPES[x.dtype]
+        if y is not None:
+            if y.shape != shape:
+                raise invalid(f"y {tuple(y.shape)}, x {tuple(shape)}")
+            ld_y = row_stride(y, "y")
+            y_type, yp = DTYPES[y.dtype], y.data_ptr()
+            same = y.get_device() == dev
+        elif gate is not None or post_weight is not None or x_out is not None:
             raise invalid("gate, post_weight and x_out need y")
-        if not pre:
+        elif not pre:
             raise invalid("nothing to compute")
-        post = False
-    else:
-        if y.shape != x.shape:
-            raise invalid(f"y {tuple(y.shape)}, x {tuple(x.shape)}")
-        ld_y = row_stride(y, "y")
-        y_type = dtype_code(y.dtype, "y")
-        yp = y.data_ptr()
-        same = y.get_device() == dev
-    if post_weight is not None:
-        if not post:
-            raise invalid("post_weight without post")
-        _weight(post_weight, M, "post_weight")
-        w_type = dtype_code(post_weight.dtype, "post_weight")
-        pp = post_weight.data_ptr()
-        same = same and post_weight.get_device() == dev
-    if pre_weight is not None:
-        if not pre:
-            raise invalid("pre_weight without pre")
-        _weight(pre_weight, M, "pre_weight")
-        if pp is not None and pre_weight.dtype != post_weight.dtype:
-            raise invalid("post_weight and pre_weight differ in dtype")
-        w_type = dtype_code(pre_weight.dtype, "pre_weight")
-        qp = pre_weight.data_ptr()
-        same = same and pre_weight.get_device() == dev
-    if gate is not None:
-        gate_type = dtype_code(gate.dtype, "gate")
-        shape = gate.shape
-        if shape == (M,) and gate.is_contiguous():
-            gate_kind = abi.WISP_GATE_CHANNEL
-        elif shape == (T, 1) and gate.is_contiguous():
-            gate_kind = abi.WISP_GATE_TOKEN
-        elif shape == (T, M):
-            gate_kind = abi.WISP_GATE_ELEMENT
-            ld_gate = row_stride(gate, "gate")
         else:
-            raise invalid(f"gate {tuple(shape)}: [{M}], [{T}, 1] or [{T}, {M}]")
-        gp = gate.data_ptr()
-        same = same and gate.get_device() == dev
-    if n_out is not None and not pre:
-        raise invalid("n_out without pre")
-    for out in (x_out, n_out):
-        if out is not None:
-            if out.shape != x.shape:
-                raise invalid(f"an output is {tuple(out.shape)}, x {tuple(x.shape)}")
-            same = same and out.get_device() == dev
+            post = False
+        if post_weight is not None:
+            if not post:
+                raise invalid("post_weight without post")
+            if post_weight.shape != vector or not post_weight.is_contiguous():
+                raise invalid(f"post_weight: a contiguous vector of {M}")
+            w_type, pp = DTYPES[post_weight.dtype], post_weight.data_ptr()
+            same = same and post_weight.get_device() == dev
+        if pre_weight is not None:
+            if not pre:
+                raise invalid("pre_weight without pre")
+            if pre_weight.shape != vector or not pre_weight.is_contiguous():
+                raise invalid(f"pre_weight: a contiguous vector of {M}")
+            t = DTYPES[pre_weight.dtype]
+            if pp is not None and t != w_type:
+                raise invalid("post_weight and pre_weight differ in dtype")
+            w_type, qp = t, pre_weight.data_ptr()
+            same = same and pre_weight.get_device() == dev
+        if gate is not None:
+            gshape = gate.shape
+            if gshape == vector and gate.is_contiguous():
+                gate_kind = abi.WISP_GATE_CHANNEL
+            elif gshape == (T, 1) and gate.is_contiguous():
+                gate_kind = abi.WISP_GATE_TOKEN
+            elif gshape == shape:
+                gate_kind = abi.WISP_GATE_ELEMENT
+                ld_gate = row_stride(gate, "gate")
+            else:
+                raise invalid(f"gate {tuple(gshape)}: [{M}], [{T}, 1] or [{T}, {M}]")
+            gate_type, gp = DTYPES[gate.dtype], gate.data_ptr()
+            same = same and gate.get_device() == dev
+        if x_out is not None:
+            if x_out.shape != shape or x_out.dtype != x.dtype:
+                raise invalid("x_out differs from x in shape or dtype")
+            ld_xo, xop = row_stride(x_out, "x_out"), x_out.data_ptr()
+            same = same and x_out.get_device() == dev
+        if n_out is not None:
+            if not pre:
+                raise invalid("n_out without pre")
+            if n_out.shape != shape:
+                raise invalid(f"n_out {tuple(n_out.shape)}, x {tuple(shape)}")
+            ld_n, nop, dtype = row_stride(n_out, "n_out"), n_out.data_ptr(), n_out.dtype
+            same = same and n_out.get_device() == dev
+        if pre:
+            n_type = DTYPES[dtype]
+    except KeyError as e:
+        raise invalid(f"{e.args[0]} (float32, bfloat16 or float16)") from None
     if not same:
         raise invalid(f"a tensor is not on {x.device} like x")
     other = elsewhere(x)
@@ -96,23 +103,15 @@ def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
                               post_weight=post_weight, pre_weight=pre_weight, post=post, pre=pre,
                               eps=eps, weight_offset=weight_offset, dtype=dtype, x_out=x_out,
                               n_out=n_out)
-    if y is not None:
-        if x_out is None:
-            x_out, ld_xo = x.new_empty((T, M)), M
-        else:
-            if x_out.dtype != x.dtype:
-                raise invalid("x_out differs from x in dtype")
-            ld_xo = row_stride(x_out, "x_out")
-        xop = x_out.data_ptr()
-    if pre:
-        if n_out is None:
-            n_out, ld_n = x.new_empty((T, M), dtype=dtype), M
-        else:
-            ld_n, dtype = row_stride(n_out, "n_out"), n_out.dtype
-        n_type = dtype_code(dtype, "n")
-        nop = n_out.data_ptr()
+    if y is not None and xop is None:
+        x_out = torch.empty_like(x) if ld_x == M else x.new_empty(shape)
+        ld_xo, xop = M, x_out.data_ptr()
+    if pre and nop is None:
+        n_out = x.new_empty(shape, dtype=dtype)
+        ld_n, nop = M, n_out.data_ptr()
     c = abi.WispBlockNorm(T, M, x_type, y_type, w_type, gate_type, n_type, 1 if post else 0,
                           gate_kind, residual_scale, eps, weight_offset, ld_x, ld_y, ld_gate,
                           ld_xo, ld_n)
-    abi.call("wisp_b200_block_norm", C.byref(c), xp, yp, gp, pp, qp, xop, nop, stream_of(x))
+    abi.call("wisp_b200_block_norm", C.byref(c), x.data_ptr(), yp, gp, pp, qp, xop, nop,
+             stream_of(x))
     return x if y is None else x_out, n_out
