@@ -92,6 +92,7 @@ struct alignas(64) Params {
   const WispSegment* segs;
   int nseg;
   int V, N, nk, ftiles;
+  int cap;                // rows per tile at most: a multiple of 32, <= kMaxN
   void* out;
   int64_t ld;
   int out_type;
@@ -161,13 +162,14 @@ struct Tile {
   int ft;                  // features 128 ft ..
 };
 
-// Rows per tile of a segment: as many tiles as kMaxN demands, of equal size
-// up to the MMA's granularity UNIT (16; 32 in a pair, 16 rows per CTA).
-template <int MAXN, int UNIT>
-WB_DEV int tile_rows(int rows) {
+// Rows per tile of a segment: as many tiles as at most `cap` rows each demand,
+// of equal size up to the MMA's granularity UNIT (16; 32 in a pair, 16 rows per
+// CTA).
+template <int UNIT>
+WB_DEV int tile_rows(int rows, int cap) {
   int per = rows;
-  if (rows > MAXN) {
-    const int t = (rows + MAXN - 1) / MAXN;
+  if (rows > cap) {
+    const int t = (rows + cap - 1) / cap;
     per = (rows + t - 1) / t;
   }
   return (per + UNIT - 1) & ~(UNIT - 1);
@@ -202,7 +204,7 @@ struct Plan {
   int fitems;
 };
 
-template <int MAXN, int UNIT>
+template <int UNIT>
 __device__ __noinline__ Tile find_tile(const Params& p, const Plan& q, int it) {
   const int fitems = q.fitems, single = q.singles * fitems;
   const int items = single + q.multi_tiles * fitems;
@@ -233,7 +235,7 @@ __device__ __noinline__ Tile find_tile(const Params& p, const Plan& q, int it) {
     tt = 0;
   }
   const WispSegment v = segment(p, q.order[at]);
-  const int per = tile_rows<MAXN, UNIT>(v.rows);
+  const int per = tile_rows<UNIT>(v.rows, p.cap);
   t.expert = v.expert;
   t.row0 = v.row_begin + tt * per;
   t.cnt = min(per, v.rows - tt * per);
@@ -494,8 +496,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       if (!segment_ok(p, v)) {
         if (p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
       } else if (v.rows > 0) {
-        per = tile_rows<C::kMaxN, kUnit>(v.rows);
-        n = v.rows <= C::kMaxN ? 1 : (v.rows + per - 1) / per;
+        per = tile_rows<kUnit>(v.rows, p.cap);
+        n = v.rows <= p.cap ? 1 : (v.rows + per - 1) / per;
       }
     }
     const int most = __reduce_max_sync(0xffffffffu, min(per, v.rows));
@@ -887,7 +889,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       v.expert = -1;
       v.row0 = v.cnt = v.ft = 0;
       if (it < items) {
-        v = find_tile<C::kMaxN, kUnit>(p, plan, it);
+        v = find_tile<kUnit>(p, plan, it);
         if (PAIR) v.ft = 2 * v.ft + rank;
       }
       if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) break;
@@ -1004,10 +1006,14 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   const bool nv = cfg->format == WISP_FP4_NV;
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
-  // Token tiles, an upper bound: at most one per row, and per segment one more
-  // than its rows fill.
-  const int64_t most = d_segs ? (int64_t)x->rows / 96 + n_segs : ((int64_t)x->rows + 95) / 96;
-  const int64_t tiles = most < x->rows ? most : x->rows;
+  // Token tiles of at most `cap` rows, an upper bound: at most one per row, and
+  // per segment one more than its rows fill.
+  int cap = nv ? Shape<true, false>::kMaxN : Shape<false, false>::kMaxN;
+  auto tiles_of = [&](int rows_per_tile) {
+    const int64_t most = (int64_t)x->rows / rows_per_tile + (d_segs ? n_segs : 1);
+    return most < x->rows ? most : x->rows;
+  };
+  const int64_t tiles = tiles_of(cap);
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 255) / 256;
   // Pairs, unless all tiles together could use at most 3/8 of the SMs as
   // single CTAs: then clusters of 4 (2) of these split K, as long as they fill
@@ -1017,8 +1023,18 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   // 9.6, 2048 x 2048 7.3 / 7.5 / 7.0, 7168 x 2048 7.6 / 7.8 / 14.0 (two waves).
   const int64_t items = tiles * ftiles;
   const int split = nk < 8 ? 1 : items * 16 <= 3 * (int64_t)sms ? 4 : items * 8 <= 3 * (int64_t)sms ? 2 : 1;
+  if (split == 1) {
+    // Smaller tiles when the largest would leave pairs without work: as many
+    // rows as give every pair one tile if the rows lay in one segment, at least
+    // 64 (what the MMA's fixed cost per weight is paid for anyway). 666 rows in
+    // 11 ragged segments, 1000 x 2080 with gate and up: 15.0 -> 13.0 us.
+    const int64_t per = ((int64_t)x->rows * ((ftiles + 1) / 2) * 2 + sms - 1) / sms;
+    const int fit = per < 64 ? 64 : per > cap ? cap : (int)((per + 31) & ~31);
+    if (fit < cap) cap = fit;
+  }
   Params p;
   memset(&p, 0, sizeof p);
+  p.cap = cap;
   const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
   if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
       (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
@@ -1047,7 +1063,7 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   if (split > 1)
     return launch_product<false>(nv, cfg->swiglu, p, dev, (unsigned)(items * split), split, stream,
                                  err);
-  const int64_t want = tiles * ((ftiles + 1) / 2) * 2;
+  const int64_t want = tiles_of(cap) * ((ftiles + 1) / 2) * 2;
   return launch_product<true>(nv, cfg->swiglu, p, dev,
                               (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2, stream, err);
 }
