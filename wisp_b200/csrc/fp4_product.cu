@@ -14,9 +14,10 @@
 // which halves what the rows cost in L2 traffic, shared memory and power; the
 // even CTA issues all MMAs, the odd CTA's MMA warp only passes on that its
 // stages are full. (At 4096 tokens over 257 experts 3 % faster than single
-// CTAs, at 40 tokens 2 %.) When there are few tiles, clusters of 2 or 4 single
-// CTAs take one tile each and split K; their partial sums meet in shared memory
-// and are added in the order of K.
+// CTAs, at 40 tokens 2 %.) Single CTAs (cta_group::1) take matrices of one
+// feature tile; and when there are few tiles, clusters of 2 or 4 of them take
+// one tile each and split K: their partial sums meet in shared memory and are
+// added in the order of K.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
 // scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 and 13-14 copy the rows'
@@ -1015,20 +1016,27 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   };
   const int64_t tiles = tiles_of(cap);
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 255) / 256;
-  // Pairs, unless all tiles together could use at most 3/8 of the SMs as
-  // single CTAs: then clusters of 4 (2) of these split K, as long as they fill
-  // at most 3/4 of the SMs (GPCs of an odd number of SMs hold fewer clusters)
-  // and have two stages of K each. One row, warm L2, us a call, as pairs / split
-  // by 2 / by 4: 2048 x 7168 11.6 / 10.4 / 8.6, with gate and up 13.1 / 11.9 /
-  // 9.6, 2048 x 2048 7.3 / 7.5 / 7.0, 7168 x 2048 7.6 / 7.8 / 14.0 (two waves).
+  // Pairs, unless there are few rows and all tiles together could use at most
+  // 3/8 of the SMs as single CTAs: then clusters of 4 (2) of these split K, as
+  // long as they fill at most 3/4 of the SMs (GPCs of an odd number of SMs hold
+  // fewer clusters) and have two stages of K each. One row, warm L2, us a call,
+  // as pairs / split by 2 / by 4: 2048 x 7168 11.6 / 10.4 / 8.6, with gate and
+  // up 13.1 / 11.9 / 9.6, 2048 x 2048 7.3 / 7.5 / 7.0, 7168 x 2048 7.6 / 7.8 /
+  // 14.0 (two waves). More rows pay a cluster round per 16.
   const int64_t items = tiles * ftiles;
-  const int split = nk < 8 ? 1 : items * 16 <= 3 * (int64_t)sms ? 4 : items * 8 <= 3 * (int64_t)sms ? 2 : 1;
+  const int split = nk < 8 || x->rows > 64              ? 1
+                    : items * 16 <= 3 * (int64_t)sms ? 4
+                    : items * 8 <= 3 * (int64_t)sms  ? 2
+                                                     : 1;
+  // With one feature tile a pair's second CTA would have none: single CTAs.
+  const bool single = split == 1 && ftiles == 1;
   if (split == 1) {
     // Smaller tiles when the largest would leave pairs without work: as many
     // rows as give every pair one tile if the rows lay in one segment, at least
     // 64 (what the MMA's fixed cost per weight is paid for anyway). 666 rows in
     // 11 ragged segments, 1000 x 2080 with gate and up: 15.0 -> 13.0 us.
-    const int64_t per = ((int64_t)x->rows * ((ftiles + 1) / 2) * 2 + sms - 1) / sms;
+    const int64_t width = single ? 1 : (ftiles + 1) / 2 * 2;
+    const int64_t per = ((int64_t)x->rows * width + sms - 1) / sms;
     const int fit = per < 64 ? 64 : per > cap ? cap : (int)((per + 31) & ~31);
     if (fit < cap) cap = fit;
   }
@@ -1038,7 +1046,7 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
   if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
       (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
-      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, split > 1 ? 32 : 16))
+      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, split > 1 || single ? 32 : 16))
     return WB_FAIL(WISP_ERR_CUDA, "fp4_product: cuTensorMapEncodeTiled failed");
   p.sf_w = static_cast<const uint8_t*>(w->prepared);
   p.ts_w = w->tensor_scale;
@@ -1063,6 +1071,11 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   if (split > 1)
     return launch_product<false>(nv, cfg->swiglu, p, dev, (unsigned)(items * split), split, stream,
                                  err);
+  if (single) {
+    const int64_t want = tiles_of(cap);
+    return launch_product<false>(nv, cfg->swiglu, p, dev, (unsigned)(want < sms ? want : sms), 1,
+                                 stream, err);
+  }
   const int64_t want = tiles_of(cap) * ((ftiles + 1) / 2) * 2;
   return launch_product<true>(nv, cfg->swiglu, p, dev,
                               (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2, stream, err);

@@ -58,6 +58,18 @@ WB_DEV float square_sum(const float (&v)[8], float s) {
 // elements 8 (k nt + i) .. + 7; otherwise (a row that does not start on 16
 // bytes) elements (8 k + j) nt + i, so that a warp's single loads are
 // consecutive.
+template <typename T>
+WB_DEV void load_strided(const T* q, int M, int e, int nt, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++, e += nt) v[j] = e < M ? (float)q[e] : 0.f;
+}
+template <typename T>
+WB_DEV void store_strided(T* q, int M, int e, int nt, const float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++, e += nt)
+    if (e < M) q[e] = (T)v[j];        // (the 16-bit types round to nearest even)
+}
+
 template <bool VEC>
 WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, int i, int nt,
                      float (&v)[8]) {
@@ -70,11 +82,13 @@ WB_DEV void load_row(const void* q, int type, int64_t base, int k, int M, int i,
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = 0.f;
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int e = (8 * k + j) * nt + i;
-      v[j] = e < M ? load_one(q, type, base + e) : 0.f;
-    }
+    const int e = 8 * k * nt + i;
+    if (type == WISP_DT_F32)
+      load_strided(static_cast<const float*>(q) + base, M, e, nt, v);
+    else if (type == WISP_DT_BF16)
+      load_strided(static_cast<const __nv_bfloat16*>(q) + base, M, e, nt, v);
+    else
+      load_strided(static_cast<const __half*>(q) + base, M, e, nt, v);
   }
 }
 
@@ -85,11 +99,13 @@ WB_DEV void store_row(void* q, int type, int64_t base, int k, int M, int i, int 
     const int e = (k * nt + i) * 8;
     if (e < M) store8(q, type, base + e, true, 8, v);
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int e = (8 * k + j) * nt + i;
-      if (e < M) store_one(q, type, base + e, v[j]);
-    }
+    const int e = 8 * k * nt + i;
+    if (type == WISP_DT_F32)
+      store_strided(static_cast<float*>(q) + base, M, e, nt, v);
+    else if (type == WISP_DT_BF16)
+      store_strided(static_cast<__nv_bfloat16*>(q) + base, M, e, nt, v);
+    else
+      store_strided(static_cast<__half*>(q) + base, M, e, nt, v);
   }
 }
 
@@ -207,6 +223,13 @@ struct RingShape {
   int stages, x_bytes, y_bytes;
 };
 
+// Rows that do not start on 16 bytes (VEC false) come as the 16-byte words
+// around them, and a thread then has columns tid, + threads, ...
+WB_DEV int64_t word_start(const void* q, int64_t byte) {
+  return (int64_t)((uintptr_t)q + byte) & ~(int64_t)15;
+}
+
+template <bool VEC>
 __global__ void __launch_bounds__(1024, 1)
 block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape rs) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -214,15 +237,24 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   __shared__ float buf[2][2][32];
   __shared__ int abort;
   const WispBlockNorm& c = p.c;
-  const int M = c.hidden, tid = threadIdx.x, T = c.tokens;
+  const int M = c.hidden, tid = threadIdx.x, nt = blockDim.x, T = c.tokens;
   const int stage = rs.x_bytes + rs.y_bytes;
-  const uint8_t* gx = static_cast<const uint8_t*>(p.x);
-  const uint8_t* gy = static_cast<const uint8_t*>(p.y);
   const int64_t sx = c.ld_x * dt_size(c.x_type), sy = c.ld_y * dt_size(c.y_type);
+  // bytes of a row in its words
+  auto words = [&](const void* q, int64_t at, int type) {
+    return (uint32_t)(word_start(q, at + M * dt_size(type) + 15) - word_start(q, at));
+  };
   auto issue = [&](int s, int64_t t) {
-    mbar_arrive_expect_tx(&full[s], rs.x_bytes + rs.y_bytes);
-    bulk_load(ring + s * stage, gx + t * sx, rs.x_bytes, &full[s]);
-    if (rs.y_bytes) bulk_load(ring + s * stage + rs.x_bytes, gy + t * sy, rs.y_bytes, &full[s]);
+    uint32_t bx = rs.x_bytes, by = rs.y_bytes;
+    if (!VEC) {
+      bx = words(p.x, t * sx, c.x_type);
+      if (by) by = words(p.y, t * sy, c.y_type);
+    }
+    mbar_arrive_expect_tx(&full[s], bx + by);
+    bulk_load(ring + s * stage, reinterpret_cast<const void*>(word_start(p.x, t * sx)), bx, &full[s]);
+    if (by)
+      bulk_load(ring + s * stage + rs.x_bytes,
+                reinterpret_cast<const void*>(word_start(p.y, t * sy)), by, &full[s]);
   };
   if (tid == 0) {
     abort = 0;
@@ -233,29 +265,24 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       if (t < T) issue(i, t);
     }
   }
-  const int i0 = tid * 8;
-  const bool in = i0 < M;
   // columns' factors: a of y / rms(y), b of x' / rms(x')
-  float a[8], b[8];
+  float a[8], b[8], w[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) a[j] = b[j] = 1.f;
-  if (in) {
-    float w[8];
-    if (p.post_w) {
-      load8(p.post_w, c.w_type, i0, true, 8, w);
+  if (p.post_w) {
+    load_row<VEC>(p.post_w, c.w_type, 0, 0, M, tid, nt, w);
 #pragma unroll
-      for (int j = 0; j < 8; j++) a[j] = c.weight_offset + w[j];
-    }
-    if (c.gate_kind == WISP_GATE_CHANNEL) {
-      load8(p.gate, c.gate_type, i0, true, 8, w);
+    for (int j = 0; j < 8; j++) a[j] = c.weight_offset + w[j];
+  }
+  if (c.gate_kind == WISP_GATE_CHANNEL) {
+    load_row<VEC>(p.gate, c.gate_type, 0, 0, M, tid, nt, w);
 #pragma unroll
-      for (int j = 0; j < 8; j++) a[j] *= w[j];
-    }
-    if (p.pre_w) {
-      load8(p.pre_w, c.w_type, i0, true, 8, w);
+    for (int j = 0; j < 8; j++) a[j] *= w[j];
+  }
+  if (p.pre_w) {
+    load_row<VEC>(p.pre_w, c.w_type, 0, 0, M, tid, nt, w);
 #pragma unroll
-      for (int j = 0; j < 8; j++) b[j] = c.weight_offset + w[j];
-    }
+    for (int j = 0; j < 8; j++) b[j] = c.weight_offset + w[j];
   }
   int s = 0, flip = 0;
   uint32_t ph = 0;
@@ -264,14 +291,17 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   // bounded) makes the row NaN. The slot may be refilled after the next
   // barrier.
   auto take = [&](int64_t t) {
-    const bool ok = mbar_wait(&full[s], ph, &abort);
-    const uint8_t* st = ring + s * stage;
-    const float none = ok ? 0.f : __uint_as_float(0x7fffffffu);
+    if (mbar_wait(&full[s], ph, &abort)) {
+      const uint8_t* st = ring + s * stage;
+      const int ox = VEC ? 0 : (int)((uintptr_t)p.x + t * sx) & 15;
+      load_row<VEC>(st + ox, c.x_type, 0, 0, M, tid, nt, x);
+      if (p.y) {
+        const int oy = VEC ? 0 : (int)((uintptr_t)p.y + t * sy) & 15;
+        load_row<VEC>(st + rs.x_bytes + oy, c.y_type, 0, 0, M, tid, nt, y);
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = y[j] = none;
-    if (in && ok) {
-      load8(st, c.x_type, i0, true, 8, x);
-      if (p.y) load8(st + rs.x_bytes, c.y_type, i0, true, 8, y);
+      for (int j = 0; j < 8; j++) x[j] = y[j] = __uint_as_float(0x7fffffffu);
     }
   };
   auto refill = [&](int64_t t) {      // the slot row t was taken from
@@ -284,6 +314,8 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       ph ^= 1;
     }
   };
+#pragma unroll
+  for (int j = 0; j < 8; j++) y[j] = 0.f;
   __syncthreads();
   int64_t t = blockIdx.x;
   take(t);
@@ -297,15 +329,14 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] *= r * a[j];
-      if (c.gate_kind == WISP_GATE_ELEMENT && in) {
-        float w[8];
-        load8(p.gate, c.gate_type, t * c.ld_gate + i0, true, 8, w);
+      if (c.gate_kind == WISP_GATE_ELEMENT) {
+        load_row<VEC>(p.gate, c.gate_type, t * c.ld_gate, 0, M, tid, nt, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] *= w[j];
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) x[j] = fmaf(c.residual_scale, x[j], y[j]);
-      if (p.x_out && in) store8(p.x_out, c.x_type, t * c.ld_x_out + i0, true, 8, x);
+      if (p.x_out) store_row<VEC>(p.x_out, c.x_type, t * c.ld_x_out, 0, M, tid, nt, x);
     }
     float xp[8];
 #pragma unroll
@@ -316,11 +347,11 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
     q[1] = square_sum(y, 0.f);
     block_sum(q, buf[flip]);
     if (tn < T) refill(tn);
-    if (p.n && in) {
+    if (p.n) {
       const float r = inv_rms(q[0] * p.inv_m, c.eps);
 #pragma unroll
       for (int j = 0; j < 8; j++) xp[j] *= r * b[j];
-      store8(p.n, c.n_type, t * c.ld_n + i0, true, 8, xp);
+      store_row<VEC>(p.n, c.n_type, t * c.ld_n, 0, M, tid, nt, xp);
     }
   }
 }
@@ -383,18 +414,23 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   const int threads1 = (c.hidden + 255) / 256 * 32, T = c.tokens;    // a vector of 8 each
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
-  if (vec && threads1 > 64 && threads1 <= 1024 && T > 2 * sms) {
+  if (threads1 > 64 && threads1 <= 1024 && T > 2 * sms) {
     RingShape rs;
-    rs.x_bytes = c.hidden * dt_size(c.x_type);
-    rs.y_bytes = d_y ? c.hidden * dt_size(c.y_type) : 0;
+    auto room = [&](int type) {     // the words of a row that starts anywhere
+      const int bytes = c.hidden * dt_size(type);
+      return vec ? bytes : (bytes + 15) / 16 * 16 + 16;
+    };
+    rs.x_bytes = room(c.x_type);
+    rs.y_bytes = d_y ? room(c.y_type) : 0;
     // as many CTAs per SM as make 1024 threads, which share its memory
     const int ctas = 1024 / threads1 < 8 ? 1024 / threads1 : 8;
     const int budget = 200 * 1024 / ctas, stage = rs.x_bytes + rs.y_bytes;
     rs.stages = budget / stage < kNormStages ? budget / stage : kNormStages;
-    static std::atomic<uint64_t> raised{0};
-    WB_CUDA_CHECK(wb::raise_smem(block_norm_stream_kernel, 200 * 1024, dev, raised));
     const int grid = ctas * sms < T ? ctas * sms : T;
-    wb::launch_k(block_norm_stream_kernel, grid, threads1, (size_t)rs.stages * stage, stream, p, rs);
+    auto kernel = vec ? block_norm_stream_kernel<true> : block_norm_stream_kernel<false>;
+    static std::atomic<uint64_t> raised[2];
+    WB_CUDA_CHECK(wb::raise_smem(kernel, 200 * 1024, dev, raised[vec]));
+    wb::launch_k(kernel, grid, threads1, (size_t)rs.stages * stage, stream, p, rs);
   } else if (vec) {
     launch_rows<true>(p, stream);
   } else {
