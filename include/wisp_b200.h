@@ -523,8 +523,8 @@ WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
 
 /* The MoE layer of wisp_b200_moe_forward over fp4 experts: route, dispatch
  * plan, quantise the gathered rows, gate/up product with SwiGLU (bf16 rows),
- * quantise, down product (fp32 rows), each token's rows summed in a fixed
- * order with the routing weights. gate, up: sets of E (+1 shared) entries
+ * quantise, down product (bf16 rows), each token's rows summed in fp32 in a
+ * fixed order with the routing weights. d_out 16-byte aligned. gate, up: sets of E (+1 shared) entries
  * [inter x hidden], down: [hidden x inter], all prepared. cfg->group_size,
  * cfg->deterministic are ignored (every run gives the same bits). x_scale,
  * h_scale: the NV tensor scales of the layer's input and of the SwiGLU output

@@ -540,7 +540,7 @@ def _check_layer(layer, x, out):
     fmt = layer.gate_up.fmt
     xs, hs = layer._keep[2:]
     h = fp4.product(fp4.quantize(x, fmt, xs, rows=tok), layer.gate_up, segs, dtype=torch.bfloat16)
-    y = fp4.product(fp4.quantize(h, fmt, hs), layer.down, segs, dtype=torch.float32).double()
+    y = fp4.product(fp4.quantize(h, fmt, hs), layer.down, segs, dtype=torch.bfloat16).double()
     wrow = torch.tensor([1.0 if e == spec.n_experts else wt[t][(idx[t] == e)].item()
                          for e, r in enumerate(rows) for t in r], dtype=torch.float64, device=DEV)
     want = torch.zeros((T, spec.hidden), dtype=torch.float64, device=DEV)
@@ -554,7 +554,7 @@ def _check_layer(layer, x, out):
 
 @pytest.mark.gpu
 @FMTS
-@pytest.mark.parametrize("tokens", [1, 3, 64, 300])
+@pytest.mark.parametrize("tokens", [1, 3, 64, 210, 300, 700])
 def test_moe_layer(fmt, tokens):
     for spec in (synth.MoeSpec("soft", 512, 256, 16, 4, has_shared=True),
                  synth.MoeSpec("sig", 384, 128, 32, 4, scoring=abi.WISP_SCORE_SIGMOID_GROUPED,
