@@ -513,9 +513,9 @@ WispError wisp_b200_fp4_prepare(const WispFp4Config* cfg, const uint8_t* d_scale
  * over the rows, which must not overlap; NULL: all rows through entry 0. Rows
  * in no segment are left as they are. A segment whose expert or rows lie
  * outside the set or the rows is skipped and sets *d_error_flag to 2. ld: elements
- * between output rows. up is NULL unless swiglu. d_error_flag as for
- * wisp_b200_grouped_ffn (may be NULL; the call does not clear it).
- * rows = 0 is allowed and launches nothing. */
+ * between output rows. up is NULL unless swiglu. d_out overlaps none of the
+ * inputs. d_error_flag as for wisp_b200_grouped_ffn (may be NULL; the call
+ * does not clear it). rows = 0 is allowed and launches nothing. */
 WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
                                 const WispFp4Mats* up, const WispFp4Rows* x,
                                 const WispSegment* d_segs, int n_segs, void* d_out, int64_t ld,
@@ -524,9 +524,10 @@ WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
 /* The MoE layer of wisp_b200_moe_forward over fp4 experts: route, dispatch
  * plan, quantise the gathered rows, gate/up product with SwiGLU (bf16 rows),
  * quantise, down product (bf16 rows), each token's rows summed in fp32 in a
- * fixed order with the routing weights. d_out 16-byte aligned. gate, up: sets of E (+1 shared) entries
- * [inter x hidden], down: [hidden x inter], all prepared. cfg->group_size,
- * cfg->deterministic are ignored (every run gives the same bits). x_scale,
+ * fixed order with the routing weights. d_out 16-byte aligned. gate, up: sets
+ * of E (+1 shared) entries [inter x hidden], down: [hidden x inter], all
+ * prepared. cfg->group_size, cfg->deterministic are ignored (every run gives
+ * the same bits). x_scale,
  * h_scale: the NV tensor scales of the layer's input and of the SwiGLU output
  * (device, from calibration; NULL for MX). */
 typedef struct {

@@ -122,6 +122,8 @@ def test_python_refusals():
                                     torch.zeros(2, 4, dtype=torch.uint8)),
                 lambda: fp4.Fp4Weights(MX, torch.zeros(2, 32, dtype=torch.uint8),
                                        torch.zeros(2, 2, dtype=torch.uint8)),
+                lambda: fp4.Fp4Weights(MX, torch.zeros(1, 2, 32, dtype=torch.uint8),
+                                       torch.zeros(1, 2, 2, dtype=torch.uint8), up=(x,)),
                 lambda: norm.block_norm(x, pre=False), lambda: norm.block_norm(x, gate=x),
                 lambda: norm.block_norm(x, x, gate=x[:, :3]),
                 lambda: norm.block_norm(x, x, post=False, post_weight=x[0]),
@@ -451,6 +453,12 @@ def test_product_on_streams_and_in_graphs(fmt):
     qs = [_rows(g, fmt, 243, 544) for _ in range(2)]
     want = [fp4.product(q, w, segs, dtype=torch.float32) for q in qs]
     torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        own = fp4.dequantize(qs[0])
+    qs[0].record_stream(side)
+    side.synchronize()
+    assert torch.equal(own, fp4.dequantize(qs[0]))
     outs = [torch.zeros_like(want[0]) for _ in qs]
     streams = [torch.cuda.Stream() for _ in qs]
     for _ in range(5):
@@ -510,6 +518,18 @@ def test_weights_from_values(fmt):
     codes, scales = (torch.stack([m[i] for m in mats]) for i in (0, 1))
     ts = torch.cat([m[2] for m in mats]) if fmt == NV else None
     ref.check_product(out, q, [(codes, scales, ts)], segs, 96)
+
+
+@pytest.mark.gpu
+@FMTS
+def test_up_without_tensor_scales(fmt):
+    g = torch.Generator(device=DEV).manual_seed(10)
+    (gc, gs, _), (uc, us, _) = _mats(g, fmt, 2, 64, 96), _mats(g, fmt, 2, 64, 96)
+    q = _rows(g, fmt, 9, 96)
+    segs, dev = _segs([4, 5])
+    out, same = (fp4.product(q, fp4.Fp4Weights(fmt, gc, gs, up=up), dev, dtype=torch.float32)
+                 for up in ((uc, us), (uc, us, None)))
+    assert torch.equal(out.view(torch.int32), same.view(torch.int32))
 
 
 # ---------------------------------------------------------------------------

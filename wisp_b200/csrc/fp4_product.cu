@@ -4,10 +4,10 @@
 //
 // The features are the MMA's M (128 per tile, so that a weight matrix streams
 // through shared memory once per token tile), the rows its N: any multiple of
-// 16 up to kMaxN, set per tile in the instruction descriptor, so one kernel
-// serves single tokens and prefill. An accumulator lane is then one feature
-// and a column one row: an epilogue warp stores 32 consecutive features of a
-// row at a time, and SwiGLU pairs the gate and up accumulators lane by lane.
+// 16 (32 in a pair) up to kMaxN, set per tile in the instruction descriptor, so
+// one kernel serves single tokens and prefill. An accumulator lane is then one
+// feature and a column one row: an epilogue warp stores 32 consecutive features
+// of a row at a time, and SwiGLU pairs the gate and up accumulators lane by lane.
 //
 // Two forms. CTA pairs (cta_group::2, M = 256) take two feature tiles of one
 // token tile, and each loads its own weights but only half of the row codes,
@@ -20,12 +20,18 @@
 // added in the order of K.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
-// scales, row codes; 128-byte swizzle, 256 k per stage), 2-3 and 13-14 copy the rows'
-// scale bytes into the layout tcgen05.cp spreads over tensor memory, 1 issues
-// the scale copies and MMAs, 4-11 are the epilogue. tcgen05.mma after
-// tcgen05.cp of one thread are ordered; the reverse is not documented, so the
-// scales in tensor memory have several buffers, and one is refilled only when
-// the MMAs that read it have completed.
+// scales, row codes; 128-byte swizzle, 256 k per stage), 2, 3 (and 13 for NV)
+// copy the rows' scale bytes into the layout tcgen05.cp spreads over tensor
+// memory, 1 issues the scale copies and MMAs, 4-11 are the epilogue, 12 hands
+// out the tiles. tcgen05.mma after tcgen05.cp of one thread are ordered; the
+// reverse is not documented, so the scales in tensor memory have several
+// buffers, and one is refilled only when the MMAs that read it have completed.
+//
+// Measured on one B200 (64 experts of 2 x 2048 x 7168, MX, L2 flushed): one row
+// per expert 150 us = 6.7 TB/s, 128 rows 168 us = 6.3 TB/s, 224 rows 197 us =
+// 4.3 PFLOP/s; a dense 8192^3 product 203 us = 5.4 PFLOP/s (NV 274 us = 4.0).
+// The weights' bytes bound it up to ~200 rows per expert, above that the MMAs,
+// and under steady load the power limit.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -101,8 +107,8 @@ struct alignas(64) Params {
 };
 
 // Instruction descriptor of the block-scaled 4-bit MMAs: A and B e2m1, both
-// K-major, M = 128 (256 for a pair); scale type bit 23 (0: e4m3, 1: e8m0); the scale bytes
-// used within each 32-bit word at bits 29 (A) and 4 (B).
+// K-major, M = 128 (256 for a pair); scale type bit 23 (0: e4m3, 1: e8m0); the
+// scale bytes used within each 32-bit word at bits 29 (A) and 4 (B).
 template <bool NV, bool PAIR>
 WB_DEV uint32_t idesc_fp4(int n) {
   return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((NV ? 0u : 1u) << 23) |

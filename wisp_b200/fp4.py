@@ -120,6 +120,12 @@ class Fp4Rows:
         q._ts = None if tensor_scale is None else tensor_scale.data_ptr()
         return q
 
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """As torch.Tensor.record_stream: the rows are in use on `stream` too."""
+        for t in (self._buf, *(self._views or ()), self.tensor_scale):
+            if t is not None:
+                t.record_stream(stream)
+
     def _split(self) -> tuple[torch.Tensor, torch.Tensor]:
         if self._views is None:
             n, m = self.rows * self.cols // 2, self.rows * self.cols // BLOCK[self.fmt]
@@ -196,10 +202,10 @@ def dequantize(q: Fp4Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 
 class Fp4Weights:
-    """V matrices [n, k] (one per expert) laid out once for the product; with ``up``, V pairs
-    for silu(gate x) * up x. codes [V, n, k/2] stay in use where they are; scales
-    [V, n, k/block] are laid out into a buffer of the object and no longer needed; scale: fp32
-    [V] tensor scales or None."""
+    """V matrices [n, k] (one per expert) laid out once for the product; with ``up`` = (codes,
+    scales[, scale]), V pairs for silu(gate x) * up x. codes [V, n, k/2] stay in use where
+    they are; scales [V, n, k/block] are laid out into a buffer of the object and no longer
+    needed; scale: fp32 [V] tensor scales or None."""
 
     def __init__(self, fmt: int, codes: torch.Tensor, scales: torch.Tensor,
                  scale: torch.Tensor | None = None, up: tuple | None = None):
@@ -210,7 +216,11 @@ class Fp4Weights:
         self.entries, self.n = codes.shape[:2]
         if self.k % 32:
             raise invalid(f"k={self.k} is no multiple of 32")
-        mats = [(codes, scales, scale)] + ([tuple(up)] if up is not None else [])
+        mats = [(codes, scales, scale)]
+        if up is not None:
+            if len(up) not in (2, 3):
+                raise invalid("up: (codes, scales) or (codes, scales, scale)")
+            mats.append(tuple(up) if len(up) == 3 else (*up, None))
         self.cfg = abi.WispFp4Config(fmt, self.entries, self.n, self.k, len(mats) - 1,
                                      abi.WISP_DT_F32)
         self._keep, structs = [], []
