@@ -546,7 +546,7 @@ def _layer(fmt, spec, tokens, seed=11):
     return fp4.Fp4MoeLayer(spec, router, None, gu, dn, tokens, x_scale=xs, h_scale=hs)
 
 
-def _check_layer(layer, x, out):
+def _check_layer(layer, x, out, keep=slice(None)):
     """The layer's output against its own stages, each of which the tests above hold to 64 bits:
     the rows each token was routed to, quantised, multiplied, quantised, multiplied, and summed
     with the routing weights in 64 bits."""
@@ -569,7 +569,28 @@ def _check_layer(layer, x, out):
     mag.index_add_(0, tok.long(), (y * wrow[:, None]).abs())
     # one fused multiply-add per row
     bound = (spec.top_k + 2) * 2.0 ** -24 * mag + 1e-30
-    assert ((out.double() - want).abs() <= bound).all()
+    assert ((out.double() - want).abs() <= bound)[keep].all()
+
+
+@pytest.mark.gpu
+@FMTS
+@pytest.mark.parametrize("tokens", [5, 700])   # rows quantised singly, and gathered
+@pytest.mark.parametrize("shared", [False, True])
+def test_moe_layer_nan_tokens_stay_apart(fmt, tokens, shared):
+    """A token of NaN has no expert under softmax scores: the plan fills fewer rows, and what the
+    workspace holds behind them is not followed."""
+    spec = synth.MoeSpec("nan", 512, 256, 16, 4, has_shared=shared)
+    layer = _layer(fmt, spec, tokens)
+    layer.workspace.fill_(0x7f)
+    x = torch.randn((tokens, spec.hidden), device=DEV).to(torch.bfloat16)
+    bad = torch.zeros(tokens, dtype=torch.bool, device=DEV)
+    bad[1::3] = True
+    x[bad] = float("nan")
+    out = layer.forward(x)
+    layer.check()
+    assert (layer.idx[bad] == -1).all() and (layer.idx[~bad] >= 0).all()
+    _check_layer(layer, x, out, ~bad)
+    assert out[bad].isnan().all() if shared else (out[bad] == 0).all()
 
 
 @pytest.mark.gpu

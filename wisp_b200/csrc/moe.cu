@@ -483,12 +483,17 @@ combine_bf16_kernel(const uint16_t* __restrict__ y, const float* __restrict__ ro
 }
 
 // dst row p = src row row_token[p], for quantised rows: codes in 16-byte and
-// scales in 4-byte words.
+// scales in 4-byte words. A token without a valid logit is routed nowhere, so
+// the plan may fill fewer rows than there are; what row_token holds behind them
+// is no index.
 __global__ void __launch_bounds__(256)
 gather_fp4_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales,
-                  const int* __restrict__ row_token, int code_words, int scale_words,
+                  const int* __restrict__ row_token, int tokens, int code_words, int scale_words,
                   uint4* __restrict__ out_codes, uint32_t* __restrict__ out_scales) {
-  const size_t p = blockIdx.x, t = row_token[p];
+  const size_t p = blockIdx.x;
+  const int src = row_token[p];
+  if (src < 0 || src >= tokens) return;
+  const size_t t = src;
   for (int i = threadIdx.x; i < code_words; i += 256)
     out_codes[p * code_words + i] = __ldg(codes + t * code_words + i);
   for (int i = threadIdx.x; i < scale_words; i += 256)
@@ -607,7 +612,7 @@ extern "C" WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const W
                                stream, err);
     if (e != WISP_OK) return e;
     wb::launch_k(gather_fp4_kernel, b.rows, 256, 0, stream, reinterpret_cast<const uint4*>(ws.tc),
-                 reinterpret_cast<const uint32_t*>(ws.ts), b.row_token, M / 32, M / block / 4,
+                 reinterpret_cast<const uint32_t*>(ws.ts), b.row_token, T, M / 32, M / block / 4,
                  reinterpret_cast<uint4*>(ws.xc), reinterpret_cast<uint32_t*>(ws.xs));
     WB_CUDA_CHECK(cudaGetLastError());
   } else {
