@@ -39,6 +39,19 @@ def test_no_tokens_launch_nothing():
     c = abi.WispBlockNorm(tokens=0, hidden=64, ld_x=64, ld_n=64)
     abi.call("wisp_b200_block_norm", C.byref(c), P, None, None, None, None, None, P, None)
 
+    # rows and a block's output of no tokens have no address
+    c = abi.WispBlockNorm(tokens=0, hidden=64, post_norm=1, gate_kind=1, ld_x=64, ld_y=64,
+                          ld_x_out=64, ld_n=64)
+    abi.call("wisp_b200_block_norm", C.byref(c), None, None, P, P, P, None, None, None)
+
+
+@pytest.mark.gpu
+def test_empty_batch():
+    x, w = torch.empty((0, 64), device=DEV, dtype=torch.bfloat16), torch.ones(64, device=DEV)
+    xo, n = norm.block_norm(x, x.float(), gate=w, post_weight=w, pre_weight=w)
+    assert xo.shape == n.shape == (0, 64)
+    assert norm.block_norm(x)[1].shape == (0, 64)
+
 
 def _run(T, M, x="bf16", y="fp32", w="bf16", gate="channel", n="bf16", post=True, pre=True, rs=1.0,
          off=0.0, eps=1e-6, seed=0, scale=3.0):

@@ -374,6 +374,7 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   if (c.gate_kind < WISP_GATE_NONE || c.gate_kind > WISP_GATE_ELEMENT)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: unknown gate_kind %d", c.gate_kind);
   if (!(c.eps >= 0.f)) return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: eps must be >= 0");
+  if (c.tokens == 0) return WISP_OK;     // (buffers of no rows may have no address)
   if (d_y ? (!d_x_out && !d_n) : !d_n)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: no output (x_out, n)");
   if (!d_y && (c.post_norm || c.gate_kind != WISP_GATE_NONE || d_post_w))
@@ -386,7 +387,6 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
   if (c.ld_x < c.hidden || (d_y && c.ld_y < c.hidden) || (d_x_out && d_y && c.ld_x_out < c.hidden) ||
       (d_n && c.ld_n < c.hidden) || (c.gate_kind == WISP_GATE_ELEMENT && c.ld_gate < c.hidden))
     return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: a row stride is less than hidden=%d", c.hidden);
-  if (c.tokens == 0) return WISP_OK;
   if (!d_x) return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: null pointer argument (x)");
   if ((uintptr_t)d_x % dt_size(c.x_type) || (uintptr_t)d_y % dt_size(c.y_type) ||
       (uintptr_t)d_x_out % dt_size(c.x_type) || (uintptr_t)d_n % dt_size(c.n_type) ||
