@@ -46,6 +46,13 @@ def test_no_tokens_launch_nothing():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 400])
+@pytest.mark.parametrize("M", [8184, 8192, 8193, 8200, 16376, 16383, 16384, 16385, 16392])
+def test_wide_rows(T, M):
+    _run(T, M)
+
+
+@pytest.mark.gpu
 def test_empty_batch():
     x, w = torch.empty((0, 64), device=DEV, dtype=torch.bfloat16), torch.ones(64, device=DEV)
     xo, n = norm.block_norm(x, x.float(), gate=w, post_weight=w, pre_weight=w)

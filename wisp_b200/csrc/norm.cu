@@ -185,7 +185,10 @@ block_norm_warp_kernel(const __grid_constant__ NormParams p) {
   });
 }
 
-// One row per CTA.
+// One row per CTA, V vectors of 8 a thread: as few as 1024 threads allow, since
+// 64 registers hold two of x and y and spill four. (bf16 x, fp32 y, by two
+// instead of four: 4096 x 8200 113 -> 82 us, 2048 x 16384 100 -> 88, 16 x 16384
+// 14.3 -> 10.2. Above 16384 four remain: 1024 x 32768 109 us = 3.1 TB/s.)
 template <int V, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float buf[2][1][32];
@@ -206,6 +209,8 @@ void launch_rows(const NormParams& p, cudaStream_t st) {
     wb::launch_k(block_norm_warp_kernel<2, VEC>, blocks, 32 * kNormWarps, 0, st, p);
   else if (vecs <= 1024)
     wb::launch_k(block_norm_kernel<1, 1024, VEC>, T, (vecs + 31) / 32 * 32, 0, st, p);
+  else if (vecs <= 2048)
+    wb::launch_k(block_norm_kernel<2, 1024, VEC>, T, ((vecs + 1) / 2 + 31) / 32 * 32, 0, st, p);
   else
     wb::launch_k(block_norm_kernel<4, 1024, VEC>, T, ((vecs + 3) / 4 + 31) / 32 * 32, 0, st, p);
 }
