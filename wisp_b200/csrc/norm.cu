@@ -221,8 +221,9 @@ void launch_rows(const NormParams& p, cudaStream_t st) {
 // weights and channel gate for good. The sum of a row's x'^2 goes round
 // together with the sum of the next row's y^2: one barrier per row. (At 4096 x
 // 7168, 10 bytes a value, one row per CTA took 117 us, this ring with two sums
-// after one another 64, with one 53 = 5.5 TB/s; 45 us are the copy rate. What
-// is left is the issue of 28 warps' arithmetic between two barriers.)
+// after one another 64, with one 57 to 59 with L2 flushed, 55 = 5.3 TB/s back to
+// back; 45 us are the copy rate. What is left is the issue of 28 warps'
+// arithmetic between two barriers.)
 constexpr int kNormStages = 8;
 struct RingShape {
   int stages, x_bytes, y_bytes;
@@ -270,6 +271,22 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       if (t < T) issue(i, t);
     }
   }
+  // A thread has columns if it has a first one. (VEC: all eight are there then,
+  // and the accesses check nothing; with a check in each, 4096 x 7168 took 63.5
+  // us instead of 59.4.)
+  const bool in = (VEC ? tid * 8 : tid) < M;
+  auto load_cols = [&](const void* q, int type, int64_t base, float (&v)[8]) {
+    if (VEC)
+      load8(q, type, base + tid * 8, true, 8, v);
+    else
+      load_row<false>(q, type, base, 0, M, tid, nt, v);
+  };
+  auto store_cols = [&](void* q, int type, int64_t base, const float (&v)[8]) {
+    if (VEC)
+      store8(q, type, base + tid * 8, true, 8, v);
+    else
+      store_row<false>(q, type, base, 0, M, tid, nt, v);
+  };
   // columns' factors: a of y / rms(y), b of x' / rms(x')
   float a[8], b[8], w[8];
 #pragma unroll
@@ -296,17 +313,18 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   // bounded) makes the row NaN. The slot may be refilled after the next
   // barrier.
   auto take = [&](int64_t t) {
-    if (mbar_wait(&full[s], ph, &abort)) {
-      const uint8_t* st = ring + s * stage;
+    const bool ok = mbar_wait(&full[s], ph, &abort);
+    const uint8_t* st = ring + s * stage;
+    const float none = ok ? 0.f : __uint_as_float(0x7fffffffu);
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = y[j] = none;
+    if (in && ok) {
       const int ox = VEC ? 0 : (int)((uintptr_t)p.x + t * sx) & 15;
-      load_row<VEC>(st + ox, c.x_type, 0, 0, M, tid, nt, x);
+      load_cols(st + ox, c.x_type, 0, x);
       if (p.y) {
         const int oy = VEC ? 0 : (int)((uintptr_t)p.y + t * sy) & 15;
-        load_row<VEC>(st + rs.x_bytes + oy, c.y_type, 0, 0, M, tid, nt, y);
+        load_cols(st + rs.x_bytes + oy, c.y_type, 0, y);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = y[j] = __uint_as_float(0x7fffffffu);
     }
   };
   auto refill = [&](int64_t t) {      // the slot row t was taken from
@@ -334,14 +352,15 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       if (c.gate_kind == WISP_GATE_TOKEN) r *= load_one(p.gate, c.gate_type, t);
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] *= r * a[j];
-      if (c.gate_kind == WISP_GATE_ELEMENT) {
-        load_row<VEC>(p.gate, c.gate_type, t * c.ld_gate, 0, M, tid, nt, w);
+      if (c.gate_kind == WISP_GATE_ELEMENT && in) {
+        float w[8];
+        load_cols(p.gate, c.gate_type, t * c.ld_gate, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) y[j] *= w[j];
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) x[j] = fmaf(c.residual_scale, x[j], y[j]);
-      if (p.x_out) store_row<VEC>(p.x_out, c.x_type, t * c.ld_x_out, 0, M, tid, nt, x);
+      if (p.x_out && in) store_cols(p.x_out, c.x_type, t * c.ld_x_out, x);
     }
     float xp[8];
 #pragma unroll
@@ -352,11 +371,11 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
     q[1] = square_sum(y, 0.f);
     block_sum(q, buf[flip]);
     if (tn < T) refill(tn);
-    if (p.n) {
+    if (p.n && in) {
       const float r = inv_rms(q[0] * p.inv_m, c.eps);
 #pragma unroll
       for (int j = 0; j < 8; j++) xp[j] *= r * b[j];
-      store_row<VEC>(p.n, c.n_type, t * c.ld_n, 0, M, tid, nt, xp);
+      store_cols(p.n, c.n_type, t * c.ld_n, xp);
     }
   }
 }
