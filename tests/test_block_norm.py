@@ -169,3 +169,49 @@ def test_streams():
         got = norm.block_norm(X, Y)
     s.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# Rows and columns at which every CTA of the many-row form goes through its ring of rows more than
+# twice, with a last round that only some of the CTAs have: 17 rows each through 4 slots (7168),
+# 14 through 5 (3373, rows that start anywhere), 17 through 4 (1024) and 19 through 8 (520).
+RING = [(2500, 7168), (2501, 7167), (4001, 3373), (20_011, 1024), (22_003, 520)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+@pytest.mark.parametrize("T,M", RING)
+def test_many_rows_parts(T, M, gate):
+    for post, pre in ((True, True), (True, False), (False, True), (False, False)):
+        _run(T, M, gate=gate, post=post, pre=pre, rs=-0.5, off=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x", list(DT))
+@pytest.mark.parametrize("y", [None, *DT])
+@pytest.mark.parametrize("T,M", [(2501, 7168), (4001, 3373)])
+def test_many_rows_types(T, M, x, y):
+    for w, n in (("fp16", "bf16"), ("bf16", "fp32"), ("fp32", "fp16")):
+        _run(T, M, x=x, y=y, w=w, n=n, gate="token" if y else "none", post=y is not None, rs=0.7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad,at", [(64, 16), (17, 3)])     # aligned rows, rows that start anywhere
+@pytest.mark.parametrize("T,M", [(11, 200), (900, 72), (2500, 7168), (4001, 3376), (20_011, 1024)])
+def test_in_place_leaves_what_lies_beside(T, M, pad, at):
+    """x' in place in the columns of a wider buffer, n into the columns of another: what lies
+    beside them, and the other inputs, stay as they were."""
+    g = torch.Generator(device=DEV).manual_seed(T + M + pad)
+    big = torch.randn((T, M + pad), generator=g, device=DEV).to(torch.bfloat16)
+    ybig = torch.randn((T, M + pad), generator=g, device=DEV).to(torch.float16)
+    X, Y = big[:, at:at + M], ybig[:, at:at + M]
+    G = torch.randn((T, M), generator=g, device=DEV).to(torch.bfloat16)
+    out = torch.full((T, M + pad), 7.0, device=DEV, dtype=torch.float32)
+    xr, dx, nr, dn = ref.block_norm(X, Y, G, 0.9, None, None, True, True, 1e-6, 0.0)
+    before, ybefore = big.clone(), ybig.clone()
+    xo, no = norm.block_norm(X, Y, gate=G, residual_scale=0.9, x_out=X, n_out=out[:, at:at + M])
+    assert xo.data_ptr() == X.data_ptr() and no.data_ptr() == out[:, at:].data_ptr()
+    ref.check_rounded(X, xr, dx)
+    ref.check_rounded(no, nr, dn)
+    for a, b in ((big, before), (out, torch.full_like(out, 7.0))):
+        assert torch.equal(a[:, :at], b[:, :at]) and torch.equal(a[:, at + M:], b[:, at + M:])
+    assert torch.equal(ybig, ybefore)

@@ -257,6 +257,35 @@ def test_quantize_gathered_strided_and_unaligned(fmt):
 
 @pytest.mark.gpu
 @FMTS
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows", [4737, 4738, 9475])     # 1, 2 and 3 left of fours, 1 of twos
+@pytest.mark.parametrize("cols", [96, 2080])
+def test_quantize_and_back_many_rows(fmt, dtype, rows, cols):
+    """Enough rows that a thread takes several of them: as they lie, gathered (indices outside the
+    input among them), and from rows that start anywhere."""
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    big = torch.randn((rows, cols + 13), generator=g, device=DEV)
+    big *= torch.exp2(torch.randint(-9, 10, (rows, 1), generator=g, device=DEV).float())
+    big = big.to(DT[dtype])
+    x = big[:, :cols].contiguous()
+    ts = fp4.tensor_scale(x) if fmt == NV else None
+    q = _check_quantize(x, fmt, ts)
+    want = ref.values(q.codes, q.scales, fmt, ts)
+    for out in DT.values():
+        ref.check_rounded(fp4.dequantize(q, out), want,
+                          want.abs() * (2.0 ** -24 if fmt == NV else 0.0))
+    apart = big[:, 5:5 + cols]
+    _check_quantize(apart, fmt, ts)
+    src = torch.randint(0, rows, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    src[::7], src[3::11], src[-1] = -1, rows, 1 << 30
+    ok = (src >= 0) & (src < rows)
+    for v in (x, apart):
+        picked = torch.where(ok[:, None], v[src.clamp(0, rows - 1).long()], torch.zeros_like(v[:1]))
+        _check_quantize(v, fmt, ts, rows=src, src=picked)
+
+
+@pytest.mark.gpu
+@FMTS
 def test_quantize_past_32_bit_offsets(fmt):
     rows, cols = 301_000, 7168                    # 2.16e9 values
     x = torch.zeros((rows, cols), dtype=torch.bfloat16, device=DEV)
@@ -348,6 +377,20 @@ def test_product_long_rows_in_short_rings(fmt, k):
         for _ in range(10):
             assert torch.equal(fp4.product(q, w, dev, dtype=torch.float32), out)
         w.check()
+
+
+@pytest.mark.gpu
+@FMTS
+@pytest.mark.parametrize("swiglu", [False, True], ids=["plain", "swiglu"])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,k,counts", [
+    (3840, 2048, [1]),              # 30 feature tiles: K split by 2, four stages each
+    (1000, 2080, [40, 3, 0, 9]),    # the same over ragged segments, nine stages as 4 and 5
+    (6900, 1824, [17]),             # 54 feature tiles, the last of 116 features
+    (200, 2080, [33, 7, 20]),       # by 4, several rounds of 16 rows
+])
+def test_product_split_over_k(fmt, swiglu, dtype, n, k, counts):
+    _run_product(fmt, swiglu, DT[dtype], n, k, counts)
 
 
 @pytest.mark.gpu
@@ -606,6 +649,20 @@ def test_moe_layer(fmt, tokens):
         layer.check()
         _check_layer(layer, x, out)
         assert torch.equal(layer.forward(x), out)
+
+
+@pytest.mark.gpu
+@FMTS
+@pytest.mark.parametrize("tokens", [1, 40, 1100])
+def test_moe_layer_of_several_k_stages(fmt, tokens):
+    """Row lengths of nine and five 256-k stages: K split for one token, a ring that goes round
+    for the others."""
+    layer = _layer(fmt, synth.MoeSpec("deep", 2304, 1152, 8, 2, has_shared=True), tokens)
+    x = torch.randn((tokens, 2304), device=DEV).to(torch.bfloat16)
+    out = layer.forward(x)
+    layer.check()
+    _check_layer(layer, x, out)
+    assert torch.equal(layer.forward(x), out)
 
 
 @pytest.mark.gpu
