@@ -186,9 +186,10 @@ WB_DEV uint32_t cluster_addr(const void* p, uint32_t rank) {
   return r;
 }
 
-// Arrive on an mbarrier of another CTA of this cluster (the default
-// semantics of the instruction; what the waiting side reads is tensor memory
-// and shared memory that the tcgen05 and TMA fences already order).
+// Arrive on an mbarrier of another CTA of this cluster, with the instruction's
+// default scope, which is no cluster's: for handing over tensor memory and
+// shared memory that asynchronous copies have written, never a thread's plain
+// stores (mbar_arrive_remote_release).
 WB_DEV void mbar_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -207,6 +208,15 @@ WB_DEV float4 ld_cluster_f4(uint32_t cluster_ptr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_ptr) : "memory");
   return v;
+}
+
+// Bytes of this CTA's shared memory (16-byte aligned, a multiple of 16) into
+// another CTA's, completing on a barrier of that CTA.
+WB_DEV void bulk_copy_cluster(uint32_t dst_cluster, const void* src, uint32_t bytes,
+                              uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(dst_cluster), "r"(smem_u32(src)), "r"(bytes), "r"(bar_cluster) : "memory");
 }
 
 WB_DEV uint32_t cluster_size() {

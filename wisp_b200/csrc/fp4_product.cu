@@ -13,8 +13,8 @@
 // token tile, and each loads its own weights but only half of the row codes,
 // which halves what the rows cost in L2 traffic, shared memory and power; the
 // even CTA issues all MMAs, the odd CTA's MMA warp only passes on that its
-// stages are full. (At 4096 tokens over 257 experts 3 % faster than single
-// CTAs, at 40 tokens 2 %.) Single CTAs (cta_group::1) take matrices of one
+// stages are full. (At 4096 tokens over 257 experts 4 to 6 % faster than single
+// CTAs, at 40 tokens 3 %, dense 8192^3 12 %.) Single CTAs (cta_group::1) take matrices of one
 // feature tile; and when there are few tiles, clusters of 2 or 4 of them take
 // one tile each and split K: their partial sums meet in shared memory and are
 // added in the order of K.
@@ -22,7 +22,7 @@
 // Warps of a persistent CTA: 0 issues the TMA copies (weights, their prepared
 // scales, row codes; 128-byte swizzle, 256 k per stage), 2, 3 (and 13 for NV)
 // copy the rows' scale bytes into the layout tcgen05.cp spreads over tensor
-// memory, 1 issues the scale copies and MMAs, 4-11 are the epilogue, 12 hands
+// memory (in a pair the even CTA's do, and send the odd one a copy), 1 issues the scale copies and MMAs, 4-11 are the epilogue, 12 hands
 // out the tiles. tcgen05.mma after tcgen05.cp of one thread are ordered; the
 // reverse is not documented, so the scales in tensor memory have several
 // buffers, and one is refilled only when the MMAs that read it have completed.
@@ -459,11 +459,13 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   // for only where another CTA's barriers are used, and the thread that holds
   // the first tile's segment hands that tile out itself.
   if (tid < kMaxStages) {
-    // the copies, a scale warp; in a pair's even CTA also the odd one's word
-    mbar_init(&bars.full[tid], PAIR && rank == 0 ? 3 : 2);
+    // the copies, a scale warp, the odd CTA's word; in the odd CTA all comes by
+    // copies
+    mbar_init(&bars.full[tid], !PAIR ? 2 : rank == 0 ? 3 : 1);
     mbar_init(&bars.empty[tid], 1);
     mbar_init(&bars.tile_full[tid], 1);
-    mbar_init(&bars.tile_empty[tid], 10 + C::kScaleWarps);   // all warps but the scheduler
+    // all warps that walk the tiles
+    mbar_init(&bars.tile_empty[tid], 10 + (rank == 0 ? C::kScaleWarps : 0));
     if (tid < 2) {
       mbar_init(&bars.acc_full[tid], 1);
       mbar_init(&bars.acc_empty[tid], PAIR ? 16 : 8);
@@ -571,7 +573,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   // Few rows leave room for more stages in flight, which is what hides the
   // memory's latency when the weights are most of the traffic.
   const int row_tiles = max_cnt > 128 ? 2 : 1;     // of 128 rows' scales
-  const int off_b = C::kOffSfb + C::kWords * 512 * row_tiles;
+  const int sfb_bytes = C::kWords * 512 * row_tiles, off_b = C::kOffSfb + sfb_bytes;
   // a pair's CTA holds half of the tile's rows, in boxes of 16
   const int stage_bytes = off_b + ((max_cnt + 31) >> 5) * (PAIR ? 2048 : 4096);
   constexpr int kRedBytes = C::kMats * kRedRows * 128 * 4;     // a cluster's partial sums
@@ -598,7 +600,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       const uint8_t* sfu = p.sf_up + sf;
       const int nb = (t.cnt + 31) >> 5;           // (in a pair: half of the rows each)
       const int xrow = t.row0 + rank * nb * 16;
-      const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * kBox * 128;
+      const uint32_t bytes = C::kMats * (kABytes + C::kSfaBytes) + nb * kBox * 128 +
+                             (rank == 1 ? sfb_bytes : 0);     // the even CTA's copy
       for (int kk = k0; kk < k1; kk++) {
         if (!first && !mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort)) { ok = false; break; }
         uint8_t* st = smem + r.s * stage_bytes;
@@ -633,7 +636,13 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     bool ok = true;
     while (ok && tiles.next(bars, t, abort)) {
       for (int kk = k0; kk < k1; kk++) {
-        if (!mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        // All of the odd CTA's stage came by asynchronous copies, whose completion
+        // the barrier reports at cluster scope; the word to the even CTA has no
+        // scope of its own. (Were there plain stores among them, as the scale
+        // warps' once were, it would need cluster-scope release, a fence of about
+        // a microsecond each under load: one token per expert 154 -> 254 us,
+        // dense 8192^3 207 -> 467, with four warps taking turns 162 and 240.)
+        if (!mbar_wait_cluster(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
         if (lane == 0) mbar_arrive_remote(cluster_addr(&bars.full[r.s], 0));
         __syncwarp();
         r.next(S);
@@ -657,7 +666,8 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       tc_fence_after();
       const uint32_t d = tmem + acc.h * cols, du = d + acc.up_offset();
       for (int kk = k0; kk < k1; kk++) {
-        if (!mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        if (PAIR ? !mbar_wait_cluster(&bars.full[r.s], r.ph, abort)
+                 : !mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
         // The scale buffer's last readers are the MMAs of the stage sf_bufs
         // before. (With as many buffers as stages they have completed: their
         // slot has been filled again.)
@@ -715,9 +725,13 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         mbar_wait(&bars.empty[s], s < r.s ? r.ph : r.ph ^ 1, abort, 20000000LL);
       }
     }
-  } else if (warp < kEpiWarp || warp > kSchedWarp) {
+  } else if (rank == 0 && (warp < kEpiWarp || warp > kSchedWarp)) {
     // Row scales. The warps take turns at units of 16 scale bytes per row (two
-    // stages of MX, one of NV). A lane reads the one or two 16-byte words
+    // stages of MX, one of NV). In a pair both CTAs' MMAs take the scales of all
+    // rows: the even CTA's warps put them down here and copy them into the odd
+    // one's stage, so that no plain store of one CTA is handed to a thread of the
+    // other. (Each CTA for itself is up to 4 % faster, and not in order by the
+    // memory model.) A lane reads the one or two 16-byte words
     // around the bytes of rows lane + 32 i (rows may start anywhere), while the
     // warp's last unit waits for its slots, and puts the four rows whose words
     // lie side by side in the layout down at once. (Measured and dropped: every
@@ -781,6 +795,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     };
     int ahead = skip(wi);   // stages of the other warps before this one's next
     fetch();
+    cluster_wait();
     while (q.more && ok) {
       const int n = min(U, k1 - q.kk), at = q.kk * W * 4, nb = min(p.xs_ld - at, 16);
       uint32_t w[4][8];     // [word][row / 32]
@@ -825,13 +840,20 @@ fp4_product_kernel(const __grid_constant__ Params p) {
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.full[r.s]);
+            if (lane == 0) {
+              if (PAIR) {       // (the MMAs of stage i - S have released both CTAs' slots)
+                const uint8_t* sfb = smem + r.s * stage_bytes + C::kOffSfb;
+                bulk_copy_cluster(cluster_addr(sfb, 1), sfb, sfb_bytes,
+                                  cluster_addr(&bars.full[r.s], 1));
+              }
+              mbar_arrive(&bars.full[r.s]);
+            }
             leave();
           }
         }
       }
     }
-  } else if (warp < kSchedWarp) {
+  } else if (warp >= kEpiWarp && warp < kSchedWarp) {
     cluster_wait();
     // Epilogue: warp % 4 is the lane quadrant, the two warps of a quadrant
     // take alternate groups of 16 rows.
@@ -884,7 +906,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       }
       acc.done();
     }
-  } else if (lane == 0) {
+  } else if (warp == kSchedWarp && lane == 0) {
     // Scheduler: finding a tile (a search, a segment read from memory, a
     // division) takes ~1 us, which cost the MMA warp 5 to 24 % of its time.
     const int items = (plan.singles + plan.multi_tiles) * fitems;
@@ -911,7 +933,9 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     }
   }
   __syncwarp();
-  if (warp != 1 && (warp < kEpiWarp || warp >= kSchedWarp)) cluster_wait();
+  // (the others have waited before their first use of the other CTA's barriers)
+  const bool scale_warp = (warp > 1 && warp < kEpiWarp) || warp > kSchedWarp;
+  if (warp == 0 || warp == kSchedWarp || (scale_warp && rank == 1)) cluster_wait();
   tc_fence_before();
   cluster_sync();      // no CTA's memory goes away while another uses it
   tc_fence_after();
