@@ -512,8 +512,8 @@ WispError wisp_b200_fp4_prepare(const WispFp4Config* cfg, const uint8_t* d_scale
  * e = the segment's expert. d_segs: DEVICE array of n_segs <= 1025 segments
  * over the rows, which must not overlap; NULL: all rows through entry 0. Rows
  * in no segment are left as they are. A segment whose expert or rows lie
- * outside the set or the rows is skipped and sets *d_error_flag to 2. ld: elements
- * between output rows. up is NULL unless swiglu. d_out overlaps none of the
+ * outside the set or the rows is skipped and sets bit 2 of *d_error_flag. ld:
+ * elements between output rows. up is NULL unless swiglu. d_out overlaps none of the
  * inputs. d_error_flag as for wisp_b200_grouped_ffn (may be NULL; the call
  * does not clear it). rows = 0 is allowed and launches nothing. */
 WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispFp4Mats* w,
@@ -587,10 +587,11 @@ WispError wisp_b200_rms_rescale(const float* d_in, uint16_t* d_out, int tokens, 
 WispError wisp_b200_pack_rows(const uint16_t* d_x, const int* d_src, int n_rows, int hidden,
                               uint16_t* d_xp, cudaStream_t stream, WispErrCtx* err);
 
-/* Device error word written by the tcgen05 kernels when a bounded wait gave
- * up (nonzero = the results of that launch are invalid): WISP_ERR_TIMEOUT. 2,
- * from wisp_b200_fp4_product alone: a segment was skipped,
- * WISP_ERR_INVALID_ARG. */
+/* Device error word, of two bits that kernels set beside what the word holds.
+ * 1: a bounded wait gave up (the results of that launch are invalid), reported
+ * as WISP_ERR_TIMEOUT whatever else is set. 2, from wisp_b200_fp4_product
+ * alone: a segment was skipped, WISP_ERR_INVALID_ARG. The word is not cleared
+ * here. */
 WispError wisp_b200_check_error_flag(const int* d_error_flag, cudaStream_t stream,
                                      WispErrCtx* err);
 

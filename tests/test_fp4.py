@@ -467,6 +467,27 @@ def test_product_skips_bad_segments(fmt):
 
 
 @pytest.mark.gpu
+def test_error_word_keeps_both_states():
+    """A segment skipped (2) does not hide a wait that was given up (1), in whichever order they
+    came; the wait is what a check reports of the two."""
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    check = lambda: abi.call("wisp_b200_check_error_flag", word.data_ptr(),
+                             torch.cuda.current_stream().cuda_stream)
+    check()
+    for v, code, text in ((1, 7, "waiting"), (2, 4, "segment"), (3, 7, "waiting.*segment")):
+        word.fill_(v)
+        with pytest.raises(RuntimeError, match=rf"wisp engine error \[{code}\].*{text}"):
+            check()
+    g = torch.Generator(device=DEV).manual_seed(15)
+    w = fp4.Fp4Weights(MX, *_mats(g, MX, 2, 64, 64))
+    bad = torch.tensor([(2, 0, 4, 0)], dtype=torch.int32, device=DEV)
+    for before, after in ((0, 2), (1, 3), (2, 2), (3, 3)):
+        w.error_word.fill_(before)
+        fp4.product(_rows(g, MX, 20, 64), w, bad)
+        assert w.error_word.item() == after
+
+
+@pytest.mark.gpu
 @FMTS
 def test_product_of_nonfinite_blocks(fmt):
     """A NaN scale spoils its row's or its feature's products only."""

@@ -123,6 +123,10 @@ WB_DEV bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Bits of a device error word: a bounded wait gave up, a segment was skipped.
+// (Set with atomicOr: neither hides the other, and a word may be shared.)
+constexpr int kErrorTimeout = 1, kErrorSkipped = 2;
+
 // Waits for the phase with the given parity to complete. Gives up after
 // `limit_cycles` SM clocks: sets *abort and returns false, so a lost
 // arrival turns into an error status instead of a hung GPU.

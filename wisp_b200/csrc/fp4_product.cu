@@ -503,7 +503,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
     if (s0 + tid < nseg) {
       v = segment(p, s0 + tid);
       if (!segment_ok(p, v)) {
-        if (p.error_flag && blockIdx.x == 0) atomicMax(p.error_flag, 2);
+        if (p.error_flag && blockIdx.x == 0) atomicOr(p.error_flag, kErrorSkipped);
       } else if (v.rows > 0) {
         per = tile_rows<kUnit>(v.rows, p.cap);
         n = v.rows <= p.cap ? 1 : (v.rows + per - 1) / per;
@@ -948,7 +948,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       tmem_dealloc(tmem, 512);
     }
   }
-  if (tid == 0 && bars.abort && p.error_flag) atomicMax(p.error_flag, 1);
+  if (tid == 0 && bars.abort && p.error_flag) atomicOr(p.error_flag, kErrorTimeout);
 }
 
 // Code rows [rows x k/2 bytes] as a 2D tensor; one box = box_rows x 128 bytes

@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_ffn_kernel(const __grid_c
       }
     }
   }
-  if (threadIdx.x == 0 && L->abort && p.error_flag) atomicExch(p.error_flag, 1);
+  if (threadIdx.x == 0 && L->abort && p.error_flag) atomicOr(p.error_flag, kErrorTimeout);
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, kTmemCols);

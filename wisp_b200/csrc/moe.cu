@@ -684,10 +684,12 @@ extern "C" WispError wisp_b200_check_error_flag(const int* d_error_flag, cudaStr
   int h = 0;
   WB_CUDA_CHECK(cudaMemcpyAsync(&h, d_error_flag, sizeof(int), cudaMemcpyDeviceToHost, stream));
   WB_CUDA_CHECK(cudaStreamSynchronize(stream));
-  if (h == 2)
+  if (h == wb::kErrorSkipped)
     return WB_FAIL(WISP_ERR_INVALID_ARG,
                    "a segment lay outside its weights or rows and was skipped (device error word 2)");
-  if (h) return WB_FAIL(WISP_ERR_TIMEOUT, "a tensor-core kernel gave up waiting (device error word %d)", h);
+  if (h)
+    return WB_FAIL(WISP_ERR_TIMEOUT, "a kernel gave up waiting%s (device error word %d)",
+                   h & wb::kErrorSkipped ? ", and a segment was skipped" : "", h);
   return WISP_OK;
 }
 

@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1) skinny_ffn_kernel(const __grid_co
   else
     sk_consumer<MODE>(p, ring, L, total, stride, warp, lane);
   __syncthreads();
-  if (threadIdx.x == 0 && L->abort && p.error_flag) atomicExch(p.error_flag, 1);
+  if (threadIdx.x == 0 && L->abort && p.error_flag) atomicOr(p.error_flag, kErrorTimeout);
 }
 
 constexpr size_t kSmemBytes = 1024 + (size_t)kStages * kStageBytes + sizeof(SkSmem);
