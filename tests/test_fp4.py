@@ -488,6 +488,22 @@ def test_error_word_keeps_both_states():
 
 
 @pytest.mark.gpu
+def test_check_reports_once():
+    """A check that raised clears what it reported: the products after it are judged by
+    themselves."""
+    g = torch.Generator(device=DEV).manual_seed(16)
+    w = fp4.Fp4Weights(MX, *_mats(g, MX, 2, 64, 64))
+    q = _rows(g, MX, 20, 64)
+    good, bad = (torch.tensor([(e, 0, 4, 0)], dtype=torch.int32, device=DEV) for e in (1, 2))
+    for _ in range(2):
+        fp4.product(q, w, bad)
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*segment"):
+            w.check()
+        fp4.product(q, w, good)
+        w.check()
+
+
+@pytest.mark.gpu
 @FMTS
 def test_product_of_nonfinite_blocks(fmt):
     """A NaN scale spoils its row's or its feature's products only."""

@@ -272,10 +272,16 @@ class Fp4Weights:
         return self.error_word.device
 
     def check(self) -> None:
-        """Raise if a product with these weights gave up waiting or skipped a bad segment."""
+        """Raise if a product with these weights gave up waiting or skipped a bad segment since
+        the last check that raised (which clears what it reports; products on other streams than
+        the current one should have finished). Waits for the current stream."""
         with elsewhere(self.error_word) or contextlib.nullcontext():
-            abi.call("wisp_b200_check_error_flag", self.error_word.data_ptr(),
-                     stream_of(self.error_word))
+            try:
+                abi.call("wisp_b200_check_error_flag", self.error_word.data_ptr(),
+                         stream_of(self.error_word))
+            except RuntimeError:
+                self.error_word.zero_()
+                raise
 
 
 def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
@@ -388,4 +394,6 @@ class Fp4MoeLayer:
         return out
 
     def check(self) -> None:
+        """Raise if a forward of this layer, or another product with its gate and up weights,
+        gave up waiting since the last check that raised."""
         self.gate_up.check()
