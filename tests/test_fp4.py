@@ -360,6 +360,45 @@ def test_product(fmt, swiglu, n, k, counts):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("k,rows", [(32, 1), (32, 200), (2048, 1), (2048, 40)])   # K whole, and split
+def test_swiglu_of_large_gates(dtype, k, rows):
+    """Gates at which exp(-g) is near the end of fp32's range or past it, and silu(g) is small but
+    not 0, times an up value that brings it back. The gates are sums of few multiples of 1/2, so
+    exact; a row of ones by 4-bit values."""
+    gates = [0.0, 0.5, 20.0, 88.0, 100.0, -20.0, -86.5, -87.5, -88.0, -88.5, -89.0, -90.5, -95.0,
+             -100.0, -103.0]
+    codes = torch.zeros((1, len(gates), k), dtype=torch.uint8)
+    for i, v in enumerate(gates):
+        left, j = abs(v), 0
+        while left:
+            c = max(c for c in range(8) if ref.GRID[c] <= left)
+            codes[0, i, j] = c + 8 * (v < 0)
+            left, j = left - ref.GRID[c].item(), j + 1
+        assert j <= 32
+    pack = lambda c: (c[..., 0::2] | c[..., 1::2] << 4).contiguous().to(DEV)
+    sc = lambda n, b: torch.full((n, len(gates), k // 32), b, dtype=torch.uint8, device=DEV)
+    one = torch.zeros((1, len(gates), k), dtype=torch.uint8)
+    one[..., 0] = 2
+    w = fp4.Fp4Weights(MX, pack(codes), sc(1, 127), up=(pack(one), sc(1, 127 + 90)))
+    x = torch.zeros((rows, k), dtype=torch.uint8)
+    x[:, :32] = 2
+    q = fp4.Fp4Rows(MX, pack(x), torch.full((rows, k // 32), 127, dtype=torch.uint8, device=DEV))
+    out = fp4.product(q, w, dtype=DT[dtype]).double().cpu()
+    g, u = torch.tensor(gates, dtype=torch.float64), 2.0 ** 90
+    want = g * torch.sigmoid(g) * u
+    # the exponential of half the gate (1 ulp, and twice for its square), two products, a sum, a
+    # quotient (2 ulp) and the product with u: 8 times 2^-23. Below fp32's normal range the
+    # products and the quotient round by half of 2^-149 each. A 16-bit output: half a step, and the
+    # fast exponential's argument, |g| / 2 * log2(e) rounded to fp32, twice over: |g| 2^-23, with
+    # a factor 2 for the instruction.
+    tol = 8 * 2.0 ** -23 * want.abs() + 3 * 2.0 ** -150 * u
+    if dtype == "bf16":
+        tol = tol + (ref.half_step(torch.bfloat16) + g.abs() * 2.0 ** -22) * want.abs() * 1.001
+    assert ((out - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 @FMTS
 def test_product_more_tiles_than_ctas(fmt):
     _run_product(fmt, False, torch.float16, 2200, 288, [1, 40, 260, 9] * 8)

@@ -94,13 +94,6 @@ __device__ __noinline__ uint32_t nv_scale_exact(float a, float g) {
 // significant bits).
 WB_DEV bool nv_plain_range(float g) { return g >= 1e-30f && g <= 1e30f; }
 
-// 1 / x to 1 ulp, for normal x and 1 / x.
-WB_DEV float rcp_approx(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
 
 // The same for a plain g: the byte of the scaled-down and scaled-up fp32

@@ -15,6 +15,13 @@ namespace wb {
 __host__ __device__ inline int dt_size(int t) { return t == WISP_DT_F32 ? 4 : 2; }
 inline bool dt_valid(int t) { return t == WISP_DT_F32 || t == WISP_DT_BF16 || t == WISP_DT_F16; }
 
+// 1 / x to 1 ulp, for normal x and 1 / x.
+WB_DEV float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 WB_DEV float load_one(const void* p, int type, int64_t i) {
   if (type == WISP_DT_F32) return static_cast<const float*>(p)[i];
   if (type == WISP_DT_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
