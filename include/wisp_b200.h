@@ -458,6 +458,7 @@ enum { WISP_DT_F32 = 0, WISP_DT_BF16 = 1, WISP_DT_F16 = 2 };
  * code, saturated at 6), decided as if by exact arithmetic. A zero scale
  * gives zero codes; a block holding an infinity or a NaN, or a tensor_scale
  * that is not positive and finite, gives the NaN scale byte and zero codes.
+ * d_tensor_scale is not read for MX.
  * rows = 0 is allowed and launches nothing. */
 WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t ld, int x_rows,
                                  const int* d_src, int rows, int cols, int format,
@@ -465,7 +466,9 @@ WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t ld, int x_
                                  uint8_t* d_scales, cudaStream_t stream, WispErrCtx* err);
 
 /* The values of quantised rows, rounded once to out_type (ld elements
- * between output rows). */
+ * between output rows). d_tensor_scale: one fp32 or NULL (1), for NV rows; MX
+ * rows have none, and one given for them is refused (here and in
+ * wisp_b200_fp4_product). */
 WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int rows,
                                    int cols, int format, const float* d_tensor_scale, void* d_out,
                                    int out_type, int64_t ld, cudaStream_t stream,
@@ -491,7 +494,7 @@ typedef struct {
 } WispFp4Mats;
 
 /* Activation rows from wisp_b200_fp4_quantize; tensor_scale: one fp32 or NULL
- * (1). codes 16-byte aligned. */
+ * (1), NULL for MX. codes 16-byte aligned. */
 typedef struct {
     const uint8_t* codes;
     const uint8_t* scales;

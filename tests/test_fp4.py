@@ -79,6 +79,20 @@ def test_product_refuses(kw, match):
              C.byref(x), a["segs"], a["n_segs"], a["out"], a["ld"], None, None, match=match)
 
 
+def test_mx_rows_have_no_tensor_scale():
+    """Refused wherever rows are used, so that their values and their products cannot differ by
+    a scale that only one of the two knows."""
+    why = "MX rows have no tensor scale"
+    _refused("wisp_b200_fp4_dequantize", P, P, 4, 64, MX, P, P, 1, 64, None, match=why)
+    cfg = abi.WispFp4Config(MX, 2, 64, 64, 0, 1)
+    m, x = abi.WispFp4Mats(P, P, P), abi.WispFp4Rows(P, P, P, 3)
+    _refused("wisp_b200_fp4_product", C.byref(cfg), C.byref(m), None, C.byref(x), P, 2, P, 64, None,
+             None, match=why)
+    with pytest.raises(RuntimeError, match=rf"wisp engine error \[4\].*{why}"):
+        fp4.Fp4Rows(MX, torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8),
+                    torch.ones(1))
+
+
 def test_prepare_sizes_and_refusals():
     cfg = abi.WispFp4Config(MX, 3, 130, 288, 0, 1)
     n = abi.lib().wisp_b200_fp4_prepared_bytes(C.byref(cfg))

@@ -328,7 +328,7 @@ template <bool NV, int TYPE, int R>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
   const int64_t row = (int64_t)blockIdx.x * R;
   const int tid = threadIdx.x;
-  const float g = NV && p.ts ? __ldg(p.ts) : 1.f;
+  const float g = p.ts ? __ldg(p.ts) : 1.f;
   const uint8_t* codes = p.codes + row * (p.cols / 2);
   const uint8_t* scales = p.scales + row * (p.cols / (NV ? 16 : 32));
   if (TYPE == WISP_DT_F32) {
@@ -522,6 +522,8 @@ extern "C" WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_dequantize: codes must be 4-byte aligned");
   if ((uintptr_t)d_out % dt_size(out_type))
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_dequantize: out not aligned to its type");
+  if (format == WISP_FP4_MX && d_tensor_scale)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_dequantize: MX rows have no tensor scale");
   DequantParams p;
   p.codes = d_codes;
   p.scales = d_scales;

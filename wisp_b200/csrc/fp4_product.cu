@@ -1043,6 +1043,8 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
     return WB_FAIL(WISP_ERR_INVALID_ARG,
                    "fp4_product: row codes must be 16-byte aligned, out to its type");
   const bool nv = cfg->format == WISP_FP4_NV;
+  if (!nv && x->tensor_scale)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: MX rows have no tensor scale");
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
   // Token tiles of at most `cap` rows, an upper bound: at most one per row, and

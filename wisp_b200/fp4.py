@@ -90,13 +90,16 @@ def _check_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor) -> int:
 
 
 class Fp4Rows:
-    """Quantised rows: codes [rows, cols/2], scales [rows, cols/block], one tensor scale (NV)."""
+    """Quantised rows: codes [rows, cols/2], scales [rows, cols/block], one tensor scale (NV; None
+    stands for 1)."""
 
     def __init__(self, fmt: int, codes: torch.Tensor, scales: torch.Tensor,
                  tensor_scale: torch.Tensor | None = None):
         if codes.dim() != 2:
             raise invalid("rows are 2D")
         self.cols = _check_codes(fmt, codes, scales)
+        if fmt == abi.WISP_FP4_MX and tensor_scale is not None:
+            raise invalid("MX rows have no tensor scale")
         _check_scale(tensor_scale, 1, "tensor_scale")
         same_device(codes, tensor_scale=tensor_scale)
         self.fmt, self.tensor_scale, self.rows = fmt, tensor_scale, codes.shape[0]
@@ -153,7 +156,8 @@ def tensor_scale(x: torch.Tensor) -> torch.Tensor:
 def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None,
              rows: torch.Tensor | None = None) -> Fp4Rows:
     """Rows of x (float32, bfloat16 or float16) as 4-bit codes; rows (int32): row p of the
-    result is row rows[p] of x, a row of zeros where rows[p] is outside x."""
+    result is row rows[p] of x, a row of zeros where rows[p] is outside x. tensor_scale: needed
+    for NV, not used for MX."""
     block = BLOCK.get(fmt)
     if block is None:
         raise invalid(f"unknown format {fmt}")
