@@ -581,6 +581,12 @@ WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* d_x, const 
                                const void* d_gate, const void* d_post_w, const void* d_pre_w,
                                void* d_x_out, void* d_n, cudaStream_t stream, WispErrCtx* err);
 
+/* Device error word of wisp_b200_block_norm on the current device, for
+ * wisp_b200_check_error_flag: set when a wait for a row gave up (that row and
+ * some after it are then NaN); cleared by nobody but its reader. NULL without a
+ * device. */
+int* wisp_b200_block_norm_error_word(void);
+
 /* Between stacked layers: d_out[t] = bf16(d_in[t] / rms(d_in[t])), fp32 in. */
 WispError wisp_b200_rms_rescale(const float* d_in, uint16_t* d_out, int tokens, int hidden,
                                 float eps, cudaStream_t stream, WispErrCtx* err);

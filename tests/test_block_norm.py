@@ -215,3 +215,18 @@ def test_in_place_leaves_what_lies_beside(T, M, pad, at):
     for a, b in ((big, before), (out, torch.full_like(out, 7.0))):
         assert torch.equal(a[:, :at], b[:, :at]) and torch.equal(a[:, at + M:], b[:, at + M:])
     assert torch.equal(ybig, ybefore)
+
+
+@pytest.mark.gpu
+def test_error_word():
+    """A wait that gave up (none can be made to here: the word is set by hand) is reported once."""
+    X = torch.randn((2500, 1024), device=DEV)
+    norm.block_norm(X)
+    norm.check()
+    word = norm.error_word()
+    assert word.shape == (1,) and word.dtype == torch.int32 and word.device == X.device
+    word.fill_(1)
+    with pytest.raises(RuntimeError, match=r"wisp engine error \[7\].*waiting"):
+        norm.check(X.device)
+    assert word.item() == 0
+    norm.check(0)

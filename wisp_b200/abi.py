@@ -162,6 +162,7 @@ SIGNATURES = {
     "wisp_b200_fp4_moe_forward": (_I, [C.POINTER(WispMoeConfig), C.POINTER(WispFp4MoeWeights), _P,
                                        _P, _P, _P, _P, _SZ, _P, _P, _E]),
     "wisp_b200_block_norm": (_I, [C.POINTER(WispBlockNorm), _P, _P, _P, _P, _P, _P, _P, _P, _E]),
+    "wisp_b200_block_norm_error_word": (_P, []),
     "wisp_b200_rms_rescale": (_I, [_P, _P, _I, _I, _F, _P, _E]),
     "wisp_b200_combine_rows": (_I, [_P, _P, _P, _I, _I, _P, _P, _E]),
     "wisp_b200_ep_block_bytes": (_SZ, [_I, _I, _I, _I]),

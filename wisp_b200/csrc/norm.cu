@@ -225,6 +225,7 @@ void launch_rows(const NormParams& p, cudaStream_t st) {
 // back; 45 us are the copy rate. What is left is the issue of 28 warps'
 // arithmetic between two barriers.)
 constexpr int kNormStages = 8;
+__device__ int norm_error;     // kErrorTimeout: a copy never landed
 struct RingShape {
   int stages, x_bytes, y_bytes;
 };
@@ -241,7 +242,7 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kNormStages];
   __shared__ float buf[2][2][32];
-  __shared__ int abort;
+  __shared__ int abort, late;
   const WispBlockNorm& c = p.c;
   const int M = c.hidden, tid = threadIdx.x, nt = blockDim.x, T = c.tokens;
   const int stage = rs.x_bytes + rs.y_bytes;
@@ -262,13 +263,17 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       bulk_load(ring + s * stage + rs.x_bytes,
                 reinterpret_cast<const void*>(word_start(p.y, t * sy)), by, &full[s]);
   };
+  int issued = 0;      // rows (thread 0)
   if (tid == 0) {
-    abort = 0;
+    abort = late = 0;
     for (int i = 0; i < rs.stages; i++) mbar_init(&full[i], 1);
     fence_barrier_init();
     for (int i = 0; i < rs.stages; i++) {
       const int64_t t = blockIdx.x + (int64_t)i * gridDim.x;
-      if (t < T) issue(i, t);
+      if (t < T) {
+        issue(i, t);
+        issued++;
+      }
     }
   }
   // A thread has columns if it has a first one. (VEC: all eight are there then,
@@ -309,11 +314,15 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   int s = 0, flip = 0;
   uint32_t ph = 0;
   float x[8], y[8];
-  // The ring's next row into x and y; a copy that never lands (the wait is
-  // bounded) makes the row NaN. The slot may be refilled after the next
-  // barrier.
+  // The ring's next row into x and y. A copy that never lands (the wait is
+  // bounded) makes its row and later ones NaN: a thread that has given up waits
+  // no more, since a slot's parity could then stand for an older phase, and
+  // thread 0 then issues no more (while it has seen a slot's copy land, the slot
+  // is free, whatever other threads saw). The slot may be refilled after the
+  // next barrier.
+  bool ok = true;
   auto take = [&](int64_t t) {
-    const bool ok = mbar_wait(&full[s], ph, &abort);
+    ok = ok && mbar_wait(&full[s], ph, &abort);
     const uint8_t* st = ring + s * stage;
     const float none = ok ? 0.f : __uint_as_float(0x7fffffffu);
 #pragma unroll
@@ -330,7 +339,10 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
   auto refill = [&](int64_t t) {      // the slot row t was taken from
     if (tid == 0) {
       const int64_t next = t + (int64_t)rs.stages * gridDim.x;
-      if (next < T) issue(s, next);
+      if (next < T && ok) {
+        issue(s, next);
+        issued++;
+      }
     }
     if (++s == rs.stages) {
       s = 0;
@@ -378,9 +390,21 @@ block_norm_stream_kernel(const __grid_constant__ NormParams p, const RingShape r
       store_cols(p.n, c.n_type, t * c.ld_n, xp);
     }
   }
+  // (every wait lies before the last barrier)
+  if (tid == 0 && *static_cast<volatile int*>(&abort)) {
+    atomicOr(&norm_error, kErrorTimeout);
+    // let the copies in flight land before the CTA's memory goes away
+    for (int i = max(issued - rs.stages, 0); i < issued; i++)
+      mbar_wait(&full[i % rs.stages], i / rs.stages & 1, &late, 20000000LL);
+  }
 }
 
 }  // namespace
+
+extern "C" int* wisp_b200_block_norm_error_word(void) {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, norm_error) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+}
 
 extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* d_x,
                                           const void* d_y, const void* d_gate,

@@ -10,6 +10,37 @@ from . import abi
 from .fp4 import DTYPES, elsewhere, invalid, row_stride, stream_of
 
 
+class _ErrorWord:
+    """The current device's error word of wisp_b200_block_norm, as torch.as_tensor takes it."""
+
+    def __init__(self):
+        ptr = abi.lib().wisp_b200_block_norm_error_word()
+        if not ptr:
+            raise RuntimeError("wisp engine error: no CUDA device")
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (ptr, False),
+                                         "version": 2}
+
+
+def error_word(device: torch.device | int | None = None) -> torch.Tensor:
+    """The device's error word (int32 [1], the library's own memory; default: the current
+    device)."""
+    with torch.cuda.device(device):
+        return torch.as_tensor(_ErrorWord(), device="cuda")
+
+
+def check(device: torch.device | int | None = None) -> None:
+    """Raise if a block_norm on the device (default: the current one) gave up waiting for a row
+    since the last check that raised; that row and some after it are NaN. Waits for the device's
+    current stream; calls on its other streams should have finished."""
+    with torch.cuda.device(device):
+        word = error_word()
+        try:
+            abi.call("wisp_b200_check_error_flag", word.data_ptr(), stream_of(word))
+        except RuntimeError:
+            word.zero_()
+            raise
+
+
 def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
                gate: torch.Tensor | None = None, residual_scale: float = 1.0,
                post_weight: torch.Tensor | None = None, pre_weight: torch.Tensor | None = None,
