@@ -45,6 +45,31 @@ def test_no_tokens_launch_nothing():
     abi.call("wisp_b200_block_norm", C.byref(c), None, None, P, P, P, None, None, None)
 
 
+@pytest.mark.parametrize("which", ["x", "y", "gate", "post_weight", "pre_weight", "x_out", "n_out"])
+def test_no_gradient(which):
+    """A gradient that would be lost without a word is refused; without grad mode the call goes on
+    (here to the refusal of CPU tensors)."""
+    kw = dict(y=torch.ones(2, 8), gate=torch.ones(8), post_weight=torch.ones(8),
+              pre_weight=torch.ones(8), x_out=torch.ones(2, 8), n_out=torch.ones(2, 8))
+    x = torch.ones(2, 8)
+    (x if which == "x" else kw[which]).requires_grad_()
+    with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*gradient"):
+        norm.block_norm(x, **kw)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode(), pytest.raises(RuntimeError, match="no CPU path"):
+            norm.block_norm(x, **kw)
+
+
+@pytest.mark.gpu
+def test_parameters_without_grad_mode():
+    x = torch.randn(5, 64, device=DEV)
+    w = torch.nn.Parameter(torch.rand(64, device=DEV))
+    with torch.no_grad():
+        got = norm.block_norm(x, x, post_weight=w, pre_weight=w)
+    want = norm.block_norm(x, x, post_weight=w.detach(), pre_weight=w.detach())
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [3, 400])
 @pytest.mark.parametrize("M", [8184, 8192, 8193, 8200, 16376, 16383, 16384, 16385, 16392])

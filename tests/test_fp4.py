@@ -146,6 +146,15 @@ def test_python_refusals():
             bad()
 
 
+def test_quantize_has_no_gradient():
+    x, ts = torch.zeros(2, 64), torch.ones(1)
+    for a, b in ((x.clone().requires_grad_(), ts), (x, ts.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*gradient"):
+            fp4.quantize(a, NV, b)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            fp4.quantize(a, NV, b)
+
+
 # ---------------------------------------------------------------------------
 # Quantisation
 # ---------------------------------------------------------------------------
@@ -651,6 +660,33 @@ def test_weights_from_values(fmt):
     codes, scales = (torch.stack([m[i] for m in mats]) for i in (0, 1))
     ts = torch.cat([m[2] for m in mats]) if fmt == NV else None
     ref.check_product(out, q, [(codes, scales, ts)], segs, 96)
+
+
+@pytest.mark.gpu
+@FMTS
+def test_products_have_no_gradient(fmt):
+    """An output or an input that requires a gradient is refused under grad mode; weights are
+    constants, laid out from parameters too."""
+    g = torch.Generator(device=DEV).manual_seed(17)
+    wv = torch.randn((2, 64, 96), generator=g, device=DEV)
+    w = fp4.Fp4Weights.from_values(fmt, torch.nn.Parameter(wv))
+    q, (_, segs) = _rows(g, fmt, 9, 96), _segs([4, 5])
+    want = fp4.product(q, fp4.Fp4Weights.from_values(fmt, wv), segs, dtype=torch.float32)
+    assert torch.equal(fp4.product(q, w, segs, dtype=torch.float32), want)
+    out = torch.zeros((9, 64), device=DEV, requires_grad=True)
+    why = r"wisp engine error \[4\].*gradient"
+    with pytest.raises(RuntimeError, match=why):
+        fp4.product(q, w, segs, out=out)
+    with torch.no_grad():
+        fp4.product(q, w, segs, out=out)
+    assert torch.equal(out.detach(), want)
+    layer = _layer(fmt, synth.MoeSpec("soft", 512, 256, 16, 4), 3)
+    x = torch.randn((3, 512), device=DEV).to(torch.bfloat16).requires_grad_()
+    with pytest.raises(RuntimeError, match=why):
+        layer.forward(x)
+    with torch.no_grad():
+        y = layer.forward(x)
+    assert torch.equal(y, layer.forward(x.detach()))
 
 
 @pytest.mark.gpu

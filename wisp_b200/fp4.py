@@ -2,7 +2,9 @@
 
 Thin wrappers over the C ABI (include/wisp_b200.h): tensors are PyTorch CUDA
 tensors used as device memory; every launch goes on the current torch stream
-of the tensors' device. The work itself runs in libwisp_b200.so.
+of the tensors' device. The work itself runs in libwisp_b200.so. For serving: no
+operator has a gradient, and tensors that require one are refused where autograd
+would record the call.
 
     q = quantize(x, abi.WISP_FP4_MX)                # rows -> codes and scales
     w = Fp4Weights(abi.WISP_FP4_MX, codes, scales)  # [V, n, k/2], [V, n, k/32]
@@ -50,6 +52,20 @@ def dtype_code(dtype: torch.dtype, what: str) -> int:
     if code is None:
         raise invalid(f"{what}: {dtype} (float32, bfloat16 or float16)")
     return code
+
+
+def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd would expect a gradient for one of the tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def refuse_grad() -> None:
+    raise invalid("a tensor requires a gradient, and this operator has none (torch.no_grad() or "
+                  "detach() for serving)")
 
 
 def row_stride(t: torch.Tensor, what: str) -> int:
@@ -161,6 +177,8 @@ def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None
     block = BLOCK.get(fmt)
     if block is None:
         raise invalid(f"unknown format {fmt}")
+    if wants_grad(x, tensor_scale):
+        refuse_grad()
     ld = row_stride(x, "x")
     n, cols = x.shape
     if cols % block or cols == 0:
@@ -258,11 +276,13 @@ class Fp4Weights:
 
     @classmethod
     def from_values(cls, fmt: int, w: torch.Tensor, up: torch.Tensor | None = None) -> "Fp4Weights":
-        """Quantises matrices w [V, n, k] (and up), one tensor scale per matrix for NV."""
+        """Quantises matrices w [V, n, k] (and up), one tensor scale per matrix for NV. The set
+        holds constants: parameters may be given, and get no gradient from it."""
         sets = []
         for m in [w] if up is None else [w, up]:
             if m.dim() != 3:
                 raise invalid("weights are [entries, n, k]")
+            m = m.detach()
             ts = None
             if fmt == abi.WISP_FP4_NV:
                 ts = torch.cat([tensor_scale(e) for e in m])
@@ -297,6 +317,8 @@ def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
     if q.fmt != w.fmt or q.cols != w.k:
         raise invalid(f"rows (format {q.fmt}, k={q.cols}) do not fit the weights (format "
                       f"{w.fmt}, k={w.k})")
+    if wants_grad(out, q.tensor_scale):
+        refuse_grad()
     n_segs = 0
     if segments is not None:
         if segments.dtype != torch.int32 or segments.dim() != 2 or segments.shape[1] != 4 or \
@@ -382,6 +404,8 @@ class Fp4MoeLayer:
         shape = (self.cfg.tokens, self.spec.hidden)
         if x.dtype != torch.bfloat16 or not x.is_contiguous() or x.shape != shape:
             raise invalid(f"x: contiguous bfloat16 {shape}")
+        if wants_grad(x, out):
+            refuse_grad()
         same_device(self.workspace, x=x, out=out)
         other = elsewhere(x)
         if other is not None:

@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import abi
-from .fp4 import DTYPES, elsewhere, invalid, row_stride, stream_of
+from .fp4 import DTYPES, elsewhere, invalid, refuse_grad, row_stride, stream_of, wants_grad
 
 
 class _ErrorWord:
@@ -55,8 +55,11 @@ def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     with post_norm(v) = v / sqrt(mean(v^2) + eps) * (weight_offset + post_weight) (v itself with
     post=False) and pre_norm alike. gate: [hidden], [tokens, 1] or [tokens, hidden]; the two
     weights share a dtype. x' has x's dtype (x_out may be x itself), n has ``dtype``; n is None
-    with pre=False."""
+    with pre=False. There is no gradient: under grad mode tensors that require one (parameters
+    among them) are refused."""
     # (One pass over the arguments: at a few rows this function takes longer than its kernel.)
+    if wants_grad(x, y, gate, post_weight, pre_weight, x_out, n_out):
+        refuse_grad()
     ld_x = row_stride(x, "x")
     shape = x.shape
     T, M = shape
