@@ -442,7 +442,8 @@ WispError wisp_b200_ep_combine_f16(const uint16_t* d_yback, const int* d_slot,
  *   WISP_FP4_MX: blocks of 32, scale = 2^(byte - 127) (byte 255: NaN)
  *   WISP_FP4_NV: blocks of 16, scale = e4m3(byte) * tensor_scale, where
  *                tensor_scale is one positive fp32 on the device per matrix
- * Rows are contiguous: cols/2 code bytes and cols/block scale bytes each.
+ * Rows are contiguous: cols/2 code bytes and cols/block scale bytes each, at
+ * most 2^31 - 256 rows a call.
  * ------------------------------------------------------------------------ */
 enum { WISP_FP4_MX = 0, WISP_FP4_NV = 1 };
 enum { WISP_DT_F32 = 0, WISP_DT_BF16 = 1, WISP_DT_F16 = 2 };
@@ -561,7 +562,7 @@ WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const WispFp4MoeWe
 enum { WISP_GATE_NONE = 0, WISP_GATE_CHANNEL = 1, WISP_GATE_TOKEN = 2, WISP_GATE_ELEMENT = 3 };
 
 typedef struct {
-    int tokens;            /* 0 allowed: launches nothing */
+    int tokens;            /* at most 2^31 - 256; 0 allowed: launches nothing */
     int hidden;            /* 1 .. 32768 */
     int x_type, y_type;    /* WISP_DT_*: residual stream, block output */
     int w_type, gate_type; /* norm weights, gate */

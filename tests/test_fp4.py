@@ -146,6 +146,31 @@ def test_python_refusals():
             bad()
 
 
+def test_counts_past_32_bits_are_refused():
+    """The ABI's counts are 32-bit ints: larger ones are refused, not cut off, and so are those
+    that a kernel would round up past 2^31."""
+    most, over = 0x7FFFFF00, 0x7FFFFF01
+    _refused("wisp_b200_fp4_quantize", P, 1, 16, 4, P, over, 16, NV, P, P, P, None, match="2\\^31")
+    _refused("wisp_b200_fp4_dequantize", P, P, over, 32, MX, None, P, 1, 32, None, match="2\\^31")
+    cfg, m = abi.WispFp4Config(MX, 1, 1, 32, 0, 1), abi.WispFp4Mats(P, P, None)
+    for rows, why in ((over, "2\\^31"), (most, "null")):
+        x = abi.WispFp4Rows(P, P, None, rows)
+        _refused("wisp_b200_fp4_product", C.byref(cfg), C.byref(m), None, C.byref(x), None, 0, None, 1,
+                 None, None, match=why)
+    c = abi.WispBlockNorm(tokens=over, hidden=1, ld_x=1, ld_n=1, n_type=1, x_type=1)
+    _refused("wisp_b200_block_norm", C.byref(c), P, None, None, None, None, None, P, None,
+             match="2\\^31")
+    big = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="meta")
+    u8, n = torch.uint8, 2 ** 32 + 4
+    for call in (lambda: fp4.quantize(big(n, 32), MX),
+                 lambda: fp4.quantize(big(4, 32), MX, rows=big(n, dtype=torch.int32)),
+                 lambda: fp4.Fp4Rows(MX, big(n, 16, dtype=u8), big(n, 1, dtype=u8)),
+                 lambda: fp4.Fp4Weights(MX, big(n, 1, 16, dtype=u8), big(n, 1, 1, dtype=u8)),
+                 lambda: norm.block_norm(big(n, 1)), lambda: norm.block_norm(big(4, n))):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*2\^31"):
+            call()
+
+
 def test_quantize_has_no_gradient():
     x, ts = torch.zeros(2, 64), torch.ones(1)
     for a, b in ((x.clone().requires_grad_(), ts), (x, ts.clone().requires_grad_())):
@@ -642,6 +667,26 @@ def test_product_past_32_bit_offsets(fmt):
     for r0 in (0, 524_280, rows - 40):
         part = fp4.Fp4Rows(fmt, q.codes[r0:r0 + 40], q.scales[r0:r0 + 40], q.tensor_scale)
         ref.check_product(out[r0:r0 + 40], part, [mats], [(0, 0, 40)], 32)
+
+
+@pytest.mark.gpu
+def test_product_of_the_most_rows():
+    """2^31 - 256 rows in one segment (34 GB of codes)."""
+    rows = 0x7FFFFF00
+    g = torch.Generator(device=DEV).manual_seed(18)
+    mats = _mats(g, MX, 1, 1, 32)
+    w = fp4.Fp4Weights(MX, *mats)
+    codes = torch.zeros((rows, 16), dtype=torch.uint8, device=DEV)
+    scales = torch.full((rows, 1), 127, dtype=torch.uint8, device=DEV)
+    spots = (0, rows // 2, rows - 50)
+    for r0 in spots:
+        codes[r0:r0 + 50] = torch.randint(0, 256, (50, 16), generator=g, device=DEV, dtype=torch.uint8)
+    out = fp4.product(fp4.Fp4Rows(MX, codes, scales), w, dtype=torch.bfloat16)
+    w.check()
+    for r0 in spots:
+        part = fp4.Fp4Rows(MX, codes[r0:r0 + 50], scales[r0:r0 + 50])
+        ref.check_product(out[r0:r0 + 50], part, [mats], [(0, 0, 50)], 32)
+    assert int((out != 0).sum()) <= 150
 
 
 @pytest.mark.gpu

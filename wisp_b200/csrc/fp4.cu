@@ -468,9 +468,11 @@ extern "C" WispError wisp_b200_fp4_quantize(const void* d_x, int x_type, int64_t
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_quantize: unknown format %d", format);
   if (!dt_valid(x_type))
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_quantize: unknown x_type %d", x_type);
-  if (rows < 0 || x_rows < 0 || cols <= 0 || cols % block_of(format) || ld < cols)
+  if (rows < 0 || rows > wb::kMaxRows || x_rows < 0 || cols <= 0 || cols % block_of(format) ||
+      ld < cols)
     return WB_FAIL(WISP_ERR_INVALID_ARG,
-                   "fp4_quantize: rows=%d x_rows=%d cols=%d ld=%lld (cols a multiple of %d, ld >= cols)",
+                   "fp4_quantize: rows=%d x_rows=%d cols=%d ld=%lld (at most 2^31 - 256 rows, cols a "
+                   "multiple of %d, ld >= cols)",
                    rows, x_rows, cols, (long long)ld, block_of(format));
   if (!d_src && rows > x_rows)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_quantize: rows=%d > x_rows=%d without d_src", rows,
@@ -511,9 +513,10 @@ extern "C" WispError wisp_b200_fp4_dequantize(const uint8_t* d_codes, const uint
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_dequantize: unknown format %d", format);
   if (!dt_valid(out_type))
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_dequantize: unknown out_type %d", out_type);
-  if (rows < 0 || cols <= 0 || cols % block_of(format) || ld < cols)
+  if (rows < 0 || rows > wb::kMaxRows || cols <= 0 || cols % block_of(format) || ld < cols)
     return WB_FAIL(WISP_ERR_INVALID_ARG,
-                   "fp4_dequantize: rows=%d cols=%d ld=%lld (cols a multiple of %d, ld >= cols)",
+                   "fp4_dequantize: rows=%d cols=%d ld=%lld (at most 2^31 - 256 rows, cols a "
+                   "multiple of %d, ld >= cols)",
                    rows, cols, (long long)ld, block_of(format));
   if (rows == 0) return WISP_OK;
   if (!d_codes || !d_scales || !d_out)

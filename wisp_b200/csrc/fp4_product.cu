@@ -176,8 +176,8 @@ template <int UNIT>
 WB_DEV int tile_rows(int rows, int cap) {
   int per = rows;
   if (rows > cap) {
-    const int t = (rows + cap - 1) / cap;
-    per = (rows + t - 1) / t;
+    const int t = (rows - 1) / cap + 1;      // (rows + t may pass 2^31)
+    per = (rows - 1) / t + 1;
   }
   return (per + UNIT - 1) & ~(UNIT - 1);
 }
@@ -514,7 +514,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
         if (p.error_flag && blockIdx.x == 0) atomicOr(p.error_flag, kErrorSkipped);
       } else if (v.rows > 0) {
         per = tile_rows<kUnit>(v.rows, p.cap);
-        n = v.rows <= p.cap ? 1 : (v.rows + per - 1) / per;
+        n = v.rows <= p.cap ? 1 : (v.rows - 1) / per + 1;
       }
     }
     const int most = __reduce_max_sync(0xffffffffu, min(per, v.rows));
@@ -1029,7 +1029,8 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   if (cfg->swiglu && (e = check_mats(up, "up weights", err)) != WISP_OK) return e;
   if (!cfg->swiglu && up)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: up weights without swiglu");
-  if (!x || x->rows < 0) return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: bad rows");
+  if (!x || x->rows < 0 || x->rows > wb::kMaxRows)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: bad rows (0 .. 2^31 - 256)");
   if (d_segs ? (n_segs < 0 || n_segs > kMaxSegs) : n_segs != 0)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: n_segs=%d (0..%d, 0 without segments)",
                    n_segs, kMaxSegs);

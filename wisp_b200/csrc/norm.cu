@@ -413,8 +413,9 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
                                           WispErrCtx* err) {
   if (!cfg) return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: null config");
   const WispBlockNorm& c = *cfg;
-  if (c.tokens < 0 || c.hidden <= 0 || c.hidden > 32768)
-    return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: tokens=%d hidden=%d (1..32768)", c.tokens,
+  if (c.tokens < 0 || c.tokens > wb::kMaxRows || c.hidden <= 0 || c.hidden > 32768)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "block_norm: tokens=%d (at most 2^31 - 256) hidden=%d (1..32768)", c.tokens,
                    c.hidden);
   if (!dt_valid(c.x_type) || !dt_valid(c.y_type) || !dt_valid(c.w_type) ||
       !dt_valid(c.gate_type) || !dt_valid(c.n_type))

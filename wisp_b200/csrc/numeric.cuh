@@ -13,6 +13,9 @@
 namespace wb {
 
 __host__ __device__ inline int dt_size(int t) { return t == WISP_DT_F32 ? 4 : 2; }
+// Rows of one call at most: counts rounded up to a tile or a block stay below
+// 2^31.
+constexpr int kMaxRows = 0x7fffff00;
 inline bool dt_valid(int t) { return t == WISP_DT_F32 || t == WISP_DT_BF16 || t == WISP_DT_F16; }
 
 // 1 / x to 1 ulp, for normal x and 1 / x.

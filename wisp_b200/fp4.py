@@ -20,6 +20,7 @@ import torch
 from . import abi
 
 BLOCK = {abi.WISP_FP4_MX: 32, abi.WISP_FP4_NV: 16}
+INT_MAX = 0x7FFFFFFF     # the ABI's counts are 32-bit; ctypes cuts larger ones off without a word
 DTYPES = {torch.float32: abi.WISP_DT_F32, torch.bfloat16: abi.WISP_DT_BF16,
           torch.float16: abi.WISP_DT_F16}
 
@@ -73,6 +74,8 @@ def row_stride(t: torch.Tensor, what: str) -> int:
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
         raise invalid(f"{what}: a 2D tensor with contiguous rows is needed")
+    if shape[0] > INT_MAX or shape[1] > INT_MAX:
+        raise invalid(f"{what}: {tuple(shape)}, more than 2^31 - 1 rows or columns")
     return stride[0] if shape[0] > 1 else shape[1]
 
 
@@ -97,6 +100,8 @@ def _check_codes(fmt: int, codes: torch.Tensor, scales: torch.Tensor) -> int:
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise invalid("codes and scales must be contiguous")
     k = codes.shape[-1] * 2
+    if max(k, *codes.shape) > INT_MAX:
+        raise invalid(f"codes {tuple(codes.shape)}: more than 2^31 - 1 entries, rows or columns")
     if codes.shape[:-1] != scales.shape[:-1] or k % BLOCK[fmt] or \
             scales.shape[-1] != k // BLOCK[fmt]:
         raise invalid(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} disagree "
@@ -193,6 +198,8 @@ def quantize(x: torch.Tensor, fmt: int, tensor_scale: torch.Tensor | None = None
     if rows is not None:
         if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
             raise invalid("rows: a contiguous 1D int32 tensor")
+        if rows.shape[0] > INT_MAX:
+            raise invalid(f"rows: {rows.shape[0]} indices, more than 2^31 - 1")
         r = rows.shape[0]
     dt = dtype_code(x.dtype, "x")
     other = elsewhere(x)
@@ -324,7 +331,7 @@ def product(q: Fp4Rows, w: Fp4Weights, segments: torch.Tensor | None = None,
         if segments.dtype != torch.int32 or segments.dim() != 2 or segments.shape[1] != 4 or \
                 not segments.is_contiguous():
             raise invalid("segments: a contiguous int32 [S, 4] tensor")
-        n_segs = segments.shape[0]
+        n_segs = min(segments.shape[0], INT_MAX)     # (1025 at most, which the call checks)
     buf = q._buf
     other = elsewhere(buf)
     if other is not None:
