@@ -576,8 +576,8 @@ typedef struct {
 } WispBlockNorm;
 
 /* d_y NULL: no block output (d_x_out, if given, is left as it is). d_post_w /
- * d_pre_w NULL: ones. d_x_out NULL: x' is not stored; it may equal d_x. d_n
- * NULL: no norm after. No other buffers may overlap. */
+ * d_pre_w NULL: ones. d_x_out NULL: x' is not stored; it may equal d_x (with
+ * the same row stride). d_n NULL: no norm after. No other buffers may overlap. */
 WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* d_x, const void* d_y,
                                const void* d_gate, const void* d_post_w, const void* d_pre_w,
                                void* d_x_out, void* d_n, cudaStream_t stream, WispErrCtx* err);

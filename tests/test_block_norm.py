@@ -35,6 +35,12 @@ def test_refusals(kw, match):
         abi.call("wisp_b200_block_norm", C.byref(c), *ptr.values(), None)
 
 
+def test_in_place_needs_the_same_rows():
+    c = abi.WispBlockNorm(tokens=2, hidden=8, x_type=1, n_type=1, ld_x=8, ld_y=8, ld_x_out=16, ld_n=8)
+    with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*in place"):
+        abi.call("wisp_b200_block_norm", C.byref(c), P, 2 * P, None, None, None, P, 3 * P, None)
+
+
 def test_no_tokens_launch_nothing():
     c = abi.WispBlockNorm(tokens=0, hidden=64, ld_x=64, ld_n=64)
     abi.call("wisp_b200_block_norm", C.byref(c), P, None, None, None, None, None, P, None)

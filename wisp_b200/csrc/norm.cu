@@ -437,6 +437,8 @@ extern "C" WispError wisp_b200_block_norm(const WispBlockNorm* cfg, const void* 
       (d_n && c.ld_n < c.hidden) || (c.gate_kind == WISP_GATE_ELEMENT && c.ld_gate < c.hidden))
     return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: a row stride is less than hidden=%d", c.hidden);
   if (!d_x) return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: null pointer argument (x)");
+  if (d_y && d_x_out == d_x && c.ld_x_out != c.ld_x && c.tokens > 1)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "block_norm: x_out in place with another row stride");
   if ((uintptr_t)d_x % dt_size(c.x_type) || (uintptr_t)d_y % dt_size(c.y_type) ||
       (uintptr_t)d_x_out % dt_size(c.x_type) || (uintptr_t)d_n % dt_size(c.n_type) ||
       (uintptr_t)d_post_w % dt_size(c.w_type) || (uintptr_t)d_pre_w % dt_size(c.w_type) ||
