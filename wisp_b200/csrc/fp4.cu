@@ -7,14 +7,14 @@
 // was divided out:
 //   MX: the scale is a power of two; x / scale is exact in fp32.
 //   NV: the scale is e4m3 * tensor_scale (4 + 24 significant bits). x times
-//       the fp32 reciprocal of that product is within 3 roundings (2^-22.4
-//       relative) of the quotient, so the codes of the products with the
-//       reciprocal made 2^-21 smaller and larger enclose the right one. Where
-//       they differ (one value in about 800 for bf16 rows under the tensor
-//       scale of their own maximum), |x| is compared with border * scale by
-//       the sign of one fused multiply-add: border * e4m3 has 7 bits, so the
-//       difference is rounded once and its sign is right. The scale byte
-//       itself is found in the same way.
+//       the fp32 reciprocal of that product, made 2^-21 smaller or larger, is
+//       within 2^-21.7 relative of where exact arithmetic has it (three
+//       roundings and the reciprocal's ulp), so the codes of the two enclose
+//       the right one. Where they differ (one value in about 800 for bf16 rows
+//       under the tensor scale of their own maximum), |x| is compared with
+//       border * scale by the sign of one fused multiply-add: border * e4m3 has
+//       7 bits, so the difference is rounded once and its sign is right. The
+//       scale byte itself is found in the same way.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -224,7 +224,7 @@ WB_DEV uint32_t nv_block(const float (&v)[16], uint32_t top, float g, uint32_t (
 // grid (ceil(rows / R), ceil(cols / 16 / blockDim)): one thread per 16 values
 // of R rows, 32 (16-bit types) or 64 (fp32) bytes read and 8 written for each;
 // the R rows' loads are issued together. 32,768 gathered bf16 rows of 7168: MX
-// 72 us (their reads, 470 MB from L2, bound it), NV 99 us (its ~190
+// 71 us (their reads, 470 MB from L2, bound it), NV 100 to 107 us (its ~190
 // instructions per block do; six CTAs per SM instead of four gave 6 us).
 template <bool NV, typename T, int R>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 6 : 4) quantize_kernel(const QuantParams p) {
@@ -320,7 +320,7 @@ WB_DEV float scale_value(uint32_t sb, bool nv) {
 
 // grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 values of R rows per
 // thread. fp32: in four chunks of 16 bytes blockDim apart, so that a warp's
-// stores are 512 consecutive bytes (14336 x 4096: 63 -> 45 us); 16-bit types:
+// stores are 512 consecutive bytes (14336 x 4096: 63 -> 45 to 48 us); 16-bit types:
 // 16 neighbours, read with one load and written as one sector. code * scale is
 // exact in fp32 (2 x 4 significant bits); the tensor scale and the output type
 // round once each.

@@ -28,10 +28,13 @@
 // buffers, and one is refilled only when the MMAs that read it have completed.
 //
 // Measured on one B200 (64 experts of 2 x 2048 x 7168, MX, L2 flushed): one row
-// per expert 150 us = 6.7 TB/s, 128 rows 168 us = 6.3 TB/s, 224 rows 197 us =
-// 4.3 PFLOP/s; a dense 8192^3 product 203 us = 5.4 PFLOP/s (NV 274 us = 4.0).
-// The weights' bytes bound it up to ~200 rows per expert, above that the MMAs,
-// and under steady load the power limit.
+// per expert 152 us = 6.6 TB/s, 128 rows 170 us = 6.3 TB/s, 224 rows 199 us =
+// 4.2 PFLOP/s; a dense 8192^3 product 209 to 215 us = 5.1 to 5.3 PFLOP/s (NV 281
+// us = 3.9). The weights' bytes bound it up to ~200 rows per expert. Above that
+// the copies into an SM do more than the MMAs: the MMA warp waits a quarter (one
+// matrix) to 45 % (gate/up) of its cycles for a full stage and 10 to 17 % for a
+// scale buffer, with the ring full of copies in flight; and under steady load the
+// power limit lowers the clock (1.27 to 1.45 GHz at prefill).
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"

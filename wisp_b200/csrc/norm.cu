@@ -171,7 +171,8 @@ WB_DEV void norm_row(const NormParams& p, int64_t t, int i, int nt, Sum sum) {
 }
 
 // Rows of at most 512: one per warp, no barrier (65,536 rows of 64: 59 us with
-// the ring below, 27 so; 16,384 of 1024 the other way round, 31 and 47).
+// the ring below, 26 so; 16,384 of 1024 the other way round, 35 and 47). At 64
+// columns 8 of the 32 lanes hold values: four times the copy rate's 6.4 us.
 constexpr int kNormWarps = 8;
 template <int V, bool VEC>
 __global__ void __launch_bounds__(32 * kNormWarps)
@@ -188,7 +189,7 @@ block_norm_warp_kernel(const __grid_constant__ NormParams p) {
 // One row per CTA, V vectors of 8 a thread: as few as 1024 threads allow, since
 // 64 registers hold two of x and y and spill four. (bf16 x, fp32 y, by two
 // instead of four: 4096 x 8200 113 -> 82 us, 2048 x 16384 100 -> 88, 16 x 16384
-// 14.3 -> 10.2. Above 16384 four remain: 1024 x 32768 109 us = 3.1 TB/s.)
+// 14.3 -> 10.2. Above 16384 four remain: 1024 x 32768 109 to 114 us = 3.0 TB/s.)
 template <int V, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) block_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float buf[2][1][32];
@@ -221,9 +222,10 @@ void launch_rows(const NormParams& p, cudaStream_t st) {
 // weights and channel gate for good. The sum of a row's x'^2 goes round
 // together with the sum of the next row's y^2: one barrier per row. (At 4096 x
 // 7168, 10 bytes a value, one row per CTA took 117 us, this ring with two sums
-// after one another 64, with one 57 to 59 with L2 flushed, 55 = 5.3 TB/s back to
+// after one another 64, with one 59 to 61 with L2 flushed, 55 = 5.3 TB/s back to
 // back; 45 us are the copy rate. What is left is the issue of 28 warps'
-// arithmetic between two barriers.)
+// arithmetic between two barriers. Rows that start anywhere, whose values are
+// read and written one by one: 3952 x 3373 44 to 51 us, copy rate 20.)
 constexpr int kNormStages = 8;
 __device__ int norm_error;     // kErrorTimeout: a copy never landed
 struct RingShape {
