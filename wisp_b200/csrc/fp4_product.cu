@@ -38,6 +38,7 @@
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
+#include "tiles.cuh"
 
 namespace {
 
@@ -45,7 +46,6 @@ using namespace wb;
 
 constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
 constexpr int kSchedWarp = 12;    // then the scale warps after 2 and 3
-constexpr int kMaxSegs = 1025;
 constexpr int kABytes = 128 * 128;
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 218 * 1024;
@@ -150,119 +150,12 @@ WB_DEV void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
                  : "memory");
 }
 
-// Arrive on a barrier (of both CTAs of a pair) when the MMAs and copies issued
-// so far have completed.
-template <bool PAIR>
-WB_DEV void commit(uint64_t* bar) {
-  if constexpr (PAIR)
-    mma_commit_pair(bar);
-  else
-    mma_commit(bar);
-}
-
 // Shared-memory descriptor of a 512-byte scale tile: no swizzle, 8-row groups
 // of 16-byte rows 128 bytes apart.
 WB_DEV uint64_t scale_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) |
          ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
 }
-
-struct Tile {
-  int expert, row0, cnt;   // rows row0 .. row0 + cnt - 1
-  int ft;                  // features 128 ft ..
-};
-
-// Rows per tile of a segment: as many tiles as at most `cap` rows each demand,
-// of equal size up to the MMA's granularity UNIT (16; 32 in a pair, 16 rows per
-// CTA).
-template <int UNIT>
-WB_DEV int tile_rows(int rows, int cap) {
-  int per = rows;
-  if (rows > cap) {
-    const int t = (rows - 1) / cap + 1;      // (rows + t may pass 2^31)
-    per = (rows - 1) / t + 1;
-  }
-  return (per + UNIT - 1) & ~(UNIT - 1);
-}
-
-WB_DEV WispSegment segment(const Params& p, int s) {
-  if (p.segs) return p.segs[s];
-  WispSegment v;
-  v.expert = 0;
-  v.row_begin = 0;
-  v.rows = p.rows;
-  v.reserved = 0;
-  return v;
-}
-
-WB_DEV bool segment_ok(const Params& p, const WispSegment& v) {
-  return v.rows >= 0 && v.row_begin >= 0 && (int64_t)v.row_begin + v.rows <= p.rows &&
-         (v.rows == 0 || (v.expert >= 0 && v.expert < p.V));
-}
-
-// The work: each token tile has `fitems` items (feature tiles, or pairs of
-// them). Segments of one token tile and those of several are listed apart, in
-// order (the second list from the end of the arrays); pref holds the tiles
-// before a segment within its list. A single tile's weights come from memory
-// while the tiles after the first of a larger segment find theirs in the L2
-// cache, so the items of the two lists are dealt out evenly over the launch,
-// each list in its order.
-struct Plan {
-  const int* pref;
-  const uint16_t* order;
-  int singles, multis, multi_tiles;     // segments of one, of several tiles; tiles of these
-  int fitems;
-};
-
-template <int UNIT>
-__device__ __noinline__ Tile find_tile(const Params& p, const Plan& q, int it) {
-  const int fitems = q.fitems, single = q.singles * fitems;
-  const int items = single + q.multi_tiles * fitems;
-  int i = it;
-  bool one = q.multi_tiles == 0;
-  if (q.multi_tiles > 0 && single > 0) {
-    const int before = (int)((int64_t)it * single / items);     // singles among the items before
-    const int after = (int)((int64_t)(it + 1) * single / items);
-    one = after > before;
-    i = one ? before : it - before;
-  }
-  int tt = i / fitems;
-  Tile t;
-  t.ft = i - tt * fitems;
-  int at = tt;                  // its place in the list
-  if (!one) {
-    int lo = 0, hi = q.multis;       // the last segment with pref <= tt
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (q.pref[kMaxSegs - 1 - m] <= tt)
-        lo = m;
-      else
-        hi = m;
-    }
-    at = kMaxSegs - 1 - lo;
-    tt -= q.pref[at];
-  } else {
-    tt = 0;
-  }
-  const WispSegment v = segment(p, q.order[at]);
-  const int per = tile_rows<UNIT>(v.rows, p.cap);
-  t.expert = v.expert;
-  t.row0 = v.row_begin + tt * per;
-  t.cnt = min(per, v.rows - tt * per);
-  return t;
-}
-
-// A position in the ring of stages.
-struct Ring {
-  int s = 0;
-  uint32_t ph = 0;     // parity of the slot's current use
-  WB_DEV void next(int S) {
-    if (++s == S) {
-      s = 0;
-      ph ^= 1;
-    }
-  }
-};
 
 // The accumulators: two halves of `cols` columns. A tile of one matrix, or a
 // gate/up tile of at most cols / 2 rows (up cols / 2 columns after gate), takes
@@ -288,26 +181,6 @@ struct Acc {
     if (!both) nxt ^= 1;
   }
 };
-
-WB_DEV void put_out(float* q, float v) { *q = v; }
-WB_DEV void put_out(__nv_bfloat16* q, float v) { *q = __float2bfloat16_rn(v); }
-WB_DEV void put_out(__half* q, float v) { *q = __float2half_rn(v); }
-
-// silu(g) * u, with h = exp(-|g| / 2): g / (1 + h^2), or g h^2 / (1 + h^2) for a
-// negative g. Nothing overflows, and the divisor lies in [1, 2]. (With
-// g / (1 + exp(-g)) and a quick quotient, which is 0 for divisors above 2^126,
-// the result is 0 from g = -87.4 down, where silu is still 1e-36; the time is
-// the same.) 16-bit outputs take the quick power of two for the exponential,
-// whose error, about |g| 2^-23 relative, is far below theirs.
-template <typename T>
-WB_DEV float swiglu(float g, float u) {
-  float h;
-  if (sizeof(T) == 4)
-    h = expf(-0.5f * fabsf(g));
-  else     // exp(-|g| / 2) = 2^(-|g| / (2 ln 2)); 0 below 2^-126, where g h^2 is 0 too
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(g) * -0.72134752f));
-  return (g < 0.f ? g * h * h : g) * rcp_approx(fmaf(h, h, 1.f)) * u;
-}
 
 // One warp's part of a tile: its lane's feature f, rows 16 half + 32 i ...
 // Everything is fp32 until the one rounding to the output type.
@@ -415,29 +288,6 @@ struct Reduce {
   }
 };
 
-// A role's walk through the tiles that the scheduler warp puts into the ring.
-struct Tiles {
-  int s = 0;
-  uint32_t ph = 0;
-  // Every lane gets the tile; false: no more, or the wait was given up.
-  WB_DEV bool next(Bars& bars, Tile& t, volatile int* abort) {
-    const bool ok = mbar_wait(&bars.tile_full[s], ph, abort);
-    if (!__all_sync(0xffffffffu, ok)) return false;
-    const int4 v = bars.tile[s];
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars.tile_empty[s]);
-    if (++s == kTileRing) {
-      s = 0;
-      ph ^= 1;
-    }
-    t.expert = __shfl_sync(0xffffffffu, v.x, 0);
-    t.row0 = __shfl_sync(0xffffffffu, v.y, 0);
-    t.cnt = __shfl_sync(0xffffffffu, v.z, 0);
-    t.ft = __shfl_sync(0xffffffffu, v.w, 0);
-    return t.expert >= 0;
-  }
-};
-
 template <bool NV, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(Shape<NV, SWIGLU>::kThreads, 1)
 fp4_product_kernel(const __grid_constant__ Params p) {
@@ -453,6 +303,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   volatile int* abort = &bars.abort;
   constexpr int kUnit = PAIR ? 32 : 16;
+  using Cut = EvenCut<kUnit>;
   constexpr int kBox = PAIR ? 16 : 32;            // rows per copy of row codes
   // pair: this CTA's place in it; else the K split: kp of ks
   const int rank = PAIR ? (int)cluster_rank() : 0;
@@ -495,84 +346,14 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   }
   const int group = PAIR ? 2 : ks;                   // CTAs that share a tile
   const int it0 = blockIdx.x / group, it_step = gridDim.x / group;
-  // The lists of segments and the largest tile: a scan over (segments of one
-  // tile | segments of several << 16, tiles of these), kThreads segments at a
-  // time. (Loops are not unrolled: this runs once, from cold instructions.)
-  Plan plan;
-  plan.pref = pref;
-  plan.order = order;
-  plan.singles = plan.multis = plan.multi_tiles = 0;
-  plan.fitems = fitems;
-  int max_cnt = 0;
-  bool first_done = false;
-  const int nseg = p.segs ? p.nseg : 1;
-#pragma unroll 1
-  for (int s0 = 0; s0 < nseg; s0 += kThreads) {
-    WispSegment v;
-    v.rows = 0;
-    int n = 0, per = 0;
-    if (s0 + tid < nseg) {
-      v = segment(p, s0 + tid);
-      if (!segment_ok(p, v)) {
-        if (p.error_flag && blockIdx.x == 0) atomicOr(p.error_flag, kErrorSkipped);
-      } else if (v.rows > 0) {
-        per = tile_rows<kUnit>(v.rows, p.cap);
-        n = v.rows <= p.cap ? 1 : (v.rows - 1) / per + 1;
-      }
-    }
-    const int most = __reduce_max_sync(0xffffffffu, min(per, v.rows));
-    const int kind = n == 0 ? 0 : n == 1 ? 1 : 1 << 16, many = n > 1 ? n : 0;
-    int x = kind, z = many;
-#pragma unroll 1
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y0 = __shfl_up_sync(0xffffffffu, x, o), y1 = __shfl_up_sync(0xffffffffu, z, o);
-      if (lane >= o) {
-        x += y0;
-        z += y1;
-      }
-    }
-    if (s0 > 0) __syncthreads();          // the last round's totals have been read
-    if (lane == 31) warp_tot[warp] = make_int4(x, z, most, 0);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (s0 == 0) cluster_arrive();
-    // every warp scans the warps' totals
-    const int4 w = lane < kThreads / 32 ? warp_tot[lane] : make_int4(0, 0, 0, 0);
-    int wx = w.x, wz = w.y;
-#pragma unroll 1
-    for (int o = 1; o < 16; o <<= 1) {
-      const int y0 = __shfl_up_sync(0xffffffffu, wx, o), y1 = __shfl_up_sync(0xffffffffu, wz, o);
-      if (lane >= o) {
-        wx += y0;
-        wz += y1;
-      }
-    }
-    max_cnt = max(max_cnt, __reduce_max_sync(0xffffffffu, w.z));
-    const int bx = __shfl_sync(0xffffffffu, wx - w.x, warp) + x - kind;
-    const int bz = __shfl_sync(0xffffffffu, wz - w.y, warp) + z - many;
-    if (n == 1) {
-      const int at = plan.singles + (bx & 0xffff);
-      order[at] = (uint16_t)(s0 + tid);
-    } else if (n > 1) {
-      const int at = kMaxSegs - 1 - (plan.multis + (bx >> 16));
-      order[at] = (uint16_t)(s0 + tid);
-      pref[at] = plan.multi_tiles + bz;
-    }
-    // The first tile, when every segment is one tile and this thread has it.
-    const int tx = __shfl_sync(0xffffffffu, wx, 15);
-    first_done = nseg <= kThreads && tx > 0 && tx < (1 << 16) && it0 < tx * fitems;
-    if (first_done && n == 1) {
-      const int ft = it0 - (bx & 0xffff) * fitems;
-      if (ft >= 0 && ft < fitems) {
+  int max_cnt;
+  bool first_done;
+  const Plan plan = make_plan<Cut, kThreads>(
+      p, fitems, it0, pref, order, warp_tot, max_cnt, first_done,
+      [&](const WispSegment& v, int ft) {
         bars.tile[0] = make_int4(v.expert, v.row_begin, v.rows, PAIR ? 2 * ft + rank : ft);
         mbar_arrive(&bars.tile_full[0]);
-      }
-    }
-    plan.singles += tx & 0xffff;
-    plan.multis += tx >> 16;
-    plan.multi_tiles += __shfl_sync(0xffffffffu, wz, 15);
-  }
+      });
   // the scheduler warp reads pref and order
   __syncwarp();
   if (warp == kSchedWarp)
@@ -596,7 +377,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
   // half can hold gate and up), buffers of scales
   const int cols = min(max((max_cnt + 31) & ~31, 32) * C::kMats, C::kMaxN);
   const int sf_bufs = min(S, (512 - 2 * cols) / C::kSfCols);
-  Tiles tiles;
+  TileWalk<kTileRing> tiles;
   Tile t;
 
   if (warp == 0) {
@@ -929,7 +710,7 @@ fp4_product_kernel(const __grid_constant__ Params p) {
       v.expert = -1;
       v.row0 = v.cnt = v.ft = 0;
       if (it < items) {
-        v = find_tile<kUnit>(p, plan, it);
+        v = find_tile<Cut>(p, plan, it);
         if (PAIR) v.ft = 2 * v.ft + rank;
       }
       if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) break;
