@@ -550,6 +550,141 @@ WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const WispFp4MoeWe
                                     int* d_error_flag, cudaStream_t stream, WispErrCtx* err);
 
 /* --------------------------------------------------------------------------
+ * 8-bit block-scaled operands ("fp8"): e4m3 values (largest 448, codes 0x7f and
+ * 0xff NaN) with fp32 scales, one per 128 consecutive values of an activation
+ * row and one per 128 x 128 block of a weight matrix; the last blocks may be
+ * shorter. No counterpart in the reference.
+ * Code rows are contiguous and 16-byte aligned, their length a multiple of 16, at
+ * most 2^27; a call takes at most 2^31 - 256 rows. The scale of row p and block b
+ * lies at scales[p * scale_row + b * scale_block] (scale_row = 1 and scale_block =
+ * the rows or more suit the product: a block's scales are then read together).
+ * ------------------------------------------------------------------------ */
+
+/* Quantises rows: row p of the result is row d_src[p] of d_x (d_src NULL: row p;
+ * an index outside [0, x_rows) gives a row of zeros). d_x has x_rows rows of cols
+ * values of x_type, ld elements apart. Per block, with a = max|x|:
+ *   scale = fp32(a / 448), or with pow2 the least power of two that is not below
+ *           a / 448, at least 2^-126; 0 for a = 0
+ * and each code is the e4m3 value nearest to x / scale (ties to the even code,
+ * saturated at 448), decided as if by exact arithmetic. A zero scale gives zero
+ * codes; a block holding an infinity or a NaN gives a NaN scale and zero codes.
+ * rows = 0 is allowed and launches nothing. */
+WispError wisp_b200_fp8_quantize(const void* d_x, int x_type, int64_t ld, int x_rows,
+                                 const int* d_src, int rows, int cols, int pow2,
+                                 uint8_t* d_codes, float* d_scales, int64_t scale_row,
+                                 int64_t scale_block, cudaStream_t stream, WispErrCtx* err);
+
+/* The values of quantised rows: code * scale in fp32, rounded to out_type (ld
+ * elements between output rows). */
+WispError wisp_b200_fp8_dequantize(const uint8_t* d_codes, const float* d_scales,
+                                   int64_t scale_row, int64_t scale_block, int rows, int cols,
+                                   void* d_out, int out_type, int64_t ld, cudaStream_t stream,
+                                   WispErrCtx* err);
+
+/* Quantises matrices d_w [n_entries x n x k] of w_type (contiguous) to codes of
+ * the same shape and scales [n_entries x ceil(n / 128) x ceil(k / 128)], by the
+ * rule above over blocks of 128 x 128. At most 65535 matrices and 65535 * 128
+ * rows each. */
+WispError wisp_b200_fp8_quantize_weights(const void* d_w, int w_type, int n_entries, int n, int k,
+                                         uint8_t* d_codes, float* d_scales, cudaStream_t stream,
+                                         WispErrCtx* err);
+
+/* A set of n_entries matrices [n x k] (one per expert), used by one product. */
+typedef struct {
+    int n_entries;
+    int n;         /* output features, any n >= 1 */
+    int k;         /* multiple of 16, at most 2^27 */
+    int swiglu;    /* 1: silu(gate x) * up x over two sets, 0: one set */
+    int out_type;  /* WISP_DT_* */
+} WispFp8Config;
+
+/* codes [n_entries x n x k], 16-byte aligned; scales [n_entries x ceil(n / 128) x
+ * ceil(k / 128)]. Both contiguous and used where they lie. */
+typedef struct {
+    const uint8_t* codes;
+    const float* scales;
+} WispFp8Mats;
+
+/* Activation rows from wisp_b200_fp8_quantize. */
+typedef struct {
+    const uint8_t* codes;
+    const float* scales;
+    int64_t scale_row, scale_block;
+    int rows;
+} WispFp8Rows;
+
+/* out[p, f] = sum_k x[p, k] w_e[f, k] for every row p of every segment, e = the
+ * segment's expert (with swiglu silu(w x) * (up x)). Each block of 128 k is summed
+ * on the tensor cores in fp32, scaled by its two scales and added up in fp32; the
+ * sum is rounded once to out_type. d_segs, n_segs, ld, up, the rows in no segment
+ * and d_error_flag as for wisp_b200_fp4_product. rows = 0 is allowed and launches
+ * nothing. */
+WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispFp8Mats* w,
+                                const WispFp8Mats* up, const WispFp8Rows* x,
+                                const WispSegment* d_segs, int n_segs, void* d_out, int64_t ld,
+                                int* d_error_flag, cudaStream_t stream, WispErrCtx* err);
+
+/* --------------------------------------------------------------------------
+ * Routing from logits, with a bias for balance.
+ *   score  = softmax(logits) over the token's experts, or sigmoid(logit)
+ *   choice = score + bias                     (the bias chooses, it does not weigh)
+ *   of n_groups groups of consecutive experts the topk_groups best are kept, by the
+ *   sum of their group_top largest choices; of the kept groups' experts the top_k
+ *   of largest choice are taken, in that order
+ *   weight = score (renormalize: / the sum over the token's top_k) * scaling
+ * Scores, choices and weights are computed in fp64 and the weights rounded once;
+ * equal choices go to the lower expert, equal groups to the lower group. An expert
+ * whose choice is NaN or -infinity is never taken and adds nothing to its group's
+ * sum (a NaN or +infinite logit makes all of a token's softmax scores NaN); where
+ * fewer than top_k are left, the remaining slots have index -1 and weight 0, which
+ * wisp_b200_dispatch_plan routes nowhere. (wisp_b200_route, whose bias enters before
+ * the scores, is the other form.)
+ * ------------------------------------------------------------------------ */
+enum { WISP_ROUTE_SOFTMAX = 0, WISP_ROUTE_SIGMOID = 1 };
+
+typedef struct {
+    int scoring;        /* WISP_ROUTE_* */
+    int n_groups;       /* 1..32, n_experts % n_groups == 0 */
+    int topk_groups;    /* 1..n_groups */
+    int group_top;      /* 1 or 2 */
+    int renormalize;
+    float scaling;
+} WispRouting;
+
+/* d_logits: tokens rows of n_experts (<= 1024) values of logits_type, ld elements
+ * apart. d_bias: fp32 [n_experts] or NULL. d_idx, d_w: [tokens x top_k], top_k <=
+ * min(32, the kept groups' experts). tokens = 0 is allowed and launches nothing. */
+WispError wisp_b200_select_experts(const WispRouting* routing, const void* d_logits,
+                                   int logits_type, int64_t ld, int tokens, int n_experts,
+                                   int top_k, const float* d_bias, int* d_idx, float* d_w,
+                                   cudaStream_t stream, WispErrCtx* err);
+
+/* The MoE layer of wisp_b200_moe_forward over fp8 experts: route, dispatch plan,
+ * quantise the rows, gate/up product with SwiGLU (bf16 rows), quantise, down
+ * product (bf16 rows), each token's rows summed in fp32 in a fixed order with the
+ * routing weights. gate, up: sets of E (+1 shared) entries [inter x hidden], down:
+ * [hidden x inter]. routing NULL: cfg's scoring, as the other layers route; else
+ * the logits (router_bias added) are routed as wisp_b200_select_experts does, with
+ * score_bias as its bias, and cfg's scoring, n_groups, topk_groups and
+ * routed_scaling are ignored, as group_size and deterministic always are (every run
+ * gives the same bits). d_x, router_w and d_out 16-byte aligned, the workspace
+ * 256-byte. One call at a time per workspace. */
+typedef struct {
+    const uint16_t* router_w;   /* as in WispMoeWeights */
+    const float* router_bias;   /* added to the logits; may be NULL */
+    const float* score_bias;    /* added to the scores for the choice; may be NULL */
+    WispFp8Mats gate, up, down;
+    int pow2;                   /* scales of the quantised rows are powers of two */
+} WispFp8MoeWeights;
+
+size_t wisp_b200_fp8_moe_workspace_bytes(const WispMoeConfig* cfg, const WispRouting* routing);
+WispError wisp_b200_fp8_moe_forward(const WispMoeConfig* cfg, const WispRouting* routing,
+                                    const WispFp8MoeWeights* w, const uint16_t* d_x, float* d_out,
+                                    int* d_topk_idx, float* d_topk_w, void* d_workspace,
+                                    size_t workspace_bytes, int* d_error_flag,
+                                    cudaStream_t stream, WispErrCtx* err);
+
+/* --------------------------------------------------------------------------
  * Norms around a block, with its gate and its residual (the reference runs
  * them as op_rmsnorm, op_residual and op_rmsnorm over fp32,
  * csrc/core/wisp_engine.c:1715-1722):
@@ -599,8 +734,8 @@ WispError wisp_b200_pack_rows(const uint16_t* d_x, const int* d_src, int n_rows,
 
 /* Device error word, of two bits that kernels set beside what the word holds.
  * 1: a bounded wait gave up (the results of that launch are invalid), reported
- * as WISP_ERR_TIMEOUT whatever else is set. 2, from wisp_b200_fp4_product
- * alone: a segment was skipped, WISP_ERR_INVALID_ARG. The word is not cleared
+ * as WISP_ERR_TIMEOUT whatever else is set. 2, from wisp_b200_fp4_product and
+ * wisp_b200_fp8_product: a segment was skipped, WISP_ERR_INVALID_ARG. The word is not cleared
  * here. */
 WispError wisp_b200_check_error_flag(const int* d_error_flag, cudaStream_t stream,
                                      WispErrCtx* err);

@@ -30,6 +30,8 @@ WISP_SCORE_SIGMOID_GROUPED = 1
 
 WISP_FP4_MX = 0
 WISP_FP4_NV = 1
+WISP_ROUTE_SOFTMAX = 0
+WISP_ROUTE_SIGMOID = 1
 WISP_DT_F32 = 0
 WISP_DT_BF16 = 1
 WISP_DT_F16 = 2
@@ -97,6 +99,31 @@ class WispFp4MoeWeights(C.Structure):
                 ("h_scale", C.c_void_p), ("format", C.c_int)]
 
 
+class WispFp8Config(C.Structure):
+    _fields_ = [("n_entries", C.c_int), ("n", C.c_int), ("k", C.c_int), ("swiglu", C.c_int),
+                ("out_type", C.c_int)]
+
+
+class WispFp8Mats(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class WispFp8Rows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("scale_row", C.c_int64),
+                ("scale_block", C.c_int64), ("rows", C.c_int)]
+
+
+class WispRouting(C.Structure):
+    _fields_ = [("scoring", C.c_int), ("n_groups", C.c_int), ("topk_groups", C.c_int),
+                ("group_top", C.c_int), ("renormalize", C.c_int), ("scaling", C.c_float)]
+
+
+class WispFp8MoeWeights(C.Structure):
+    _fields_ = [("router_w", C.c_void_p), ("router_bias", C.c_void_p), ("score_bias", C.c_void_p),
+                ("gate", WispFp8Mats), ("up", WispFp8Mats), ("down", WispFp8Mats),
+                ("pow2", C.c_int)]
+
+
 class WispBlockNorm(C.Structure):
     _fields_ = [("tokens", C.c_int), ("hidden", C.c_int), ("x_type", C.c_int), ("y_type", C.c_int),
                 ("w_type", C.c_int), ("gate_type", C.c_int), ("n_type", C.c_int),
@@ -161,6 +188,18 @@ SIGNATURES = {
     "wisp_b200_fp4_moe_workspace_bytes": (_SZ, [C.POINTER(WispMoeConfig), _I]),
     "wisp_b200_fp4_moe_forward": (_I, [C.POINTER(WispMoeConfig), C.POINTER(WispFp4MoeWeights), _P,
                                        _P, _P, _P, _P, _SZ, _P, _P, _E]),
+    "wisp_b200_fp8_quantize": (_I, [_P, _I, _L, _I, _P, _I, _I, _I, _P, _P, _L, _L, _P, _E]),
+    "wisp_b200_fp8_dequantize": (_I, [_P, _P, _L, _L, _I, _I, _P, _I, _L, _P, _E]),
+    "wisp_b200_fp8_quantize_weights": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _E]),
+    "wisp_b200_fp8_product": (_I, [C.POINTER(WispFp8Config), C.POINTER(WispFp8Mats),
+                                   C.POINTER(WispFp8Mats), C.POINTER(WispFp8Rows), _P, _I, _P, _L,
+                                   _P, _P, _E]),
+    "wisp_b200_select_experts": (_I, [C.POINTER(WispRouting), _P, _I, _L, _I, _I, _I, _P, _P, _P,
+                                      _P, _E]),
+    "wisp_b200_fp8_moe_workspace_bytes": (_SZ, [C.POINTER(WispMoeConfig), C.POINTER(WispRouting)]),
+    "wisp_b200_fp8_moe_forward": (_I, [C.POINTER(WispMoeConfig), C.POINTER(WispRouting),
+                                       C.POINTER(WispFp8MoeWeights), _P, _P, _P, _P, _P, _SZ, _P,
+                                       _P, _E]),
     "wisp_b200_block_norm": (_I, [C.POINTER(WispBlockNorm), _P, _P, _P, _P, _P, _P, _P, _P, _E]),
     "wisp_b200_block_norm_error_word": (_P, []),
     "wisp_b200_rms_rescale": (_I, [_P, _P, _I, _I, _F, _P, _E]),

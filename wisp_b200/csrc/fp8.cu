@@ -1,0 +1,524 @@
+// fp8.cu -- rows to e4m3 codes with one fp32 scale per 128 values and back, and
+// matrices to codes with one per block of 128 x 128.
+//
+// scale = fp32(max|x| / 448) or the least power of two that is not below max|x| /
+// 448; a code is the e4m3 value nearest to x / scale, ties to the even code. The
+// result is the one exact arithmetic gives, so that codes do not depend on how the
+// scale was divided out: x times the fp32 reciprocal of the scale, made 2^-21
+// smaller or larger, is within 2^-22 relative of where exact arithmetic has it (a
+// reciprocal's ulp and two roundings), so the codes of the two enclose the right
+// one. Where they differ (one value in about 65,000) |x| is compared with border *
+// scale in 64 bits, where the product of 5 and 24 significant bits is exact. (With
+// a power of two as the scale the first product is exact.)
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "internal.h"
+#include "numeric.cuh"
+
+namespace {
+
+using namespace wb;
+
+constexpr int kUnit = 16;      // values per thread; 8 threads hold a block of 128
+constexpr int kBlock = 128;
+constexpr int kLanes = kBlock / kUnit;
+constexpr int kMaxCols = 1 << 27;    // what a launch's grid holds, with room
+constexpr float kTop = 448.f;
+constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
+
+// A row of `units` threads split over equal CTAs of at most 256.
+int row_threads(int units) {
+  const int blocks = (units + 255) / 256;
+  return ((units + blocks - 1) / blocks + 31) / 32 * 32;
+}
+
+// 16 values of one thread as they lie in memory.
+template <typename T>
+struct Raw {
+  uint32_t u[4 * sizeof(T)];
+};
+
+template <typename T>
+WB_DEV void load_raw(const T* x, bool wide, Raw<T>& r) {
+  constexpr int W = 4 * sizeof(T);
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < W / 8; j++) load32(reinterpret_cast<const uint8_t*>(x) + 32 * j, r.u + 8 * j);
+  } else if (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < W; j++) r.u[j] = __ldg(reinterpret_cast<const uint32_t*>(x) + j);
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(x);
+#pragma unroll
+    for (int j = 0; j < W; j++) r.u[j] = __ldg(q + 2 * j) | (uint32_t)__ldg(q + 2 * j + 1) << 16;
+  }
+}
+
+// The bits of the largest magnitude in fp32 (found on integers, so that a NaN is
+// the largest of all).
+template <typename T>
+WB_DEV uint32_t top_of(const Raw<T>& r) {
+  uint32_t top = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) top = max(top, r.u[j] & 0x7fffffffu);
+    return top;
+  } else {
+    constexpr int type = std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = __vmaxu2(top, r.u[j] & 0x7fff7fffu);
+    return __float_as_uint(unpack2(max(top & 0xffffu, top >> 16), type).x);
+  }
+}
+
+template <typename T>
+WB_DEV float2 pair_of(const Raw<T>& r, int j) {
+  if constexpr (sizeof(T) == 4)
+    return make_float2(__uint_as_float(r.u[2 * j]), __uint_as_float(r.u[2 * j + 1]));
+  else
+    return unpack2(r.u[j], std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+}
+
+// The scale of a block whose largest magnitude has the bits `top`. An infinity or
+// a NaN in the block: NaN.
+template <bool POW2>
+WB_DEV float scale_of(uint32_t top) {
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+  if (!POW2) return __fdiv_rn(__uint_as_float(top), kTop);
+  // top = m 2^e, 448 = 1.75 2^8: 2^(e - 8), one more where m > 1.75
+  if (top == 0) return 0.f;
+  const int e = (int)((top + 0x1fffffu) >> 23) - 8;
+  return __uint_as_float((uint32_t)max(e, 1) << 23);
+}
+
+WB_DEV float e4m3_value(uint32_t b) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+}
+
+// Codes of four values, the first in the low byte. Round to nearest even,
+// saturating.
+WB_DEV uint32_t e4m3x4(float2 a, float2 b, float r) {
+  uint32_t o;
+  asm("{\n\t.reg .b64 x, y, z;\n\t.reg .b16 p, q;\n\t.reg .f32 f, g;\n\t"
+      "mov.b64 z, {%5, %5};\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\t"
+      "mul.rn.f32x2 x, x, z;\n\tmul.rn.f32x2 y, y, z;\n\t"
+      "mov.b64 {f, g}, x;\n\tcvt.rn.satfinite.e4m3x2.f32 p, g, f;\n\t"
+      "mov.b64 {f, g}, y;\n\tcvt.rn.satfinite.e4m3x2.f32 q, g, f;\n\t"
+      "mov.b32 %0, {p, q};\n\t}"
+      : "=r"(o) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(r));
+  return o;
+}
+
+// Of two neighbouring codes' magnitudes lo < hi, the one nearer to |x| / s.
+WB_DEV uint32_t nearer(float ax, float s, uint32_t lo, uint32_t hi) {
+  const double border = 0.5 * ((double)e4m3_value(lo) + (double)e4m3_value(hi)) * (double)s;
+  const double a = (double)ax;
+  return a > border || (a == border && !(hi & 1)) ? hi : lo;
+}
+
+// Decides the values among four whose two candidate codes differ.
+__device__ __noinline__ uint32_t settle(float2 a, float2 b, float s, uint32_t lo, uint32_t hi) {
+  const float v[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t l = lo >> (8 * j) & 127u, h = hi >> (8 * j) & 127u;
+    if (l != h) {
+      const uint32_t c = nearer(fabsf(v[j]), s, l, h);
+      lo = (lo & ~(127u << (8 * j))) | c << (8 * j);
+    }
+  }
+  return lo;
+}
+
+// Code of x for a scale whose reciprocal is no normal number.
+__device__ __noinline__ uint32_t code_exact(float x, float s) {
+  const double q = fabs((double)x) / (double)s;      // a guess, put right below
+  uint32_t c = __nv_cvt_double_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+  if (c > 0) c = nearer(fabsf(x), s, c - 1, c);
+  if (c < 126) c = nearer(fabsf(x), s, c, c + 1);
+  return c | (__float_as_uint(x) >> 24 & 128u);
+}
+
+template <bool POW2, typename T>
+WB_DEV void codes_of(const Raw<T>& raw, float s, uint32_t (&c)[4]) {
+  c[0] = c[1] = c[2] = c[3] = 0u;
+  if (!(s > 0.f)) return;           // a zero block, or NaN
+  if (s < 1.17549435e-38f) {        // subnormal: has no reciprocal
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 a = pair_of(raw, 2 * i), b = pair_of(raw, 2 * i + 1);
+      c[i] = code_exact(a.x, s) | code_exact(a.y, s) << 8 | code_exact(b.x, s) << 16 |
+             code_exact(b.y, s) << 24;
+    }
+    return;
+  }
+  const float r = POW2 ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : rcp_approx(s);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 a = pair_of(raw, 2 * i), b = pair_of(raw, 2 * i + 1);
+    if (POW2) {
+      c[i] = e4m3x4(a, b, r);
+    } else {
+      c[i] = e4m3x4(a, b, r * kBelow);
+      const uint32_t hi = e4m3x4(a, b, r * kAbove);
+      if (c[i] != hi) c[i] = settle(a, b, s, c[i], hi);
+    }
+  }
+}
+
+struct QuantParams {
+  const void* x;
+  int64_t ld;
+  int x_rows;
+  const int* src;
+  int rows, cols;
+  uint8_t* codes;
+  float* scales;
+  int64_t s_row, s_block;
+  int wide;   // rows of x start on 32-byte boundaries
+};
+
+// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): one thread per 16 values of R
+// rows, 32 (16-bit types) or 64 (fp32) bytes read and 16 written for each; the R
+// rows' loads are issued together. Lane i of a block's eight writes the scale of
+// row i, so that scales stored block by block go out 4 R bytes at a time.
+template <bool POW2, typename T, int R>
+__global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
+  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x;
+  const int units = p.cols / kUnit;
+  const bool in = u < units;
+  Raw<T> raw[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int64_t row = row0 + i;
+    int64_t sr = -1;
+    if (row < p.rows) sr = p.src ? (int64_t)__ldg(p.src + row) : row;
+#pragma unroll
+    for (int j = 0; j < 4 * (int)sizeof(T); j++) raw[i].u[j] = 0;
+    if (in && sr >= 0 && sr < p.x_rows)
+      load_raw(static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit, p.wide, raw[i]);
+  }
+  float mine = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int64_t row = row0 + i;
+    uint32_t top = top_of(raw[i]);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float s = scale_of<POW2>(top);
+    if ((u & (kLanes - 1)) == i) mine = s;
+    uint32_t c[4];
+    codes_of<POW2>(raw[i], s, c);
+    if (in && row < p.rows)
+      *reinterpret_cast<uint4*>(p.codes + row * p.cols + (int64_t)u * kUnit) =
+          make_uint4(c[0], c[1], c[2], c[3]);
+  }
+  // (the last block of a row may have fewer lanes than R rows)
+  const int i = u & (kLanes - 1), b = u / kLanes;
+  if (i < R && b * kBlock < p.cols && row0 + i < p.rows)
+    p.scales[(row0 + i) * p.s_row + b * p.s_block] = mine;
+}
+
+template <bool POW2, typename T>
+void launch_quantize(const QuantParams& p, cudaStream_t st) {
+  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
+  const int gy = (units + threads - 1) / threads;
+  constexpr int R = sizeof(T) == 4 ? 2 : 4;
+  // Several rows per thread once there are enough to fill the GPU all the same.
+  if ((int64_t)p.rows * gy >= 148 * 8 * R)
+    wb::launch_k(quantize_kernel<POW2, T, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
+  else
+    wb::launch_k(quantize_kernel<POW2, T, 1>, dim3(p.rows, gy), threads, 0, st, p);
+}
+
+template <bool POW2>
+void launch_quantize(const QuantParams& p, int type, cudaStream_t st) {
+  if (type == WISP_DT_F32)
+    launch_quantize<POW2, float>(p, st);
+  else if (type == WISP_DT_BF16)
+    launch_quantize<POW2, __nv_bfloat16>(p, st);
+  else
+    launch_quantize<POW2, __half>(p, st);
+}
+
+struct BlockParams {
+  const void* x;
+  int n, k, kb, nb;
+  uint8_t* codes;
+  float* scales;
+  int wide;
+};
+
+// One CTA per block of 128 x 128 (grid kb x nb x entries): a thread holds 16
+// values of four rows.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const BlockParams p) {
+  __shared__ uint32_t tops[8];
+  const int tid = threadIdx.x, c0 = blockIdx.x * kBlock + (tid & 7) * kUnit;
+  const int64_t first = (int64_t)blockIdx.z * p.n;
+  Raw<T> raw[4];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = blockIdx.y * kBlock + (tid >> 3) + 32 * i;
+#pragma unroll
+    for (int j = 0; j < 4 * (int)sizeof(T); j++) raw[i].u[j] = 0;
+    if (r < p.n && c0 < p.k)
+      load_raw(static_cast<const T*>(p.x) + (first + r) * p.k + c0, p.wide, raw[i]);
+    top = max(top, top_of(raw[i]));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = max(top, tops[i]);
+  const float s = scale_of<false>(top);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = blockIdx.y * kBlock + (tid >> 3) + 32 * i;
+    if (r < p.n && c0 < p.k) {
+      uint32_t c[4];
+      codes_of<false>(raw[i], s, c);
+      *reinterpret_cast<uint4*>(p.codes + (first + r) * p.k + c0) =
+          make_uint4(c[0], c[1], c[2], c[3]);
+    }
+  }
+  if (tid == 0) p.scales[((int64_t)blockIdx.z * p.nb + blockIdx.y) * p.kb + blockIdx.x] = s;
+}
+
+struct DequantParams {
+  const uint8_t* codes;
+  const float* scales;
+  int64_t s_row, s_block;
+  int rows, cols;
+  void* out;
+  int64_t ld;
+  int wide;
+};
+
+WB_DEV float2 e4m3_values(uint32_t two) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(two));
+  return __half22float2(u2h2(h));
+}
+
+// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 values of R rows per
+// thread. code * scale is rounded to fp32, then to the output's type.
+template <int TYPE, int R>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
+  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool in = u < p.cols / kUnit;
+  const int lane = u & (kLanes - 1), b = u / kLanes;
+  // lane i of a block's eight reads the scale of row i
+  float mine = 0.f;
+  if (lane < R && b * kBlock < p.cols && row0 + lane < p.rows)
+    mine = __ldg(p.scales + (row0 + lane) * p.s_row + b * p.s_block);
+  uint4 c[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    c[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (in && row0 + i < p.rows)
+      c[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + (row0 + i) * p.cols) + u);
+  }
+  float scale[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) scale[i] = __shfl_sync(0xffffffffu, mine, i, kLanes);
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if (!in || row0 + i >= p.rows) continue;
+    const float s = scale[i];
+    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float2 f = e4m3_values(w[j >> 1] >> (16 * (j & 1)) & 0xffffu);
+      v[2 * j] = f.x * s;
+      v[2 * j + 1] = f.y * s;
+    }
+    const int64_t at = (row0 + i) * p.ld + (int64_t)u * kUnit;
+    if constexpr (TYPE == WISP_DT_F32) {
+      float* q = static_cast<float*>(p.out) + at;
+      if (p.wide) {
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(v[j]);
+        store32(q, o);
+        store32(q + 8, o + 8);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) q[j] = v[j];
+      }
+    } else {
+      uint16_t* q = static_cast<uint16_t*>(p.out) + at;
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) o[j] = pack2(v[2 * j], v[2 * j + 1], TYPE);
+      if (p.wide) {
+        store32(q, o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          q[2 * j] = (uint16_t)o[j];
+          q[2 * j + 1] = (uint16_t)(o[j] >> 16);
+        }
+      }
+    }
+  }
+}
+
+template <int TYPE>
+void launch_dequantize(const DequantParams& p, cudaStream_t st) {
+  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
+  const int gy = (units + threads - 1) / threads;
+  constexpr int R = 2;
+  if ((int64_t)p.rows * gy >= 148 * 8 * R)
+    wb::launch_k(dequantize_kernel<TYPE, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
+  else
+    wb::launch_k(dequantize_kernel<TYPE, 1>, dim3(p.rows, gy), threads, 0, st, p);
+}
+
+}  // namespace
+
+extern "C" WispError wisp_b200_fp8_quantize(const void* d_x, int x_type, int64_t ld, int x_rows,
+                                            const int* d_src, int rows, int cols, int pow2,
+                                            uint8_t* d_codes, float* d_scales, int64_t scale_row,
+                                            int64_t scale_block, cudaStream_t stream,
+                                            WispErrCtx* err) {
+  if (!dt_valid(x_type))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize: unknown x_type %d", x_type);
+  if (rows < 0 || rows > wb::kMaxRows || x_rows < 0 || cols <= 0 || cols > kMaxCols ||
+      cols % kUnit || ld < cols)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_quantize: rows=%d x_rows=%d cols=%d ld=%lld (at most 2^31 - 256 rows, cols a "
+                   "multiple of 16 up to 2^27, ld >= cols)",
+                   rows, x_rows, cols, (long long)ld);
+  if (!d_src && rows > x_rows)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize: rows=%d > x_rows=%d without d_src", rows,
+                   x_rows);
+  if (scale_row < 1 || scale_block < 1)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize: scale strides %lld, %lld (at least 1)",
+                   (long long)scale_row, (long long)scale_block);
+  if (rows == 0) return WISP_OK;
+  if ((!d_x && x_rows > 0) || !d_codes || !d_scales)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize: null pointer argument (x, codes, scales)");
+  if (((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_quantize: codes must be 16-byte, scales 4-byte aligned");
+  if ((uintptr_t)d_x % dt_size(x_type) || ((uintptr_t)d_src & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize: x or d_src not aligned to its type");
+  QuantParams p;
+  p.x = d_x;
+  p.ld = ld;
+  p.x_rows = x_rows;
+  p.src = d_src;
+  p.rows = rows;
+  p.cols = cols;
+  p.codes = d_codes;
+  p.scales = d_scales;
+  p.s_row = scale_row;
+  p.s_block = scale_block;
+  p.wide = !((uintptr_t)d_x & 31) && (ld * dt_size(x_type)) % 32 == 0;
+  if (pow2)
+    launch_quantize<true>(p, x_type, stream);
+  else
+    launch_quantize<false>(p, x_type, stream);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
+extern "C" WispError wisp_b200_fp8_dequantize(const uint8_t* d_codes, const float* d_scales,
+                                              int64_t scale_row, int64_t scale_block, int rows,
+                                              int cols, void* d_out, int out_type, int64_t ld,
+                                              cudaStream_t stream, WispErrCtx* err) {
+  if (!dt_valid(out_type))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_dequantize: unknown out_type %d", out_type);
+  if (rows < 0 || rows > wb::kMaxRows || cols <= 0 || cols > kMaxCols ||
+      cols % kUnit || ld < cols)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_dequantize: rows=%d cols=%d ld=%lld (at most 2^31 - 256 rows, cols a "
+                   "multiple of 16 up to 2^27, ld >= cols)",
+                   rows, cols, (long long)ld);
+  if (rows == 0) return WISP_OK;
+  if (!d_codes || !d_scales || !d_out)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_dequantize: null pointer argument");
+  if (((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_dequantize: codes must be 16-byte, scales 4-byte aligned");
+  if ((uintptr_t)d_out % dt_size(out_type))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_dequantize: out not aligned to its type");
+  DequantParams p;
+  p.codes = d_codes;
+  p.scales = d_scales;
+  p.s_row = scale_row;
+  p.s_block = scale_block;
+  p.rows = rows;
+  p.cols = cols;
+  p.out = d_out;
+  p.ld = ld;
+  p.wide = !((uintptr_t)d_out & 31) && ld * dt_size(out_type) % 32 == 0;
+  if (out_type == WISP_DT_F32)
+    launch_dequantize<WISP_DT_F32>(p, stream);
+  else if (out_type == WISP_DT_BF16)
+    launch_dequantize<WISP_DT_BF16>(p, stream);
+  else
+    launch_dequantize<WISP_DT_F16>(p, stream);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
+WispError wb::fp8_validate(const WispFp8Config* c, const char* who, WispErrCtx* err) {
+  if (!c) return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: null config", who);
+  if (c->n_entries <= 0 || c->n <= 0 || c->k <= 0 || c->k > kMaxCols || c->k % kUnit)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: n_entries=%d n=%d k=%d (k a multiple of 16 up to 2^27)",
+                   who, c->n_entries, c->n, c->k);
+  // the tensor map's row index (entries x n, plus one tile) is 32-bit
+  if ((int64_t)c->n_entries * c->n > wb::kMaxRows)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: n_entries * n = %lld exceeds 2^31 - 256", who,
+                   (long long)c->n_entries * c->n);
+  if (!dt_valid(c->out_type))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: unknown out_type %d", who, c->out_type);
+  return WISP_OK;
+}
+
+extern "C" WispError wisp_b200_fp8_quantize_weights(const void* d_w, int w_type, int n_entries,
+                                                    int n, int k, uint8_t* d_codes,
+                                                    float* d_scales, cudaStream_t stream,
+                                                    WispErrCtx* err) {
+  const WispFp8Config c = {n_entries, n, k, 0, w_type};
+  WispError e = wb::fp8_validate(&c, "fp8_quantize_weights", err);
+  if (e != WISP_OK) return e;
+  BlockParams p;
+  p.kb = (k + kBlock - 1) / kBlock;
+  p.nb = (int)(((int64_t)n + kBlock - 1) / kBlock);
+  if (n_entries > 65535 || p.nb > 65535)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize_weights: n_entries=%d n=%d (65535 matrices "
+                   "or blocks of rows at most)", n_entries, n);
+  if (!d_w || !d_codes || !d_scales)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_quantize_weights: null pointer argument");
+  if (((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 3) ||
+      (uintptr_t)d_w % dt_size(w_type))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_quantize_weights: codes must be 16-byte, scales and weights aligned to "
+                   "their types");
+  p.x = d_w;
+  p.n = n;
+  p.k = k;
+  p.codes = d_codes;
+  p.scales = d_scales;
+  // (16 values are 32 bytes or more, so every row start is as aligned as the first)
+  p.wide = !((uintptr_t)d_w & 31);
+  const dim3 grid(p.kb, p.nb, n_entries);
+  if (w_type == WISP_DT_F32)
+    wb::launch_k(quantize_blocks_kernel<float>, grid, 256, 0, stream, p);
+  else if (w_type == WISP_DT_BF16)
+    wb::launch_k(quantize_blocks_kernel<__nv_bfloat16>, grid, 256, 0, stream, p);
+  else
+    wb::launch_k(quantize_blocks_kernel<__half>, grid, 256, 0, stream, p);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}

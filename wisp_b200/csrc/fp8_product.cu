@@ -1,0 +1,849 @@
+// fp8_product.cu -- out[p, f] = sum_b xs[p, b] ws_e[f / 128, b] sum_{k in b} x[p, k] w_e[f, k]
+// over e4m3 rows with one fp32 scale per block b of 128 k and e4m3 expert
+// matrices with one per block of 128 x 128 (one expert per segment of rows).
+//
+// The scales are no powers of two, so the tensor cores cannot apply them: each
+// block of 128 k is one MMA accumulation in tensor memory (four tcgen05.mma of
+// 32 k), which the epilogue warps scale and add to fp32 sums in registers while
+// the MMAs of the next blocks fill other buffers.
+//
+// Two forms of tile, for one CTA pair (cta_group::2, M = 256) or a single CTA
+// (cta_group::1, M = 128):
+//   narrow (at most 128 rows): the features are the MMA's M (128 per CTA), the
+//     rows its N, any multiple of 16 (32 in a pair), so that a weight matrix
+//     streams through once and few rows cost little. An accumulator lane is one
+//     feature: the weight scale is the tile's, the rows' scales run over the
+//     columns and are read from shared memory.
+//   wide (129 to 256 rows, pairs only): the rows are M (128 per CTA), N is 256
+//     features, one block of 128 in either CTA's shared memory: two of one
+//     matrix, or gate in the even and up in the odd CTA. A lane is one row: its
+//     scale is one register, where the narrow form would read 4 bytes of shared
+//     memory per accumulator and block (and takes two passes over the weights).
+//
+// Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
+// swizzle), 1 the MMAs, 2 hands out the tiles, 4-11 are the epilogue, with the
+// registers that the first four give up.
+#include "common.cuh"
+#include "internal.h"
+#include "numeric.cuh"
+#include "tiles.cuh"
+
+namespace {
+
+using namespace wb;
+
+constexpr int kThreads = 384;
+constexpr int kSchedWarp = 2;
+constexpr int kEpiWarp = 4;       // first of 8 epilogue warps
+constexpr int kABytes = 128 * 128;
+constexpr int kNarrow = 128;      // rows of a narrow tile at most
+constexpr int kWide = 256;
+constexpr int kMaxStages = 12;
+constexpr int kMaxBufs = 8;       // accumulators of one block of k
+constexpr int kRingBytes = 208 * 1024;
+constexpr int kTileRing = 8;
+// Registers: launch 168 x 384 = 64,512; 256 x 208 + 128 x 80 = 63,488.
+constexpr int kEpiRegs = 208, kOtherRegs = 80;
+// Scales of one epilogue warp and block of k: of its rows (64 columns of a
+// narrow tile, 32 lanes of a wide one), then the weights' two.
+constexpr int kScaleSlots = 4, kSlotFloats = 68;
+
+struct Bars {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[kMaxBufs];
+  uint64_t acc_empty[kMaxBufs];
+  uint64_t red_full, red_empty;     // partial sums of a cluster's CTAs
+  uint64_t tile_full[kTileRing];
+  uint64_t tile_empty[kTileRing];
+  int4 tile[kTileRing];     // expert (-1: no more), first row, rows, feature tile
+  uint32_t tmem;
+  int abort;
+};
+
+struct alignas(64) Params {
+  CUtensorMap tm_w, tm_up, tm_x, tm_x128;     // tm_x: boxes of 16 rows, tm_x128 of 128
+  const float* ws_w;
+  const float* ws_up;
+  const float* xs;        // scale of row p, block b: xs[p * xs_row + b * xs_block]
+  int64_t xs_row, xs_block;
+  int rows;
+  const WispSegment* segs;
+  int nseg;
+  int V, N, nk, ftiles;
+  int cap;                // rows per tile at most: a multiple of 32 up to kNarrow, or kWide
+  void* out;
+  int64_t ld;
+  int out_type;
+  int wide_out;           // output rows start on 32-byte boundaries
+  int* error_flag;
+};
+
+// kWide: whole wide tiles and a rest, so that the rest can be a narrow one.
+template <int UNIT>
+struct Cut8 {
+  WB_DEV static int rows(int rows, int cap) {
+    return cap == kWide && rows > kWide ? kWide : EvenCut<UNIT>::rows(rows, cap);
+  }
+};
+
+// Instruction descriptor of kind::f8f6f4: A and B e4m3, both K-major, fp32 sums.
+WB_DEV uint32_t idesc_fp8(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+template <bool PAIR>
+WB_DEV void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+
+// The wait for a tmem_ld16's registers; as operands of it, they cannot be read
+// before.
+WB_DEV void tmem_wait_regs(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
+WB_DEV void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+}
+
+// Two products, two sums of products per instruction.
+WB_DEV float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+WB_DEV void fma2(float2& c, float2 a, float2 b) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%0, %1};\n\tfma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "+f"(c.x), "+f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
+// The sums of one thread, 128 or fewer in use.
+//   narrow: [matrix][chunk j: rows (2 j + half) 16 ..][16]; one matrix uses the
+//           first 64
+//   wide:   features [half 64 ..][64] of the first block of 128, then of the second
+struct Sums {
+  float2 v[64];
+};
+
+// The epilogue's scales of coming blocks: every warp fetches its own, kScaleSlots
+// - 1 blocks ahead, with cp.async (4 bytes, so that rows' scales may lie
+// anywhere).
+struct Scales {
+  float* ring;              // this warp's [kScaleSlots][kSlotFloats]
+  const float* x0;          // the lane's (up to) two rows
+  const float* x1;
+  const float* w;           // lanes 0, 1: a weight scale
+  int64_t step;
+  int kk, k1, slot;
+
+  WB_DEV void fetch() {
+    if (kk < k1) {
+      float* s = ring + slot * kSlotFloats;
+      const int lane = threadIdx.x & 31;
+      if (x0) cp_async_4(s + lane, x0 + kk * step);
+      if (x1) cp_async_4(s + 32 + lane, x1 + kk * step);
+      if (w) cp_async_4(s + 64 + lane, w + kk);
+    }
+    cp_async_commit();
+    kk++;
+    if (++slot == kScaleSlots) slot = 0;
+  }
+};
+
+template <bool SWIGLU, bool PAIR>
+struct Epilogue {
+  const Params& p;
+  int lane, quad, half, rank;
+
+  WB_DEV bool wide(const Tile& t) const { return PAIR && t.cnt > kNarrow; }
+
+  // Starts the fetches of a tile's scales. (Rows past the tile's have none:
+  // what their lanes and columns hold is not stored.)
+  WB_DEV void begin(Scales& sc, const Tile& t, int k0, int k1) const {
+    sc.step = p.xs_block;
+    sc.kk = k0;
+    sc.k1 = k1;
+    sc.slot = 0;
+    sc.x0 = sc.x1 = sc.w = nullptr;
+    const int nfb = p.ftiles;
+    const int last = nfb - 1;
+    if (wide(t)) {
+      const int r = rank * 128 + quad * 32 + lane;
+      if (r < t.cnt) sc.x0 = p.xs + (t.row0 + (int64_t)r) * p.xs_row;
+      if (lane < 2) {
+        const float* w = SWIGLU && lane ? p.ws_up : p.ws_w;
+        const int fb = SWIGLU ? t.ft : (t.ft & ~1) + lane;
+        sc.w = w + ((int64_t)t.expert * nfb + min(fb, last)) * p.nk;
+      }
+    } else {
+      const int c0 = (lane >> 4) * 32 + half * 16 + (lane & 15);
+      if (c0 < t.cnt) sc.x0 = p.xs + (t.row0 + (int64_t)c0) * p.xs_row;
+      if (c0 + 64 < t.cnt) sc.x1 = p.xs + (t.row0 + (int64_t)c0 + 64) * p.xs_row;
+      if (lane < (SWIGLU ? 2 : 1))
+        sc.w = (lane ? p.ws_up : p.ws_w) + ((int64_t)t.expert * nfb + min(t.ft, last)) * p.nk;
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleSlots - 1; i++) sc.fetch();
+  }
+
+  // sums += scales * one block's accumulators at column d (up: at du).
+  WB_DEV void add(Sums& a, const Tile& t, const float* s, uint32_t d, uint32_t du) const {
+    if (wide(t)) {
+      const float x = s[lane];
+      const float2 s0 = make_float2(x * s[64], x * s[64]), s1 = make_float2(x * s[65], x * s[65]);
+      uint32_t u[2][16];
+      tmem_ld16(d + half * 64, u[0]);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {      // 16 columns each
+        tmem_wait_regs(u[j & 1]);
+        if (j < 7) tmem_ld16(d + half * 64 + (j + 1 >> 2) * 128 + (j + 1 & 3) * 16, u[j + 1 & 1]);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          fma2(a.v[j * 8 + i],
+               make_float2(__uint_as_float(u[j & 1][2 * i]), __uint_as_float(u[j & 1][2 * i + 1])),
+               j < 4 ? s0 : s1);
+      }
+    } else {
+      const float2 wg = make_float2(s[64], s[64]);
+      const float2 wu = SWIGLU ? make_float2(s[65], s[65]) : wg;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = (2 * j + half) * 16;
+        if (c < t.cnt) {
+          uint32_t g[16], u[16];
+          tmem_ld16(d + c, g);
+          if (SWIGLU) tmem_ld16(du + c, u);
+          tmem_wait_regs(g);
+          if (SWIGLU) tmem_wait_regs(u);
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float4 x = *reinterpret_cast<const float4*>(s + j * 16 + i * 2);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const float2 xs = h ? make_float2(x.z, x.w) : make_float2(x.x, x.y);
+              const int r = 2 * (i + h);
+              fma2(a.v[j * 8 + i + h],
+                   mul2(make_float2(__uint_as_float(g[r]), __uint_as_float(g[r + 1])), wg), xs);
+              if (SWIGLU)
+                fma2(a.v[32 + j * 8 + i + h],
+                     mul2(make_float2(__uint_as_float(u[r]), __uint_as_float(u[r + 1])), wu), xs);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  template <typename T>
+  WB_DEV void store(const Sums& a, const Tile& t) const {
+    const int64_t ld = p.ld;
+    if (wide(t)) {
+      const int r = rank * 128 + quad * 32 + lane;
+      if (r >= t.cnt) return;
+      T* row = static_cast<T*>(p.out) + (t.row0 + (int64_t)r) * ld;
+#pragma unroll
+      for (int b = 0; b < (SWIGLU ? 1 : 2); b++) {
+        const int f = (SWIGLU ? t.ft : (t.ft & ~1) + b) * 128 + half * 64;
+        constexpr int kRun = 32 / (int)sizeof(T);      // values of a 32-byte store
+#pragma unroll
+        for (int i = 0; i < 64; i += kRun) {
+          float o[kRun];
+#pragma unroll
+          for (int j = 0; j < kRun; j++) {
+            const float2 g = a.v[b * 32 + (i + j) / 2];
+            o[j] = j & 1 ? g.y : g.x;
+            if (SWIGLU) {
+              const float2 u = a.v[32 + (i + j) / 2];
+              o[j] = swiglu<T>(o[j], j & 1 ? u.y : u.x);
+            }
+          }
+          if (p.wide_out && f + i + kRun <= p.N) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              if constexpr (sizeof(T) == 4)
+                w[j] = __float_as_uint(o[j]);
+              else
+                w[j] = pack2(o[2 * j], o[2 * j + 1],
+                             std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+            }
+            store32(row + f + i, w);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kRun; j++)
+              if (f + i + j < p.N) put_out(row + f + i + j, o[j]);
+          }
+        }
+      }
+    } else {
+      const int f = t.ft * 128 + quad * 32 + lane;
+      if (f >= p.N) return;
+      T* out = static_cast<T*>(p.out) + (int64_t)t.row0 * ld + f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = (2 * j + half) * 16;
+        if (c < t.cnt) {
+          T* q = out + c * ld;
+#pragma unroll
+          for (int i = 0; i < 16; i++, q += ld) {
+            if (c + i < t.cnt) {
+              const float2 g = a.v[j * 8 + i / 2];
+              float o = i & 1 ? g.y : g.x;
+              if (SWIGLU) {
+                const float2 u = a.v[32 + j * 8 + i / 2];
+                o = swiglu<T>(o, i & 1 ? u.y : u.x);
+              }
+              put_out(q, o);
+            }
+          }
+        }
+      }
+    }
+  }
+};
+
+// The join of a cluster whose CTAs split K (narrow tiles of at most 64 rows).
+// 32 rows at a time, every CTA puts its sums into its shared memory, and CTA kp
+// adds those of all, in the order of K, for the rows kp, kp + ks, ... (a warp per
+// row, 4 features per lane).
+constexpr int kRedRows = 32, kSplitRows = 64;
+template <bool SWIGLU>
+struct Reduce {
+  float* buf;        // [gate, up][kRedRows][128 features]
+  Bars* bars;
+  int ks, kp;
+  uint32_t uses = 0;
+
+  WB_DEV void arrive_all(uint64_t* bar) const {
+    __syncwarp();
+    const int j = threadIdx.x & 31;
+    if (j < ks) mbar_arrive_remote_release(cluster_addr(bar, j));
+  }
+
+  template <typename T>
+  WB_DEV bool store(const Params& p, const Sums& a, const Tile& t, int quad, int half,
+                    volatile int* abort) {
+    const int lane = threadIdx.x & 31, w = half * 4 + quad;
+#pragma unroll
+    for (int j = 0; j < kSplitRows / kRedRows; j++) {
+      const int c = j * kRedRows;
+      if (c >= t.cnt) break;
+      bool ok = uses == 0 || mbar_wait_cluster(&bars->red_empty, (uses - 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (c + half * 16 < t.cnt) {
+        float* q = buf + half * 16 * 128 + quad * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float2 g = a.v[j * 8 + i / 2];
+          q[i * 128] = i & 1 ? g.y : g.x;
+          if (SWIGLU) {
+            const float2 u = a.v[32 + j * 8 + i / 2];
+            q[(kRedRows + i) * 128] = i & 1 ? u.y : u.x;
+          }
+        }
+      }
+      arrive_all(&bars->red_full);
+      ok = mbar_wait_cluster(&bars->red_full, uses & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      for (int r = kp + ks * w; r < min(kRedRows, t.cnt - c); r += ks * 8) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < ks; i++) {
+          const uint32_t at = cluster_addr(buf + r * 128 + lane * 4, i);
+          const float4 y = ld_cluster_f4(at);
+          v[0] += y.x;
+          v[1] += y.y;
+          v[2] += y.z;
+          v[3] += y.w;
+          if (SWIGLU) {
+            const float4 z = ld_cluster_f4(at + kRedRows * 128 * 4);
+            x[0] += z.x;
+            x[1] += z.y;
+            x[2] += z.z;
+            x[3] += z.w;
+          }
+        }
+        const int f = t.ft * 128 + lane * 4;
+        T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)(c + r)) * p.ld + f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (f + i < p.N) put_out(out + i, SWIGLU ? swiglu<T>(v[i], x[i]) : v[i]);
+      }
+      arrive_all(&bars->red_empty);
+      uses++;
+    }
+    return true;
+  }
+};
+
+template <bool SWIGLU, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_product_kernel(const __grid_constant__ Params p) {
+  constexpr int kMats = SWIGLU ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ Bars bars;
+  __shared__ alignas(16) float scales[8][kScaleSlots][kSlotFloats];
+  __shared__ int pref[kMaxSegs];
+  __shared__ uint16_t order[kMaxSegs];
+  __shared__ int4 warp_tot[kThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  volatile int* abort = &bars.abort;
+  constexpr int kUnit = PAIR ? 32 : 16;
+  using Cut = Cut8<kUnit>;
+  // pair: this CTA's place in it; else the K split: kp of ks
+  const int rank = PAIR ? (int)cluster_rank() : 0;
+  const int ks = PAIR ? 1 : (int)cluster_size(), kp = PAIR ? 0 : (int)cluster_rank();
+  const int fitems = PAIR ? (p.ftiles + 1) / 2 : p.ftiles;
+
+  if (warp == 0 && elect_sync()) {
+    tma_prefetch_desc(&p.tm_w);
+    tma_prefetch_desc(&p.tm_x);
+    if (SWIGLU) tma_prefetch_desc(&p.tm_up);
+    if (PAIR) tma_prefetch_desc(&p.tm_x128);
+  }
+  __syncwarp();
+  if (tid < kMaxStages) {
+    // the copies; the odd CTA's word
+    mbar_init(&bars.full[tid], PAIR && rank == 0 ? 2 : 1);
+    mbar_init(&bars.empty[tid], 1);
+    if (tid < kTileRing) {
+      mbar_init(&bars.tile_full[tid], 1);
+      mbar_init(&bars.tile_empty[tid], 10);     // all warps that walk the tiles
+    }
+    if (tid < kMaxBufs) {
+      mbar_init(&bars.acc_full[tid], 1);
+      mbar_init(&bars.acc_empty[tid], PAIR ? 16 : 8);
+    } else if (tid == kMaxBufs) {
+      mbar_init(&bars.red_full, 8 * ks);
+      mbar_init(&bars.red_empty, 8 * ks);
+      bars.abort = 0;
+    }
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if (PAIR)
+      tmem_alloc_pair(&bars.tmem, 512);
+    else
+      tmem_alloc(&bars.tmem, 512);
+  }
+  const int group = PAIR ? 2 : ks;                   // CTAs that share a tile
+  const int it0 = blockIdx.x / group, it_step = gridDim.x / group;
+  // a wide item of gate and up is two tiles, which only the scheduler hands out
+  const bool two_tiles = PAIR && SWIGLU && p.cap > kNarrow;
+  int max_cnt;
+  bool first_done;
+  const Plan plan = make_plan<Cut, kThreads>(
+      p, fitems, it0, pref, order, warp_tot, max_cnt, first_done,
+      [&](const WispSegment& v, int ft) {
+        if (two_tiles) return;
+        bars.tile[0] = make_int4(v.expert, v.row_begin, v.rows, PAIR ? 2 * ft + rank : ft);
+        mbar_arrive(&bars.tile_full[0]);
+      });
+  if (two_tiles) first_done = false;
+  const bool wides = PAIR && max_cnt > kNarrow;
+  // the scheduler warp reads pref and order
+  __syncthreads();
+  const uint32_t tmem = bars.tmem;
+  const int k0 = p.nk * kp / ks, k1 = p.nk * (kp + 1) / ks;     // this CTA's stages
+  // A stage: weights (in narrow tiles gate and up), then rows: of a narrow tile n
+  // (a pair's CTA half of them), of a wide one 128. Few rows leave room for more
+  // stages, which is what hides the memory's latency when the weights are most of
+  // the traffic.
+  const int narrow_n = (min(max_cnt, kNarrow) + kUnit - 1) / kUnit * kUnit;
+  const int narrow_bytes = kMats * kABytes + narrow_n / (PAIR ? 2 : 1) * 128;
+  const int stage_bytes = wides ? max(narrow_bytes, 2 * kABytes) : narrow_bytes;
+  constexpr int kRedBytes = kMats * kRedRows * 128 * 4;     // a cluster's partial sums
+  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
+  // accumulators: buffers of `cols` columns (gate, then up)
+  const int up_offset = (narrow_n + 31) & ~31;
+  const int cols = wides ? kWide : up_offset * kMats;
+  const int bufs = min(kMaxBufs, 512 / cols);
+  TileWalk<kTileRing> tiles;
+  Tile t;
+
+  // (within each role, so that the compiler knows what the role may use)
+  if (warp == 0) {
+    give_registers();
+    Ring r;
+    bool first = true, ok = true;
+    while (ok && tiles.next(bars, t, abort)) {
+      const bool wide = PAIR && t.cnt > kNarrow;
+      const int wrow = t.expert * p.N + t.ft * 128;
+      const bool second = SWIGLU && wide && rank == 1;      // this CTA's block is up's
+      const int nb = ((t.cnt + kUnit - 1) / kUnit);         // boxes of 16 rows
+      const int xrow = t.row0 + rank * (wide ? 128 : nb * 16);
+      const uint32_t bytes = wide ? 2 * kABytes : kMats * kABytes + nb * 2048;
+      for (int kk = k0; kk < k1; kk++) {
+        if (!first && !mbar_wait(&bars.empty[r.s], r.ph ^ 1, abort)) { ok = false; break; }
+        uint8_t* st = smem + r.s * stage_bytes;
+        uint64_t* full = &bars.full[r.s];
+        if (elect_sync()) {
+          mbar_arrive_expect_tx(full, bytes);
+          if (wide) {
+            tma_load_2d(st, second ? &p.tm_up : &p.tm_w, full, kk * 128, wrow);
+            tma_load_2d(st + kABytes, &p.tm_x128, full, kk * 128, xrow);
+          } else {
+            tma_load_2d(st, &p.tm_w, full, kk * 128, wrow);
+            if (SWIGLU) tma_load_2d(st + kABytes, &p.tm_up, full, kk * 128, wrow);
+            for (int b = 0; b < nb; b++)
+              tma_load_2d(st + kMats * kABytes + b * 2048, &p.tm_x, full, kk * 128, xrow + b * 16);
+          }
+        }
+        __syncwarp();
+        r.next(S);
+        if (r.s == 0) first = false;
+      }
+    }
+    if (*abort) {
+      // let the copies in flight land before the CTA's memory goes away
+      for (int i = 0; i < S; i++) {
+        const int s = (r.s + i) % S;
+        const bool wrapped = s >= r.s;
+        if (first && wrapped) continue;      // never used
+        mbar_wait(&bars.full[s], wrapped ? r.ph ^ 1 : r.ph, abort, 20000000LL);
+      }
+    }
+    cluster_wait();
+  } else if (warp == 1 && rank == 1) {
+    give_registers();
+    cluster_wait();
+    Ring r;
+    bool ok = true;
+    while (ok && tiles.next(bars, t, abort)) {
+      for (int kk = k0; kk < k1; kk++) {
+        // All of the odd CTA's stage came by asynchronous copies, whose completion
+        // the barrier reports at cluster scope; the word to the even CTA has no
+        // scope of its own.
+        if (!mbar_wait_cluster(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        if (lane == 0) mbar_arrive_remote(cluster_addr(&bars.full[r.s], 0));
+        __syncwarp();
+        r.next(S);
+      }
+    }
+  } else if (warp == 1) {
+    give_registers();
+    cluster_wait();
+    Ring r, b;                    // stages, accumulators
+    int uses = 0;                 // stages so far, up to S
+    bool fresh = true, ok = true;
+    while (ok && tiles.next(bars, t, abort)) {
+      const bool wide = PAIR && t.cnt > kNarrow;
+      const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
+      const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kWide : n);
+      for (int kk = k0; kk < k1; kk++) {
+        if (!fresh && !(PAIR ? mbar_wait_cluster(&bars.acc_empty[b.s], b.ph ^ 1, abort)
+                             : mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort))) { ok = false; break; }
+        if (PAIR ? !mbar_wait_cluster(&bars.full[r.s], r.ph, abort)
+                 : !mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
+        const uint32_t d = tmem + b.s * cols, du = d + up_offset;
+        if (elect_sync()) {
+          const uint64_t dw = smem_desc_sw128(st);
+          const uint64_t dx = smem_desc_sw128(st + (wide ? kABytes : kMats * kABytes));
+#pragma unroll
+          for (int j = 0; j < 4; j++) {          // 32 k (32 bytes) each
+            if (wide) {
+              mma_fp8<PAIR>(d, dx + j * 2, dw + j * 2, idesc, j ? 1u : 0u);
+            } else {
+              mma_fp8<PAIR>(d, dw + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
+              if (SWIGLU)
+                mma_fp8<PAIR>(du, dw + (kABytes >> 4) + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
+            }
+          }
+          commit<PAIR>(&bars.empty[r.s]);
+          commit<PAIR>(&bars.acc_full[b.s]);
+        }
+        __syncwarp();
+        r.next(S);
+        b.next(bufs);
+        if (b.s == 0) fresh = false;
+        uses = min(uses + 1, S);
+      }
+    }
+    if (*abort) {
+      // MMAs in flight read shared memory: wait for the last stages issued
+      for (int i = 0; i < uses; i++) {
+        const int s = (r.s + 2 * S - 1 - i) % S;
+        mbar_wait(&bars.empty[s], s < r.s ? r.ph : r.ph ^ 1, abort, 20000000LL);
+      }
+    }
+  } else if (warp >= kEpiWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+    cluster_wait();
+    // warp % 4 is the lane quadrant; the two warps of a quadrant take alternate
+    // groups of 16 rows of a narrow tile, a half of each 128 features of a wide one
+    Epilogue<SWIGLU, PAIR> epi{p, lane, warp & 3, (warp - kEpiWarp) >> 2, rank};
+    Reduce<SWIGLU> red;
+    red.buf = reinterpret_cast<float*>(smem + kRingBytes - kRedBytes);
+    red.bars = &bars;
+    red.ks = ks;
+    red.kp = kp;
+    Scales sc;
+    sc.ring = &scales[warp - kEpiWarp][0][0];
+    Ring b;
+    const uint32_t quad_lane = (uint32_t)(epi.quad * 32) << 16;
+    bool ok = true;
+    while (ok && tiles.next(bars, t, abort)) {
+      epi.begin(sc, t, k0, k1);
+      Sums a;
+#pragma unroll
+      for (int i = 0; i < 64; i++) a.v[i] = make_float2(0.f, 0.f);
+      int slot = 0;
+      for (int kk = k0; kk < k1; kk++) {
+        __syncwarp();          // the slot that is filled next has been read
+        sc.fetch();
+        ok = mbar_wait(&bars.acc_full[b.s], b.ph, abort);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        cp_async_wait<kScaleSlots - 1>();
+        __syncwarp();          // every lane's copies of this block have landed
+        tc_fence_after();
+        const uint32_t d = tmem + quad_lane + b.s * cols;
+        epi.add(a, t, sc.ring + slot * kSlotFloats, d, d + up_offset);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR)
+            mbar_arrive_remote(cluster_addr(&bars.acc_empty[b.s], 0));
+          else
+            mbar_arrive(&bars.acc_empty[b.s]);
+        }
+        b.next(bufs);
+        if (++slot == kScaleSlots) slot = 0;
+      }
+      if (!ok) break;
+      cp_async_wait_all();
+      __syncwarp();
+      if (!PAIR && ks > 1) {
+        if (p.out_type == WISP_DT_F32)
+          ok = red.template store<float>(p, a, t, epi.quad, epi.half, abort);
+        else if (p.out_type == WISP_DT_BF16)
+          ok = red.template store<__nv_bfloat16>(p, a, t, epi.quad, epi.half, abort);
+        else
+          ok = red.template store<__half>(p, a, t, epi.quad, epi.half, abort);
+      } else if (p.out_type == WISP_DT_F32) {
+        epi.template store<float>(a, t);
+      } else if (p.out_type == WISP_DT_BF16) {
+        epi.template store<__nv_bfloat16>(a, t);
+      } else {
+        epi.template store<__half>(a, t);
+      }
+      __syncwarp();
+    }
+    cp_async_wait_all();
+  } else if (warp == kSchedWarp) {
+    give_registers();
+    if (lane == 0) {
+      const int items = (plan.singles + plan.multi_tiles) * fitems;
+      int s = first_done ? 1 : 0;
+      uint32_t ph = 0;
+      bool first = true, ok = true;
+      for (int it = first_done ? it0 + it_step : it0; ok; it += it_step) {
+        Tile v;
+        v.expert = -1;
+        v.row0 = v.cnt = v.ft = 0;
+        int n = 1;
+        if (it < items) {
+          v = find_tile<Cut>(p, plan, it);
+          if (PAIR && SWIGLU && v.cnt > kNarrow) {
+            // both feature tiles, one after the other, each by the whole pair
+            v.ft *= 2;
+            n = min(2, p.ftiles - v.ft);
+          } else if (PAIR) {
+            v.ft = 2 * v.ft + rank;
+          }
+        }
+        for (int i = 0; i < n; i++) {
+          if (!first && !mbar_wait(&bars.tile_empty[s], ph ^ 1, abort)) { ok = false; break; }
+          bars.tile[s] = make_int4(v.expert, v.row0, v.cnt, v.ft + i);
+          mbar_arrive(&bars.tile_full[s]);
+          if (++s == kTileRing) {
+            s = 0;
+            ph ^= 1;
+            first = false;
+          }
+        }
+        if (it >= items) break;
+      }
+    }
+    __syncwarp();
+    cluster_wait();
+  } else {
+    give_registers();
+    cluster_wait();
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();      // no CTA's memory goes away while another uses it
+  tc_fence_after();
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_relinquish_pair();
+      tmem_dealloc_pair(tmem, 512);
+    } else {
+      tmem_relinquish();
+      tmem_dealloc(tmem, 512);
+    }
+  }
+  if (tid == 0 && bars.abort && p.error_flag) atomicOr(p.error_flag, kErrorTimeout);
+}
+
+// e4m3 rows [rows x k bytes] as a 2D tensor; one box = box_rows x 128 bytes (one
+// block of k), 128-byte swizzle. Bytes past a row and rows past the end read 0.
+bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box_rows) {
+  wb::TensorMapEncodeFn fn = wb::tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)k};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// grid CTAs in clusters of `cluster`.
+template <bool SWIGLU, bool PAIR>
+WispError launch_product(const Params& p, int dev, unsigned grid, int cluster, cudaStream_t stream,
+                         WispErrCtx* err) {
+  const int smem = kRingBytes + 1024;
+  auto kernel = fp8_product_kernel<SWIGLU, PAIR>;
+  static std::atomic<uint64_t> raised{0};
+  WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  WB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+  return WISP_OK;
+}
+
+template <bool PAIR>
+WispError launch_product(bool swiglu, const Params& p, int dev, unsigned grid, int cluster,
+                         cudaStream_t stream, WispErrCtx* err) {
+  return swiglu ? launch_product<true, PAIR>(p, dev, grid, cluster, stream, err)
+                : launch_product<false, PAIR>(p, dev, grid, cluster, stream, err);
+}
+
+WispError check_mats(const WispFp8Mats* m, const char* what, WispErrCtx* err) {
+  if (!m || !m->codes || !m->scales)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: null pointer argument (%s)", what);
+  if (((uintptr_t)m->codes & 15) || ((uintptr_t)m->scales & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_product: %s codes must be 16-byte, scales 4-byte aligned", what);
+  return WISP_OK;
+}
+
+}  // namespace
+
+extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispFp8Mats* w,
+                                           const WispFp8Mats* up, const WispFp8Rows* x,
+                                           const WispSegment* d_segs, int n_segs, void* d_out,
+                                           int64_t ld, int* d_error_flag, cudaStream_t stream,
+                                           WispErrCtx* err) {
+  WispError e = wb::fp8_validate(cfg, "fp8_product", err);
+  if (e != WISP_OK) return e;
+  if ((e = check_mats(w, "weights", err)) != WISP_OK) return e;
+  if (cfg->swiglu && (e = check_mats(up, "up weights", err)) != WISP_OK) return e;
+  if (!cfg->swiglu && up)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: up weights without swiglu");
+  if (!x || x->rows < 0 || x->rows > wb::kMaxRows)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: bad rows (0 .. 2^31 - 256)");
+  if (d_segs ? (n_segs < 0 || n_segs > kMaxSegs) : n_segs != 0)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: n_segs=%d (0..%d, 0 without segments)",
+                   n_segs, kMaxSegs);
+  if (ld < cfg->n)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: ld=%lld < n=%d", (long long)ld, cfg->n);
+  if (x->rows == 0 || (d_segs && n_segs == 0)) return WISP_OK;
+  if (!x->codes || !x->scales || !d_out)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: null pointer argument (rows, out)");
+  if (((uintptr_t)x->codes & 15) || ((uintptr_t)x->scales & 3) ||
+      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_product: row codes must be 16-byte aligned, scales and out to their types");
+  int dev = 0, sms = 0;
+  WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
+  auto tiles_of = [&](int rows_per_tile) {     // an upper bound: at most one per row, and
+    // per segment one more than its rows fill
+    const int64_t most = (int64_t)x->rows / rows_per_tile + (d_segs ? n_segs : 1);
+    return most < x->rows ? most : x->rows;
+  };
+  const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 127) / 128;
+  const int64_t items = tiles_of(kNarrow) * ftiles;
+  const int split = nk < 16 || x->rows > kSplitRows    ? 1
+                    : items * 16 <= 3 * (int64_t)sms ? 4
+                    : items * 8 <= 3 * (int64_t)sms  ? 2
+                                                     : 1;
+  // With one feature tile a pair's second CTA would have none: single CTAs.
+  const bool single = split == 1 && ftiles == 1;
+  int cap = split > 1 || single ? kNarrow : kWide;
+  if (split == 1) {
+    // Smaller tiles when the largest would leave SMs without work: as many rows
+    // as give every CTA one tile if the rows lay in one segment, at least 64.
+    const int64_t width = single ? 1 : (ftiles + 1) / 2 * 2;
+    const int64_t per = ((int64_t)x->rows * width + sms - 1) / sms;
+    if (per <= kNarrow) cap = per < 64 ? 64 : (int)((per + 31) & ~31);
+  }
+  Params p;
+  memset(&p, 0, sizeof p);
+  p.cap = cap;
+  const int64_t wrows = (int64_t)cfg->n_entries * cfg->n;
+  if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
+      (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
+      !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, 16) ||
+      !encode_codes(&p.tm_x128, x->codes, x->rows, cfg->k, 128))
+    return WB_FAIL(WISP_ERR_CUDA, "fp8_product: cuTensorMapEncodeTiled failed");
+  p.ws_w = w->scales;
+  p.ws_up = cfg->swiglu ? up->scales : nullptr;
+  p.xs = x->scales;
+  p.xs_row = x->scale_row;
+  p.xs_block = x->scale_block;
+  p.rows = x->rows;
+  p.segs = d_segs;
+  p.nseg = n_segs;
+  p.V = cfg->n_entries;
+  p.N = cfg->n;
+  p.nk = nk;
+  p.ftiles = ftiles;
+  p.out = d_out;
+  p.ld = ld;
+  p.out_type = cfg->out_type;
+  p.wide_out = !((uintptr_t)d_out & 31) && ld * dt_size(cfg->out_type) % 32 == 0;
+  p.error_flag = d_error_flag;
+  if (split > 1)
+    return launch_product<false>(cfg->swiglu, p, dev, (unsigned)(items * split), split, stream, err);
+  if (single) {
+    const int64_t want = tiles_of(cap);
+    return launch_product<false>(cfg->swiglu, p, dev, (unsigned)(want < sms ? want : sms), 1,
+                                 stream, err);
+  }
+  const int64_t want = tiles_of(cap) * ((ftiles + 1) / 2) * 2;
+  return launch_product<true>(cfg->swiglu, p, dev,
+                              (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2, stream, err);
+}

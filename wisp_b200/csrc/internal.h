@@ -101,6 +101,17 @@ inline cudaError_t raise_smem(K* kernel, int bytes, int dev, std::atomic<uint64_
 // Checks shared by the fp4 weight-set entry points (fp4.cu).
 WispError fp4_validate(const WispFp4Config* c, const char* who, WispErrCtx* err);
 
+// The same for fp8 (fp8.cu) and for a routing (select.cu).
+WispError fp8_validate(const WispFp8Config* c, const char* who, WispErrCtx* err);
+WispError routing_validate(const WispRouting* r, int tokens, int n_experts, int top_k,
+                           const char* who, WispErrCtx* err);
+
+// wisp_b200_select_experts over the sum of `splits` sets of fp32 logits [tokens x
+// n_experts] and logit_bias (may be NULL).
+WispError launch_select(const WispRouting* r, const float* part, int splits,
+                        const float* logit_bias, const float* bias, int tokens, int n_experts,
+                        int top_k, int* idx, float* w, cudaStream_t st, WispErrCtx* err);
+
 // Fill a WispErrCtx the way the reference's WISP_ERR_SET does
 // (csrc/core/wisp_engine.h:66-72) and return the code.
 inline WispError set_err(WispErrCtx* err, WispError code, const char* file, int line,

@@ -20,6 +20,8 @@
 
 namespace wb {
 size_t router_splits(int T, int E, int M);
+int launch_logits(const WispMoeConfig* c, const uint16_t* x, const uint16_t* W, float* part,
+                  size_t splits, cudaStream_t st);
 WispError launch_route(const WispMoeConfig* c, const uint16_t* x, const uint16_t* W,
                        const float* bias, float* part, size_t splits, float* logits_out, int* idx,
                        float* w, cudaStream_t st, WispErrCtx* err);
@@ -482,6 +484,24 @@ combine_bf16_kernel(const uint16_t* __restrict__ y, const float* __restrict__ ro
   o[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
 
+// Each token's bf16 expert outputs summed with their weights.
+WispError combine_bf16(const Workspace& b, const uint16_t* y, int V, int T, int M, float* out,
+                       cudaStream_t stream, WispErrCtx* err) {
+  const dim3 grid(T, (M + 2047) / 2048);
+  if (b.rows <= kScanRows) {
+    wb::launch_k(combine_bf16_kernel<true>, grid, 256, 0, stream, y, b.row_weight, b.row_token,
+                 b.segs, V, b.rows, nullptr, nullptr, b.lanes, M, out);
+  } else {
+    WB_CUDA_CHECK(cudaMemsetAsync(b.tok_cnt, 0, (size_t)T * sizeof(int), stream));
+    wb::launch_k(token_rows_kernel, (b.rows + 255) / 256, 256, 0, stream, b.row_token, b.segs, V,
+                 b.rows, b.lanes, b.tok_cnt, b.tok_list);
+    wb::launch_k(combine_bf16_kernel<false>, grid, 256, 0, stream, y, b.row_weight, b.row_token,
+                 b.segs, V, b.rows, b.tok_cnt, b.tok_list, b.lanes, M, out);
+  }
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
 // dst row p = src row row_token[p], for quantised rows: codes in 16-byte and
 // scales in 4-byte words. A token without a valid logit is routed nowhere, so
 // the plan may fill fewer rows than there are; what row_token holds behind them
@@ -633,19 +653,165 @@ extern "C" WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const W
   e = wisp_b200_fp4_product(&dn, &w->down, nullptr, &hr, b.segs, V, ws.y, M, d_error_flag, stream,
                             err);
   if (e != WISP_OK) return e;
-  const dim3 grid(T, (M + 2047) / 2048);
-  if (b.rows <= kScanRows) {
-    wb::launch_k(combine_bf16_kernel<true>, grid, 256, 0, stream, ws.y, b.row_weight, b.row_token,
-                 b.segs, V, b.rows, nullptr, nullptr, b.lanes, M, d_out);
+  return combine_bf16(b, ws.y, V, T, M, d_out, stream, err);
+}
+
+namespace {
+
+// The same for fp8 rows, whose scales are stored block by block.
+__global__ void __launch_bounds__(256)
+gather_fp8_kernel(const uint4* __restrict__ codes, const float* __restrict__ scales,
+                  const int* __restrict__ row_token, int tokens, int scale_ld, int code_words,
+                  int blocks, uint4* __restrict__ out_codes, float* __restrict__ out_scales,
+                  int out_scale_ld) {
+  const size_t p = blockIdx.x;
+  const int src = row_token[p];
+  if (src < 0 || src >= tokens) return;
+  const size_t t = src;
+  for (int i = threadIdx.x; i < code_words; i += 256)
+    out_codes[p * code_words + i] = __ldg(codes + t * code_words + i);
+  for (int i = threadIdx.x; i < blocks; i += 256)
+    out_scales[p + (size_t)i * out_scale_ld] = __ldg(scales + t + (size_t)i * scale_ld);
+}
+
+struct Fp8Ws {
+  Workspace base;      // routing, plan, token lists
+  float* part;
+  uint16_t* y;         // bf16 expert outputs
+  uint8_t* tc;         // the tokens' codes and scales (kGatherRows)
+  float* ts;
+  uint8_t* xc;
+  float* xs;
+  uint16_t* h;
+  uint8_t* hc;
+  float* hs;
+  size_t bytes;
+};
+
+Fp8Ws carve_fp8(const WispMoeConfig* c, void* base) {
+  Fp8Ws ws;
+  Carve cv;
+  const int T = c->tokens, E = c->n_experts, k = c->top_k, M = c->hidden, I = c->inter;
+  const int V = E + (c->has_shared ? 1 : 0);
+  Workspace& b = ws.base;
+  b.lanes = k + (c->has_shared ? 1 : 0);
+  b.rows = T * b.lanes;
+  b.splits = wb::router_splits(T, E, M);
+  ws.part = cv.take<float>(base, b.splits * (size_t)T * E);
+  b.plan_scratch = cv.take<int>(base, std::max<size_t>(1, wb::plan_scratch_ints(c)));
+  b.idx = cv.take<int>(base, (size_t)T * k);
+  b.w = cv.take<float>(base, (size_t)T * k);
+  b.counts = cv.take<int>(base, V);
+  b.segs = cv.take<WispSegment>(base, V);
+  b.row_token = cv.take<int>(base, b.rows);
+  b.row_weight = cv.take<float>(base, b.rows);
+  b.y = nullptr;
+  ws.y = cv.take<uint16_t>(base, (size_t)b.rows * M);
+  b.tok_cnt = cv.take<int>(base, T);
+  b.tok_list = cv.take<int>(base, (size_t)T * b.lanes);
+  const size_t tokens = b.rows >= kGatherRows ? T : 0;
+  ws.tc = cv.take<uint8_t>(base, tokens * M);
+  ws.ts = cv.take<float>(base, tokens * (M / 128));
+  ws.xc = cv.take<uint8_t>(base, (size_t)b.rows * M);
+  ws.xs = cv.take<float>(base, (size_t)b.rows * (M / 128));
+  ws.h = cv.take<uint16_t>(base, (size_t)b.rows * I);
+  ws.hc = cv.take<uint8_t>(base, (size_t)b.rows * I);
+  ws.hs = cv.take<float>(base, (size_t)b.rows * (I / 128));
+  ws.bytes = (cv.off + 255) & ~(size_t)255;
+  return ws;
+}
+
+// group_size is the int4 layer's, and with a routing of its own the layer does not
+// use the config's: any valid values pass those checks.
+WispError validate_fp8(const WispMoeConfig* c, const WispRouting* r, WispErrCtx* err) {
+  if (!c) return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe: null config");
+  WispMoeConfig v = *c;
+  v.group_size = 128;
+  if (r) v.scoring = WISP_SCORE_SOFTMAX;
+  WispError e = validate(&v, err);
+  if (e != WISP_OK) return e;
+  // rows are counted in 32 bits
+  if ((int64_t)c->tokens * (c->top_k + (c->has_shared ? 1 : 0)) > 0x7fffff00LL)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe: %d tokens of %d experts are more than 2^31 - 256 "
+                   "rows", c->tokens, c->top_k);
+  return r ? wb::routing_validate(r, c->tokens, c->n_experts, c->top_k, "fp8_moe", err) : WISP_OK;
+}
+
+}  // namespace
+
+extern "C" size_t wisp_b200_fp8_moe_workspace_bytes(const WispMoeConfig* cfg,
+                                                    const WispRouting* routing) {
+  if (validate_fp8(cfg, routing, nullptr) != WISP_OK) return 0;
+  return carve_fp8(cfg, nullptr).bytes;
+}
+
+extern "C" WispError wisp_b200_fp8_moe_forward(const WispMoeConfig* cfg, const WispRouting* routing,
+                                               const WispFp8MoeWeights* w, const uint16_t* d_x,
+                                               float* d_out, int* d_topk_idx, float* d_topk_w,
+                                               void* d_workspace, size_t workspace_bytes,
+                                               int* d_error_flag, cudaStream_t stream,
+                                               WispErrCtx* err) {
+  WispError e = validate_fp8(cfg, routing, err);
+  if (e != WISP_OK) return e;
+  if (!w || !w->router_w || !d_x || !d_out || !d_workspace)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_moe_forward: null pointer argument (weights, router_w, x, out, workspace)");
+  if (((uintptr_t)d_x | (uintptr_t)w->router_w | (uintptr_t)d_out) & 15 ||
+      (uintptr_t)d_workspace & 255)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_moe_forward: x, out and router_w must be 16-byte, workspace 256-byte aligned");
+  if (w->score_bias && !routing)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe_forward: score_bias without a routing");
+  const Fp8Ws ws = carve_fp8(cfg, d_workspace);
+  if (workspace_bytes < ws.bytes)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe_forward: workspace %zu < required %zu",
+                   workspace_bytes, ws.bytes);
+  const Workspace& b = ws.base;
+  const int T = cfg->tokens, M = cfg->hidden, I = cfg->inter;
+  const int V = cfg->n_experts + (cfg->has_shared ? 1 : 0);
+  int* idx = d_topk_idx ? d_topk_idx : b.idx;
+  float* wt = d_topk_w ? d_topk_w : b.w;
+
+  if (routing) {
+    const int parts = wb::launch_logits(cfg, d_x, w->router_w, ws.part, b.splits, stream);
+    WB_CUDA_CHECK(cudaGetLastError());
+    e = wb::launch_select(routing, ws.part, parts, w->router_bias, w->score_bias, T, cfg->n_experts,
+                          cfg->top_k, idx, wt, stream, err);
   } else {
-    WB_CUDA_CHECK(cudaMemsetAsync(b.tok_cnt, 0, (size_t)T * sizeof(int), stream));
-    wb::launch_k(token_rows_kernel, (b.rows + 255) / 256, 256, 0, stream, b.row_token, b.segs, V,
-                 b.rows, b.lanes, b.tok_cnt, b.tok_list);
-    wb::launch_k(combine_bf16_kernel<false>, grid, 256, 0, stream, ws.y, b.row_weight, b.row_token,
-                 b.segs, V, b.rows, b.tok_cnt, b.tok_list, b.lanes, M, d_out);
+    e = wb::launch_route(cfg, d_x, w->router_w, w->router_bias, ws.part, b.splits, nullptr, idx, wt,
+                         stream, err);
   }
-  WB_CUDA_CHECK(cudaGetLastError());
-  return WISP_OK;
+  if (e != WISP_OK) return e;
+  e = wb::launch_plan(cfg, idx, wt, b.counts, b.segs, b.row_token, b.row_weight, stream, err,
+                      b.plan_scratch);
+  if (e != WISP_OK) return e;
+  if (b.rows >= kGatherRows) {
+    e = wisp_b200_fp8_quantize(d_x, WISP_DT_BF16, M, T, nullptr, T, M, w->pow2, ws.tc, ws.ts, 1, T,
+                               stream, err);
+    if (e != WISP_OK) return e;
+    wb::launch_k(gather_fp8_kernel, b.rows, 256, 0, stream, reinterpret_cast<const uint4*>(ws.tc),
+                 ws.ts, b.row_token, T, T, M / 16, M / 128, reinterpret_cast<uint4*>(ws.xc), ws.xs,
+                 b.rows);
+    WB_CUDA_CHECK(cudaGetLastError());
+  } else {
+    e = wisp_b200_fp8_quantize(d_x, WISP_DT_BF16, M, T, b.row_token, b.rows, M, w->pow2, ws.xc,
+                               ws.xs, 1, b.rows, stream, err);
+    if (e != WISP_OK) return e;
+  }
+  const WispFp8Config gu = {V, I, M, 1, WISP_DT_BF16};
+  const WispFp8Rows xr = {ws.xc, ws.xs, 1, b.rows, b.rows};
+  e = wisp_b200_fp8_product(&gu, &w->gate, &w->up, &xr, b.segs, V, ws.h, I, d_error_flag, stream,
+                            err);
+  if (e != WISP_OK) return e;
+  e = wisp_b200_fp8_quantize(ws.h, WISP_DT_BF16, I, b.rows, nullptr, b.rows, I, w->pow2, ws.hc,
+                             ws.hs, 1, b.rows, stream, err);
+  if (e != WISP_OK) return e;
+  const WispFp8Config dn = {V, M, I, 0, WISP_DT_BF16};
+  const WispFp8Rows hr = {ws.hc, ws.hs, 1, b.rows, b.rows};
+  e = wisp_b200_fp8_product(&dn, &w->down, nullptr, &hr, b.segs, V, ws.y, M, d_error_flag, stream,
+                            err);
+  if (e != WISP_OK) return e;
+  return combine_bf16(b, ws.y, V, T, M, d_out, stream, err);
 }
 
 // Pointers into a reference blob (header at offset 0) from its parsed meta.

@@ -1400,30 +1400,38 @@ size_t router_splits(int T, int E, int M) {
   return (size_t)splits;
 }
 
-WispError launch_route(const WispMoeConfig* c, const uint16_t* x, const uint16_t* W,
-                       const float* bias, float* part, size_t splits, float* logits_out, int* idx,
-                       float* w, cudaStream_t st, WispErrCtx* err) {
+// The router's logits (no bias) as sums over parts of K, [parts][T x E]; returns
+// the number of parts, at most `splits`. Errors are left for cudaGetLastError.
+int launch_logits(const WispMoeConfig* c, const uint16_t* x, const uint16_t* W, float* part,
+                  size_t splits, cudaStream_t st) {
   const int T = c->tokens, E = c->n_experts, M = c->hidden;
-  int nsplit = 1;
   if (T <= kGemvMaxT) {
     const int g = (E + 1) / 2;
     if (c->router_fp16)
       wb::launch_k(router_gemv_kernel<true>, g, 256, 0, st, x, W, part, T, E, M);
     else
       wb::launch_k(router_gemv_kernel<false>, g, 256, 0, st, x, W, part, T, E, M);
-  } else {
-    // fp16 weights stay on the fp32 SIMT kernel (the tensor cores would need
-    // the bf16 activations rounded to fp16).
-    const int gran = c->router_fp16 ? kRK : kMK;
-    int kspan = (M + (int)splits - 1) / (int)splits;
-    kspan = (kspan + gran - 1) / gran * gran;
-    nsplit = (M + kspan - 1) / kspan;
-    dim3 g1((E + kRE - 1) / kRE, (T + kRT - 1) / kRT, nsplit);
-    if (c->router_fp16)
-      wb::launch_k(router_logits_kernel<true>, g1, 256, 0, st, x, W, part, T, E, M, kspan);
-    else
-      wb::launch_k(router_mma_kernel, g1, 128, 0, st, x, W, part, T, E, M, kspan);
+    return 1;
   }
+  // fp16 weights stay on the fp32 SIMT kernel (the tensor cores would need
+  // the bf16 activations rounded to fp16).
+  const int gran = c->router_fp16 ? kRK : kMK;
+  int kspan = (M + (int)splits - 1) / (int)splits;
+  kspan = (kspan + gran - 1) / gran * gran;
+  const int nsplit = (M + kspan - 1) / kspan;
+  dim3 g1((E + kRE - 1) / kRE, (T + kRT - 1) / kRT, nsplit);
+  if (c->router_fp16)
+    wb::launch_k(router_logits_kernel<true>, g1, 256, 0, st, x, W, part, T, E, M, kspan);
+  else
+    wb::launch_k(router_mma_kernel, g1, 128, 0, st, x, W, part, T, E, M, kspan);
+  return nsplit;
+}
+
+WispError launch_route(const WispMoeConfig* c, const uint16_t* x, const uint16_t* W,
+                       const float* bias, float* part, size_t splits, float* logits_out, int* idx,
+                       float* w, cudaStream_t st, WispErrCtx* err) {
+  const int T = c->tokens, E = c->n_experts;
+  const int nsplit = launch_logits(c, x, W, part, splits, st);
   auto topk = E <= 32 ? topk_kernel<1> : E <= 64 ? topk_kernel<2> : E <= 128 ? topk_kernel<4>
             : E <= 256 ? topk_kernel<8> : E <= 512 ? topk_kernel<16> : topk_kernel<32>;
   // two tokens per block (one warp each), so a few hundred tokens still

@@ -1,0 +1,65 @@
+"""Which experts each token goes to, from the router's logits: softmax or sigmoid scores, a
+bias that chooses without weighing, groups, top-k (wisp_b200_select_experts in
+include/wisp_b200.h)."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import abi
+from .fp4 import dtype_code, elsewhere, invalid, refuse_grad, row_stride, same_device, stream_of, \
+    wants_grad
+
+
+def policy(scoring: int = abi.WISP_ROUTE_SIGMOID, n_groups: int = 1, topk_groups: int = 1,
+           group_top: int = 2, renormalize: bool = True, scaling: float = 1.0) -> abi.WispRouting:
+    """How tokens are routed, for select_experts and fp8.Fp8MoeLayer."""
+    return abi.WispRouting(scoring, n_groups, topk_groups, group_top, 1 if renormalize else 0,
+                           scaling)
+
+
+def check_bias(bias: torch.Tensor | None, n_experts: int, what: str = "bias") -> None:
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n_experts,) or
+                             not bias.is_contiguous()):
+        raise invalid(f"{what}: contiguous float32 [{n_experts}]")
+
+
+def select_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = None,
+                   scoring: int = abi.WISP_ROUTE_SIGMOID, n_groups: int = 1, topk_groups: int = 1,
+                   group_top: int = 2, renormalize: bool = True, scaling: float = 1.0):
+    """(idx int32 [tokens, top_k], weights float32 [tokens, top_k]) of logits [tokens, experts]
+    (float32, bfloat16 or float16):
+
+        score  = softmax(logits) or sigmoid(logits);  choice = score + bias
+        the topk_groups of n_groups groups with the largest sum of their group_top best choices
+        idx    = the top_k of their experts by choice, largest first
+        weight = score (renormalize: / the sum over the top_k) * scaling
+
+    Computed in 64 bits; ties go to the lower index. NaN and -infinite choices are never taken;
+    slots without an expert have idx -1 and weight 0. No gradient: tensors that require one are
+    refused under grad mode."""
+    if wants_grad(logits, bias):
+        refuse_grad()
+    ld = row_stride(logits, "logits")
+    tokens, experts = logits.shape
+    dt = dtype_code(logits.dtype, "logits")
+    check_bias(bias, experts)
+    other = elsewhere(logits)
+    if other is not None:
+        with other:
+            return select_experts(logits, top_k, bias=bias, scoring=scoring, n_groups=n_groups,
+                                  topk_groups=topk_groups, group_top=group_top,
+                                  renormalize=renormalize, scaling=scaling)
+    if bias is not None:
+        same_device(logits, bias=bias)
+    if not 0 < top_k <= 32:
+        raise invalid(f"top_k={top_k} (1..32)")
+    r = abi.WispRouting(scoring, n_groups, topk_groups, group_top, 1 if renormalize else 0, scaling)
+    # one allocation: indices, then weights
+    buf = logits.new_empty((2, tokens, top_k), dtype=torch.int32)
+    idx, w = buf[0], buf[1].view(torch.float32)
+    abi.call("wisp_b200_select_experts", C.byref(r), logits.data_ptr(), dt, ld, tokens, experts,
+             top_k, None if bias is None else bias.data_ptr(), idx.data_ptr(), w.data_ptr(),
+             stream_of(logits))
+    return idx, w
