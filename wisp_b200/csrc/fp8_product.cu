@@ -3,26 +3,37 @@
 // matrices with one per block of 128 x 128 (one expert per segment of rows).
 //
 // The scales are no powers of two, so the tensor cores cannot apply them: each
-// block of 128 k is one MMA accumulation in tensor memory (four tcgen05.mma of
-// 32 k), which the epilogue warps scale and add to fp32 sums in registers while
-// the MMAs of the next blocks fill other buffers.
+// block of 128 k is an MMA accumulation of its own in tensor memory (four
+// tcgen05.mma of 32 k), which the epilogue warps scale and add to fp32 sums in
+// registers while the MMAs of the next blocks fill other buffers.
 //
 // Two forms of tile, for one CTA pair (cta_group::2, M = 256) or a single CTA
 // (cta_group::1, M = 128):
 //   narrow (at most 128 rows): the features are the MMA's M (128 per CTA), the
 //     rows its N, any multiple of 16 (32 in a pair), so that a weight matrix
 //     streams through once and few rows cost little. An accumulator lane is one
-//     feature: the weight scale is the tile's, the rows' scales run over the
-//     columns and are read from shared memory.
+//     feature; the rows' scales run over the columns and are read from shared
+//     memory.
 //   wide (129 to 256 rows, pairs only): the rows are M (128 per CTA), N is 256
 //     features, one block of 128 in either CTA's shared memory: two of one
 //     matrix, or gate in the even and up in the odd CTA. A lane is one row: its
 //     scale is one register, where the narrow form would read 4 bytes of shared
-//     memory per accumulator and block (and takes two passes over the weights).
+//     memory per accumulator and block (and take two passes over the weights).
+//
+// What a buffer of accumulators waits for bounds a product of many rows: from its
+// MMAs' issue to the next ones' into it pass their own time, 400 cycles until the
+// barriers have reported them, the loads into registers, and 160 until the MMA
+// warp has seen it free. So a buffer is a group of at most 128 columns (gate, up,
+// or half of a wide tile's features), four of which or more take turns, and it is
+// free as soon as it has been read, before the last of it is added.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
-// swizzle), 1 the MMAs, 2 hands out the tiles, 4-11 are the epilogue, with the
-// registers that the first four give up.
+// swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
+// epilogue, with the registers that the first four give up. An epilogue warp's work
+// on a group is a chain of dependent steps (wait, load, release, add) that its one
+// companion on the scheduler cannot hide, so the steps around the additions are kept
+// few: one wait a group, no branch by lane, no addresses to work out, and of a wide
+// tile each group to four of the warps.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -39,20 +50,22 @@ constexpr int kABytes = 128 * 128;
 constexpr int kNarrow = 128;      // rows of a narrow tile at most
 constexpr int kWide = 256;
 constexpr int kMaxStages = 12;
-constexpr int kMaxBufs = 8;       // accumulators of one block of k
+constexpr int kGroup = 128;       // columns of a group of accumulators at most
+constexpr int kMaxBufs = 8;
 constexpr int kRingBytes = 208 * 1024;
+// Blocks whose products of scales are ready, and whose scales are held or on their
+// way; scales of a block: of the CTA's rows, then the weights' two.
+constexpr int kScaleSlots = 4, kRawSlots = 8, kRawFloats = 132;
 constexpr int kTileRing = 8;
-// Registers: launch 168 x 384 = 64,512; 256 x 208 + 128 x 80 = 63,488.
-constexpr int kEpiRegs = 208, kOtherRegs = 80;
-// Scales of one epilogue warp and block of k: of its rows (64 columns of a
-// narrow tile, 32 lanes of a wide one), then the weights' two.
-constexpr int kScaleSlots = 4, kSlotFloats = 68;
-
+// Registers: launch 168 x 384 = 64,512; 256 x 232 + 128 x 40 = 64,512.
+constexpr int kEpiRegs = 232, kOtherRegs = 40;
 struct Bars {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
   uint64_t acc_full[kMaxBufs];
   uint64_t acc_empty[kMaxBufs];
+  uint64_t scale_full[kScaleSlots];
+  uint64_t scale_empty[kScaleSlots];
   uint64_t red_full, red_empty;     // partial sums of a cluster's CTAs
   uint64_t tile_full[kTileRing];
   uint64_t tile_empty[kTileRing];
@@ -74,7 +87,6 @@ struct alignas(64) Params {
   int cap;                // rows per tile at most: a multiple of 32 up to kNarrow, or kWide
   void* out;
   int64_t ld;
-  int out_type;
   int wide_out;           // output rows start on 32-byte boundaries
   int* error_flag;
 };
@@ -106,222 +118,211 @@ WB_DEV void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 
-// The wait for a tmem_ld16's registers; as operands of it, they cannot be read
-// before.
-WB_DEV void tmem_wait_regs(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
+// Registers that a wait for loads has covered: as operands, they cannot be read
+// before it.
+WB_DEV void waited(uint32_t (&v)[32]) {
+  asm volatile(""
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
                  "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
-                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
+                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31])
                :
                : "memory");
+}
+// Arrivals of one lane without a branch.
+WB_DEV void arrive_one(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+template <int COUNT>
+WB_DEV void arrive_one_remote(uint32_t cluster_bar) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+      "@p mbarrier.arrive.shared::cluster.b64 _, [%0], %1;\n\t}"
+      ::"r"(cluster_bar), "n"(COUNT) : "memory");
 }
 
 WB_DEV void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
 }
 
-// Two products, two sums of products per instruction.
-WB_DEV float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
+// Two sums of products per instruction.
 WB_DEV void fma2(float2& c, float2 a, float2 b) {
   asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
       "mov.b64 z, {%0, %1};\n\tfma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
       : "+f"(c.x), "+f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
 }
 
-// The sums of one thread, 128 or fewer in use.
-//   narrow: [matrix][chunk j: rows (2 j + half) 16 ..][16]; one matrix uses the
-//           first 64
+// The sums of one thread.
 //   wide:   features [half 64 ..][64] of the first block of 128, then of the second
+//   narrow: [matrix][chunk j: rows (2 j + half) 32 ..][32]; one matrix uses the
+//           first 32
 struct Sums {
   float2 v[64];
 };
 
-// The epilogue's scales of coming blocks: every warp fetches its own, kScaleSlots
-// - 1 blocks ahead, with cp.async (4 bytes, so that rows' scales may lie
-// anywhere).
-struct Scales {
-  float* ring;              // this warp's [kScaleSlots][kSlotFloats]
-  const float* x0;          // the lane's (up to) two rows
-  const float* x1;
-  const float* w;           // lanes 0, 1: a weight scale
-  int64_t step;
-  int kk, k1, slot;
+// A warp of the epilogue.
+struct Warp {
+  int lane, quad, half, rank;
+};
 
-  WB_DEV void fetch() {
+// Waits for two barriers at once; all lanes get the same answer, false: given up.
+WB_DEV bool wait_both(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, volatile int* abort) {
+  const bool ra = mbar_try_wait(a, pa), rb = mbar_try_wait(b, pb);
+  bool ok = ra && rb;
+  if (__all_sync(0xffffffffu, ok)) return true;
+  ok = mbar_wait(a, pa, abort) && mbar_wait(b, pb, abort);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// sums += accumulators * a scale each, of 32 columns.
+WB_DEV void add32(float2* v, const uint32_t (&u)[32], float y) {
+#pragma unroll
+  for (int q = 0; q < 16; q++)
+    fma2(v[q], make_float2(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1])),
+         make_float2(y, y));
+}
+WB_DEV void add32(float2* v, const uint32_t (&u)[32], const float* s) {
+#pragma unroll
+  for (int q = 0; q < 16; q += 2) {
+    const float4 y = *reinterpret_cast<const float4*>(s + 2 * q);
+    fma2(v[q], make_float2(__uint_as_float(u[2 * q]), __uint_as_float(u[2 * q + 1])),
+         make_float2(y.x, y.y));
+    fma2(v[q + 1], make_float2(__uint_as_float(u[2 * q + 2]), __uint_as_float(u[2 * q + 3])),
+         make_float2(y.z, y.w));
+  }
+}
+
+// The scale warp: of a tile's scales, block by block, the products of each row's
+// with the weights' two (gate and up, or a wide tile's blocks of features). The
+// scales come by cp.async (4 bytes, so that rows' scales may lie anywhere)
+// kRawSlots - 1 blocks ahead. Rows past the tile's have none: what their lanes and
+// columns hold is not stored.
+template <bool SWIGLU>
+WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank, int k0, int k1,
+                            Bars& bars, float (*raw)[kRawFloats], float (*products)[256], Ring& r,
+                            bool& first, volatile int* abort) {
+  const int lane = threadIdx.x & 31;
+  const int row = (wide ? rank * 128 : 0) + lane, left = t.cnt - row;
+  const float* x = p.xs + (t.row0 + (int64_t)row) * p.xs_row + k0 * p.xs_block;
+  const int fb = wide && !SWIGLU ? (t.ft & ~1) + lane : t.ft;
+  const float* w = (SWIGLU && lane ? p.ws_up : p.ws_w) +
+                   ((int64_t)t.expert * p.ftiles + min(fb, p.ftiles - 1)) * p.nk + k0;
+  const bool two = SWIGLU || wide, has_w = lane < (two ? 2 : 1);
+  const int groups = min(4, (t.cnt - (wide ? rank * 128 : 0) + 31) >> 5);     // of 32 rows
+  int in = 0;
+  auto fetch = [&](int kk) {
     if (kk < k1) {
-      float* s = ring + slot * kSlotFloats;
-      const int lane = threadIdx.x & 31;
-      if (x0) cp_async_4(s + lane, x0 + kk * step);
-      if (x1) cp_async_4(s + 32 + lane, x1 + kk * step);
-      if (w) cp_async_4(s + 64 + lane, w + kk);
+      float* s = raw[in] + lane;
+      if (left > 0) cp_async_4(s, x);
+      if (left > 32) cp_async_4(s + 32, x + 32 * p.xs_row);
+      if (left > 64) cp_async_4(s + 64, x + 64 * p.xs_row);
+      if (left > 96) cp_async_4(s + 96, x + 96 * p.xs_row);
+      if (has_w) cp_async_4(s + 128, w);
+      x += p.xs_block;
+      w++;
     }
     cp_async_commit();
-    kk++;
-    if (++slot == kScaleSlots) slot = 0;
-  }
-};
-
-template <bool SWIGLU, bool PAIR>
-struct Epilogue {
-  const Params& p;
-  int lane, quad, half, rank;
-
-  WB_DEV bool wide(const Tile& t) const { return PAIR && t.cnt > kNarrow; }
-
-  // Starts the fetches of a tile's scales. (Rows past the tile's have none:
-  // what their lanes and columns hold is not stored.)
-  WB_DEV void begin(Scales& sc, const Tile& t, int k0, int k1) const {
-    sc.step = p.xs_block;
-    sc.kk = k0;
-    sc.k1 = k1;
-    sc.slot = 0;
-    sc.x0 = sc.x1 = sc.w = nullptr;
-    const int nfb = p.ftiles;
-    const int last = nfb - 1;
-    if (wide(t)) {
-      const int r = rank * 128 + quad * 32 + lane;
-      if (r < t.cnt) sc.x0 = p.xs + (t.row0 + (int64_t)r) * p.xs_row;
-      if (lane < 2) {
-        const float* w = SWIGLU && lane ? p.ws_up : p.ws_w;
-        const int fb = SWIGLU ? t.ft : (t.ft & ~1) + lane;
-        sc.w = w + ((int64_t)t.expert * nfb + min(fb, last)) * p.nk;
-      }
-    } else {
-      const int c0 = (lane >> 4) * 32 + half * 16 + (lane & 15);
-      if (c0 < t.cnt) sc.x0 = p.xs + (t.row0 + (int64_t)c0) * p.xs_row;
-      if (c0 + 64 < t.cnt) sc.x1 = p.xs + (t.row0 + (int64_t)c0 + 64) * p.xs_row;
-      if (lane < (SWIGLU ? 2 : 1))
-        sc.w = (lane ? p.ws_up : p.ws_w) + ((int64_t)t.expert * nfb + min(t.ft, last)) * p.nk;
+    in = (in + 1) % kRawSlots;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kRawSlots - 1; i++) fetch(k0 + i);
+  for (int kk = k0; kk < k1; kk++) {
+    __syncwarp();                // the slot that is filled next has been read
+    const float* s = raw[(in + 1) % kRawSlots];
+    fetch(kk + kRawSlots - 1);
+    cp_async_wait<kRawSlots - 1>();
+    const bool ok = first || mbar_wait(&bars.scale_empty[r.s], r.ph ^ 1, abort);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    __syncwarp();                // every lane's copies of this block have landed
+    float* o = products[r.s] + lane;
+    const float w0 = s[128], w1 = two ? s[129] : 0.f;
+    for (int i = 0; i < groups; i++) {
+      const float v = s[32 * i + lane];
+      o[32 * i] = v * w0;
+      if (two) o[128 + 32 * i] = v * w1;
     }
-#pragma unroll
-    for (int i = 0; i < kScaleSlots - 1; i++) sc.fetch();
+    __syncwarp();
+    arrive_one(&bars.scale_full[r.s]);
+    r.next(kScaleSlots);
+    if (r.s == 0) first = false;
   }
+  return true;
+}
 
-  // sums += scales * one block's accumulators at column d (up: at du).
-  WB_DEV void add(Sums& a, const Tile& t, const float* s, uint32_t d, uint32_t du) const {
-    if (wide(t)) {
-      const float x = s[lane];
-      const float2 s0 = make_float2(x * s[64], x * s[64]), s1 = make_float2(x * s[65], x * s[65]);
-      uint32_t u[2][16];
-      tmem_ld16(d + half * 64, u[0]);
+template <bool SWIGLU, typename T>
+WB_DEV void store_wide(const Params& p, const Sums& a, const Tile& t, const Warp& me) {
+  const int r = me.rank * 128 + me.quad * 32 + me.lane;
+  if (r >= t.cnt) return;
+  T* row = static_cast<T*>(p.out) + (t.row0 + (int64_t)r) * p.ld;
+  constexpr int kRun = 32 / (int)sizeof(T);      // values of a 32-byte store
 #pragma unroll
-      for (int j = 0; j < 8; j++) {      // 16 columns each
-        tmem_wait_regs(u[j & 1]);
-        if (j < 7) tmem_ld16(d + half * 64 + (j + 1 >> 2) * 128 + (j + 1 & 3) * 16, u[j + 1 & 1]);
+  for (int q = 0; q < (SWIGLU ? 1 : 2); q++) {
+    const int f = (SWIGLU ? t.ft : (t.ft & ~1) + q) * 128 + me.half * 64;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          fma2(a.v[j * 8 + i],
-               make_float2(__uint_as_float(u[j & 1][2 * i]), __uint_as_float(u[j & 1][2 * i + 1])),
-               j < 4 ? s0 : s1);
+    for (int i = 0; i < 64; i += kRun) {
+      float o[kRun];
+#pragma unroll
+      for (int j = 0; j < kRun; j++) {
+        const float2 g = a.v[q * 32 + (i + j) / 2];
+        o[j] = j & 1 ? g.y : g.x;
+        if (SWIGLU) {
+          const float2 u = a.v[32 + (i + j) / 2];
+          o[j] = swiglu<T>(o[j], j & 1 ? u.y : u.x);
+        }
       }
-    } else {
-      const float2 wg = make_float2(s[64], s[64]);
-      const float2 wu = SWIGLU ? make_float2(s[65], s[65]) : wg;
+      if (p.wide_out && f + i + kRun <= p.N) {
+        uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int c = (2 * j + half) * 16;
-        if (c < t.cnt) {
-          uint32_t g[16], u[16];
-          tmem_ld16(d + c, g);
-          if (SWIGLU) tmem_ld16(du + c, u);
-          tmem_wait_regs(g);
-          if (SWIGLU) tmem_wait_regs(u);
+        for (int j = 0; j < 8; j++) {
+          if constexpr (sizeof(T) == 4)
+            w[j] = __float_as_uint(o[j]);
+          else
+            w[j] = pack2(o[2 * j], o[2 * j + 1],
+                         std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+        }
+        store32(row + f + i, w);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float4 x = *reinterpret_cast<const float4*>(s + j * 16 + i * 2);
+        for (int j = 0; j < kRun; j++)
+          if (f + i + j < p.N) put_out(row + f + i + j, o[j]);
+      }
+    }
+  }
+}
+
+template <bool SWIGLU, typename T>
+WB_DEV void store_narrow(const Params& p, const Sums& a, const Tile& t, const Warp& me) {
+  const int64_t ld = p.ld;
+  const int f = t.ft * 128 + me.quad * 32 + me.lane;
+  if (f >= p.N) return;
+  T* out = static_cast<T*>(p.out) + (int64_t)t.row0 * ld + f;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const float2 xs = h ? make_float2(x.z, x.w) : make_float2(x.x, x.y);
-              const int r = 2 * (i + h);
-              fma2(a.v[j * 8 + i + h],
-                   mul2(make_float2(__uint_as_float(g[r]), __uint_as_float(g[r + 1])), wg), xs);
-              if (SWIGLU)
-                fma2(a.v[32 + j * 8 + i + h],
-                     mul2(make_float2(__uint_as_float(u[r]), __uint_as_float(u[r + 1])), wu), xs);
-            }
+  for (int j = 0; j < 2; j++) {
+    const int c = (2 * j + me.half) * 32;
+    if (c < t.cnt) {
+      T* q = out + c * ld;
+#pragma unroll
+      for (int i = 0; i < 32; i++, q += ld) {
+        if (c + i < t.cnt) {
+          const float2 g = a.v[j * 16 + i / 2];
+          float o = i & 1 ? g.y : g.x;
+          if (SWIGLU) {
+            const float2 u = a.v[32 + j * 16 + i / 2];
+            o = swiglu<T>(o, i & 1 ? u.y : u.x);
           }
+          put_out(q, o);
         }
       }
     }
   }
-
-  template <typename T>
-  WB_DEV void store(const Sums& a, const Tile& t) const {
-    const int64_t ld = p.ld;
-    if (wide(t)) {
-      const int r = rank * 128 + quad * 32 + lane;
-      if (r >= t.cnt) return;
-      T* row = static_cast<T*>(p.out) + (t.row0 + (int64_t)r) * ld;
-#pragma unroll
-      for (int b = 0; b < (SWIGLU ? 1 : 2); b++) {
-        const int f = (SWIGLU ? t.ft : (t.ft & ~1) + b) * 128 + half * 64;
-        constexpr int kRun = 32 / (int)sizeof(T);      // values of a 32-byte store
-#pragma unroll
-        for (int i = 0; i < 64; i += kRun) {
-          float o[kRun];
-#pragma unroll
-          for (int j = 0; j < kRun; j++) {
-            const float2 g = a.v[b * 32 + (i + j) / 2];
-            o[j] = j & 1 ? g.y : g.x;
-            if (SWIGLU) {
-              const float2 u = a.v[32 + (i + j) / 2];
-              o[j] = swiglu<T>(o[j], j & 1 ? u.y : u.x);
-            }
-          }
-          if (p.wide_out && f + i + kRun <= p.N) {
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              if constexpr (sizeof(T) == 4)
-                w[j] = __float_as_uint(o[j]);
-              else
-                w[j] = pack2(o[2 * j], o[2 * j + 1],
-                             std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
-            }
-            store32(row + f + i, w);
-          } else {
-#pragma unroll
-            for (int j = 0; j < kRun; j++)
-              if (f + i + j < p.N) put_out(row + f + i + j, o[j]);
-          }
-        }
-      }
-    } else {
-      const int f = t.ft * 128 + quad * 32 + lane;
-      if (f >= p.N) return;
-      T* out = static_cast<T*>(p.out) + (int64_t)t.row0 * ld + f;
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int c = (2 * j + half) * 16;
-        if (c < t.cnt) {
-          T* q = out + c * ld;
-#pragma unroll
-          for (int i = 0; i < 16; i++, q += ld) {
-            if (c + i < t.cnt) {
-              const float2 g = a.v[j * 8 + i / 2];
-              float o = i & 1 ? g.y : g.x;
-              if (SWIGLU) {
-                const float2 u = a.v[32 + j * 8 + i / 2];
-                o = swiglu<T>(o, i & 1 ? u.y : u.x);
-              }
-              put_out(q, o);
-            }
-          }
-        }
-      }
-    }
-  }
-};
+}
 
 // The join of a cluster whose CTAs split K (narrow tiles of at most 64 rows).
-// 32 rows at a time, every CTA puts its sums into its shared memory, and CTA kp
+// 16 rows of each half at a time, every CTA puts its sums into its shared memory, and CTA kp
 // adds those of all, in the order of K, for the rows kp, kp + ks, ... (a warp per
 // row, 4 features per lane).
 constexpr int kRedRows = 32, kSplitRows = 64;
@@ -339,17 +340,17 @@ struct Reduce {
   }
 
   template <typename T>
-  WB_DEV bool store(const Params& p, const Sums& a, const Tile& t, int quad, int half,
+  WB_DEV bool store(const Params& p, const Sums& a, const Tile& t, const Warp& me,
                     volatile int* abort) {
-    const int lane = threadIdx.x & 31, w = half * 4 + quad;
+    const int lane = me.lane, w = me.half * 4 + me.quad;
 #pragma unroll
     for (int j = 0; j < kSplitRows / kRedRows; j++) {
-      const int c = j * kRedRows;
-      if (c >= t.cnt) break;
+      // rows 16 j + (0 .. 15) and 32 + 16 j + (0 .. 15)
+      if (16 * j >= t.cnt) break;
       bool ok = uses == 0 || mbar_wait_cluster(&bars->red_empty, (uses - 1) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) return false;
-      if (c + half * 16 < t.cnt) {
-        float* q = buf + half * 16 * 128 + quad * 32 + lane;
+      if (me.half * 32 + 16 * j < t.cnt) {
+        float* q = buf + me.half * 16 * 128 + me.quad * 32 + lane;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const float2 g = a.v[j * 8 + i / 2];
@@ -363,7 +364,9 @@ struct Reduce {
       arrive_all(&bars->red_full);
       ok = mbar_wait_cluster(&bars->red_full, uses & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) return false;
-      for (int r = kp + ks * w; r < min(kRedRows, t.cnt - c); r += ks * 8) {
+      for (int r = kp + ks * w; r < kRedRows; r += ks * 8) {
+        const int row = (r & 16) * 2 + 16 * j + (r & 15);
+        if (row >= t.cnt) continue;
         float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
         for (int i = 0; i < ks; i++) {
           const uint32_t at = cluster_addr(buf + r * 128 + lane * 4, i);
@@ -381,7 +384,7 @@ struct Reduce {
           }
         }
         const int f = t.ft * 128 + lane * 4;
-        T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)(c + r)) * p.ld + f;
+        T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)row) * p.ld + f;
 #pragma unroll
         for (int i = 0; i < 4; i++)
           if (f + i < p.N) put_out(out + i, SWIGLU ? swiglu<T>(v[i], x[i]) : v[i]);
@@ -393,14 +396,18 @@ struct Reduce {
   }
 };
 
-template <bool SWIGLU, bool PAIR>
+// One output type per kernel: with all three in one, the sums' unrolled stores do
+// not stay in the instruction cache, and a tile's first pass through them cost 3 to
+// 12 us.
+template <typename T, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_product_kernel(const __grid_constant__ Params p) {
   constexpr int kMats = SWIGLU ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
-  __shared__ alignas(16) float scales[8][kScaleSlots][kSlotFloats];
+  __shared__ alignas(16) float raw[kRawSlots][kRawFloats];
+  __shared__ alignas(16) float products[kScaleSlots][256];      // of scales
   __shared__ int pref[kMaxSegs];
   __shared__ uint16_t order[kMaxSegs];
   __shared__ int4 warp_tot[kThreads / 32];
@@ -427,7 +434,11 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     mbar_init(&bars.empty[tid], 1);
     if (tid < kTileRing) {
       mbar_init(&bars.tile_full[tid], 1);
-      mbar_init(&bars.tile_empty[tid], 10);     // all warps that walk the tiles
+      mbar_init(&bars.tile_empty[tid], 11);     // all warps that walk the tiles
+    }
+    if (tid < kScaleSlots) {
+      mbar_init(&bars.scale_full[tid], 1);
+      mbar_init(&bars.scale_empty[tid], 8);
     }
     if (tid < kMaxBufs) {
       mbar_init(&bars.acc_full[tid], 1);
@@ -473,9 +484,11 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   const int stage_bytes = wides ? max(narrow_bytes, 2 * kABytes) : narrow_bytes;
   constexpr int kRedBytes = kMats * kRedRows * 128 * 4;     // a cluster's partial sums
   const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
-  // accumulators: buffers of `cols` columns (gate, then up)
-  const int up_offset = (narrow_n + 31) & ~31;
-  const int cols = wides ? kWide : up_offset * kMats;
+  // accumulators: buffers of `cols` columns, one for a group; gate and up are one
+  // group where both fit
+  const int cols1 = (narrow_n + 31) & ~31;
+  const bool together = SWIGLU && !wides && 2 * cols1 <= kGroup;
+  const int cols = wides ? kGroup : together ? 2 * cols1 : cols1;
   const int bufs = min(kMaxBufs, 512 / cols);
   TileWalk<kTileRing> tiles;
   Tile t;
@@ -548,35 +561,40 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     while (ok && tiles.next(bars, t, abort)) {
       const bool wide = PAIR && t.cnt > kNarrow;
       const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
-      const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kWide : n);
+      const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kGroup : n);
       for (int kk = k0; kk < k1; kk++) {
-        if (!fresh && !(PAIR ? mbar_wait_cluster(&bars.acc_empty[b.s], b.ph ^ 1, abort)
-                             : mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort))) { ok = false; break; }
         if (PAIR ? !mbar_wait_cluster(&bars.full[r.s], r.ph, abort)
                  : !mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
-        tc_fence_after();
+        // A, B: rows and weights of a wide tile, weights and rows of a narrow one. A
+        // second group takes the other 64 of each CTA's features, or up's weights.
         const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
-        const uint32_t d = tmem + b.s * cols, du = d + up_offset;
-        if (elect_sync()) {
-          const uint64_t dw = smem_desc_sw128(st);
-          const uint64_t dx = smem_desc_sw128(st + (wide ? kABytes : kMats * kABytes));
+        const uint64_t dw = smem_desc_sw128(st);
+        const uint64_t dx = smem_desc_sw128(st + (wide ? kABytes : kMats * kABytes));
+        const int groups = wide ? 2 : together ? 1 : kMats;
+        for (int g = 0; g < groups; g++) {
+          if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem + b.s * cols;
+          const uint64_t da = wide ? dx : dw + g * (kABytes >> 4);
+          const uint64_t db = wide ? dw + g * (kABytes / 2 >> 4) : dx;
+          if (elect_sync()) {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {          // 32 k (32 bytes) each
-            if (wide) {
-              mma_fp8<PAIR>(d, dx + j * 2, dw + j * 2, idesc, j ? 1u : 0u);
-            } else {
-              mma_fp8<PAIR>(d, dw + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
-              if (SWIGLU)
-                mma_fp8<PAIR>(du, dw + (kABytes >> 4) + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
+            for (int j = 0; j < 4; j++)            // 32 k (32 bytes) each
+              mma_fp8<PAIR>(d, da + j * 2, db + j * 2, idesc, j ? 1u : 0u);
+            if (together) {
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                mma_fp8<PAIR>(d + cols1, da + (kABytes >> 4) + j * 2, db + j * 2, idesc, j ? 1u : 0u);
             }
+            commit<PAIR>(&bars.acc_full[b.s]);
+            if (g == groups - 1) commit<PAIR>(&bars.empty[r.s]);
           }
-          commit<PAIR>(&bars.empty[r.s]);
-          commit<PAIR>(&bars.acc_full[b.s]);
+          __syncwarp();
+          b.next(bufs);
+          if (b.s == 0) fresh = false;
         }
-        __syncwarp();
+        if (!ok) break;
         r.next(S);
-        b.next(bufs);
-        if (b.s == 0) fresh = false;
         uses = min(uses + 1, S);
       }
     }
@@ -592,64 +610,129 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     cluster_wait();
     // warp % 4 is the lane quadrant; the two warps of a quadrant take alternate
     // groups of 16 rows of a narrow tile, a half of each 128 features of a wide one
-    Epilogue<SWIGLU, PAIR> epi{p, lane, warp & 3, (warp - kEpiWarp) >> 2, rank};
+    const Warp me = {lane, warp & 3, (warp - kEpiWarp) >> 2, rank};
     Reduce<SWIGLU> red;
     red.buf = reinterpret_cast<float*>(smem + kRingBytes - kRedBytes);
     red.bars = &bars;
     red.ks = ks;
     red.kp = kp;
-    Scales sc;
-    sc.ring = &scales[warp - kEpiWarp][0][0];
-    Ring b;
-    const uint32_t quad_lane = (uint32_t)(epi.quad * 32) << 16;
+    Ring b, sc;                  // accumulators, scales
+    const uint32_t base = tmem + ((uint32_t)(me.quad * 32) << 16);
+    const uint32_t empty0 = cluster_addr(&bars.acc_empty[0], PAIR ? 0 : kp);
     bool ok = true;
+    // A group's turn: waits for its accumulators, the first of a block also for its
+    // products of scales.
+    auto full = [&](bool first) {
+      if (first)
+        ok = wait_both(&bars.acc_full[b.s], b.ph, &bars.scale_full[sc.s], sc.ph, abort);
+      else
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.acc_full[b.s], b.ph, abort));
+      tc_fence_after();
+      return ok;
+    };
+    // The accumulators have been read.
+    auto release = [&](bool alone) {
+      tc_fence_before();
+      __syncwarp();
+      if (!PAIR)
+        arrive_one(&bars.acc_empty[b.s]);
+      else if (alone)
+        arrive_one_remote<2>(empty0 + b.s * 8);      // (for the other half's warp too)
+      else
+        arrive_one_remote<1>(empty0 + b.s * 8);
+      b.next(bufs);
+    };
+    auto release_scales = [&]() {
+      __syncwarp();
+      arrive_one(&bars.scale_empty[sc.s]);
+      sc.next(kScaleSlots);
+    };
     while (ok && tiles.next(bars, t, abort)) {
-      epi.begin(sc, t, k0, k1);
+      const bool wide = PAIR && t.cnt > kNarrow;
       Sums a;
 #pragma unroll
       for (int i = 0; i < 64; i++) a.v[i] = make_float2(0.f, 0.f);
-      int slot = 0;
-      for (int kk = k0; kk < k1; kk++) {
-        __syncwarp();          // the slot that is filled next has been read
-        sc.fetch();
-        ok = mbar_wait(&bars.acc_full[b.s], b.ph, abort);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        cp_async_wait<kScaleSlots - 1>();
-        __syncwarp();          // every lane's copies of this block have landed
-        tc_fence_after();
-        const uint32_t d = tmem + quad_lane + b.s * cols;
-        epi.add(a, t, sc.ring + slot * kSlotFloats, d, d + up_offset);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR)
-            mbar_arrive_remote(cluster_addr(&bars.acc_empty[b.s], 0));
-          else
-            mbar_arrive(&bars.acc_empty[b.s]);
+      if (wide) {
+        if (me.half) b.next(bufs);       // each half of the warps has a group of its own
+        for (int kk = k0; kk < k1; kk++) {
+          if (!full(true)) break;
+          uint32_t u[2][32];
+          const uint32_t d = base + b.s * cols;
+          tmem_ld32(d, u[0]);
+          tmem_ld32(d + 32, u[1]);
+          const float* s = products[sc.s] + me.quad * 32 + lane;
+          const float y0 = s[0], y1 = s[128];
+          tmem_wait_ld();
+          waited(u[0]);
+          add32(a.v, u[0], y0);
+          tmem_ld32(d + 64, u[0]);
+          waited(u[1]);
+          add32(a.v + 16, u[1], y0);
+          tmem_ld32(d + 96, u[1]);
+          release_scales();
+          tmem_wait_ld();
+          waited(u[0]);
+          waited(u[1]);
+          release(true);
+          b.next(bufs);
+          add32(a.v + 32, u[0], y1);
+          add32(a.v + 48, u[1], y1);
         }
-        b.next(bufs);
-        if (++slot == kScaleSlots) slot = 0;
+        if (me.half) b.back(bufs);
+      } else {
+        const int left = t.cnt - me.half * 32;
+        const int chunks = left > 64 ? 2 : left > 0 ? 1 : 0;
+        for (int kk = k0; kk < k1; kk++) {
+          const uint32_t c = me.half * 32;
+          const float* s = products[sc.s] + c;
+          uint32_t u[2][32];
+          if (together) {
+            if (!full(true)) break;
+            const uint32_t d = base + b.s * cols + c;
+            if (chunks > 0) {
+              tmem_ld32(d, u[0]);
+              tmem_ld32(d + cols1, u[1]);
+            }
+            tmem_wait_ld();
+            release(false);
+            if (chunks > 0) {
+              waited(u[0]);
+              waited(u[1]);
+              add32(a.v, u[0], s);
+              add32(a.v + 32, u[1], s + 128);
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < kMats; g++) {
+              if (!full(g == 0)) break;
+              const uint32_t d = base + b.s * cols + c;
+              if (chunks > 0) tmem_ld32(d, u[0]);
+              if (chunks > 1) tmem_ld32(d + 64, u[1]);
+              tmem_wait_ld();
+              release(false);
+              if (chunks > 0) {
+                waited(u[0]);
+                add32(a.v + g * 32, u[0], s + g * 128);
+              }
+              if (chunks > 1) {
+                waited(u[1]);
+                add32(a.v + g * 32 + 16, u[1], s + g * 128 + 64);
+              }
+            }
+            if (!ok) break;
+          }
+          release_scales();
+        }
       }
       if (!ok) break;
-      cp_async_wait_all();
-      __syncwarp();
-      if (!PAIR && ks > 1) {
-        if (p.out_type == WISP_DT_F32)
-          ok = red.template store<float>(p, a, t, epi.quad, epi.half, abort);
-        else if (p.out_type == WISP_DT_BF16)
-          ok = red.template store<__nv_bfloat16>(p, a, t, epi.quad, epi.half, abort);
-        else
-          ok = red.template store<__half>(p, a, t, epi.quad, epi.half, abort);
-      } else if (p.out_type == WISP_DT_F32) {
-        epi.template store<float>(a, t);
-      } else if (p.out_type == WISP_DT_BF16) {
-        epi.template store<__nv_bfloat16>(a, t);
-      } else {
-        epi.template store<__half>(a, t);
-      }
+      if (!PAIR && ks > 1)
+        ok = red.template store<T>(p, a, t, me, abort);
+      else if (wide)
+        store_wide<SWIGLU, T>(p, a, t, me);
+      else
+        store_narrow<SWIGLU, T>(p, a, t, me);
       __syncwarp();
     }
-    cp_async_wait_all();
   } else if (warp == kSchedWarp) {
     give_registers();
     if (lane == 0) {
@@ -689,6 +772,13 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     cluster_wait();
   } else {
     give_registers();
+    Ring r;
+    bool first = true;
+    while (tiles.next(bars, t, abort))
+      if (!multiply_scales<SWIGLU>(p, t, PAIR && t.cnt > kNarrow, rank, k0, k1, bars, raw, products,
+                                   r, first, abort))
+        break;
+    cp_async_wait_all();
     cluster_wait();
   }
   __syncwarp();
@@ -722,11 +812,11 @@ bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box
 }
 
 // grid CTAs in clusters of `cluster`.
-template <bool SWIGLU, bool PAIR>
-WispError launch_product(const Params& p, int dev, unsigned grid, int cluster, cudaStream_t stream,
-                         WispErrCtx* err) {
+template <typename T, bool SWIGLU, bool PAIR>
+WispError launch_kernel(const Params& p, int dev, unsigned grid, int cluster, cudaStream_t stream,
+                        WispErrCtx* err) {
   const int smem = kRingBytes + 1024;
-  auto kernel = fp8_product_kernel<SWIGLU, PAIR>;
+  auto kernel = fp8_product_kernel<T, SWIGLU, PAIR>;
   static std::atomic<uint64_t> raised{0};
   WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
   cudaLaunchConfig_t cfg = {};
@@ -744,11 +834,21 @@ WispError launch_product(const Params& p, int dev, unsigned grid, int cluster, c
   return WISP_OK;
 }
 
+template <typename T, bool PAIR>
+WispError launch_typed(bool swiglu, const Params& p, int dev, unsigned grid, int cluster,
+                       cudaStream_t stream, WispErrCtx* err) {
+  return swiglu ? launch_kernel<T, true, PAIR>(p, dev, grid, cluster, stream, err)
+                : launch_kernel<T, false, PAIR>(p, dev, grid, cluster, stream, err);
+}
+
 template <bool PAIR>
-WispError launch_product(bool swiglu, const Params& p, int dev, unsigned grid, int cluster,
-                         cudaStream_t stream, WispErrCtx* err) {
-  return swiglu ? launch_product<true, PAIR>(p, dev, grid, cluster, stream, err)
-                : launch_product<false, PAIR>(p, dev, grid, cluster, stream, err);
+WispError launch_product(const WispFp8Config* c, const Params& p, int dev, unsigned grid,
+                         int cluster, cudaStream_t stream, WispErrCtx* err) {
+  if (c->out_type == WISP_DT_F32)
+    return launch_typed<float, PAIR>(c->swiglu, p, dev, grid, cluster, stream, err);
+  if (c->out_type == WISP_DT_BF16)
+    return launch_typed<__nv_bfloat16, PAIR>(c->swiglu, p, dev, grid, cluster, stream, err);
+  return launch_typed<__half, PAIR>(c->swiglu, p, dev, grid, cluster, stream, err);
 }
 
 WispError check_mats(const WispFp8Mats* m, const char* what, WispErrCtx* err) {
@@ -833,17 +933,16 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   p.ftiles = ftiles;
   p.out = d_out;
   p.ld = ld;
-  p.out_type = cfg->out_type;
   p.wide_out = !((uintptr_t)d_out & 31) && ld * dt_size(cfg->out_type) % 32 == 0;
   p.error_flag = d_error_flag;
   if (split > 1)
-    return launch_product<false>(cfg->swiglu, p, dev, (unsigned)(items * split), split, stream, err);
+    return launch_product<false>(cfg, p, dev, (unsigned)(items * split), split, stream, err);
   if (single) {
     const int64_t want = tiles_of(cap);
-    return launch_product<false>(cfg->swiglu, p, dev, (unsigned)(want < sms ? want : sms), 1,
+    return launch_product<false>(cfg, p, dev, (unsigned)(want < sms ? want : sms), 1,
                                  stream, err);
   }
   const int64_t want = tiles_of(cap) * ((ftiles + 1) / 2) * 2;
-  return launch_product<true>(cfg->swiglu, p, dev,
+  return launch_product<true>(cfg, p, dev,
                               (unsigned)(want < (sms & ~1) ? want : sms & ~1), 2, stream, err);
 }
