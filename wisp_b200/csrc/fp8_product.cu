@@ -23,17 +23,17 @@
 // What a buffer of accumulators waits for bounds a product of many rows: from its
 // MMAs' issue to the next ones' into it pass their own time, 400 cycles until the
 // barriers have reported them, the loads into registers, and 160 until the MMA
-// warp has seen it free. So a buffer is a group of at most 128 columns (gate, up,
-// or half of a wide tile's features), four of which or more take turns, and it is
-// free as soon as it has been read, before the last of it is added.
+// warp has seen it free. So it is free as soon as it has been read, before the last
+// of it is added. (A wide tile's accumulators as two groups of 128 columns, released
+// one by one: the MMAs then read the rows twice from shared memory, which cost more
+// than the shorter cycle gained, 8192 x 8192 x 7168 457 us.)
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
 // epilogue, with the registers that the first four give up. An epilogue warp's work
 // on a group is a chain of dependent steps (wait, load, release, add) that its one
 // companion on the scheduler cannot hide, so the steps around the additions are kept
-// few: one wait a group, no branch by lane, no addresses to work out, and of a wide
-// tile each group to four of the warps.
+// few: one wait a group, no branch by lane, no addresses to work out.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -137,12 +137,10 @@ WB_DEV void arrive_one(uint64_t* bar) {
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
       "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
-template <int COUNT>
 WB_DEV void arrive_one_remote(uint32_t cluster_bar) {
   asm volatile(
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
-      "@p mbarrier.arrive.shared::cluster.b64 _, [%0], %1;\n\t}"
-      ::"r"(cluster_bar), "n"(COUNT) : "memory");
+      "@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_bar) : "memory");
 }
 
 WB_DEV void give_registers() {
@@ -561,30 +559,52 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     while (ok && tiles.next(bars, t, abort)) {
       const bool wide = PAIR && t.cnt > kNarrow;
       const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
-      const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kGroup : n);
+      const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kWide : n);
+      if (wide && (b.s & 1)) {       // its two buffers are neighbours: one goes round unused
+        if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) break;
+        if (elect_sync()) commit<PAIR>(&bars.acc_full[b.s]);
+        __syncwarp();
+        b.next(bufs);
+        if (b.s == 0) fresh = false;
+      }
       for (int kk = k0; kk < k1; kk++) {
         if (PAIR ? !mbar_wait_cluster(&bars.full[r.s], r.ph, abort)
                  : !mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
-        // A, B: rows and weights of a wide tile, weights and rows of a narrow one. A
-        // second group takes the other 64 of each CTA's features, or up's weights.
+        // A, B: rows and weights of a wide tile, weights and rows of a narrow one.
         const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
         const uint64_t dw = smem_desc_sw128(st);
         const uint64_t dx = smem_desc_sw128(st + (wide ? kABytes : kMats * kABytes));
-        const int groups = wide ? 2 : together ? 1 : kMats;
+        if (wide) {       // two buffers
+          if (!fresh && !(mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort) &&
+                          mbar_wait(&bars.acc_empty[b.s + 1], b.ph ^ 1, abort))) { ok = false; break; }
+          tc_fence_after();
+          if (elect_sync()) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)            // 32 k (32 bytes) each
+              mma_fp8<PAIR>(tmem + b.s * cols, dx + j * 2, dw + j * 2, idesc, j ? 1u : 0u);
+            commit<PAIR>(&bars.acc_full[b.s]);
+            commit<PAIR>(&bars.acc_full[b.s + 1]);
+            commit<PAIR>(&bars.empty[r.s]);
+          }
+          __syncwarp();
+          b.next(bufs);
+          b.next(bufs);
+          if (b.s == 0) fresh = false;
+        }
+        const int groups = wide ? 0 : together ? 1 : kMats;
         for (int g = 0; g < groups; g++) {
           if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem + b.s * cols;
-          const uint64_t da = wide ? dx : dw + g * (kABytes >> 4);
-          const uint64_t db = wide ? dw + g * (kABytes / 2 >> 4) : dx;
+          const uint64_t da = dw + g * (kABytes >> 4);
           if (elect_sync()) {
 #pragma unroll
-            for (int j = 0; j < 4; j++)            // 32 k (32 bytes) each
-              mma_fp8<PAIR>(d, da + j * 2, db + j * 2, idesc, j ? 1u : 0u);
+            for (int j = 0; j < 4; j++)
+              mma_fp8<PAIR>(d, da + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
             if (together) {
 #pragma unroll
               for (int j = 0; j < 4; j++)
-                mma_fp8<PAIR>(d + cols1, da + (kABytes >> 4) + j * 2, db + j * 2, idesc, j ? 1u : 0u);
+                mma_fp8<PAIR>(d + cols1, da + (kABytes >> 4) + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
             }
             commit<PAIR>(&bars.acc_full[b.s]);
             if (g == groups - 1) commit<PAIR>(&bars.empty[r.s]);
@@ -631,15 +651,13 @@ fp8_product_kernel(const __grid_constant__ Params p) {
       return ok;
     };
     // The accumulators have been read.
-    auto release = [&](bool alone) {
+    auto release = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (!PAIR)
-        arrive_one(&bars.acc_empty[b.s]);
-      else if (alone)
-        arrive_one_remote<2>(empty0 + b.s * 8);      // (for the other half's warp too)
+      if (PAIR)
+        arrive_one_remote(empty0 + b.s * 8);
       else
-        arrive_one_remote<1>(empty0 + b.s * 8);
+        arrive_one(&bars.acc_empty[b.s]);
       b.next(bufs);
     };
     auto release_scales = [&]() {
@@ -653,11 +671,14 @@ fp8_product_kernel(const __grid_constant__ Params p) {
 #pragma unroll
       for (int i = 0; i < 64; i++) a.v[i] = make_float2(0.f, 0.f);
       if (wide) {
-        if (me.half) b.next(bufs);       // each half of the warps has a group of its own
+        if (b.s & 1) {                   // (see the MMA warp)
+          if (!full(false)) break;
+          release();
+        }
         for (int kk = k0; kk < k1; kk++) {
           if (!full(true)) break;
           uint32_t u[2][32];
-          const uint32_t d = base + b.s * cols;
+          const uint32_t d = base + b.s * cols + me.half * 64;
           tmem_ld32(d, u[0]);
           tmem_ld32(d + 32, u[1]);
           const float* s = products[sc.s] + me.quad * 32 + lane;
@@ -665,20 +686,19 @@ fp8_product_kernel(const __grid_constant__ Params p) {
           tmem_wait_ld();
           waited(u[0]);
           add32(a.v, u[0], y0);
-          tmem_ld32(d + 64, u[0]);
+          tmem_ld32(d + 128, u[0]);
           waited(u[1]);
           add32(a.v + 16, u[1], y0);
-          tmem_ld32(d + 96, u[1]);
+          tmem_ld32(d + 160, u[1]);
           release_scales();
           tmem_wait_ld();
           waited(u[0]);
           waited(u[1]);
-          release(true);
-          b.next(bufs);
+          release();
+          release();
           add32(a.v + 32, u[0], y1);
           add32(a.v + 48, u[1], y1);
         }
-        if (me.half) b.back(bufs);
       } else {
         const int left = t.cnt - me.half * 32;
         const int chunks = left > 64 ? 2 : left > 0 ? 1 : 0;
@@ -694,7 +714,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
               tmem_ld32(d + cols1, u[1]);
             }
             tmem_wait_ld();
-            release(false);
+            release();
             if (chunks > 0) {
               waited(u[0]);
               waited(u[1]);
@@ -709,7 +729,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
               if (chunks > 0) tmem_ld32(d, u[0]);
               if (chunks > 1) tmem_ld32(d + 64, u[1]);
               tmem_wait_ld();
-              release(false);
+              release();
               if (chunks > 0) {
                 waited(u[0]);
                 add32(a.v + g * 32, u[0], s + g * 128);

@@ -205,12 +205,6 @@ struct Ring {
       ph ^= 1;
     }
   }
-  WB_DEV void back(int S) {
-    if (--s < 0) {
-      s = S - 1;
-      ph ^= 1;
-    }
-  }
 };
 
 // A role's walk through the tiles that the scheduler warp puts into a ring of
