@@ -23,17 +23,18 @@
 // What a buffer of accumulators waits for bounds a product of many rows: from its
 // MMAs' issue to the next ones' into it pass their own time, 400 cycles until the
 // barriers have reported them, the loads into registers, and 160 until the MMA
-// warp has seen it free. So it is free as soon as it has been read, before the last
-// of it is added. (A wide tile's accumulators as two groups of 128 columns, released
-// one by one: the MMAs then read the rows twice from shared memory, which cost more
-// than the shorter cycle gained, 8192 x 8192 x 7168 457 us.)
+// warp has seen it free. So one barrier stands for a whole block (gate and up, or
+// both blocks of features), and a buffer is free as soon as it has been read,
+// before the last of it is added. (Groups of 128 columns with barriers of their
+// own: twice the waits, and a wide tile's MMAs then read the rows twice from shared
+// memory. 8192 x 8192 x 7168 457 us.)
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
 // epilogue, with the registers that the first four give up. An epilogue warp's work
-// on a group is a chain of dependent steps (wait, load, release, add) that its one
+// on a block is a chain of dependent steps (wait, load, release, add) that its one
 // companion on the scheduler cannot hide, so the steps around the additions are kept
-// few: one wait a group, no branch by lane, no addresses to work out.
+// few: one wait a block, no branch by lane, no addresses to work out.
 #include "common.cuh"
 #include "internal.h"
 #include "numeric.cuh"
@@ -50,7 +51,6 @@ constexpr int kABytes = 128 * 128;
 constexpr int kNarrow = 128;      // rows of a narrow tile at most
 constexpr int kWide = 256;
 constexpr int kMaxStages = 12;
-constexpr int kGroup = 128;       // columns of a group of accumulators at most
 constexpr int kMaxBufs = 8;
 constexpr int kRingBytes = 208 * 1024;
 // Blocks whose products of scales are ready, and whose scales are held or on their
@@ -482,11 +482,9 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   const int stage_bytes = wides ? max(narrow_bytes, 2 * kABytes) : narrow_bytes;
   constexpr int kRedBytes = kMats * kRedRows * 128 * 4;     // a cluster's partial sums
   const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
-  // accumulators: buffers of `cols` columns, one for a group; gate and up are one
-  // group where both fit
-  const int cols1 = (narrow_n + 31) & ~31;
-  const bool together = SWIGLU && !wides && 2 * cols1 <= kGroup;
-  const int cols = wides ? kGroup : together ? 2 * cols1 : cols1;
+  // accumulators: buffers of `cols` columns, one for a block of k (gate, then up)
+  const int up_offset = (narrow_n + 31) & ~31;
+  const int cols = wides ? kWide : up_offset * kMats;
   const int bufs = min(kMaxBufs, 512 / cols);
   TileWalk<kTileRing> tiles;
   Tile t;
@@ -560,13 +558,6 @@ fp8_product_kernel(const __grid_constant__ Params p) {
       const bool wide = PAIR && t.cnt > kNarrow;
       const int n = (t.cnt + kUnit - 1) / kUnit * kUnit;
       const uint32_t idesc = idesc_fp8(PAIR ? 256 : 128, wide ? kWide : n);
-      if (wide && (b.s & 1)) {       // its two buffers are neighbours: one goes round unused
-        if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) break;
-        if (elect_sync()) commit<PAIR>(&bars.acc_full[b.s]);
-        __syncwarp();
-        b.next(bufs);
-        if (b.s == 0) fresh = false;
-      }
       for (int kk = k0; kk < k1; kk++) {
         if (PAIR ? !mbar_wait_cluster(&bars.full[r.s], r.ph, abort)
                  : !mbar_wait(&bars.full[r.s], r.ph, abort)) { ok = false; break; }
@@ -574,46 +565,22 @@ fp8_product_kernel(const __grid_constant__ Params p) {
         const uint32_t st = smem_u32(smem) + r.s * stage_bytes;
         const uint64_t dw = smem_desc_sw128(st);
         const uint64_t dx = smem_desc_sw128(st + (wide ? kABytes : kMats * kABytes));
-        if (wide) {       // two buffers
-          if (!fresh && !(mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort) &&
-                          mbar_wait(&bars.acc_empty[b.s + 1], b.ph ^ 1, abort))) { ok = false; break; }
-          tc_fence_after();
-          if (elect_sync()) {
+        const uint32_t d = tmem + b.s * cols;
+        if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_sync()) {
 #pragma unroll
-            for (int j = 0; j < 4; j++)            // 32 k (32 bytes) each
-              mma_fp8<PAIR>(tmem + b.s * cols, dx + j * 2, dw + j * 2, idesc, j ? 1u : 0u);
-            commit<PAIR>(&bars.acc_full[b.s]);
-            commit<PAIR>(&bars.acc_full[b.s + 1]);
-            commit<PAIR>(&bars.empty[r.s]);
+          for (int j = 0; j < 4; j++) {          // 32 k (32 bytes) each
+            mma_fp8<PAIR>(d, (wide ? dx : dw) + j * 2, (wide ? dw : dx) + j * 2, idesc, j ? 1u : 0u);
+            if (SWIGLU && !wide)
+              mma_fp8<PAIR>(d + up_offset, dw + (kABytes >> 4) + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
           }
-          __syncwarp();
-          b.next(bufs);
-          b.next(bufs);
-          if (b.s == 0) fresh = false;
+          commit<PAIR>(&bars.acc_full[b.s]);
+          commit<PAIR>(&bars.empty[r.s]);
         }
-        const int groups = wide ? 0 : together ? 1 : kMats;
-        for (int g = 0; g < groups; g++) {
-          if (!fresh && !mbar_wait(&bars.acc_empty[b.s], b.ph ^ 1, abort)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t d = tmem + b.s * cols;
-          const uint64_t da = dw + g * (kABytes >> 4);
-          if (elect_sync()) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              mma_fp8<PAIR>(d, da + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
-            if (together) {
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                mma_fp8<PAIR>(d + cols1, da + (kABytes >> 4) + j * 2, dx + j * 2, idesc, j ? 1u : 0u);
-            }
-            commit<PAIR>(&bars.acc_full[b.s]);
-            if (g == groups - 1) commit<PAIR>(&bars.empty[r.s]);
-          }
-          __syncwarp();
-          b.next(bufs);
-          if (b.s == 0) fresh = false;
-        }
-        if (!ok) break;
+        __syncwarp();
+        b.next(bufs);
+        if (b.s == 0) fresh = false;
         r.next(S);
         uses = min(uses + 1, S);
       }
@@ -640,17 +607,13 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     const uint32_t base = tmem + ((uint32_t)(me.quad * 32) << 16);
     const uint32_t empty0 = cluster_addr(&bars.acc_empty[0], PAIR ? 0 : kp);
     bool ok = true;
-    // A group's turn: waits for its accumulators, the first of a block also for its
-    // products of scales.
-    auto full = [&](bool first) {
-      if (first)
-        ok = wait_both(&bars.acc_full[b.s], b.ph, &bars.scale_full[sc.s], sc.ph, abort);
-      else
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.acc_full[b.s], b.ph, abort));
+    // The next block's accumulators and products of scales are there, and have been
+    // read.
+    auto full = [&]() {
+      ok = wait_both(&bars.acc_full[b.s], b.ph, &bars.scale_full[sc.s], sc.ph, abort);
       tc_fence_after();
       return ok;
     };
-    // The accumulators have been read.
     auto release = [&]() {
       tc_fence_before();
       __syncwarp();
@@ -671,12 +634,8 @@ fp8_product_kernel(const __grid_constant__ Params p) {
 #pragma unroll
       for (int i = 0; i < 64; i++) a.v[i] = make_float2(0.f, 0.f);
       if (wide) {
-        if (b.s & 1) {                   // (see the MMA warp)
-          if (!full(false)) break;
-          release();
-        }
         for (int kk = k0; kk < k1; kk++) {
-          if (!full(true)) break;
+          if (!full()) break;
           uint32_t u[2][32];
           const uint32_t d = base + b.s * cols + me.half * 64;
           tmem_ld32(d, u[0]);
@@ -690,56 +649,48 @@ fp8_product_kernel(const __grid_constant__ Params p) {
           waited(u[1]);
           add32(a.v + 16, u[1], y0);
           tmem_ld32(d + 160, u[1]);
-          release_scales();
           tmem_wait_ld();
           waited(u[0]);
           waited(u[1]);
           release();
-          release();
+          release_scales();
           add32(a.v + 32, u[0], y1);
           add32(a.v + 48, u[1], y1);
         }
       } else {
-        const int left = t.cnt - me.half * 32;
-        const int chunks = left > 64 ? 2 : left > 0 ? 1 : 0;
+        const uint32_t c = me.half * 32;
+        const int chunks = t.cnt > (int)c + 64 ? 2 : t.cnt > (int)c ? 1 : 0;
         for (int kk = k0; kk < k1; kk++) {
-          const uint32_t c = me.half * 32;
-          const float* s = products[sc.s] + c;
+          if (!full()) break;
           uint32_t u[2][32];
-          if (together) {
-            if (!full(true)) break;
-            const uint32_t d = base + b.s * cols + c;
-            if (chunks > 0) {
-              tmem_ld32(d, u[0]);
-              tmem_ld32(d + cols1, u[1]);
-            }
-            tmem_wait_ld();
-            release();
-            if (chunks > 0) {
-              waited(u[0]);
-              waited(u[1]);
-              add32(a.v, u[0], s);
-              add32(a.v + 32, u[1], s + 128);
-            }
-          } else {
-#pragma unroll
-            for (int g = 0; g < kMats; g++) {
-              if (!full(g == 0)) break;
-              const uint32_t d = base + b.s * cols + c;
-              if (chunks > 0) tmem_ld32(d, u[0]);
-              if (chunks > 1) tmem_ld32(d + 64, u[1]);
+          const uint32_t d = base + b.s * cols + c, du = d + up_offset;
+          const float* s = products[sc.s] + c;
+          if (chunks > 0) tmem_ld32(d, u[0]);
+          if (SWIGLU && chunks == 1) tmem_ld32(du, u[1]);
+          if (chunks == 2) tmem_ld32(d + 64, u[1]);
+          tmem_wait_ld();
+          if (!SWIGLU || chunks < 2) release();
+          if (chunks > 0) {
+            waited(u[0]);
+            add32(a.v, u[0], s);
+          }
+          if (SWIGLU && chunks == 1) {
+            waited(u[1]);
+            add32(a.v + 32, u[1], s + 128);
+          }
+          if (chunks == 2) {
+            if (SWIGLU) tmem_ld32(du, u[0]);
+            waited(u[1]);
+            add32(a.v + 16, u[1], s + 64);
+            if (SWIGLU) {
+              tmem_ld32(du + 64, u[1]);
               tmem_wait_ld();
               release();
-              if (chunks > 0) {
-                waited(u[0]);
-                add32(a.v + g * 32, u[0], s + g * 128);
-              }
-              if (chunks > 1) {
-                waited(u[1]);
-                add32(a.v + g * 32 + 16, u[1], s + g * 128 + 64);
-              }
+              waited(u[0]);
+              waited(u[1]);
+              add32(a.v + 32, u[0], s + 128);
+              add32(a.v + 48, u[1], s + 192);
             }
-            if (!ok) break;
           }
           release_scales();
         }
