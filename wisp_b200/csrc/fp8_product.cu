@@ -52,10 +52,10 @@ constexpr int kNarrow = 128;      // rows of a narrow tile at most
 constexpr int kWide = 256;
 constexpr int kMaxStages = 12;
 constexpr int kMaxBufs = 8;
-constexpr int kRingBytes = 208 * 1024;
-// Blocks whose products of scales are ready, and whose scales are held or on their
-// way; scales of a block: of the CTA's rows, then the weights' two.
-constexpr int kScaleSlots = 4, kRawSlots = 8, kRawFloats = 132;
+constexpr int kRingBytes = 206 * 1024;
+// Blocks whose scales are held or on their way; scales of a block: of the CTA's rows,
+// then the weights' two.
+constexpr int kRawSlots = 8, kRawFloats = 132;
 constexpr int kTileRing = 8;
 // Registers: launch 168 x 384 = 64,512; 256 x 232 + 128 x 40 = 64,512.
 constexpr int kEpiRegs = 232, kOtherRegs = 40;
@@ -64,8 +64,7 @@ struct Bars {
   uint64_t empty[kMaxStages];
   uint64_t acc_full[kMaxBufs];
   uint64_t acc_empty[kMaxBufs];
-  uint64_t scale_full[kScaleSlots];
-  uint64_t scale_empty[kScaleSlots];
+  uint64_t scale_empty[kMaxBufs];
   uint64_t red_full, red_empty;     // partial sums of a cluster's CTAs
   uint64_t tile_full[kTileRing];
   uint64_t tile_empty[kTileRing];
@@ -167,15 +166,6 @@ struct Warp {
   int lane, quad, half, rank;
 };
 
-// Waits for two barriers at once; all lanes get the same answer, false: given up.
-WB_DEV bool wait_both(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, volatile int* abort) {
-  const bool ra = mbar_try_wait(a, pa), rb = mbar_try_wait(b, pb);
-  bool ok = ra && rb;
-  if (__all_sync(0xffffffffu, ok)) return true;
-  ok = mbar_wait(a, pa, abort) && mbar_wait(b, pb, abort);
-  return __all_sync(0xffffffffu, ok);
-}
-
 // sums += accumulators * a scale each, of 32 columns.
 WB_DEV void add32(float2* v, const uint32_t (&u)[32], float y) {
 #pragma unroll
@@ -197,12 +187,13 @@ WB_DEV void add32(float2* v, const uint32_t (&u)[32], const float* s) {
 // The scale warp: of a tile's scales, block by block, the products of each row's
 // with the weights' two (gate and up, or a wide tile's blocks of features). The
 // scales come by cp.async (4 bytes, so that rows' scales may lie anywhere)
-// kRawSlots - 1 blocks ahead. Rows past the tile's have none: what their lanes and
+// kRawSlots - 1 blocks ahead; the products go where the block's buffer of
+// accumulators has its place. Rows past the tile's have none: what their lanes and
 // columns hold is not stored.
 template <bool SWIGLU>
 WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank, int k0, int k1,
                             Bars& bars, float (*raw)[kRawFloats], float (*products)[256], Ring& r,
-                            bool& first, volatile int* abort) {
+                            bool& first, int bufs, volatile int* abort) {
   const int lane = threadIdx.x & 31;
   const int row = (wide ? rank * 128 : 0) + lane, left = t.cnt - row;
   const float* x = p.xs + (t.row0 + (int64_t)row) * p.xs_row + k0 * p.xs_block;
@@ -244,8 +235,9 @@ WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank,
       if (two) o[128 + 32 * i] = v * w1;
     }
     __syncwarp();
-    arrive_one(&bars.scale_full[r.s]);
-    r.next(kScaleSlots);
+    // (its last reads being over, so is the barrier's last phase)
+    arrive_one(&bars.acc_full[r.s]);
+    r.next(bufs);
     if (r.s == 0) first = false;
   }
   return true;
@@ -405,7 +397,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
   __shared__ alignas(16) float raw[kRawSlots][kRawFloats];
-  __shared__ alignas(16) float products[kScaleSlots][256];      // of scales
+  __shared__ alignas(16) float products[kMaxBufs][256];      // of scales
   __shared__ int pref[kMaxSegs];
   __shared__ uint16_t order[kMaxSegs];
   __shared__ int4 warp_tot[kThreads / 32];
@@ -434,12 +426,9 @@ fp8_product_kernel(const __grid_constant__ Params p) {
       mbar_init(&bars.tile_full[tid], 1);
       mbar_init(&bars.tile_empty[tid], 11);     // all warps that walk the tiles
     }
-    if (tid < kScaleSlots) {
-      mbar_init(&bars.scale_full[tid], 1);
-      mbar_init(&bars.scale_empty[tid], 8);
-    }
     if (tid < kMaxBufs) {
-      mbar_init(&bars.acc_full[tid], 1);
+      mbar_init(&bars.acc_full[tid], 2);        // the MMAs, the products of scales
+      mbar_init(&bars.scale_empty[tid], 8);
       mbar_init(&bars.acc_empty[tid], PAIR ? 16 : 8);
     } else if (tid == kMaxBufs) {
       mbar_init(&bars.red_full, 8 * ks);
@@ -603,14 +592,14 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     red.bars = &bars;
     red.ks = ks;
     red.kp = kp;
-    Ring b, sc;                  // accumulators, scales
+    Ring b;
     const uint32_t base = tmem + ((uint32_t)(me.quad * 32) << 16);
     const uint32_t empty0 = cluster_addr(&bars.acc_empty[0], PAIR ? 0 : kp);
     bool ok = true;
     // The next block's accumulators and products of scales are there, and have been
     // read.
     auto full = [&]() {
-      ok = wait_both(&bars.acc_full[b.s], b.ph, &bars.scale_full[sc.s], sc.ph, abort);
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars.acc_full[b.s], b.ph, abort));
       tc_fence_after();
       return ok;
     };
@@ -621,12 +610,11 @@ fp8_product_kernel(const __grid_constant__ Params p) {
         arrive_one_remote(empty0 + b.s * 8);
       else
         arrive_one(&bars.acc_empty[b.s]);
-      b.next(bufs);
     };
     auto release_scales = [&]() {
       __syncwarp();
-      arrive_one(&bars.scale_empty[sc.s]);
-      sc.next(kScaleSlots);
+      arrive_one(&bars.scale_empty[b.s]);
+      b.next(bufs);
     };
     while (ok && tiles.next(bars, t, abort)) {
       const bool wide = PAIR && t.cnt > kNarrow;
@@ -640,7 +628,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
           const uint32_t d = base + b.s * cols + me.half * 64;
           tmem_ld32(d, u[0]);
           tmem_ld32(d + 32, u[1]);
-          const float* s = products[sc.s] + me.quad * 32 + lane;
+          const float* s = products[b.s] + me.quad * 32 + lane;
           const float y0 = s[0], y1 = s[128];
           tmem_wait_ld();
           waited(u[0]);
@@ -664,7 +652,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
           if (!full()) break;
           uint32_t u[2][32];
           const uint32_t d = base + b.s * cols + c, du = d + up_offset;
-          const float* s = products[sc.s] + c;
+          const float* s = products[b.s] + c;
           if (chunks > 0) tmem_ld32(d, u[0]);
           if (SWIGLU && chunks == 1) tmem_ld32(du, u[1]);
           if (chunks == 2) tmem_ld32(d + 64, u[1]);
@@ -747,7 +735,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     bool first = true;
     while (tiles.next(bars, t, abort))
       if (!multiply_scales<SWIGLU>(p, t, PAIR && t.cnt > kNarrow, rank, k0, k1, bars, raw, products,
-                                   r, first, abort))
+                                   r, first, bufs, abort))
         break;
     cp_async_wait_all();
     cluster_wait();
