@@ -7,9 +7,11 @@
 // scale was divided out: x times the fp32 reciprocal of the scale, made 2^-21
 // smaller or larger, is within 2^-22 relative of where exact arithmetic has it (a
 // reciprocal's ulp and two roundings), so the codes of the two enclose the right
-// one. Where they differ (one value in about 65,000) |x| is compared with border *
-// scale in 64 bits, where the product of 5 and 24 significant bits is exact. (With
-// a power of two as the scale the first product is exact.)
+// one. Where they differ, |x| is compared with border * scale by the sign of one
+// fused multiply-add: a border has 5 significant bits, so the difference is rounded
+// once and its sign is right. (For 16-bit rows that is no rare event: the quotient of
+// two 8-bit significands by 7 * 64 lies on a border for one value in a few hundred.)
+// With a power of two as the scale the first product is exact.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -27,6 +29,8 @@ constexpr int kBlock = 128;
 constexpr int kLanes = kBlock / kUnit;
 constexpr int kMaxCols = 1 << 27;    // what a launch's grid holds, with room
 constexpr float kTop = 448.f;
+// Below this, products and remainders of fp32 may lose bits to its range.
+constexpr float kTiny = 1e-30f, kRaise = 1.2676506002282294e30f;     // 2^100
 constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
 
 // A row of `units` threads split over equal CTAs of at most 256.
@@ -87,15 +91,26 @@ WB_DEV float2 pair_of(const Raw<T>& r, int j) {
 template <bool POW2>
 WB_DEV float scale_of(uint32_t top) {
   if (top >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
-  if (!POW2) return __fdiv_rn(__uint_as_float(top), kTop);
+  if (!POW2) {
+    // a / 448 rounded to nearest: the quotient by the rounded reciprocal, corrected
+    // once by its exact remainder (Markstein 1990: the correction by a correctly
+    // rounded reciprocal gives the correctly rounded quotient). Where the remainder
+    // would drop below fp32's last bit, the same in fp64. (A division is a call, which
+    // keeps registers of what comes after it.)
+    const float a = __uint_as_float(top);
+    if (a < kTiny) {
+      constexpr double r = 1.0 / kTop;
+      const double q = a * r;
+      return (float)fma(fma(-q, (double)kTop, (double)a), r, q);
+    }
+    constexpr float r = 1.f / kTop;
+    const float q = a * r;
+    return fmaf(fmaf(-q, kTop, a), r, q);
+  }
   // top = m 2^e, 448 = 1.75 2^8: 2^(e - 8), one more where m > 1.75
   if (top == 0) return 0.f;
   const int e = (int)((top + 0x1fffffu) >> 23) - 8;
   return __uint_as_float((uint32_t)max(e, 1) << 23);
-}
-
-WB_DEV float e4m3_value(uint32_t b) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
 }
 
 // Codes of four values, the first in the low byte. Round to nearest even,
@@ -112,60 +127,73 @@ WB_DEV uint32_t e4m3x4(float2 a, float2 b, float r) {
   return o;
 }
 
-// Of two neighbouring codes' magnitudes lo < hi, the one nearer to |x| / s.
-WB_DEV uint32_t nearer(float ax, float s, uint32_t lo, uint32_t hi) {
-  const double border = 0.5 * ((double)e4m3_value(lo) + (double)e4m3_value(hi)) * (double)s;
-  const double a = (double)ax;
-  return a > border || (a == border && !(hi & 1)) ? hi : lo;
-}
-
-// Decides the values among four whose two candidate codes differ.
-__device__ __noinline__ uint32_t settle(float2 a, float2 b, float s, uint32_t lo, uint32_t hi) {
-  const float v[4] = {a.x, a.y, b.x, b.y};
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const uint32_t l = lo >> (8 * j) & 127u, h = hi >> (8 * j) & 127u;
-    if (l != h) {
-      const uint32_t c = nearer(fabsf(v[j]), s, l, h);
-      lo = (lo & ~(127u << (8 * j))) | c << (8 * j);
-    }
-  }
-  return lo;
-}
-
-// Code of x for a scale whose reciprocal is no normal number.
-__device__ __noinline__ uint32_t code_exact(float x, float s) {
-  const double q = fabs((double)x) / (double)s;      // a guess, put right below
-  uint32_t c = __nv_cvt_double_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-  if (c > 0) c = nearer(fabsf(x), s, c - 1, c);
-  if (c < 126) c = nearer(fabsf(x), s, c, c + 1);
-  return c | (__float_as_uint(x) >> 24 & 128u);
-}
-
+// The codes of a thread's 16 values, which lie at x.
 template <bool POW2, typename T>
-WB_DEV void codes_of(const Raw<T>& raw, float s, uint32_t (&c)[4]) {
+WB_DEV void codes_of(Raw<T> raw, const T* x, float s, uint32_t (&c)[4]) {
   c[0] = c[1] = c[2] = c[3] = 0u;
   if (!(s > 0.f)) return;           // a zero block, or NaN
-  if (s < 1.17549435e-38f) {        // subnormal: has no reciprocal
+  float raise = 1.f;
+  if (!POW2 && !std::is_same<T, __half>::value && s < kTiny) {
+    // the same quotients from values and scale times 2^100, which is exact (fp16 has
+    // no values as small)
+    raise = kRaise;
+    s *= kRaise;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 a = pair_of(raw, 2 * i), b = pair_of(raw, 2 * i + 1);
-      c[i] = code_exact(a.x, s) | code_exact(a.y, s) << 8 | code_exact(b.x, s) << 16 |
-             code_exact(b.y, s) << 24;
+    for (int j = 0; j < (int)(4 * sizeof(T)); j++) {
+      if constexpr (sizeof(T) == 4) {
+        raw.u[j] = __float_as_uint(__uint_as_float(raw.u[j]) * kRaise);
+      } else {
+        const float2 v = pair_of(raw, j);
+        raw.u[j] = pack2(v.x * kRaise, v.y * kRaise, WISP_DT_BF16);
+      }
     }
-    return;
   }
   const float r = POW2 ? __uint_as_float(0x7f000000u - __float_as_uint(s)) : rcp_approx(s);
+  uint32_t hi[4], differ = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const float2 a = pair_of(raw, 2 * i), b = pair_of(raw, 2 * i + 1);
-    if (POW2) {
-      c[i] = e4m3x4(a, b, r);
-    } else {
-      c[i] = e4m3x4(a, b, r * kBelow);
-      const uint32_t hi = e4m3x4(a, b, r * kAbove);
-      if (c[i] != hi) c[i] = settle(a, b, s, c[i], hi);
+    c[i] = e4m3x4(a, b, POW2 ? r : r * kBelow);
+    if (!POW2) {
+      hi[i] = e4m3x4(a, b, r * kAbove);
+      differ |= c[i] ^ hi[i];
     }
+  }
+  if (!POW2 && differ) {
+    // One value of each lane after the other.
+    uint32_t left = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)      // a bit per byte that differs
+      left |= ((__vcmpne4(c[i], hi[i]) & 0x08040201u) * 0x01010101u >> 24) << 4 * i;
+#pragma unroll 1
+    do {
+      const int j = __ffs(left) - 1, i = j >> 2, at = 8 * (j & 3);
+      left &= left - 1;
+      const uint32_t cl = i < 2 ? (i < 1 ? c[0] : c[1]) : (i < 3 ? c[2] : c[3]);
+      const uint32_t ch = i < 2 ? (i < 1 ? hi[0] : hi[1]) : (i < 3 ? hi[2] : hi[3]);
+      float ax;
+      if constexpr (sizeof(T) == 4) {
+        ax = fabsf(x[j]) * raise;       // (rare: read again)
+      } else {
+        const int w = j >> 1;
+        const uint32_t w0 = w & 1 ? raw.u[1] : raw.u[0], w1 = w & 1 ? raw.u[3] : raw.u[2];
+        const uint32_t w2 = w & 1 ? raw.u[5] : raw.u[4], w3 = w & 1 ? raw.u[7] : raw.u[6];
+        const uint32_t lo = w & 2 ? w1 : w0, up = w & 2 ? w3 : w2;
+        const float2 v = unpack2(w & 4 ? up : lo,
+                                 std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+        ax = fabsf(j & 1 ? v.y : v.x);
+      }
+      // the border: the quotient, which is next to it, to 5 significant bits
+      const float border = __uint_as_float((__float_as_uint(ax * r) + 0x40000u) & 0xfff80000u);
+      const float d = fmaf(border, s, -ax);
+      if (d < 0.f || (d == 0.f && !(ch >> at & 1u))) {
+        const uint32_t m = 255u << at, v = (cl & ~m) | (ch & m);
+        if (i == 0) c[0] = v;
+        if (i == 1) c[1] = v;
+        if (i == 2) c[2] = v;
+        if (i == 3) c[3] = v;
+      }
+    } while (left);
   }
 }
 
@@ -192,15 +220,16 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   const int units = p.cols / kUnit;
   const bool in = u < units;
   Raw<T> raw[R];
+  const T* x[R];
 #pragma unroll
   for (int i = 0; i < R; i++) {
     const int64_t row = row0 + i;
     int64_t sr = -1;
     if (row < p.rows) sr = p.src ? (int64_t)__ldg(p.src + row) : row;
+    x[i] = static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit;
 #pragma unroll
     for (int j = 0; j < 4 * (int)sizeof(T); j++) raw[i].u[j] = 0;
-    if (in && sr >= 0 && sr < p.x_rows)
-      load_raw(static_cast<const T*>(p.x) + sr * p.ld + (int64_t)u * kUnit, p.wide, raw[i]);
+    if (in && sr >= 0 && sr < p.x_rows) load_raw(x[i], p.wide, raw[i]);
   }
   float mine = 0.f;
 #pragma unroll
@@ -212,7 +241,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     const float s = scale_of<POW2>(top);
     if ((u & (kLanes - 1)) == i) mine = s;
     uint32_t c[4];
-    codes_of<POW2>(raw[i], s, c);
+    codes_of<POW2>(raw[i], x[i], s, c);
     if (in && row < p.rows)
       *reinterpret_cast<uint4*>(p.codes + row * p.cols + (int64_t)u * kUnit) =
           make_uint4(c[0], c[1], c[2], c[3]);
@@ -260,6 +289,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const BlockParams 
   __shared__ uint32_t tops[8];
   const int tid = threadIdx.x, c0 = blockIdx.x * kBlock + (tid & 7) * kUnit;
   const int64_t first = (int64_t)blockIdx.z * p.n;
+  const T* x = static_cast<const T*>(p.x) + first * p.k + c0;
   Raw<T> raw[4];
   uint32_t top = 0;
 #pragma unroll
@@ -267,8 +297,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const BlockParams 
     const int r = blockIdx.y * kBlock + (tid >> 3) + 32 * i;
 #pragma unroll
     for (int j = 0; j < 4 * (int)sizeof(T); j++) raw[i].u[j] = 0;
-    if (r < p.n && c0 < p.k)
-      load_raw(static_cast<const T*>(p.x) + (first + r) * p.k + c0, p.wide, raw[i]);
+    if (r < p.n && c0 < p.k) load_raw(x + (int64_t)r * p.k, p.wide, raw[i]);
     top = max(top, top_of(raw[i]));
   }
   top = __reduce_max_sync(0xffffffffu, top);
@@ -282,7 +311,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const BlockParams 
     const int r = blockIdx.y * kBlock + (tid >> 3) + 32 * i;
     if (r < p.n && c0 < p.k) {
       uint32_t c[4];
-      codes_of<false>(raw[i], s, c);
+      codes_of<false>(raw[i], x + (int64_t)r * p.k, s, c);
       *reinterpret_cast<uint4*>(p.codes + (first + r) * p.k + c0) =
           make_uint4(c[0], c[1], c[2], c[3]);
     }

@@ -461,7 +461,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   // the scheduler warp reads pref and order
   __syncthreads();
   const uint32_t tmem = bars.tmem;
-  const int k0 = p.nk * kp / ks, k1 = p.nk * (kp + 1) / ks;     // this CTA's stages
+  const int k0 = PAIR ? 0 : p.nk * kp / ks, k1 = PAIR ? p.nk : p.nk * (kp + 1) / ks;     // this CTA's stages
   // A stage: weights (in narrow tiles gate and up), then rows: of a narrow tile n
   // (a pair's CTA half of them), of a wide one 128. Few rows leave room for more
   // stages, which is what hides the memory's latency when the weights are most of
