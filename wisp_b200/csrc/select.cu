@@ -23,46 +23,80 @@ struct Params {
   const float* bias;
   int T, E, k;
   int scoring, groups, kept, group_top, renorm;
+  int gsz, lanes;                  // experts of a group, lanes that look at them
+  uint32_t by_gsz;                 // 2^32 / gsz rounded up
   float scaling;
   int* idx;
   float* w;
 };
 
-// A double as an unsigned integer in the same order; 0 for what cannot be chosen
-// (NaN and -infinity).
+// A double, a float as an unsigned integer in the same order; 0 for what cannot be
+// chosen (NaN and -infinity).
 WB_DEV uint64_t order_key(double v) {
   if (!(v > -INFINITY)) return 0;
   if (v == 0.0) v = 0.0;           // -0 and +0 are equal
   const int64_t b = __double_as_longlong(v);
   return (uint64_t)(b ^ ((b >> 63) | INT64_MIN));
 }
+WB_DEV uint32_t order_key(float v) {
+  const int32_t b = __float_as_int(v + 0.f);
+  return (uint32_t)(b ^ ((b >> 31) | INT32_MIN));
+}
+WB_DEV float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+WB_DEV float to_float(float v) { return v; }
+WB_DEV float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+WB_DEV float to_float(__half v) { return __half2float(v); }
 
 WB_DEV double shfl_xor(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+WB_DEV float shfl_xor(float v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
 
-// One warp per token; lane l holds experts l + 32 j, j < PER. Scores and choice
-// are 64-bit: two experts whose choices lie closer than fp32 resolves still come
-// out in their order, and only equal choices are ties, which go to the lower
-// expert.
+WB_DEV int group_of(const Params& p, int e) { return p.gsz == 1 ? e : (int)__umulhi(e, p.by_gsz); }
+
+// The best two of a lane's group (-infinity where there are fewer), from the choices
+// in shared memory: lanes g L .. g L + L - 1 look at group g's.
+template <typename R>
+WB_DEV void best_two(const Params& p, const R* choices, int lane, R& a, R& b) {
+  a = b = -INFINITY;
+  const int gsz = p.gsz, L = p.lanes, g = lane / L;
+  if (g < p.groups) {
+    for (int i = lane % L; i < gsz; i += L) {
+      const R c = choices[g * gsz + i];
+      if (c > a) {
+        b = a;
+        a = c;
+      } else if (c > b) {
+        b = c;
+      }
+    }
+  }
+  for (int o = 1; o < L; o <<= 1) {
+    const R oa = shfl_xor(a, o), ob = shfl_xor(b, o);
+    b = fmax(fmin(a, oa), fmax(b, ob));
+    a = fmax(a, oa);
+  }
+}
+
+// The weights of a token's choices: lane r < k holds expert `mine` (-1: none), its
+// score and its place in the row.
+WB_DEV void put_weights(const Params& p, int64_t t, int lane, int mine, double score, double total) {
+  if (lane < p.k) {
+    if (p.renorm) score = total > 0.0 ? score / total : 0.0;
+    p.idx[t * p.k + lane] = mine;
+    p.w[t * p.k + lane] = (float)(score * (double)p.scaling);
+  }
+}
+
+// The routing of one token in 64 bits. logits: of experts lane + 32 j.
 template <int PER>
-__global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
-  extern __shared__ double choices[];       // [kWarps][E], with groups
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
-  if (t >= p.T) return;
+__device__ __noinline__ void select_exact(const Params& p, int64_t t, const float* logits, int lane,
+                                          double* choices) {
   const int E = p.E;
   double score[PER];
 #pragma unroll
-  for (int j = 0; j < PER; j++) {
-    const int e = lane + 32 * j;
-    score[j] = -INFINITY;
-    if (e < E) {
-      float v = load_one(p.logits, p.type, t * p.ld + e);
-      for (int z = 1; z < p.splits; z++)
-        v += static_cast<const float*>(p.logits)[z * p.split + t * p.ld + e];
-      if (p.logit_bias) v += p.logit_bias[e];
-      score[j] = (double)v;
-    }
-  }
+  for (int j = 0; j < PER; j++) score[j] = lane + 32 * j < E ? (double)logits[32 * j] : -INFINITY;
   if (p.scoring == WISP_ROUTE_SOFTMAX) {
     // (a NaN logit makes every score NaN, as does +infinity)
     double mx = -INFINITY, sum = 0.0;
@@ -84,6 +118,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     for (int j = 0; j < PER; j++) score[j] = 1.0 / (1.0 + exp(-score[j]));
   }
   uint64_t key[PER];
+  __syncwarp();                      // the choices in 32 bits have been read
 #pragma unroll
   for (int j = 0; j < PER; j++) {
     const int e = lane + 32 * j;
@@ -91,33 +126,14 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     if (e < E) {
       const double c = p.bias ? score[j] + (double)p.bias[e] : score[j];
       key[j] = order_key(c);
-      if (p.kept < p.groups) choices[warp * E + e] = c;
+      if (p.kept < p.groups) choices[e] = c;
     }
   }
   if (p.kept < p.groups) {
-    // lanes g L .. g L + L - 1 read group g's choices, and find its best two
     __syncwarp();
-    const int gsz = E / p.groups;
-    int L = 1;
-    while (2 * L * p.groups <= 32) L *= 2;
-    const int g = lane / L;
-    double a = -INFINITY, b = -INFINITY;
-    if (g < p.groups) {
-      for (int i = lane % L; i < gsz; i += L) {
-        const double c = choices[warp * E + g * gsz + i];
-        if (c > a) {
-          b = a;
-          a = c;
-        } else if (c > b) {
-          b = c;
-        }
-      }
-    }
-    for (int o = 1; o < L; o <<= 1) {
-      const double oa = shfl_xor(a, o), ob = shfl_xor(b, o);
-      b = fmax(fmin(a, oa), fmax(b, ob));
-      a = fmax(a, oa);
-    }
+    const int L = p.lanes, g = lane / L;
+    double a, b;
+    best_two(p, choices, lane, a, b);
     // choices that cannot be made (-infinity, NaN) count nothing; a group of
     // those alone is never kept
     const double s = p.group_top > 1 && b > -INFINITY ? a + b : a;
@@ -131,7 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       const int e = lane + 32 * j;
-      if (e < E && !(keep >> (e / gsz * L) & 1u)) key[j] = 0;
+      if (e < E && !(keep >> (group_of(p, e) * L) & 1u)) key[j] = 0;
     }
   }
   // k rounds of the largest key, the lowest expert among equal ones
@@ -168,14 +184,190 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     }
     total += s;
   }
-  if (lane < p.k) {
-    if (p.renorm) weight = total > 0.0 ? weight / total : 0.0;
-    p.idx[t * p.k + lane] = mine;
-    p.w[t * p.k + lane] = (float)(weight * (double)p.scaling);
-  }
+  put_weights(p, t, lane, mine, weight, total);
 }
 
-WispError launch(const Params& p, cudaStream_t st, WispErrCtx* err) {
+// The largest of a warp's keys and the lowest expert that has it.
+template <int PER>
+WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
+  uint32_t best = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) best = max(best, key[j]);
+  best = __reduce_max_sync(0xffffffffu, best);
+  uint32_t e = 0xffffffffu;
+#pragma unroll
+  for (int j = PER - 1; j >= 0; j--)
+    if (key[j] == best) e = lane + 32 * j;
+  e = __reduce_min_sync(0xffffffffu, e);
+#pragma unroll
+  for (int j = 0; j < PER; j++)
+    if (e == (uint32_t)(lane + 32 * j)) key[j] = 0;
+  expert = e;
+  return best;
+}
+
+// One warp per token; lane l holds experts l + 32 j, j < PER.
+//
+// The result is that of 64-bit scores and choices (select_exact), found in 32 bits
+// where that decides it. The quick exponential of x is off by 2 + 1.2 |x| ulp, which
+// makes at most 1.5 * 2^-23 of a sigmoid s (s (1 - s) |x| < 0.23) and, with a sum and
+// the quick reciprocal, 7 * 2^-24; a choice rounds by 2^-24 of itself more, so two
+// that differ by 2^-20 * max(1, |choice|) are in order. A softmax score is off by
+// 9 * 2^-24 (e^-x x < 0.37) and, with all of the token's, by the sum's error of at
+// most 43 * 2^-24: there it takes 2^-18. Without a bias the scores are in the
+// logits' order, which needs no scores at all: equal logits are ties, and those 2^-20
+// apart have different 64-bit scores as long as these are not near 1 (logits above
+// 16) or 0 (logits, from the largest on for softmax, below -700). Only a token with a
+// closer pair where it matters, or with a value that is not finite, goes the 64-bit
+// way, as does a softmax whose weights are not renormalised, which needs the 64-bit
+// sum over all experts. 256 experts with bias and groups, one token: 7.9 -> 4.6 us a
+// launch, 4096: 14.3 -> 11.7, 16,384: 47 -> 34; bound by its instructions, 1700 a token.
+template <int PER>
+__global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
+  extern __shared__ double choices64[];       // [kWarps][E], with groups
+  __shared__ float logits[kWarps][32 * PER];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+  if (t >= p.T) return;
+  const int E = p.E;
+  const bool softmax = p.scoring == WISP_ROUTE_SOFTMAX, grouped = p.kept < p.groups;
+  float v[PER], mx = -INFINITY, span = 0.f;
+  // (one branch on the type for all loads, none on the experts that there are: what
+  // is read past them is the last one's)
+  auto load = [&](auto* q) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] = to_float(q[min(lane + 32 * j, E - 1)]);
+  };
+  if (p.type == WISP_DT_F32)
+    load(static_cast<const float*>(p.logits) + t * p.ld);
+  else if (p.type == WISP_DT_BF16)
+    load(static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld);
+  else
+    load(static_cast<const __half*>(p.logits) + t * p.ld);
+  for (int z = 1; z < p.splits; z++) {
+    const float* q = static_cast<const float*>(p.logits) + z * p.split + t * p.ld;
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] += q[min(lane + 32 * j, E - 1)];
+  }
+  if (p.logit_bias) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] += p.logit_bias[min(lane + 32 * j, E - 1)];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    span += v[j] - v[j];                // NaN where a value is not finite
+    v[j] = lane + 32 * j < E ? v[j] : -INFINITY;
+    mx = fmaxf(mx, v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < PER; j++) logits[warp][lane + 32 * j] = v[j];
+  const float* mine_v = logits[warp] + lane;
+  double* choices = choices64 + (grouped ? warp * E : 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, shfl_xor(mx, o));
+  // what the experts are ordered by, as keys
+  const bool scores = p.bias || (grouped && p.group_top > 1);
+  uint32_t key[PER];
+  if (scores) {
+    float s[PER], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      s[j] = __expf(softmax ? v[j] - mx : -v[j]);      // (softmax: 0 past the experts)
+      sum += s[j];
+    }
+    if (softmax) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += shfl_xor(sum, o);
+      sum = rcp_approx(sum);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; j++) s[j] = softmax ? s[j] * sum : rcp_approx(1.f + s[j]);
+    if (p.bias) {
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        s[j] += p.bias[min(lane + 32 * j, E - 1)];
+        span += s[j] - s[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      key[j] = lane + 32 * j < E ? order_key(s[j]) : 0u;
+      if (grouped && lane + 32 * j < E) reinterpret_cast<float*>(choices)[lane + 32 * j] = s[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      key[j] = lane + 32 * j < E ? order_key(v[j]) : 0u;
+      if (grouped && lane + 32 * j < E) reinterpret_cast<float*>(choices)[lane + 32 * j] = v[j];
+    }
+  }
+  bool sure = __all_sync(0xffffffffu, span == 0.f) && (scores || softmax || mx <= 16.f) &&
+              (!softmax || p.renorm);
+  const float margin = scores && softmax ? 3.814697265625e-6f : 9.5367431640625e-7f;   // 2^-18, -20
+  const float least = scores ? -INFINITY : softmax ? mx - 700.f : -700.f;
+  // Whether a > b is beyond doubt, or both are the same for certain; `of`: how many
+  // scores they are sums of.
+  auto apart = [&](float a, float b, float of) {
+    const float d = a - b;
+    return a >= least && (d >= of * margin * fmaxf(1.f, fabsf(a)) || (d == 0.f && !scores));
+  };
+  if (grouped && sure) {
+    __syncwarp();
+    const int L = p.lanes, g = lane / L;
+    float a, b;
+    best_two(p, reinterpret_cast<const float*>(choices), lane, a, b);
+    const float s = p.group_top > 1 && p.gsz > 1 ? a + b : a;
+    int rank = 0;
+    for (int h = 0; h < p.groups; h++) {
+      const float o = __shfl_sync(0xffffffffu, s, h * L);
+      rank += o > s || (o == s && h < g);
+    }
+    const bool head = g < p.groups && lane % L == 0, kept = head && rank < p.kept;
+    const uint32_t keep = __ballot_sync(0xffffffffu, kept);
+    // the worst that is kept against the best that is not
+    const uint32_t sk = order_key(s);
+    const float worst = key_value(__reduce_min_sync(0xffffffffu, kept ? sk : 0xffffffffu));
+    const float next = key_value(__reduce_max_sync(0xffffffffu, head && !kept ? sk : 0u));
+    sure = apart(worst, next, (float)p.group_top);
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int e = lane + 32 * j;
+      if (e < E && !(keep >> (group_of(p, e) * L) & 1u)) key[j] = 0;
+    }
+  }
+  int mine = -1;
+  float last = INFINITY;
+  for (int r = 0; r <= p.k && sure; r++) {       // one round more, for the last one's distance
+    uint32_t e;
+    const uint32_t best = take_best(key, lane, e);
+    if (best == 0) break;          // (all of the kept groups' experts are taken)
+    const float c = key_value(best);
+    if (r > 0) sure = apart(last, c, 1.f);
+    last = c;
+    if (lane == r && r < p.k) mine = (int)e;
+  }
+  if (!sure) {
+    select_exact<PER>(p, t, mine_v, lane, choices);
+    return;
+  }
+  // the weights, of these experts alone: the sum over all of a softmax cancels
+  __syncwarp();
+  const double l = mine >= 0 ? (double)logits[warp][mine] : 0.0;
+  double score = 0.0, total = 0.0;
+  if (mine >= 0) score = softmax ? exp(l - (double)mx) : 1.0 / (1.0 + exp(-l));
+  if (p.renorm) {
+    total = score;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += shfl_xor(total, o);
+  }
+  put_weights(p, t, lane, mine, score, total);
+}
+
+WispError launch(Params& p, cudaStream_t st, WispErrCtx* err) {
+  p.gsz = p.E / p.groups;
+  p.by_gsz = (uint32_t)(((1ull << 32) + p.gsz - 1) / p.gsz);
+  p.lanes = 1;
+  while (2 * p.lanes * p.groups <= 32) p.lanes *= 2;
   auto kernel = p.E <= 32 ? select_kernel<1> : p.E <= 64 ? select_kernel<2>
               : p.E <= 128 ? select_kernel<4> : p.E <= 256 ? select_kernel<8>
               : p.E <= 512 ? select_kernel<16> : select_kernel<32>;
