@@ -89,14 +89,14 @@ WB_DEV void put_weights(const Params& p, int64_t t, int lane, int mine, double s
   }
 }
 
-// The routing of one token in 64 bits. logits: of experts lane + 32 j.
+// The routing of one token in 64 bits. v: the logits of experts lane + 32 j,
+// -infinity where there is none.
 template <int PER>
-__device__ __noinline__ void select_exact(const Params& p, int64_t t, const float* logits, int lane,
-                                          double* choices) {
+WB_DEV void route_exact(const Params& p, int64_t t, const float (&v)[PER], int lane, double* choices) {
   const int E = p.E;
   double score[PER];
 #pragma unroll
-  for (int j = 0; j < PER; j++) score[j] = lane + 32 * j < E ? (double)logits[32 * j] : -INFINITY;
+  for (int j = 0; j < PER; j++) score[j] = (double)v[j];
   if (p.scoring == WISP_ROUTE_SOFTMAX) {
     // (a NaN logit makes every score NaN, as does +infinity)
     double mx = -INFINITY, sum = 0.0;
@@ -187,6 +187,57 @@ __device__ __noinline__ void select_exact(const Params& p, int64_t t, const floa
   put_weights(p, t, lane, mine, weight, total);
 }
 
+// The same out of line, for logits in shared memory: a rare path whose registers the
+// usual one does without.
+template <int PER>
+__device__ __noinline__ void route_exact_from(const Params& p, int64_t t, const float* logits,
+                                              int lane, double* choices) {
+  float v[PER];
+#pragma unroll
+  for (int j = 0; j < PER; j++) v[j] = logits[32 * j];
+  route_exact<PER>(p, t, v, lane, choices);
+}
+
+// A token's logits; past the experts -infinity. (One branch on the type for all loads,
+// none on the experts that there are: what is read past them is the last one's.)
+template <int PER>
+WB_DEV void load_logits(const Params& p, int64_t t, int lane, float (&v)[PER]) {
+  auto load = [&](auto* q) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] = to_float(q[min(lane + 32 * j, p.E - 1)]);
+  };
+  if (p.type == WISP_DT_F32)
+    load(static_cast<const float*>(p.logits) + t * p.ld);
+  else if (p.type == WISP_DT_BF16)
+    load(static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld);
+  else
+    load(static_cast<const __half*>(p.logits) + t * p.ld);
+  for (int z = 1; z < p.splits; z++) {
+    const float* q = static_cast<const float*>(p.logits) + z * p.split + t * p.ld;
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] += q[min(lane + 32 * j, p.E - 1)];
+  }
+  if (p.logit_bias) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) v[j] += p.logit_bias[min(lane + 32 * j, p.E - 1)];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; j++)
+    if (lane + 32 * j >= p.E) v[j] = -INFINITY;
+}
+
+// One warp per token, all in 64 bits.
+template <int PER>
+__global__ void __launch_bounds__(kWarps * 32) select_exact_kernel(const Params p) {
+  extern __shared__ double choices64[];       // [kWarps][E], with groups
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+  if (t >= p.T) return;
+  float v[PER];
+  load_logits<PER>(p, t, lane, v);
+  route_exact<PER>(p, t, v, lane, choices64 + (p.kept < p.groups ? warp * p.E : 0));
+}
+
 // The largest of a warp's keys and the lowest expert that has it.
 template <int PER>
 WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
@@ -208,7 +259,7 @@ WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
 
 // One warp per token; lane l holds experts l + 32 j, j < PER.
 //
-// The result is that of 64-bit scores and choices (select_exact), found in 32 bits
+// The result is that of 64-bit scores and choices (route_exact), found in 32 bits
 // where that decides it. The quick exponential of x is off by 2 + 1.2 |x| ulp, which
 // makes at most 1.5 * 2^-23 of a sigmoid s (s (1 - s) |x| < 0.23) and, with a sum and
 // the quick reciprocal, 7 * 2^-24; a choice rounds by 2^-24 of itself more, so two
@@ -219,8 +270,8 @@ WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
 // apart have different 64-bit scores as long as these are not near 1 (logits above
 // 16) or 0 (logits, from the largest on for softmax, below -700). Only a token with a
 // closer pair where it matters, or with a value that is not finite, goes the 64-bit
-// way, as does a softmax whose weights are not renormalised, which needs the 64-bit
-// sum over all experts. 256 experts with bias and groups, one token: 7.9 -> 4.6 us a
+// way. (A softmax whose weights are not renormalised needs the 64-bit sum over all
+// experts, and goes that way at once: 12.6 us where this takes 15.6.) 256 experts with bias and groups, one token: 7.9 -> 4.6 us a
 // launch, 4096: 14.3 -> 11.7, 16,384: 47 -> 34; bound by its instructions, 1700 a token.
 template <int PER>
 __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
@@ -232,31 +283,10 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
   const int E = p.E;
   const bool softmax = p.scoring == WISP_ROUTE_SOFTMAX, grouped = p.kept < p.groups;
   float v[PER], mx = -INFINITY, span = 0.f;
-  // (one branch on the type for all loads, none on the experts that there are: what
-  // is read past them is the last one's)
-  auto load = [&](auto* q) {
-#pragma unroll
-    for (int j = 0; j < PER; j++) v[j] = to_float(q[min(lane + 32 * j, E - 1)]);
-  };
-  if (p.type == WISP_DT_F32)
-    load(static_cast<const float*>(p.logits) + t * p.ld);
-  else if (p.type == WISP_DT_BF16)
-    load(static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld);
-  else
-    load(static_cast<const __half*>(p.logits) + t * p.ld);
-  for (int z = 1; z < p.splits; z++) {
-    const float* q = static_cast<const float*>(p.logits) + z * p.split + t * p.ld;
-#pragma unroll
-    for (int j = 0; j < PER; j++) v[j] += q[min(lane + 32 * j, E - 1)];
-  }
-  if (p.logit_bias) {
-#pragma unroll
-    for (int j = 0; j < PER; j++) v[j] += p.logit_bias[min(lane + 32 * j, E - 1)];
-  }
+  load_logits<PER>(p, t, lane, v);
 #pragma unroll
   for (int j = 0; j < PER; j++) {
-    span += v[j] - v[j];                // NaN where a value is not finite
-    v[j] = lane + 32 * j < E ? v[j] : -INFINITY;
+    if (lane + 32 * j < E) span += v[j] - v[j];       // NaN where a value is not finite
     mx = fmaxf(mx, v[j]);
   }
 #pragma unroll
@@ -301,8 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
       if (grouped && lane + 32 * j < E) reinterpret_cast<float*>(choices)[lane + 32 * j] = v[j];
     }
   }
-  bool sure = __all_sync(0xffffffffu, span == 0.f) && (scores || softmax || mx <= 16.f) &&
-              (!softmax || p.renorm);
+  bool sure = __all_sync(0xffffffffu, span == 0.f) && (scores || softmax || mx <= 16.f);
   const float margin = scores && softmax ? 3.814697265625e-6f : 9.5367431640625e-7f;   // 2^-18, -20
   const float least = scores ? -INFINITY : softmax ? mx - 700.f : -700.f;
   // Whether a > b is beyond doubt, or both are the same for certain; `of`: how many
@@ -347,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     if (lane == r && r < p.k) mine = (int)e;
   }
   if (!sure) {
-    select_exact<PER>(p, t, mine_v, lane, choices);
+    route_exact_from<PER>(p, t, mine_v, lane, choices);
     return;
   }
   // the weights, of these experts alone: the sum over all of a softmax cancels
@@ -368,9 +397,14 @@ WispError launch(Params& p, cudaStream_t st, WispErrCtx* err) {
   p.by_gsz = (uint32_t)(((1ull << 32) + p.gsz - 1) / p.gsz);
   p.lanes = 1;
   while (2 * p.lanes * p.groups <= 32) p.lanes *= 2;
-  auto kernel = p.E <= 32 ? select_kernel<1> : p.E <= 64 ? select_kernel<2>
-              : p.E <= 128 ? select_kernel<4> : p.E <= 256 ? select_kernel<8>
-              : p.E <= 512 ? select_kernel<16> : select_kernel<32>;
+  const bool exact = p.scoring == WISP_ROUTE_SOFTMAX && !p.renorm;
+  auto of = [&](auto usual, auto all64) { return exact ? all64 : usual; };
+  auto kernel = p.E <= 32 ? of(select_kernel<1>, select_exact_kernel<1>)
+              : p.E <= 64 ? of(select_kernel<2>, select_exact_kernel<2>)
+              : p.E <= 128 ? of(select_kernel<4>, select_exact_kernel<4>)
+              : p.E <= 256 ? of(select_kernel<8>, select_exact_kernel<8>)
+              : p.E <= 512 ? of(select_kernel<16>, select_exact_kernel<16>)
+                           : of(select_kernel<32>, select_exact_kernel<32>);
   const size_t smem = p.kept < p.groups ? sizeof(double) * kWarps * p.E : 0;
   wb::launch_k(kernel, (unsigned)(((int64_t)p.T + kWarps - 1) / kWarps), kWarps * 32, smem, st, p);
   WB_CUDA_CHECK(cudaGetLastError());
