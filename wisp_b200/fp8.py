@@ -61,18 +61,19 @@ class Fp8Rows:
         self._views = (codes, scales)
         self._buf = codes
         self._codes, self._scales = codes.data_ptr(), scales.data_ptr()
-        self._strides = scales.stride()
+        self._row, self._block = scales.stride()
 
     @classmethod
     def _empty(cls, x: torch.Tensor, rows: int, cols: int) -> "Fp8Rows":
         """Rows to be written, in one allocation on x's device; the codes and scales tensors
         are made when someone asks for them."""
         q = cls.__new__(cls)
-        q._buf = buf = x.new_empty(rows * cols + 4 * rows * _blocks(cols), dtype=torch.uint8)
+        n = rows * cols             # (a multiple of 16)
+        q._buf = buf = x.new_empty(n + 4 * rows * ((cols + BLOCK - 1) // BLOCK), dtype=torch.uint8)
         q._views = None
-        q._codes = buf.data_ptr()
-        q._scales = q._codes + rows * cols       # (a multiple of 16)
-        q._strides = (1, max(rows, 1))
+        q._codes = at = buf.data_ptr()
+        q._scales = at + n
+        q._row, q._block = 1, rows or 1
         q.rows, q.cols = rows, cols
         return q
 
@@ -85,7 +86,8 @@ class Fp8Rows:
         if self._views is None:
             n = self.rows * self.cols
             self._views = (self._buf[:n].view(CODES).view(self.rows, self.cols),
-                           self._buf[n:].view(torch.float32).view(_blocks(self.cols), self.rows).t())
+                           self._buf.view(torch.float32).as_strided(
+                               (self.rows, _blocks(self.cols)), (1, self._block), n // 4))
         return self._views
 
     @property
@@ -124,7 +126,7 @@ def quantize(x: torch.Tensor, rows: torch.Tensor | None = None, pow2: bool = Fal
     q = Fp8Rows._empty(x, r, cols)
     abi.call("wisp_b200_fp8_quantize", x.data_ptr(), dt, ld, n,
              None if rows is None else rows.data_ptr(), r, cols, 1 if pow2 else 0, q._codes,
-             q._scales, 1, max(r, 1), stream_of(x))
+             q._scales, 1, q._block, stream_of(x))
     return q
 
 
@@ -138,7 +140,7 @@ def dequantize(q: Fp8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
             return dequantize(q, dtype)
     cols = q.cols
     out = buf.new_empty((q.rows, cols), dtype=dtype)
-    abi.call("wisp_b200_fp8_dequantize", q._codes, q._scales, *q._strides, q.rows, cols,
+    abi.call("wisp_b200_fp8_dequantize", q._codes, q._scales, q._row, q._block, q.rows, cols,
              out.data_ptr(), dt, cols, stream_of(buf))
     return out
 
@@ -266,7 +268,7 @@ def product(q: Fp8Rows, w: Fp8Weights, segments: torch.Tensor | None = None,
         ld = row_stride(out, "out")
     if segments is not None and n_segs == 0:
         return out          # (an empty tensor has no address, which would mean "all rows")
-    x = abi.WispFp8Rows(q._codes, q._scales, *q._strides, rows)
+    x = abi.WispFp8Rows(q._codes, q._scales, q._row, q._block, rows)
     abi.call("wisp_b200_fp8_product", w._cfgs[dtype], w._mats, w._up_mats, C.byref(x),
              None if segments is None else segments.data_ptr(), n_segs, out.data_ptr(), ld,
              w._error, stream_of(buf))

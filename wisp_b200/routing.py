@@ -4,6 +4,7 @@ include/wisp_b200.h)."""
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 
@@ -17,6 +18,12 @@ def policy(scoring: int = abi.WISP_ROUTE_SIGMOID, n_groups: int = 1, topk_groups
     """How tokens are routed, for select_experts and fp8.Fp8MoeLayer."""
     return abi.WispRouting(scoring, n_groups, topk_groups, group_top, 1 if renormalize else 0,
                            scaling)
+
+
+@lru_cache(maxsize=64)
+def _policy(scoring, n_groups, topk_groups, group_top, renormalize, scaling):
+    r = policy(scoring, n_groups, topk_groups, group_top, renormalize, scaling)
+    return r, C.byref(r)
 
 
 def check_bias(bias: torch.Tensor | None, n_experts: int, what: str = "bias") -> None:
@@ -55,11 +62,10 @@ def select_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | Non
         same_device(logits, bias=bias)
     if not 0 < top_k <= 32:
         raise invalid(f"top_k={top_k} (1..32)")
-    r = abi.WispRouting(scoring, n_groups, topk_groups, group_top, 1 if renormalize else 0, scaling)
-    # one allocation: indices, then weights
-    buf = logits.new_empty((2, tokens, top_k), dtype=torch.int32)
-    idx, w = buf[0], buf[1].view(torch.float32)
-    abi.call("wisp_b200_select_experts", C.byref(r), logits.data_ptr(), dt, ld, tokens, experts,
+    _, r = _policy(scoring, n_groups, topk_groups, group_top, bool(renormalize), scaling)
+    idx = logits.new_empty((tokens, top_k), dtype=torch.int32)
+    w = logits.new_empty((tokens, top_k), dtype=torch.float32)
+    abi.call("wisp_b200_select_experts", r, logits.data_ptr(), dt, ld, tokens, experts,
              top_k, None if bias is None else bias.data_ptr(), idx.data_ptr(), w.data_ptr(),
              stream_of(logits))
     return idx, w
