@@ -201,7 +201,6 @@ WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank,
   const float* w = (SWIGLU && lane ? p.ws_up : p.ws_w) +
                    ((int64_t)t.expert * p.ftiles + min(fb, p.ftiles - 1)) * p.nk + k0;
   const bool two = SWIGLU || wide, has_w = lane < (two ? 2 : 1);
-  const int groups = min(4, (t.cnt - (wide ? rank * 128 : 0) + 31) >> 5);     // of 32 rows
   int in = 0;
   auto fetch = [&](int kk) {
     if (kk < k1) {
@@ -224,16 +223,15 @@ WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank,
     const float* s = raw[(in + 1) % kRawSlots];
     fetch(kk + kRawSlots - 1);
     cp_async_wait<kRawSlots - 1>();
+    __syncwarp();                // every lane's copies of this block have landed
+    // four rows a lane, ready before the place they go to
+    const float4 v = reinterpret_cast<const float4*>(s)[lane];
+    const float w0 = s[128], w1 = s[129];
     const bool ok = first || mbar_wait(&bars.scale_empty[r.s], r.ph ^ 1, abort);
     if (!__all_sync(0xffffffffu, ok)) return false;
-    __syncwarp();                // every lane's copies of this block have landed
-    float* o = products[r.s] + lane;
-    const float w0 = s[128], w1 = two ? s[129] : 0.f;
-    for (int i = 0; i < groups; i++) {
-      const float v = s[32 * i + lane];
-      o[32 * i] = v * w0;
-      if (two) o[128 + 32 * i] = v * w1;
-    }
+    float4* o = reinterpret_cast<float4*>(products[r.s]) + lane;
+    o[0] = make_float4(v.x * w0, v.y * w0, v.z * w0, v.w * w0);
+    if (two) o[32] = make_float4(v.x * w1, v.y * w1, v.z * w1, v.w * w1);
     __syncwarp();
     // (its last reads being over, so is the barrier's last phase)
     arrive_one(&bars.acc_full[r.s]);
@@ -856,6 +854,7 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 127) / 128;
   const int64_t items = tiles_of(kNarrow) * ftiles;
   const int split = nk < 16 || x->rows > kSplitRows    ? 1
+                    : nk >= 32 && items * 32 <= 3 * (int64_t)sms ? 8
                     : items * 16 <= 3 * (int64_t)sms ? 4
                     : items * 8 <= 3 * (int64_t)sms  ? 2
                                                      : 1;
