@@ -581,6 +581,22 @@ WispError wisp_b200_fp8_dequantize(const uint8_t* d_codes, const float* d_scales
                                    void* d_out, int out_type, int64_t ld, cudaStream_t stream,
                                    WispErrCtx* err);
 
+/* Activation rows from wisp_b200_fp8_quantize. */
+typedef struct {
+    const uint8_t* codes;
+    const float* scales;
+    int64_t scale_row, scale_block;
+    int rows;
+} WispFp8Rows;
+
+/* Copies quantised rows: row p of the result is row d_src[p] of x, codes and scales as
+ * they are, or a row of zeros (codes and scales) for an index outside [0, x->rows).
+ * What quantising the gathered rows gives, where each row is wanted several times. The
+ * result lies nowhere in x. rows = 0 is allowed and launches nothing. */
+WispError wisp_b200_fp8_gather(const WispFp8Rows* x, const int* d_src, int rows, int cols,
+                               uint8_t* d_codes, float* d_scales, int64_t scale_row,
+                               int64_t scale_block, cudaStream_t stream, WispErrCtx* err);
+
 /* Quantises matrices d_w [n_entries x n x k] of w_type (contiguous) to codes of
  * the same shape and scales [n_entries x ceil(n / 128) x ceil(k / 128)], by the
  * rule above over blocks of 128 x 128. At most 65535 matrices and 65535 * 128
@@ -604,14 +620,6 @@ typedef struct {
     const uint8_t* codes;
     const float* scales;
 } WispFp8Mats;
-
-/* Activation rows from wisp_b200_fp8_quantize. */
-typedef struct {
-    const uint8_t* codes;
-    const float* scales;
-    int64_t scale_row, scale_block;
-    int rows;
-} WispFp8Rows;
 
 /* out[p, f] = sum_k x[p, k] w_e[f, k] for every row p of every segment, e = the
  * segment's expert (with swiglu silu(w x) * (up x)). Each block of 128 k is summed

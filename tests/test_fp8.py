@@ -54,6 +54,22 @@ def test_dequantize_refuses(kw, match):
 
 
 @pytest.mark.parametrize("kw,match", [
+    (dict(cols=24), "cols"), (dict(cols=0), "cols"), (dict(cols=(1 << 27) + 16), "2\\^27"),
+    (dict(rows=-1), "rows"), (dict(rows=0x7FFFFF01), "2\\^31"), (dict(x_rows=-1), "x="),
+    (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(src=None), "null"),
+    (dict(out=None), "null"), (dict(out_scales=None), "null"), (dict(codes=P + 8), "aligned"),
+    (dict(scales=P + 2), "aligned"), (dict(src=P + 2), "aligned"), (dict(out=P + 8), "aligned"),
+    (dict(out_scales=P + 1), "aligned"), (dict(srow=0), "strides"), (dict(sblock=0), "strides"),
+])
+def test_gather_refuses(kw, match):
+    a = dict(codes=P, scales=P, x_rows=4, src=P, rows=4, cols=64, out=P, out_scales=P, srow=1, sblock=4)
+    a.update(kw)
+    x = abi.WispFp8Rows(a["codes"], a["scales"], 1, 4, a["x_rows"])
+    _refused("wisp_b200_fp8_gather", C.byref(x), a["src"], a["rows"], a["cols"], a["out"],
+             a["out_scales"], a["srow"], a["sblock"], None, match=match)
+
+
+@pytest.mark.parametrize("kw,match", [
     (dict(dt=4), "out_type"), (dict(V=0), "n_entries"), (dict(n=0), "n=0"), (dict(k=24), "k=24"),
     (dict(V=65536), "65535"), (dict(n=65535 * 128 + 1), "65535"), (dict(w=None), "null"),
     (dict(codes=P + 4), "aligned"), (dict(w=P + 2, dt=0), "aligned"),
@@ -71,6 +87,7 @@ def test_calls_without_rows_launch_nothing():
     cfg = abi.WispFp8Config(2, 64, 64, 0, 1)
     m = abi.WispFp8Mats(P, P)
     x = abi.WispFp8Rows(None, None, 1, 1, 0)
+    abi.call("wisp_b200_fp8_gather", C.byref(x), None, 0, 64, None, None, 1, 1, None)
     abi.call("wisp_b200_fp8_product", C.byref(cfg), C.byref(m), None, C.byref(x), None, 0, None, 64,
              None, None)
 
@@ -313,6 +330,53 @@ def test_dequantize_scales_of_any_strides():
         want = fp8.dequantize(q)
         for s in (q.scales.contiguous(), torch.stack([q.scales, q.scales * 0], 2)[:, :, 0]):
             assert torch.equal(fp8.dequantize(fp8.Fp8Rows(q.codes, s)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16, 112, 2064])
+@pytest.mark.parametrize("rows", [0, 1, 9473, 9479])     # 1 and 7 left of eights
+def test_gather(cols, rows):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    n = 300
+    codes = torch.randint(0, 256, (n, cols), generator=g, device=DEV, dtype=torch.uint8)
+    wide = torch.rand((n, 2 * ref.blocks(cols) + 1), generator=g, device=DEV)
+    scales = wide[:, 1::2]
+    scales[3] = float("nan")
+    src = torch.randint(-2, n + 2, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    if rows:
+        src[0], src[-1] = 3, 2 ** 31 - 1
+        src[rows // 2] = -2 ** 31
+    got = fp8.gather(fp8.Fp8Rows(codes, scales), src)
+    inside = ((src >= 0) & (src < n))[:, None]
+    at = src.clamp(0, n - 1).long()
+    assert torch.equal(got.codes.view(torch.uint8), torch.where(inside, codes[at], 0))
+    _same_scales(got.scales, torch.where(inside, scales[at], 0.0).double())
+
+
+@pytest.mark.gpu
+def test_gather_of_no_rows_gives_zeros():
+    q = fp8.quantize(torch.ones((0, 64), device=DEV))
+    for m in (5, 2 ** 19):             # (the second as a quantise of many rows does it)
+        rows = torch.arange(m, device=DEV, dtype=torch.int32)
+        for got in (fp8.gather(q, rows), fp8.quantize(torch.ones((0, 64), device=DEV), rows)):
+            assert got.rows == m and not got.codes.view(torch.uint8).any() and not got.scales.any()
+
+
+@pytest.mark.gpu
+@POW2
+@pytest.mark.parametrize("dtype", list(DT))
+def test_quantize_of_rows_wanted_often(pow2, dtype):
+    # 16,300 x 2064 values are enough for every row of x to be quantised once and copied
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x = torch.randn((1100, 2064), generator=g, device=DEV).to(DT[dtype])[:1000]
+    x[5, 7], x[6] = float("inf"), 0
+    src = torch.randint(-3, 1003, (16300,), generator=g, device=DEV, dtype=torch.int32)
+    src[:2] = torch.tensor([5, 6], device=DEV, dtype=torch.int32)
+    many = fp8.quantize(x, src, pow2=pow2)
+    for a in range(0, 16300, 3000):    # too few at a time for that
+        few = fp8.quantize(x, src[a:a + 3000].clone(), pow2=pow2)
+        assert torch.equal(many.codes.view(torch.uint8)[a:a + 3000], few.codes.view(torch.uint8))
+        _same_scales(many.scales[a:a + 3000], few.scales.double())
 
 
 @pytest.mark.gpu

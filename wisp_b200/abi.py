@@ -190,6 +190,7 @@ SIGNATURES = {
                                        _P, _P, _P, _P, _SZ, _P, _P, _E]),
     "wisp_b200_fp8_quantize": (_I, [_P, _I, _L, _I, _P, _I, _I, _I, _P, _P, _L, _L, _P, _E]),
     "wisp_b200_fp8_dequantize": (_I, [_P, _P, _L, _L, _I, _I, _P, _I, _L, _P, _E]),
+    "wisp_b200_fp8_gather": (_I, [C.POINTER(WispFp8Rows), _P, _I, _I, _P, _P, _L, _L, _P, _E]),
     "wisp_b200_fp8_quantize_weights": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _E]),
     "wisp_b200_fp8_product": (_I, [C.POINTER(WispFp8Config), C.POINTER(WispFp8Mats),
                                    C.POINTER(WispFp8Mats), C.POINTER(WispFp8Rows), _P, _I, _P, _L,

@@ -411,6 +411,57 @@ void launch_dequantize(const DequantParams& p, cudaStream_t st) {
     wb::launch_k(dequantize_kernel<TYPE, 1>, dim3(p.rows, gy), threads, 0, st, p);
 }
 
+struct GatherParams {
+  const uint8_t* codes;
+  const float* scales;
+  int64_t s_row, s_block;
+  int x_rows;
+  const int* src;
+  int rows, cols;
+  uint8_t* out;
+  float* out_scales;
+  int64_t o_row, o_block;
+};
+
+// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 codes of R rows per thread.
+// Lane i of a block's eight moves the scale of row i, so that scales stored block by
+// block go out 4 R bytes at a time. 32,768 of 4096 rows of 7168 take 54 us, of which
+// the 242 MB that are written are 37 at the copy rate.
+template <int R>
+__global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
+  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool in = u < p.cols / kUnit;
+  uint4 c[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int64_t sr = row0 + i < p.rows ? (int64_t)__ldg(p.src + row0 + i) : -1;
+    c[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (in && sr >= 0 && sr < p.x_rows)
+      c[i] = __ldg(reinterpret_cast<const uint4*>(p.codes + sr * p.cols) + u);
+  }
+  const int lane = u & (kLanes - 1), b = u / kLanes;
+  if (lane < R && b * kBlock < p.cols && row0 + lane < p.rows) {
+    const int64_t sr = __ldg(p.src + row0 + lane);
+    p.out_scales[(row0 + lane) * p.o_row + b * p.o_block] =
+        sr >= 0 && sr < p.x_rows ? __ldg(p.scales + sr * p.s_row + b * p.s_block) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++)
+    if (in && row0 + i < p.rows)
+      reinterpret_cast<uint4*>(p.out + (row0 + i) * p.cols)[u] = c[i];
+}
+
+void launch_gather(const GatherParams& p, cudaStream_t st) {
+  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
+  const int gy = (units + threads - 1) / threads;
+  constexpr int R = 8;
+  if ((int64_t)p.rows * gy >= 148 * 8 * R)
+    wb::launch_k(gather_kernel<R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
+  else
+    wb::launch_k(gather_kernel<1>, dim3(p.rows, gy), threads, 0, st, p);
+}
+
 }  // namespace
 
 extern "C" WispError wisp_b200_fp8_quantize(const void* d_x, int x_type, int64_t ld, int x_rows,
@@ -496,6 +547,33 @@ extern "C" WispError wisp_b200_fp8_dequantize(const uint8_t* d_codes, const floa
     launch_dequantize<WISP_DT_BF16>(p, stream);
   else
     launch_dequantize<WISP_DT_F16>(p, stream);
+  WB_CUDA_CHECK(cudaGetLastError());
+  return WISP_OK;
+}
+
+extern "C" WispError wisp_b200_fp8_gather(const WispFp8Rows* x, const int* d_src, int rows, int cols,
+                                          uint8_t* d_codes, float* d_scales, int64_t scale_row,
+                                          int64_t scale_block, cudaStream_t stream,
+                                          WispErrCtx* err) {
+  if (!x || x->rows < 0 || rows < 0 || rows > wb::kMaxRows || cols <= 0 || cols > kMaxCols ||
+      cols % kUnit)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_gather: x=%p rows=%d cols=%d (at most 2^31 - 256 rows, cols a multiple of 16 "
+                   "up to 2^27)",
+                   (const void*)x, rows, cols);
+  if (scale_row < 1 || scale_block < 1)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_gather: scale strides %lld, %lld (at least 1)",
+                   (long long)scale_row, (long long)scale_block);
+  if (rows == 0) return WISP_OK;
+  if (((!x->codes || !x->scales) && x->rows > 0) || !d_src || !d_codes || !d_scales)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_gather: null pointer argument");
+  if (((uintptr_t)x->codes & 15) || ((uintptr_t)x->scales & 3) || ((uintptr_t)d_src & 3) ||
+      ((uintptr_t)d_codes & 15) || ((uintptr_t)d_scales & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_gather: codes must be 16-byte, scales and d_src 4-byte aligned");
+  launch_gather({x->codes, x->scales, x->scale_row, x->scale_block, x->rows, d_src, rows, cols,
+                 d_codes, d_scales, scale_row, scale_block},
+                stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
 }

@@ -658,22 +658,6 @@ extern "C" WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const W
 
 namespace {
 
-// The same for fp8 rows, whose scales are stored block by block.
-__global__ void __launch_bounds__(256)
-gather_fp8_kernel(const uint4* __restrict__ codes, const float* __restrict__ scales,
-                  const int* __restrict__ row_token, int tokens, int scale_ld, int code_words,
-                  int blocks, uint4* __restrict__ out_codes, float* __restrict__ out_scales,
-                  int out_scale_ld) {
-  const size_t p = blockIdx.x;
-  const int src = row_token[p];
-  if (src < 0 || src >= tokens) return;
-  const size_t t = src;
-  for (int i = threadIdx.x; i < code_words; i += 256)
-    out_codes[p * code_words + i] = __ldg(codes + t * code_words + i);
-  for (int i = threadIdx.x; i < blocks; i += 256)
-    out_scales[p + (size_t)i * out_scale_ld] = __ldg(scales + t + (size_t)i * scale_ld);
-}
-
 struct Fp8Ws {
   Workspace base;      // routing, plan, token lists
   float* part;
@@ -789,10 +773,9 @@ extern "C" WispError wisp_b200_fp8_moe_forward(const WispMoeConfig* cfg, const W
     e = wisp_b200_fp8_quantize(d_x, WISP_DT_BF16, M, T, nullptr, T, M, w->pow2, ws.tc, ws.ts, 1, T,
                                stream, err);
     if (e != WISP_OK) return e;
-    wb::launch_k(gather_fp8_kernel, b.rows, 256, 0, stream, reinterpret_cast<const uint4*>(ws.tc),
-                 ws.ts, b.row_token, T, T, M / 16, M / 128, reinterpret_cast<uint4*>(ws.xc), ws.xs,
-                 b.rows);
-    WB_CUDA_CHECK(cudaGetLastError());
+    const WispFp8Rows tr = {ws.tc, ws.ts, 1, T, T};
+    e = wisp_b200_fp8_gather(&tr, b.row_token, b.rows, M, ws.xc, ws.xs, 1, b.rows, stream, err);
+    if (e != WISP_OK) return e;
   } else {
     e = wisp_b200_fp8_quantize(d_x, WISP_DT_BF16, M, T, b.row_token, b.rows, M, w->pow2, ws.xc,
                                ws.xs, 1, b.rows, stream, err);

@@ -7,6 +7,7 @@ operator has a gradient, and tensors that require one are refused where autograd
 would record the call.
 
     q = quantize(x)                       # rows -> codes, a scale per 128 values
+    q = gather(q, rows)                   # the rows of each expert's tokens
     w = Fp8Weights(codes, scales)         # [V, n, k], [V, n/128, k/128]
     y = product(q, w, segments)           # rows by their experts' matrices
 """
@@ -99,6 +100,14 @@ class Fp8Rows:
         return self._split()[1]
 
 
+def _indices(rows: torch.Tensor) -> int:
+    if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+        raise invalid("rows: a contiguous 1D int32 tensor")
+    if rows.shape[0] > INT_MAX:
+        raise invalid(f"rows: {rows.shape[0]} indices, more than 2^31 - 1")
+    return rows.shape[0]
+
+
 def quantize(x: torch.Tensor, rows: torch.Tensor | None = None, pow2: bool = False) -> Fp8Rows:
     """Rows of x (float32, bfloat16 or float16) as e4m3 codes, with one scale max|x| / 448 per
     128 values (pow2: the least power of two that is not below it); rows (int32): row p of the
@@ -109,13 +118,7 @@ def quantize(x: torch.Tensor, rows: torch.Tensor | None = None, pow2: bool = Fal
     n, cols = x.shape
     if cols % 16 or cols == 0:
         raise invalid(f"row length {cols} is no multiple of 16")
-    r = n
-    if rows is not None:
-        if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
-            raise invalid("rows: a contiguous 1D int32 tensor")
-        if rows.shape[0] > INT_MAX:
-            raise invalid(f"rows: {rows.shape[0]} indices, more than 2^31 - 1")
-        r = rows.shape[0]
+    r = n if rows is None else _indices(rows)
     dt = dtype_code(x.dtype, "x")
     other = elsewhere(x)
     if other is not None:
@@ -123,11 +126,32 @@ def quantize(x: torch.Tensor, rows: torch.Tensor | None = None, pow2: bool = Fal
             return quantize(x, rows, pow2)
     if rows is not None:
         same_device(x, rows=rows)
+        # Every row of x once and copies, where rows are wanted several times and there is
+        # enough to do: 4096 bf16 rows of 7168 to 32,768 142 -> 77 us, 1024 to 8192 42 -> 27; 256
+        # to 2048 16.4 against 17.4, 4096 to 8192 43 against 42.
+        if r >= 4 * n and r * cols >= 1 << 25:
+            return gather(quantize(x, pow2=pow2), rows)
     q = Fp8Rows._empty(x, r, cols)
     abi.call("wisp_b200_fp8_quantize", x.data_ptr(), dt, ld, n,
              None if rows is None else rows.data_ptr(), r, cols, 1 if pow2 else 0, q._codes,
              q._scales, 1, q._block, stream_of(x))
     return q
+
+
+def gather(q: Fp8Rows, rows: torch.Tensor) -> Fp8Rows:
+    """Rows of q, codes and scales as they are: row p of the result is row rows[p] (int32) of q, a
+    row of zeros where rows[p] is outside q."""
+    r, buf, cols = _indices(rows), q._buf, q.cols
+    other = elsewhere(buf)
+    if other is not None:
+        with other:
+            return gather(q, rows)
+    same_device(buf, rows=rows)
+    out = Fp8Rows._empty(buf, r, cols)
+    x = abi.WispFp8Rows(q._codes, q._scales, q._row, q._block, q.rows)
+    abi.call("wisp_b200_fp8_gather", C.byref(x), rows.data_ptr(), r, cols, out._codes, out._scales,
+             1, out._block, stream_of(buf))
+    return out
 
 
 def dequantize(q: Fp8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
