@@ -59,8 +59,8 @@ class Fp8Rows:
             raise invalid(f"scales: float32 {(self.rows, _blocks(self.cols))}, not {scales.dtype} "
                           f"{tuple(scales.shape)}")
         same_device(codes, scales=scales)
-        self._views = (codes, scales)
-        self._buf = codes
+        self._buf = self._codes_view = codes
+        self._scales_view = scales
         self._codes, self._scales = codes.data_ptr(), scales.data_ptr()
         self._row, self._block = scales.stride()
 
@@ -70,8 +70,9 @@ class Fp8Rows:
         are made when someone asks for them."""
         q = cls.__new__(cls)
         n = rows * cols             # (a multiple of 16)
-        q._buf = buf = x.new_empty(n + 4 * rows * ((cols + BLOCK - 1) // BLOCK), dtype=torch.uint8)
-        q._views = None
+        q._buf = buf = x.new_empty(n // 4 + rows * ((cols + BLOCK - 1) // BLOCK),
+                                   dtype=torch.float32)
+        q._codes_view = q._scales_view = None
         q._codes = at = buf.data_ptr()
         q._scales = at + n
         q._row, q._block = 1, rows or 1
@@ -80,24 +81,23 @@ class Fp8Rows:
 
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """As torch.Tensor.record_stream: the rows are in use on `stream` too."""
-        for t in (self._buf, *(self._views or ())):
-            t.record_stream(stream)
-
-    def _split(self) -> tuple[torch.Tensor, torch.Tensor]:
-        if self._views is None:
-            n = self.rows * self.cols
-            self._views = (self._buf[:n].view(CODES).view(self.rows, self.cols),
-                           self._buf.view(torch.float32).as_strided(
-                               (self.rows, _blocks(self.cols)), (1, self._block), n // 4))
-        return self._views
+        for t in (self._buf, self._codes_view, self._scales_view):
+            if t is not None:
+                t.record_stream(stream)
 
     @property
     def codes(self) -> torch.Tensor:
-        return self._split()[0]
+        if self._codes_view is None:
+            self._codes_view = self._buf.view(CODES).as_strided((self.rows, self.cols),
+                                                                (self.cols, 1))
+        return self._codes_view
 
     @property
     def scales(self) -> torch.Tensor:
-        return self._split()[1]
+        if self._scales_view is None:
+            self._scales_view = self._buf.as_strided((self.rows, _blocks(self.cols)),
+                                                     (1, self._block), self.rows * self.cols // 4)
+        return self._scales_view
 
 
 def _indices(rows: torch.Tensor) -> int:
