@@ -24,10 +24,16 @@
 // MMAs' issue to the next ones' into it pass their own time, 400 cycles until the
 // barriers have reported them, the loads into registers, and 160 until the MMA
 // warp has seen it free. So one barrier stands for a whole block (gate and up, or
-// both blocks of features), and a buffer is free as soon as it has been read,
-// before the last of it is added. (Groups of 128 columns with barriers of their
-// own: twice the waits, and a wide tile's MMAs then read the rows twice from shared
-// memory. 8192 x 8192 x 7168 457 us.)
+// both blocks of features: groups of 128 columns with barriers of their own have
+// twice the waits, and a wide tile's MMAs then read the rows twice from shared
+// memory), and a buffer is free as soon as it has been read, before the last of it is
+// added.
+//
+// Measured (L2 flushed; us): 64 experts of 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows
+// each 297 / 308 / 344 / 455, where the weights take 287 at the copy rate; 64 of 7168 x
+// 2048 175 / 192 / 229 / 303 (143): bound by HBM up to ~100 rows. 8192 x 8192 x 7168 387
+// = 2.48 PFLOP/s, of which MMAs and copies alone are nine tenths; without a pause
+// between calls 480, as the power limit lowers the clock.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
@@ -384,9 +390,6 @@ struct Reduce {
   }
 };
 
-// One output type per kernel: with all three in one, the sums' unrolled stores do
-// not stay in the instruction cache, and a tile's first pass through them cost 3 to
-// 12 us.
 template <typename T, bool SWIGLU, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_product_kernel(const __grid_constant__ Params p) {
@@ -853,6 +856,10 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   };
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 127) / 128;
   const int64_t items = tiles_of(kNarrow) * ftiles;
+  // Few tiles of few rows: clusters of 8, 4 or 2 CTAs split K, as long as they fill 3/4
+  // of the SMs (at one CTA an SM, more of them do not fit the GPCs in one wave) and each
+  // has enough of K. One row, us, by half as many / by the rule's: gate/up 1536 x 7168 (12
+  // tiles) 12.7 / 10.5; 2048 x 7168 (16 tiles) by 4 9.9, by 8 in two waves 15.6.
   const int split = nk < 16 || x->rows > kSplitRows    ? 1
                     : nk >= 32 && items * 32 <= 3 * (int64_t)sms ? 8
                     : items * 16 <= 3 * (int64_t)sms ? 4

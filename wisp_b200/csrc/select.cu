@@ -271,8 +271,9 @@ WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
 // 16) or 0 (logits, from the largest on for softmax, below -700). Only a token with a
 // closer pair where it matters, or with a value that is not finite, goes the 64-bit
 // way. (A softmax whose weights are not renormalised needs the 64-bit sum over all
-// experts, and goes that way at once: 12.6 us where this takes 15.6.) 256 experts with bias and groups, one token: 7.9 -> 4.6 us a
-// launch, 4096: 14.3 -> 11.7, 16,384: 47 -> 34; bound by its instructions, 1700 a token.
+// experts, and goes that way at once: 12.6 us where this takes 15.6.) 256 experts with
+// bias and groups, us a launch, in 64 bits alone and so: one token 7.9 and 4.6, 4096
+// 14.3 and 11.7, 16,384 47 and 34; bound by its instructions, 1700 a token.
 template <int PER>
 __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
   extern __shared__ double choices64[];       // [kWarps][E], with groups
