@@ -31,9 +31,10 @@
 //
 // Measured (L2 flushed; us): 64 experts of 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows
 // each 297 / 308 / 344 / 455, where the weights take 287 at the copy rate; 64 of 7168 x
-// 2048 175 / 192 / 229 / 303 (143): bound by HBM up to ~100 rows. 8192 x 8192 x 7168 387
-// = 2.48 PFLOP/s, of which MMAs and copies alone are nine tenths; without a pause
-// between calls 480, as the power limit lowers the clock.
+// 2048 175 / 195 / 225 / 282 (143): bound by HBM up to ~100 rows. 8192 x 8192 x 7168 375
+// = 2.57 PFLOP/s; without a pause between calls 470, as the power limit lowers the
+// clock. A block of a wide tile takes 0.44 us (0.27 at the MMAs' nominal rate), a change
+// of tiles 2.5 more.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
@@ -59,10 +60,12 @@ constexpr int kWide = 256;
 constexpr int kMaxStages = 12;
 constexpr int kMaxBufs = 8;
 constexpr int kRingBytes = 206 * 1024;
+constexpr int kStoreBytes = 8 * 4096;     // of these, where wide tiles' outputs change places
 // Blocks whose scales are held or on their way; scales of a block: of the CTA's rows,
 // then the weights' two.
 constexpr int kRawSlots = 8, kRawFloats = 132;
 constexpr int kTileRing = 8;
+static_assert(kMaxStages > kMaxBufs && kMaxStages >= kTileRing, "threads that initialise barriers");
 // Registers: launch 168 x 384 = 64,512; 256 x 232 + 128 x 40 = 64,512.
 constexpr int kEpiRegs = 232, kOtherRegs = 40;
 struct Bars {
@@ -247,43 +250,92 @@ WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank,
   return true;
 }
 
-template <bool SWIGLU, typename T>
-WB_DEV void store_wide(const Params& p, const Sums& a, const Tile& t, const Warp& me) {
+// A wide tile's outputs: a lane holds a row. 128 bytes of each row at a time change
+// places in the warp's 4 KB of shared memory (16-byte words, swizzled), so that eight
+// lanes write a line of one row. (Straight from the registers, 32 bytes of 32 rows per
+// instruction, the lines pass one a cycle: 8192 x 8192 x 7168 385 us, so 373; 64 experts of
+// 7168 x 2048 with 256 rows and fp32 outputs 300 and 282.)
+template <typename T>
+WB_DEV void store_wide(const Params& p, const Sums& a, const Tile& t, const Warp& me, uint4* stage) {
+  const int row0 = me.rank * 128 + me.quad * 32, rows = min(t.cnt - row0, 32);
+  if (rows <= 0) return;
+  constexpr int kWord = 16 / (int)sizeof(T), kLine = 8 * kWord;      // values
+  const int r = me.lane >> 3, c = me.lane & 7;
+  T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)row0 + r) * p.ld;
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+#pragma unroll
+    for (int l = 0; l < 64; l += kLine) {
+      __syncwarp();                      // the last line has been read
+#pragma unroll
+      for (int w = 0; w < 8; w++) {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float* g = reinterpret_cast<const float*>(a.v) + q * 64 + l + w * kWord;
+          if constexpr (sizeof(T) == 4)
+            v[j] = __float_as_uint(g[j]);
+          else
+            v[j] = pack2(g[2 * j], g[2 * j + 1],
+                         std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+        }
+        stage[me.lane * 8 + (w ^ (me.lane & 7))] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      __syncwarp();
+      const int f = ((t.ft & ~1) + q) * 128 + me.half * 64 + l + c * kWord;
+      T* o = out + f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 4, o += 4 * p.ld) {
+        if (r + i >= rows) break;
+        const uint4 v = stage[(r + i) * 8 + (c ^ ((r + i) & 7))];
+        if (p.wide_out && f + kWord <= p.N) {
+          *reinterpret_cast<uint4*>(o) = v;
+        } else {
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+          Bits* e = reinterpret_cast<Bits*>(o);
+#pragma unroll
+          for (int j = 0; j < kWord; j++)
+            if (f + j < p.N) e[j] = (Bits)(sizeof(T) == 4 ? u[j] : u[j / 2] >> (16 * (j & 1)));
+        }
+      }
+    }
+  }
+}
+
+// The same for silu(gate) * up, straight from the registers: half the values, and the
+// shared memory is a stage of the ring (64 experts of 2 x 2048 x 7168 with 256 rows 457 us;
+// through it 467).
+template <typename T>
+WB_DEV void store_wide_swiglu(const Params& p, const Sums& a, const Tile& t, const Warp& me) {
   const int r = me.rank * 128 + me.quad * 32 + me.lane;
   if (r >= t.cnt) return;
   T* row = static_cast<T*>(p.out) + (t.row0 + (int64_t)r) * p.ld;
   constexpr int kRun = 32 / (int)sizeof(T);      // values of a 32-byte store
+  const int f = t.ft * 128 + me.half * 64;
 #pragma unroll
-  for (int q = 0; q < (SWIGLU ? 1 : 2); q++) {
-    const int f = (SWIGLU ? t.ft : (t.ft & ~1) + q) * 128 + me.half * 64;
+  for (int i = 0; i < 64; i += kRun) {
+    float o[kRun];
 #pragma unroll
-    for (int i = 0; i < 64; i += kRun) {
-      float o[kRun];
+    for (int j = 0; j < kRun; j++) {
+      const float2 g = a.v[(i + j) / 2], u = a.v[32 + (i + j) / 2];
+      o[j] = swiglu<T>(j & 1 ? g.y : g.x, j & 1 ? u.y : u.x);
+    }
+    if (p.wide_out && f + i + kRun <= p.N) {
+      uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < kRun; j++) {
-        const float2 g = a.v[q * 32 + (i + j) / 2];
-        o[j] = j & 1 ? g.y : g.x;
-        if (SWIGLU) {
-          const float2 u = a.v[32 + (i + j) / 2];
-          o[j] = swiglu<T>(o[j], j & 1 ? u.y : u.x);
-        }
+      for (int j = 0; j < 8; j++) {
+        if constexpr (sizeof(T) == 4)
+          w[j] = __float_as_uint(o[j]);
+        else
+          w[j] = pack2(o[2 * j], o[2 * j + 1],
+                       std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
       }
-      if (p.wide_out && f + i + kRun <= p.N) {
-        uint32_t w[8];
+      store32(row + f + i, w);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          if constexpr (sizeof(T) == 4)
-            w[j] = __float_as_uint(o[j]);
-          else
-            w[j] = pack2(o[2 * j], o[2 * j + 1],
-                         std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
-        }
-        store32(row + f + i, w);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kRun; j++)
-          if (f + i + j < p.N) put_out(row + f + i + j, o[j]);
-      }
+      for (int j = 0; j < kRun; j++)
+        if (f + i + j < p.N) put_out(row + f + i + j, o[j]);
     }
   }
 }
@@ -471,7 +523,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   const int narrow_bytes = kMats * kABytes + narrow_n / (PAIR ? 2 : 1) * 128;
   const int stage_bytes = wides ? max(narrow_bytes, 2 * kABytes) : narrow_bytes;
   constexpr int kRedBytes = kMats * kRedRows * 128 * 4;     // a cluster's partial sums
-  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : 0)) / stage_bytes);
+  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : wides && !SWIGLU ? kStoreBytes : 0)) / stage_bytes);
   // accumulators: buffers of `cols` columns, one for a block of k (gate, then up)
   const int up_offset = (narrow_n + 31) & ~31;
   const int cols = wides ? kWide : up_offset * kMats;
@@ -593,6 +645,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     red.bars = &bars;
     red.ks = ks;
     red.kp = kp;
+    uint4* stage = reinterpret_cast<uint4*>(smem + kRingBytes - kStoreBytes) + (warp - kEpiWarp) * 256;
     Ring b;
     const uint32_t base = tmem + ((uint32_t)(me.quad * 32) << 16);
     const uint32_t empty0 = cluster_addr(&bars.acc_empty[0], PAIR ? 0 : kp);
@@ -685,12 +738,16 @@ fp8_product_kernel(const __grid_constant__ Params p) {
         }
       }
       if (!ok) break;
-      if (!PAIR && ks > 1)
+      if (!PAIR && ks > 1) {
         ok = red.template store<T>(p, a, t, me, abort);
-      else if (wide)
-        store_wide<SWIGLU, T>(p, a, t, me);
-      else
+      } else if (wide) {
+        if constexpr (SWIGLU)
+          store_wide_swiglu<T>(p, a, t, me);
+        else
+          store_wide<T>(p, a, t, me, stage);
+      } else {
         store_narrow<SWIGLU, T>(p, a, t, me);
+      }
       __syncwarp();
     }
   } else if (warp == kSchedWarp) {
