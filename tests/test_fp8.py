@@ -538,6 +538,23 @@ def test_product_split_over_k(swiglu, dtype, n, k, counts):
 
 
 @pytest.mark.gpu
+@SWIGLU
+@pytest.mark.parametrize("n,k,counts", [
+    (300, 4112, [9, 0, 30]),        # clusters of eight, 33 stages in uneven parts
+    (1400, 4096, [1]),
+    (60, 5120, [5, 22, 31]),        # one feature tile
+])
+def test_product_split_over_k_by_eight(swiglu, n, k, counts):
+    for dtype in DT.values():
+        q, w, mats, segs, dev, out = _run_product(swiglu, dtype, n, k, counts, extra=3)
+        for _ in range(3):
+            again = torch.full_like(out, 7.0)
+            fp8.product(q, w, dev, out=again)
+            assert torch.equal(again[:-3], out[:-3]) and (again[-3:] == 7.0).all()
+        w.check()
+
+
+@pytest.mark.gpu
 def test_product_many_segments_same_expert():
     """1025 segments, experts out of order and repeated."""
     counts = [(i * 7) % 4 for i in range(1025)]
@@ -584,6 +601,103 @@ def test_product_leaves_other_rows_and_columns(dtype, sizes):
         for _, r0, r in segs:
             touched[r0:r0 + r, at:at + 200] = True
         assert (big[~touched] == 7.0).all()
+
+
+WIDE = (2200, [(2, 5, 300), (0, 310, 0), (1, 311, 200), (3, 520, 700), (0, 1230, 90)], 1340)
+
+
+@pytest.mark.gpu
+@SWIGLU
+@pytest.mark.parametrize("dtype", list(DT))
+def test_wide_tiles_leave_other_rows_and_columns(swiglu, dtype):
+    """The same where there is enough for tiles of 256 rows: 1340 rows of 2200 features."""
+    n, segs, rows = WIDE
+    g = torch.Generator(device=DEV).manual_seed(24)
+    mats = [_mats(g, 4, n, 400, 3.0 if swiglu and i == 0 else 1.0) for i in range(2 if swiglu else 1)]
+    w = fp8.Fp8Weights(*mats[0], up=mats[1] if swiglu else None)
+    q = _rows(g, rows, 400)
+    dev = torch.tensor([(*s, 0) for s in segs], dtype=torch.int32, device=DEV)
+    for at, ld in ((9, 2333), (16, 2336), (8, 2264)):
+        big = torch.full((rows, ld), 7.0, device=DEV, dtype=DT[dtype])
+        fp8.product(q, w, dev, out=big[:, at:at + n])
+        _check(big[:, at:at + n], q, mats, segs, 400)
+        touched = torch.zeros_like(big, dtype=torch.bool)
+        for _, r0, r in segs:
+            touched[r0:r0 + r, at:at + n] = True
+        assert (big[~touched] == 7.0).all()
+    w.check()
+
+
+@pytest.mark.gpu
+def test_wide_tiles_keep_nan_apart():
+    """NaN in the rows beside a segment, in a row's and in a block of features' scales, and in a
+    code, where tiles are of 256 rows."""
+    n, segs, rows = WIDE
+    g = torch.Generator(device=DEV).manual_seed(25)
+    codes, scales = _mats(g, 4, n, 400)
+    w = fp8.Fp8Weights(codes, scales)
+    q = _rows(g, rows, 400)
+    dev = torch.tensor([(*s, 0) for s in segs], dtype=torch.int32, device=DEV)
+    out = fp8.product(q, w, dev, dtype=torch.float32)
+    inside = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    for _, r0, r in segs:
+        inside[r0:r0 + r] = True
+    q.codes.view(torch.uint8)[~inside] = 0x7F
+    q.scales[~inside] = float("nan")
+    assert torch.equal(fp8.product(q, w, dev, dtype=torch.float32)[inside], out[inside])
+    q.scales[600, 2] = q.scales[304, 3] = float("nan")
+    scales[3, 17, 0] = float("nan")       # features 2176 .. 2199, the last block
+    codes.view(torch.uint8)[2, 1000, 399] = 0xFF
+    bad = torch.isnan(fp8.product(q, w, dev, dtype=torch.float32))
+    want = torch.zeros_like(bad)
+    want[600] = want[304] = True
+    want[520:1220, 2176:] = True
+    want[5:305, 1000] = True
+    assert torch.equal(bad[inside], want[inside])
+    w.check()
+
+
+@pytest.mark.gpu
+@SWIGLU
+def test_wide_tiles_on_streams_and_in_graphs(swiglu):
+    """Two streams at once and two replayed graphs, over scales of other strides, give the bits of
+    a call alone."""
+    n, segs, rows = WIDE
+    g = torch.Generator(device=DEV).manual_seed(26)
+    mats = [_mats(g, 4, n, 1040) for _ in range(2 if swiglu else 1)]
+    w = fp8.Fp8Weights(*mats[0], up=mats[1] if swiglu else None)
+    dev = torch.tensor([(*s, 0) for s in segs], dtype=torch.int32, device=DEV)
+    qs = [_rows(g, rows, 1040) for _ in range(2)]
+    same = fp8.Fp8Rows(qs[1].codes, qs[1].scales[:1].expand(rows, -1))        # one row's scales
+    qs.append(fp8.Fp8Rows(same.codes, same.scales.contiguous()))
+    want = [torch.zeros((rows, n), device=DEV, dtype=torch.bfloat16) for _ in qs]
+    for q, o in zip(qs, want):
+        fp8.product(q, w, dev, out=o)
+    qs[2] = same
+    outs = [torch.zeros_like(o) for o in want]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for q, o, s in zip(qs, outs, streams):
+            with torch.cuda.stream(s):
+                fp8.product(q, w, dev, out=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    graphs = []
+    for q, o in zip(qs, outs):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            fp8.product(q, w, dev, out=o)
+        graphs.append(gr)
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    for gr, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    w.check()
 
 
 @pytest.mark.gpu

@@ -44,6 +44,13 @@ def test_select_without_a_routing_or_tokens():
     abi.call("wisp_b200_select_experts", C.byref(r), None, 0, 32, 0, 32, 4, None, None, None, None)
 
 
+def test_policy_refuses_what_would_be_cut_off():
+    for kw in (dict(n_groups=2 ** 32 + 1), dict(topk_groups=-1), dict(scoring=2 ** 32),
+               dict(group_top=2 ** 33 + 2)):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\]"):
+            routing.policy(**kw)
+
+
 def test_python_refusals():
     x = torch.zeros(2, 16)
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -110,6 +117,26 @@ def test_ties_and_close_choices(scoring):
                    group_top=top)
     idx, _ = routing.select_experts(x[3:4], 4, scoring=scoring)
     assert idx.tolist() == [[63, 62, 61, 60]]
+
+
+@pytest.mark.gpu
+@SCORING
+@pytest.mark.parametrize("base", [-500.0, -3.0, 0.0, 12.0, 40.0])
+def test_logits_a_few_roundings_apart(scoring, base):
+    """Logits, and choices under a bias that brings them next to each other, apart by 2^-24 to 2^-15
+    of their size: on both sides of where fp32 can tell."""
+    g = torch.Generator(device=DEV).manual_seed(int(base) + 600)
+    e = 40
+    for step in range(15, 25):
+        i = torch.randint(-6, 7, (30, e), generator=g, device=DEV).double()
+        x = (base + i * max(abs(base), 1.0) * 2.0 ** -step).float()
+        # choices around 1/2, `step` binary places apart, for the first token's logits
+        score = torch.softmax(x[0].double(), 0) if scoring == 0 else torch.sigmoid(x[0].double())
+        bias = (0.5 + i[1] * 2.0 ** -step - score).float()
+        x[10:20] = x[0]
+        for b in (None, bias):
+            for groups, kept, top in ((1, 1, 1), (8, 3, 2), (10, 4, 1)):
+                _check(x, 7, scoring, b, n_groups=groups, topk_groups=kept, group_top=top)
 
 
 @pytest.mark.gpu

@@ -328,6 +328,8 @@ class Fp8MoeLayer:
                     down=down.error_word, score_bias=score_bias)
         if wants_grad(router_w, router_bias, score_bias):
             refuse_grad()
+        if not 0 < tokens <= INT_MAX:
+            raise invalid(f"tokens={tokens}")
         self.spec, self.gate_up, self.down, self.routing = spec, gate_up, down, routing
         self.cfg = spec.cfg(tokens)
         self.cfg.router_fp16 = 1 if router_w.dtype == torch.float16 else 0

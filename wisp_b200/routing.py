@@ -9,15 +9,17 @@ from functools import lru_cache
 import torch
 
 from . import abi
-from .fp4 import dtype_code, elsewhere, invalid, refuse_grad, row_stride, same_device, stream_of, \
+from .fp4 import INT_MAX, dtype_code, elsewhere, invalid, refuse_grad, row_stride, same_device, stream_of, \
     wants_grad
 
 
 def policy(scoring: int = abi.WISP_ROUTE_SIGMOID, n_groups: int = 1, topk_groups: int = 1,
            group_top: int = 2, renormalize: bool = True, scaling: float = 1.0) -> abi.WispRouting:
     """How tokens are routed, for select_experts and fp8.Fp8MoeLayer."""
-    return abi.WispRouting(scoring, n_groups, topk_groups, group_top, 1 if renormalize else 0,
-                           scaling)
+    counts = [int(v) for v in (scoring, n_groups, topk_groups, group_top)]
+    if not all(0 <= v <= INT_MAX for v in counts):
+        raise invalid(f"scoring, n_groups, topk_groups, group_top: {counts}")
+    return abi.WispRouting(*counts, 1 if renormalize else 0, float(scaling))
 
 
 @lru_cache(maxsize=64)
@@ -62,7 +64,9 @@ def select_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | Non
         same_device(logits, bias=bias)
     if not 0 < top_k <= 32:
         raise invalid(f"top_k={top_k} (1..32)")
-    _, r = _policy(scoring, n_groups, topk_groups, group_top, bool(renormalize), scaling)
+    # (as numbers: what the cache keeps may not change behind it)
+    _, r = _policy(int(scoring), int(n_groups), int(topk_groups), int(group_top),
+                   bool(renormalize), float(scaling))
     idx = logits.new_empty((tokens, top_k), dtype=torch.int32)
     w = logits.new_empty((tokens, top_k), dtype=torch.float32)
     abi.call("wisp_b200_select_experts", r, logits.data_ptr(), dt, ld, tokens, experts,
