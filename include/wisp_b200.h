@@ -623,8 +623,9 @@ typedef struct {
 
 /* out[p, f] = sum_k x[p, k] w_e[f, k] for every row p of every segment, e = the
  * segment's expert (with swiglu silu(w x) * (up x)). Each block of 128 k is summed
- * on the tensor cores in fp32, scaled by its two scales and added up in fp32; the
- * sum is rounded once to out_type. d_segs, n_segs, ld, up, the rows in no segment
+ * on the tensor cores in fp32, scaled by the product of its two scales (in fp32, whose
+ * range that product has to stay in) and added up in fp32; the sum is rounded once to
+ * out_type. d_segs, n_segs, ld, up, the rows in no segment
  * and d_error_flag as for wisp_b200_fp4_product. rows = 0 is allowed and launches
  * nothing. */
 WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispFp8Mats* w,

@@ -380,6 +380,43 @@ def test_quantize_of_rows_wanted_often(pow2, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [900, 16300], ids=["singly", "copied"])
+def test_quantize_on_streams_and_in_graphs(rows):
+    """Two streams at once, and a graph that is replayed over other values, other indices and
+    another graph's replays, give what a call alone gives."""
+    g = torch.Generator(device=DEV).manual_seed(27)
+    xs = [torch.randn((1000, 2064), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2)]
+    srcs = [torch.randint(-3, 1003, (rows,), generator=g, device=DEV, dtype=torch.int32) for _ in xs]
+    run = lambda x, src: fp8.dequantize(fp8.quantize(x, src), torch.bfloat16)
+    want = [run(x, s) for x, s in zip(xs, srcs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(3):
+        got = []
+        for x, src, s in zip(xs, srcs, streams):
+            with torch.cuda.stream(s):
+                got.append(run(x, src))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for _ in xs:
+        x, src, gr = xs[0].clone(), srcs[0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = run(x, src)
+        graphs.append((gr, x, src, out))
+    for order in ((0, 1), (1, 0)):
+        for (gr, x, src, out), i in zip(graphs, order):
+            x.copy_(xs[i])
+            src.copy_(srcs[i])
+        torch.cuda.synchronize()
+        for (gr, *_), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[i]) for (_, _, _, out), i in zip(graphs, order))
+
+
+@pytest.mark.gpu
 def test_quantize_past_32_bit_offsets():
     rows, cols = 301_000, 7168                    # 2.16e9 values
     x = torch.zeros((rows, cols), dtype=torch.bfloat16, device=DEV)
