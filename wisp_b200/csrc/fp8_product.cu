@@ -95,7 +95,7 @@ struct alignas(64) Params {
   int cap;                // rows per tile at most: a multiple of 32 up to kNarrow, or kWide
   void* out;
   int64_t ld;
-  int wide_out;           // output rows start on 32-byte boundaries
+  int wide_out, even_out;   // output rows start on 32-byte, 4-byte boundaries
   int* error_flag;
 };
 
@@ -252,60 +252,80 @@ WB_DEV bool multiply_scales(const Params& p, const Tile& t, bool wide, int rank,
 
 // A wide tile's outputs: a lane holds a row. 128 bytes of each row at a time change
 // places in the warp's 4 KB of shared memory (16-byte words, swizzled), so that eight
-// lanes write a line of one row. (Straight from the registers, 32 bytes of 32 rows per
-// instruction, the lines pass one a cycle: 8192 x 8192 x 7168 385 us, so 373; 64 experts of
-// 7168 x 2048 with 256 rows and fp32 outputs 300 and 282.)
-template <typename T>
+// lanes write a line of one row, or the whole warp where rows start anywhere. (Straight
+// from the registers, 32 bytes or one value of 32 rows per instruction, the lines pass one
+// a cycle: 8192 x 8192 x 7168 385 us, so 375; 64 experts of 7168 x 2048 with 256 rows and
+// fp32 outputs 300 and 282; 31 experts of 2 x 3754 x 224 with ~150 rows, whose rows start
+// on 4 bytes, 263 and 64.)
+template <bool SWIGLU, typename T>
 WB_DEV void store_wide(const Params& p, const Sums& a, const Tile& t, const Warp& me, uint4* stage) {
   const int row0 = me.rank * 128 + me.quad * 32, rows = min(t.cnt - row0, 32);
   if (rows <= 0) return;
   constexpr int kWord = 16 / (int)sizeof(T), kLine = 8 * kWord;      // values
-  const int r = me.lane >> 3, c = me.lane & 7;
-  T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)row0 + r) * p.ld;
+  constexpr int kType = sizeof(T) == 4 ? WISP_DT_F32
+                                       : std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16;
+  T* out = static_cast<T*>(p.out) + (t.row0 + (int64_t)row0) * p.ld;
 #pragma unroll
-  for (int q = 0; q < 2; q++) {
+  for (int q = 0; q < (SWIGLU ? 1 : 2); q++) {
 #pragma unroll
     for (int l = 0; l < 64; l += kLine) {
       __syncwarp();                      // the last line has been read
 #pragma unroll
       for (int w = 0; w < 8; w++) {
+        float o[kWord];
+#pragma unroll
+        for (int j = 0; j < kWord; j++) {
+          const int i = l + w * kWord + j;
+          const float2 g = a.v[q * 32 + i / 2], u = a.v[32 + i / 2];
+          o[j] = i & 1 ? g.y : g.x;
+          if (SWIGLU) o[j] = swiglu<T>(o[j], i & 1 ? u.y : u.x);
+        }
         uint32_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float* g = reinterpret_cast<const float*>(a.v) + q * 64 + l + w * kWord;
           if constexpr (sizeof(T) == 4)
-            v[j] = __float_as_uint(g[j]);
+            v[j] = __float_as_uint(o[j]);
           else
-            v[j] = pack2(g[2 * j], g[2 * j + 1],
-                         std::is_same<T, __half>::value ? WISP_DT_F16 : WISP_DT_BF16);
+            v[j] = pack2(o[2 * j], o[2 * j + 1], kType);
         }
         stage[me.lane * 8 + (w ^ (me.lane & 7))] = make_uint4(v[0], v[1], v[2], v[3]);
       }
       __syncwarp();
-      const int f = ((t.ft & ~1) + q) * 128 + me.half * 64 + l + c * kWord;
-      T* o = out + f;
+      const int f = (SWIGLU ? t.ft : (t.ft & ~1) + q) * 128 + me.half * 64 + l;
+      if (f >= p.N) return;
+      const int left = p.N - f;          // values of the line that there are
+      if (p.wide_out && left >= kLine) {
+        const int r = me.lane >> 3, c = me.lane & 7;
+        T* o = out + f + r * p.ld + c * kWord;
 #pragma unroll
-      for (int i = 0; i < 32; i += 4, o += 4 * p.ld) {
-        if (r + i >= rows) break;
-        const uint4 v = stage[(r + i) * 8 + (c ^ ((r + i) & 7))];
-        if (p.wide_out && f + kWord <= p.N) {
-          *reinterpret_cast<uint4*>(o) = v;
-        } else {
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-          using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
-          Bits* e = reinterpret_cast<Bits*>(o);
-#pragma unroll
-          for (int j = 0; j < kWord; j++)
-            if (f + j < p.N) e[j] = (Bits)(sizeof(T) == 4 ? u[j] : u[j / 2] >> (16 * (j & 1)));
+        for (int i = 0; i < 32; i += 4, o += 4 * p.ld)
+          if (r + i < rows)
+            *reinterpret_cast<uint4*>(o) = stage[(r + i) * 8 + (c ^ ((r + i) & 7))];
+      } else {
+        using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+        const bool pairs = sizeof(T) == 2 && p.even_out;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(stage) + (me.lane & 3);
+        Bits* o = reinterpret_cast<Bits*>(out + f);
+#pragma unroll 4
+        for (int i = 0; i < rows; i++, o += p.ld) {
+          const uint32_t v = words[i * 32 + 4 * (me.lane / 4 ^ (i & 7))];
+          if constexpr (sizeof(T) == 4) {
+            if (me.lane < left) o[me.lane] = v;
+          } else if (pairs && 2 * me.lane + 1 < left) {
+            *reinterpret_cast<uint32_t*>(o + 2 * me.lane) = v;
+          } else {
+            if (2 * me.lane < left) o[2 * me.lane] = (Bits)v;
+            if (2 * me.lane + 1 < left) o[2 * me.lane + 1] = (Bits)(v >> 16);
+          }
         }
       }
     }
   }
 }
 
-// The same for silu(gate) * up, straight from the registers: half the values, and the
-// shared memory is a stage of the ring (64 experts of 2 x 2048 x 7168 with 256 rows 457 us;
-// through it 467).
+// The same for silu(gate) * up on rows that start on 32 bytes, straight from the
+// registers: half the values, and the shared memory is a stage of the ring (64 experts
+// of 2 x 2048 x 7168 with 256 rows 457 us; through it 467).
 template <typename T>
 WB_DEV void store_wide_swiglu(const Params& p, const Sums& a, const Tile& t, const Warp& me) {
   const int r = me.rank * 128 + me.quad * 32 + me.lane;
@@ -321,7 +341,7 @@ WB_DEV void store_wide_swiglu(const Params& p, const Sums& a, const Tile& t, con
       const float2 g = a.v[(i + j) / 2], u = a.v[32 + (i + j) / 2];
       o[j] = swiglu<T>(j & 1 ? g.y : g.x, j & 1 ? u.y : u.x);
     }
-    if (p.wide_out && f + i + kRun <= p.N) {
+    if (f + i + kRun <= p.N) {
       uint32_t w[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -442,7 +462,9 @@ struct Reduce {
   }
 };
 
-template <typename T, bool SWIGLU, bool PAIR>
+// DIRECT: wide tiles' outputs leave by store_wide_swiglu. (Both forms in one kernel: the
+// 457 us above became 467.)
+template <typename T, bool SWIGLU, bool PAIR, bool DIRECT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_product_kernel(const __grid_constant__ Params p) {
   constexpr int kMats = SWIGLU ? 2 : 1;
@@ -523,7 +545,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
   const int narrow_bytes = kMats * kABytes + narrow_n / (PAIR ? 2 : 1) * 128;
   const int stage_bytes = wides ? max(narrow_bytes, 2 * kABytes) : narrow_bytes;
   constexpr int kRedBytes = kMats * kRedRows * 128 * 4;     // a cluster's partial sums
-  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : wides && !SWIGLU ? kStoreBytes : 0)) / stage_bytes);
+  const int S = min(kMaxStages, (kRingBytes - (ks > 1 ? kRedBytes : wides && !DIRECT ? kStoreBytes : 0)) / stage_bytes);
   // accumulators: buffers of `cols` columns, one for a block of k (gate, then up)
   const int up_offset = (narrow_n + 31) & ~31;
   const int cols = wides ? kWide : up_offset * kMats;
@@ -741,10 +763,10 @@ fp8_product_kernel(const __grid_constant__ Params p) {
       if (!PAIR && ks > 1) {
         ok = red.template store<T>(p, a, t, me, abort);
       } else if (wide) {
-        if constexpr (SWIGLU)
+        if constexpr (DIRECT)
           store_wide_swiglu<T>(p, a, t, me);
         else
-          store_wide<T>(p, a, t, me, stage);
+          store_wide<SWIGLU, T>(p, a, t, me, stage);
       } else {
         store_narrow<SWIGLU, T>(p, a, t, me);
       }
@@ -829,11 +851,11 @@ bool encode_codes(CUtensorMap* m, const void* base, int64_t rows, int k, int box
 }
 
 // grid CTAs in clusters of `cluster`.
-template <typename T, bool SWIGLU, bool PAIR>
+template <typename T, bool SWIGLU, bool PAIR, bool DIRECT>
 WispError launch_kernel(const Params& p, int dev, unsigned grid, int cluster, cudaStream_t stream,
                         WispErrCtx* err) {
   const int smem = kRingBytes + 1024;
-  auto kernel = fp8_product_kernel<T, SWIGLU, PAIR>;
+  auto kernel = fp8_product_kernel<T, SWIGLU, PAIR, DIRECT>;
   static std::atomic<uint64_t> raised{0};
   WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
   cudaLaunchConfig_t cfg = {};
@@ -854,8 +876,12 @@ WispError launch_kernel(const Params& p, int dev, unsigned grid, int cluster, cu
 template <typename T, bool PAIR>
 WispError launch_typed(bool swiglu, const Params& p, int dev, unsigned grid, int cluster,
                        cudaStream_t stream, WispErrCtx* err) {
-  return swiglu ? launch_kernel<T, true, PAIR>(p, dev, grid, cluster, stream, err)
-                : launch_kernel<T, false, PAIR>(p, dev, grid, cluster, stream, err);
+  if constexpr (PAIR) {
+    if (swiglu && p.wide_out && p.cap > kNarrow)
+      return launch_kernel<T, true, true, true>(p, dev, grid, cluster, stream, err);
+  }
+  return swiglu ? launch_kernel<T, true, PAIR, false>(p, dev, grid, cluster, stream, err)
+                : launch_kernel<T, false, PAIR, false>(p, dev, grid, cluster, stream, err);
 }
 
 template <bool PAIR>
@@ -956,6 +982,7 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   p.out = d_out;
   p.ld = ld;
   p.wide_out = !((uintptr_t)d_out & 31) && ld * dt_size(cfg->out_type) % 32 == 0;
+  p.even_out = !((uintptr_t)d_out & 3) && ld * dt_size(cfg->out_type) % 4 == 0;
   p.error_flag = d_error_flag;
   if (split > 1)
     return launch_product<false>(cfg, p, dev, (unsigned)(items * split), split, stream, err);
