@@ -580,6 +580,7 @@ def test_product_split_over_k(swiglu, dtype, n, k, counts):
     (300, 4112, [9, 0, 30]),        # clusters of eight, 33 stages in uneven parts
     (1400, 4096, [1]),
     (60, 5120, [5, 22, 31]),        # one feature tile
+    (250, 4128, [0, 63, 64, 1]),    # around the rows of a tile
 ])
 def test_product_split_over_k_by_eight(swiglu, n, k, counts):
     for dtype in DT.values():
@@ -588,6 +589,22 @@ def test_product_split_over_k_by_eight(swiglu, n, k, counts):
             again = torch.full_like(out, 7.0)
             fp8.product(q, w, dev, out=again)
             assert torch.equal(again[:-3], out[:-3]) and (again[-3:] == 7.0).all()
+        w.check()
+
+
+@pytest.mark.gpu
+@SWIGLU
+@pytest.mark.parametrize("n,k,counts", [
+    (121, 4608, [733]),             # tiles of 61 and 62 rows, by eight
+    (300, 2080, [65, 0, 200, 3]),   # by two, 17 stages
+    (60, 2064, [129, 64, 128]),     # by four
+    (128, 2048, [2900]),
+])
+def test_product_split_over_k_of_many_rows(swiglu, n, k, counts):
+    for dtype in DT.values():
+        q, w, mats, segs, dev, out = _run_product(swiglu, dtype, n, k, counts)
+        for _ in range(3):
+            assert torch.equal(fp8.product(q, w, dev, dtype=dtype), out)
         w.check()
 
 

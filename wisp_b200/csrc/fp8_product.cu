@@ -387,7 +387,7 @@ WB_DEV void store_narrow(const Params& p, const Sums& a, const Tile& t, const Wa
   }
 }
 
-// The join of a cluster whose CTAs split K (narrow tiles of at most 64 rows).
+// The join of a cluster whose CTAs split K (tiles of at most 64 rows).
 // 16 rows of each half at a time, every CTA puts its sums into its shared memory, and CTA kp
 // adds those of all, in the order of K, for the rows kp, kp + ks, ... (a warp per
 // row, 4 features per lane).
@@ -938,19 +938,21 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
     return most < x->rows ? most : x->rows;
   };
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 127) / 128;
-  const int64_t items = tiles_of(kNarrow) * ftiles;
-  // Few tiles of few rows: clusters of 8, 4 or 2 CTAs split K, as long as they fill 3/4
-  // of the SMs (at one CTA an SM, more of them do not fit the GPCs in one wave) and each
-  // has enough of K. One row, us, by half as many / by the rule's: gate/up 1536 x 7168 (12
-  // tiles) 12.7 / 10.5; 2048 x 7168 (16 tiles) by 4 9.9, by 8 in two waves 15.6.
-  const int split = nk < 16 || x->rows > kSplitRows    ? 1
+  const int64_t items = tiles_of(kSplitRows) * ftiles;
+  // Few tiles: clusters of 8, 4 or 2 CTAs split K, as long as they fill 3/4 of the SMs
+  // (at one CTA an SM, more of them do not fit the GPCs in one wave) and each has enough
+  // of K. One row, us, by half as many / by the rule's: gate/up 1536 x 7168 (12 tiles) 12.7 /
+  // 10.5; 2048 x 7168 (16 tiles) by 4 9.9, by 8 in two waves 15.6. More rows as tiles of 64,
+  // as pairs / split: 100 rows of 256 x 7168 23.7 / 12.8, of 2048 x 7168 24.1 / 18.8, of
+  // gate/up 1536 x 2048 15.9 / 13.8; 3000 rows of 128 x 7168 23.9 / 19.0.
+  const int split = nk < 16                            ? 1
                     : nk >= 32 && items * 32 <= 3 * (int64_t)sms ? 8
                     : items * 16 <= 3 * (int64_t)sms ? 4
                     : items * 8 <= 3 * (int64_t)sms  ? 2
                                                      : 1;
   // With one feature tile a pair's second CTA would have none: single CTAs.
   const bool single = split == 1 && ftiles == 1;
-  int cap = split > 1 || single ? kNarrow : kWide;
+  int cap = split > 1 ? kSplitRows : single ? kNarrow : kWide;
   if (split == 1) {
     // Smaller tiles when the largest would leave SMs without work: as many rows
     // as give every CTA one tile if the rows lay in one segment, at least 64.
