@@ -141,6 +141,28 @@ def test_logits_a_few_roundings_apart(scoring, base):
 
 @pytest.mark.gpu
 @SCORING
+@pytest.mark.parametrize("size", [3.0, 100.0, 2.0 ** 20, 3.0e38])
+def test_groups_of_large_biases_that_cancel(scoring, size):
+    """The two best choices of a group are a large bias and its negative, so that its sum is that of
+    the scores, which fp32 has lost."""
+    g = torch.Generator(device=DEV).manual_seed(13)
+    x = torch.randn((256, 8, 5), generator=g, device=DEV) * 0.5
+    x[:, :, 1] = x[:, :, 0]
+    # the groups beside them: one score up and one down, by nearly the same
+    d, e = torch.randn((2, 256, 4), generator=g, device=DEV)
+    x[:, 1::2, 0] = x[:, ::2, 0] + d * 2.0 ** -16
+    x[:, 1::2, 1] = x[:, ::2, 1] - d * 2.0 ** -16 + e * 2.0 ** -21
+    bias = torch.full((8, 5), -3.2e38, device=DEV)
+    bias[:, 0], bias[:, 1] = size, -size
+    # one group whose sum is larger than fp32's range holds
+    if size > 1e38:
+        bias[6, 1] = size
+    for kept in (1, 3, 4):
+        _check(x.reshape(256, 40), 2, scoring, bias.reshape(40), n_groups=8, topk_groups=kept)
+
+
+@pytest.mark.gpu
+@SCORING
 def test_values_that_cannot_be_chosen(scoring):
     """-infinite logits and biases, NaN, infinities, extreme logits, rows with too few experts left
     or none."""

@@ -262,12 +262,12 @@ WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
 // The result is that of 64-bit scores and choices (route_exact), found in 32 bits
 // where that decides it. The quick exponential of x is off by 2 + 1.2 |x| ulp, which
 // makes at most 1.5 * 2^-23 of a sigmoid s (s (1 - s) |x| < 0.23) and, with a sum and
-// the quick reciprocal, 7 * 2^-24; a choice rounds by 2^-24 of itself more, so two
-// that differ by 2^-20 * max(1, |choice|) are in order. A softmax score is off by
-// 9 * 2^-24 (e^-x x < 0.37) and, with all of the token's, by the sum's error of at
-// most 43 * 2^-24: there it takes 2^-18. Without a bias the scores are in the
-// logits' order, which needs no scores at all: equal logits are ties, and those 2^-20
-// apart have different 64-bit scores as long as these are not near 1 (logits above
+// the quick reciprocal, 7 * 2^-24: 2^-21 covers it. A softmax score is off by 9 * 2^-24 of
+// the largest score (e^-x x < 0.37) and by the sum's error of at most 43 * 2^-24 of itself:
+// 2^-18 of the largest. Adding the bias rounds by 2^-24 of the choice, the sum of two choices
+// by as much, and the comparison again: 2^-22 of each choice. Without a bias the scores
+// are in the logits' order, which needs no scores at all: equal logits are ties, and
+// those 2^-20 apart have different 64-bit scores as long as these are not near 1 (logits above
 // 16) or 0 (logits, from the largest on for softmax, below -700). Only a token with a
 // closer pair where it matters, or with a value that is not finite, goes the 64-bit
 // way. (A softmax whose weights are not renormalised needs the 64-bit sum over all
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, shfl_xor(mx, o));
   // what the experts are ordered by, as keys
   const bool scores = p.bias || (grouped && p.group_top > 1);
+  float top = 1.f;                   // the largest score of a softmax
   uint32_t key[PER];
   if (scores) {
     float s[PER], sum = 0.f;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     if (softmax) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += shfl_xor(sum, o);
-      sum = rcp_approx(sum);
+      sum = top = rcp_approx(sum);
     }
 #pragma unroll
     for (int j = 0; j < PER; j++) s[j] = softmax ? s[j] * sum : rcp_approx(1.f + s[j]);
@@ -333,13 +334,15 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     }
   }
   bool sure = __all_sync(0xffffffffu, span == 0.f) && (scores || softmax || mx <= 16.f);
-  const float margin = scores && softmax ? 3.814697265625e-6f : 9.5367431640625e-7f;   // 2^-18, -20
-  const float least = scores ? -INFINITY : softmax ? mx - 700.f : -700.f;
-  // Whether a > b is beyond doubt, or both are the same for certain; `of`: how many
-  // scores they are sums of.
-  auto apart = [&](float a, float b, float of) {
+  // How far a choice may be off (with scores), see above.
+  const float off = softmax ? 3.814697265625e-6f * top : 4.76837158203125e-7f;   // 2^-18, 2^-21
+  auto err = [&](float c) { return off + 2.384185791015625e-7f * fabsf(c); };
+  const float least = softmax ? mx - 700.f : -700.f;
+  // Whether a > b is beyond doubt, or (without scores) both are the same for certain.
+  auto apart = [&](float a, float b) {
     const float d = a - b;
-    return a >= least && (d >= of * margin * fmaxf(1.f, fabsf(a)) || (d == 0.f && !scores));
+    if (scores) return d > err(a) + err(b);
+    return a >= least && (d >= 9.5367431640625e-7f * fmaxf(1.f, fabsf(a)) || d == 0.f);   // 2^-20
   };
   if (grouped && sure) {
     __syncwarp();
@@ -354,11 +357,12 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     }
     const bool head = g < p.groups && lane % L == 0, kept = head && rank < p.kept;
     const uint32_t keep = __ballot_sync(0xffffffffu, kept);
-    // the worst that is kept against the best that is not
-    const uint32_t sk = order_key(s);
-    const float worst = key_value(__reduce_min_sync(0xffffffffu, kept ? sk : 0xffffffffu));
-    const float next = key_value(__reduce_max_sync(0xffffffffu, head && !kept ? sk : 0u));
-    sure = apart(worst, next, (float)p.group_top);
+    // the worst that is kept, at its lowest, against the best that is not, at its highest
+    // (two choices of opposite signs leave a sum that is smaller than what they are off by)
+    const float e = !scores ? 0.f : p.group_top > 1 && p.gsz > 1 ? err(a) + err(b) : err(a);
+    const float worst = key_value(__reduce_min_sync(0xffffffffu, kept ? order_key(s - e) : 0xffffffffu));
+    const float next = key_value(__reduce_max_sync(0xffffffffu, head && !kept ? order_key(s + e) : 0u));
+    sure = scores ? worst > next : apart(worst, next);
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       const int e = lane + 32 * j;
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const Params p) {
     const uint32_t best = take_best(key, lane, e);
     if (best == 0) break;          // (all of the kept groups' experts are taken)
     const float c = key_value(best);
-    if (r > 0) sure = apart(last, c, 1.f);
+    if (r > 0) sure = apart(last, c);
     last = c;
     if (lane == r && r < p.k) mine = (int)e;
   }
