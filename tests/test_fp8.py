@@ -323,6 +323,23 @@ def test_quantize_and_back_many_rows(dtype, rows, cols):
 
 
 @pytest.mark.gpu
+@POW2
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows,cols", [(80_003, 16), (75_777, 144), (30_011, 272), (9_473, 1024),
+                                       (5_000, 2048)])
+def test_short_rows_several_to_a_block(pow2, dtype, rows, cols):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x = torch.randn((rows, cols), generator=g, device=DEV).to(DT[dtype])
+    q = _check_quantize(x, pow2)
+    assert torch.equal(fp8.dequantize(q, DT[dtype]).double(),
+                       ref.row_values(q.codes, q.scales).float().to(DT[dtype]).double())
+    src = torch.randint(0, rows, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    got = fp8.gather(q, src)
+    assert torch.equal(got.codes.view(torch.uint8), q.codes.view(torch.uint8)[src.long()])
+    assert torch.equal(got.scales, q.scales[src.long()])
+
+
+@pytest.mark.gpu
 def test_dequantize_scales_of_any_strides():
     g = torch.Generator(device=DEV).manual_seed(20)
     for rows in (7, 3000):

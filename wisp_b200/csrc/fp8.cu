@@ -33,10 +33,25 @@ constexpr float kTop = 448.f;
 constexpr float kTiny = 1e-30f, kRaise = 1.2676506002282294e30f;     // 2^100
 constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
 
-// A row of `units` threads split over equal CTAs of at most 256.
-int row_threads(int units) {
-  const int blocks = (units + 255) / 256;
-  return ((units + blocks - 1) / blocks + 31) / 32 * 32;
+// How `rows` rows of `cols` values lie over the grid, at R rows per thread: a row's
+// threads over equal CTAs of at most 256, or, of short rows, several in one CTA as long as
+// that leaves four CTAs an SM (100,000 bf16 rows of 64, us: quantise 23.6 -> 9.6, back 27.3 ->
+// 4.6; 65,536 of 128: 17.3 -> 8.0, 18.5 -> 4.1).
+struct Layout {
+  dim3 grid, block;
+};
+Layout layout_rows(int rows, int cols, int R) {
+  const int units = (cols + kBlock - 1) / kBlock * kLanes;
+  for (int k = 256 / units; k > 1; k--)
+    if (units * k % 32 == 0 && rows >= (int64_t)148 * 4 * R * k)
+      return {dim3(((int64_t)rows + R * k - 1) / (R * k)), dim3(units, k)};
+  const int parts = (units + 255) / 256;
+  const int threads = ((units + parts - 1) / parts + 31) / 32 * 32;
+  return {dim3(((int64_t)rows + R - 1) / R, (units + threads - 1) / threads), dim3(threads)};
+}
+// Several rows per thread once there are enough to fill the GPU all the same.
+bool many_rows(int rows, int cols, int R) {
+  return (int64_t)rows * layout_rows(1, cols, 1).grid.y >= 148 * 8 * R;
 }
 
 // 16 values of one thread as they lie in memory.
@@ -209,13 +224,13 @@ struct QuantParams {
   int wide;   // rows of x start on 32-byte boundaries
 };
 
-// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): one thread per 16 values of R
-// rows, 32 (16-bit types) or 64 (fp32) bytes read and 16 written for each; the R
+// layout_rows: one thread per 16 values of R rows, 32 (16-bit types) or 64 (fp32)
+// bytes read and 16 written for each; the R
 // rows' loads are issued together. Lane i of a block's eight writes the scale of
 // row i, so that scales stored block by block go out 4 R bytes at a time.
 template <bool POW2, typename T, int R>
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
-  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
   const int units = p.cols / kUnit;
   const bool in = u < units;
@@ -254,14 +269,11 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
 
 template <bool POW2, typename T>
 void launch_quantize(const QuantParams& p, cudaStream_t st) {
-  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
-  const int gy = (units + threads - 1) / threads;
   constexpr int R = sizeof(T) == 4 ? 2 : 4;
-  // Several rows per thread once there are enough to fill the GPU all the same.
-  if ((int64_t)p.rows * gy >= 148 * 8 * R)
-    wb::launch_k(quantize_kernel<POW2, T, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
-  else
-    wb::launch_k(quantize_kernel<POW2, T, 1>, dim3(p.rows, gy), threads, 0, st, p);
+  const bool many = many_rows(p.rows, p.cols, R);
+  const Layout l = layout_rows(p.rows, p.cols, many ? R : 1);
+  wb::launch_k(many ? quantize_kernel<POW2, T, R> : quantize_kernel<POW2, T, 1>, l.grid, l.block, 0,
+               st, p);
 }
 
 template <bool POW2>
@@ -335,11 +347,11 @@ WB_DEV float2 e4m3_values(uint32_t two) {
   return __half22float2(u2h2(h));
 }
 
-// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 values of R rows per
-// thread. code * scale is rounded to fp32, then to the output's type.
+// layout_rows: 16 values of R rows per thread. code * scale is rounded to fp32, then to
+// the output's type.
 template <int TYPE, int R>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
-  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
   const bool in = u < p.cols / kUnit;
   const int lane = u & (kLanes - 1), b = u / kLanes;
@@ -402,13 +414,11 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) 
 
 template <int TYPE>
 void launch_dequantize(const DequantParams& p, cudaStream_t st) {
-  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
-  const int gy = (units + threads - 1) / threads;
   constexpr int R = 2;
-  if ((int64_t)p.rows * gy >= 148 * 8 * R)
-    wb::launch_k(dequantize_kernel<TYPE, R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
-  else
-    wb::launch_k(dequantize_kernel<TYPE, 1>, dim3(p.rows, gy), threads, 0, st, p);
+  const bool many = many_rows(p.rows, p.cols, R);
+  const Layout l = layout_rows(p.rows, p.cols, many ? R : 1);
+  wb::launch_k(many ? dequantize_kernel<TYPE, R> : dequantize_kernel<TYPE, 1>, l.grid, l.block, 0,
+               st, p);
 }
 
 struct GatherParams {
@@ -423,13 +433,13 @@ struct GatherParams {
   int64_t o_row, o_block;
 };
 
-// grid (ceil(rows / R), ceil(cols / 16 / blockDim)): 16 codes of R rows per thread.
+// layout_rows: 16 codes of R rows per thread.
 // Lane i of a block's eight moves the scale of row i, so that scales stored block by
 // block go out 4 R bytes at a time. 32,768 of 4096 rows of 7168 take 54 us, of which
 // the 242 MB that are written are 37 at the copy rate.
 template <int R>
 __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
-  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
   const int u = blockIdx.y * blockDim.x + threadIdx.x;
   const bool in = u < p.cols / kUnit;
   uint4 c[R];
@@ -453,13 +463,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
 }
 
 void launch_gather(const GatherParams& p, cudaStream_t st) {
-  const int units = (p.cols + kBlock - 1) / kBlock * kLanes, threads = row_threads(units);
-  const int gy = (units + threads - 1) / threads;
   constexpr int R = 8;
-  if ((int64_t)p.rows * gy >= 148 * 8 * R)
-    wb::launch_k(gather_kernel<R>, dim3((p.rows + R - 1) / R, gy), threads, 0, st, p);
-  else
-    wb::launch_k(gather_kernel<1>, dim3(p.rows, gy), threads, 0, st, p);
+  const bool many = many_rows(p.rows, p.cols, R);
+  const Layout l = layout_rows(p.rows, p.cols, many ? R : 1);
+  wb::launch_k(many ? gather_kernel<R> : gather_kernel<1>, l.grid, l.block, 0, st, p);
 }
 
 }  // namespace
