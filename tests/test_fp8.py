@@ -177,6 +177,15 @@ def test_python_refusals():
         fp8.quantize(x.clone().requires_grad_())
 
 
+def test_scales_that_require_a_gradient_are_refused():
+    codes = torch.zeros((2, 32), dtype=torch.uint8)
+    for make in (lambda s: fp8.Fp8Rows(codes, s), lambda s: fp8.Fp8Weights(codes[None], s[None, :1])):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*gradient"):
+            make(torch.ones((2, 1), requires_grad=True))
+    with torch.no_grad():
+        assert fp8.Fp8Rows(codes, torch.ones((2, 1), requires_grad=True)).rows == 2
+
+
 # ---------------------------------------------------------------------------
 # Quantisation
 # ---------------------------------------------------------------------------

@@ -58,6 +58,8 @@ class Fp8Rows:
         if scales.dtype != torch.float32 or scales.shape != (self.rows, _blocks(self.cols)):
             raise invalid(f"scales: float32 {(self.rows, _blocks(self.cols))}, not {scales.dtype} "
                           f"{tuple(scales.shape)}")
+        if wants_grad(scales):
+            refuse_grad()
         same_device(codes, scales=scales)
         self._buf = self._codes_view = codes
         self._scales_view = scales
