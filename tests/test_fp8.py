@@ -380,6 +380,22 @@ def test_gather(cols, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [70_001, 1_050_001], ids=["past the L2 cache", "past 32-bit offsets"])
+def test_gather_of_large_results(rows):
+    g = torch.Generator(device=DEV).manual_seed(28)
+    q = fp8.quantize(torch.randn((700, 2064), generator=g, device=DEV))
+    src = torch.randint(0, 702, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    got = fp8.gather(q, src)
+    for r0 in (0, rows // 2, rows - 5000):
+        at, s = slice(r0, r0 + 5000), src[r0:r0 + 5000].long()
+        inside = (s < 700)[:, None]
+        s = s.clamp(max=699)
+        assert torch.equal(got.codes.view(torch.uint8)[at],
+                           torch.where(inside, q.codes.view(torch.uint8)[s], 0))
+        assert torch.equal(got.scales[at], torch.where(inside, q.scales[s], 0.0))
+
+
+@pytest.mark.gpu
 def test_gather_of_no_rows_gives_zeros():
     q = fp8.quantize(torch.ones((0, 64), device=DEV))
     for m in (5, 2 ** 19):             # (the second as a quantise of many rows does it)

@@ -431,12 +431,14 @@ struct GatherParams {
   uint8_t* out;
   float* out_scales;
   int64_t o_row, o_block;
+  int past_l2;       // the result is larger than the L2 cache
 };
 
 // layout_rows: 16 codes of R rows per thread.
 // Lane i of a block's eight moves the scale of row i, so that scales stored block by
-// block go out 4 R bytes at a time. 32,768 of 4096 rows of 7168 take 54 us, of which
-// the 242 MB that are written are 37 at the copy rate.
+// block go out 4 R bytes at a time. 32,768 of 4096 rows of 7168 take 49 us, of which
+// the 242 MB that are written are 37 at the copy rate (without the hint that what the L2
+// cannot hold need not stay there: 55).
 template <int R>
 __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   const int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * R;
@@ -458,8 +460,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
   }
 #pragma unroll
   for (int i = 0; i < R; i++)
-    if (in && row0 + i < p.rows)
-      reinterpret_cast<uint4*>(p.out + (row0 + i) * p.cols)[u] = c[i];
+    if (in && row0 + i < p.rows) {
+      uint4* o = reinterpret_cast<uint4*>(p.out + (row0 + i) * p.cols) + u;
+      if (p.past_l2)
+        __stcs(o, c[i]);
+      else
+        *o = c[i];
+    }
 }
 
 void launch_gather(const GatherParams& p, cudaStream_t st) {
@@ -579,7 +586,7 @@ extern "C" WispError wisp_b200_fp8_gather(const WispFp8Rows* x, const int* d_src
     return WB_FAIL(WISP_ERR_INVALID_ARG,
                    "fp8_gather: codes must be 16-byte, scales and d_src 4-byte aligned");
   launch_gather({x->codes, x->scales, x->scale_row, x->scale_block, x->rows, d_src, rows, cols,
-                 d_codes, d_scales, scale_row, scale_block},
+                 d_codes, d_scales, scale_row, scale_block, (int64_t)rows * cols > 1 << 27},
                 stream);
   WB_CUDA_CHECK(cudaGetLastError());
   return WISP_OK;
