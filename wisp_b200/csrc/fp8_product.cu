@@ -29,12 +29,12 @@
 // memory), and a buffer is free as soon as it has been read, before the last of it is
 // added.
 //
-// Measured (L2 flushed; us): 64 experts of 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows
-// each 297 / 308 / 344 / 455, where the weights take 287 at the copy rate; 64 of 7168 x
-// 2048 175 / 195 / 225 / 282 (143): bound by HBM up to ~100 rows. 8192 x 8192 x 7168 375
-// = 2.57 PFLOP/s; without a pause between calls 470, as the power limit lowers the
-// clock. A block of a wide tile takes 0.44 us (0.27 at the MMAs' nominal rate), a change
-// of tiles 2.5 more.
+// Measured (us; L2 flushed by writes, whose way back to memory costs ~20): 64 experts of
+// 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows each 297 / 308 / 344 / 455, where the
+// weights take 287 at the copy rate; 64 of 7168 x 2048 175 / 195 / 225 / 282 (143): bound
+// by HBM up to ~100 rows. 8192 x 8192 x 7168 375 = 2.57 PFLOP/s; without a pause between
+// calls 470, as the power limit lowers the clock. A block of a wide tile takes 0.44 (0.27
+// at the MMAs' nominal rate), a change of tiles 2.5 more.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
