@@ -373,15 +373,16 @@ WB_DEV void store_narrow(const Params& p, const Sums& a, const Tile& t, const Wa
       T* q = out + c * ld;
 #pragma unroll
       for (int i = 0; i < 32; i++, q += ld) {
-        if (c + i < t.cnt) {
-          const float2 g = a.v[j * 16 + i / 2];
-          float o = i & 1 ? g.y : g.x;
-          if (SWIGLU) {
-            const float2 u = a.v[32 + j * 16 + i / 2];
-            o = swiglu<T>(o, i & 1 ? u.y : u.x);
-          }
-          put_out(q, o);
+        // (out of the unrolled code at once: walking past it, from cold instructions, is
+        // 1 us of a call with one row: gate/up 2048 x 1024 10.3, so 9.3)
+        if (c + i >= t.cnt) break;
+        const float2 g = a.v[j * 16 + i / 2];
+        float o = i & 1 ? g.y : g.x;
+        if (SWIGLU) {
+          const float2 u = a.v[32 + j * 16 + i / 2];
+          o = swiglu<T>(o, i & 1 ? u.y : u.x);
         }
+        put_out(q, o);
       }
     }
   }
