@@ -637,12 +637,18 @@ def test_product_split_over_k_by_eight(swiglu, n, k, counts):
 @pytest.mark.gpu
 @SWIGLU
 @pytest.mark.parametrize("n,k,counts", [
-    (121, 4608, [733]),             # tiles of 61 and 62 rows, by eight
-    (300, 2080, [65, 0, 200, 3]),   # by two, 17 stages
-    (60, 2064, [129, 64, 128]),     # by four
+    (121, 4608, [733]),             # tiles of 61 and 62 rows
+    (300, 2080, [65, 0, 200, 3]),   # 17 stages
+    (60, 2064, [129, 64, 128]),
     (128, 2048, [2900]),
+    (4700, 2064, [9]),              # by three
+    (2300, 2320, [20, 50]),
+    (3100, 2576, [2]),              # by five
+    (2000, 4000, [3]),              # by six, 32 stages
+    (1100, 3616, [1]),              # by seven, 29 stages
+    (7000, 2064, [16]),             # by two, 55 feature tiles
 ])
-def test_product_split_over_k_of_many_rows(swiglu, n, k, counts):
+def test_product_split_over_k_by_any_number(swiglu, n, k, counts):
     for dtype in DT.values():
         q, w, mats, segs, dev, out = _run_product(swiglu, dtype, n, k, counts)
         for _ in range(3):

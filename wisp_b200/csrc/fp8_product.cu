@@ -895,6 +895,31 @@ WispError launch_product(const WispFp8Config* c, const Params& p, int dev, unsig
   return launch_typed<__half, PAIR>(c->swiglu, p, dev, grid, cluster, stream, err);
 }
 
+// Clusters of `size` single CTAs that run at once on device dev. (Asked once per device
+// and size; the kernel's forms all take the same registers and shared memory.)
+WispError cluster_room(int dev, int size, int* room, WispErrCtx* err) {
+  static std::atomic<int> known[64][9];
+  const bool keep = dev >= 0 && dev < 64;
+  if (keep && (*room = known[dev][size].load(std::memory_order_relaxed)) > 0) return WISP_OK;
+  auto kernel = fp8_product_kernel<__nv_bfloat16, false, false, false>;
+  const int smem = kRingBytes + 1024;
+  static std::atomic<uint64_t> raised{0};
+  WB_CUDA_CHECK(wb::raise_smem(kernel, smem, dev, raised));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  WB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(room, kernel, &cfg));
+  if (keep) known[dev][size].store(*room, std::memory_order_relaxed);
+  return WISP_OK;
+}
+
 WispError check_mats(const WispFp8Mats* m, const char* what, WispErrCtx* err) {
   if (!m || !m->codes || !m->scales)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: null pointer argument (%s)", what);
@@ -940,17 +965,24 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   };
   const int ftiles = (cfg->n + 127) / 128, nk = (cfg->k + 127) / 128;
   const int64_t items = tiles_of(kSplitRows) * ftiles;
-  // Few tiles: clusters of 8, 4 or 2 CTAs split K, as long as they fill 3/4 of the SMs
-  // (at one CTA an SM, more of them do not fit the GPCs in one wave) and each has enough
-  // of K. One row, us, by half as many / by the rule's: gate/up 1536 x 7168 (12 tiles) 12.7 /
-  // 10.5; 2048 x 7168 (16 tiles) by 4 9.9, by 8 in two waves 15.6. More rows as tiles of 64,
-  // as pairs / split: 100 rows of 256 x 7168 23.7 / 12.8, of 2048 x 7168 24.1 / 18.8, of
-  // gate/up 1536 x 2048 15.9 / 13.8; 3000 rows of 128 x 7168 23.9 / 19.0.
-  const int split = nk < 16                            ? 1
-                    : nk >= 32 && items * 32 <= 3 * (int64_t)sms ? 8
-                    : items * 16 <= 3 * (int64_t)sms ? 4
-                    : items * 8 <= 3 * (int64_t)sms  ? 2
-                                                     : 1;
+  // Few tiles: clusters of up to 8 CTAs split K, the largest that all run at once (one CTA
+  // an SM; a GPC's SMs past the last whole cluster hold none: 74, 45, 33, 26, 22, 15 and 15
+  // clusters of 2 to 8) with at least four blocks each. One row, us, as pairs / split:
+  // 7168 x 7168 21.1 / 14.2 (by two); by half as many or fewer / so: 2048 x 7168 10.2 / 9.5
+  // (six), 4096 x 7168 14.0 / 10.7 (four), 7168 x 2048 10.1 / 8.8 (two). 100 rows as pairs / as
+  // tiles of 64: 256 x 7168 23.7 / 12.8, 2048 x 7168 24.1 / 14.9, gate/up 1536 x 2048 15.9 /
+  // 13.8; 3000 rows of 128 x 7168 23.9 / 19.0. (Where many segments make the bound on tiles
+  // too large it may be too few: 8 of 512 x 2048 with 64 rows 11.0 as pairs, 11.8 by two.)
+  int split = 1;
+  if (nk >= 16) {
+    for (int k = 8; k > 1 && split == 1; k--) {
+      int room = 0;
+      if (nk >= 4 * k && items * k <= sms) {
+        if ((e = cluster_room(dev, k, &room, err)) != WISP_OK) return e;
+        if (items <= room) split = k;
+      }
+    }
+  }
   // With one feature tile a pair's second CTA would have none: single CTAs.
   const bool single = split == 1 && ftiles == 1;
   int cap = split > 1 ? kSplitRows : single ? kNarrow : kWide;
