@@ -3,6 +3,9 @@ definition in 64 bits; refusals on the CPU."""
 from __future__ import annotations
 
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -908,6 +911,28 @@ def test_product_on_streams_and_in_graphs():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
     w.check()
+
+
+@pytest.mark.gpu
+def test_first_calls_in_a_capture():
+    """A process whose first calls are captured: what is asked of the device once is asked then."""
+    code = """
+import torch
+from wisp_b200 import fp8, routing
+codes = torch.randint(0, 120, (1, 2048, 4096), device="cuda", dtype=torch.uint8)
+w = fp8.Fp8Weights(codes, torch.rand((1, 16, 32), device="cuda"))
+x, l = torch.randn((1, 4096), device="cuda"), torch.randn((4, 64), device="cuda")
+run = lambda: (fp8.product(fp8.quantize(x), w), *routing.select_experts(l, 4))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+w.check()
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], cwd=root, check=True, timeout=300)
 
 
 @pytest.mark.gpu

@@ -491,7 +491,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     tma_prefetch_desc(&p.tm_w);
     tma_prefetch_desc(&p.tm_x);
     if (SWIGLU) tma_prefetch_desc(&p.tm_up);
-    if (PAIR) tma_prefetch_desc(&p.tm_x128);
+    if (PAIR && p.cap > kNarrow) tma_prefetch_desc(&p.tm_x128);
   }
   __syncwarp();
   if (tid < kMaxStages) {
@@ -1000,7 +1000,7 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   if (!encode_codes(&p.tm_w, w->codes, wrows, cfg->k, 128) ||
       (cfg->swiglu && !encode_codes(&p.tm_up, up->codes, wrows, cfg->k, 128)) ||
       !encode_codes(&p.tm_x, x->codes, x->rows, cfg->k, 16) ||
-      !encode_codes(&p.tm_x128, x->codes, x->rows, cfg->k, 128))
+      (cap > kNarrow && !encode_codes(&p.tm_x128, x->codes, x->rows, cfg->k, 128)))
     return WB_FAIL(WISP_ERR_CUDA, "fp8_product: cuTensorMapEncodeTiled failed");
   p.ws_w = w->scales;
   p.ws_up = cfg->swiglu ? up->scales : nullptr;
