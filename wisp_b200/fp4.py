@@ -3,8 +3,8 @@
 Thin wrappers over the C ABI (include/wisp_b200.h): tensors are PyTorch CUDA
 tensors used as device memory; every launch goes on the current torch stream
 of the tensors' device. The work itself runs in libwisp_b200.so. For serving: no
-operator has a gradient, and tensors that require one are refused where autograd
-would record the call.
+operator has a gradient or a tangent, and tensors that require or carry one are refused
+where autograd would follow the call.
 
     q = quantize(x, abi.WISP_FP4_MX)                # rows -> codes and scales
     w = Fp4Weights(abi.WISP_FP4_MX, codes, scales)  # [V, n, k/2], [V, n, k/32]
@@ -16,6 +16,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import abi
 
@@ -56,17 +57,21 @@ def dtype_code(dtype: torch.dtype, what: str) -> int:
 
 
 def wants_grad(*tensors: torch.Tensor | None) -> bool:
-    """Whether autograd would expect a gradient for one of the tensors."""
+    """Whether autograd would expect a gradient for one of the tensors, or a tangent from it."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:       # (forward mode goes on under torch.no_grad())
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False
 
 
 def refuse_grad() -> None:
-    raise invalid("a tensor requires a gradient, and this operator has none (torch.no_grad() or "
-                  "detach() for serving)")
+    raise invalid("a tensor requires a gradient or has a tangent, and this operator has neither "
+                  "(for serving: torch.no_grad() for gradients, detach() for both)")
 
 
 def row_stride(t: torch.Tensor, what: str) -> int:

@@ -3,8 +3,8 @@
 Thin wrappers over the C ABI (include/wisp_b200.h): tensors are PyTorch CUDA
 tensors used as device memory; every launch goes on the current torch stream
 of the tensors' device. The work itself runs in libwisp_b200.so. For serving: no
-operator has a gradient, and tensors that require one are refused where autograd
-would record the call.
+operator has a gradient or a tangent, and tensors that require or carry one are refused
+where autograd would follow the call.
 
     q = quantize(x)                       # rows -> codes, a scale per 128 values
     q = gather(q, rows)                   # the rows of each expert's tokens

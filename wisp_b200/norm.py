@@ -56,7 +56,7 @@ def block_norm(x: torch.Tensor, y: torch.Tensor | None = None, *,
     post=False) and pre_norm alike. gate: [hidden], [tokens, 1] or [tokens, hidden]; the two
     weights share a dtype. x' has x's dtype (x_out may be x itself), n has ``dtype``; n is None
     with pre=False. There is no gradient: under grad mode tensors that require one (parameters
-    among them) are refused."""
+    among them) are refused, and so are those with a tangent."""
     # (One pass over the arguments: at a few rows this function takes longer than its kernel.)
     if wants_grad(x, y, gate, post_weight, pre_weight, x_out, n_out):
         refuse_grad()

@@ -47,7 +47,7 @@ def select_experts(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | Non
 
     Computed in 64 bits; ties go to the lower index. NaN and -infinite choices are never taken;
     slots without an expert have idx -1 and weight 0. No gradient: tensors that require one are
-    refused under grad mode."""
+    refused under grad mode, and those with a tangent."""
     if wants_grad(logits, bias):
         refuse_grad()
     ld = row_stride(logits, "logits")
