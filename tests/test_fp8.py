@@ -189,6 +189,17 @@ def test_scales_that_require_a_gradient_are_refused():
         assert fp8.Fp8Rows(codes, torch.ones((2, 1), requires_grad=True)).rows == 2
 
 
+def test_codes_that_require_a_gradient_are_refused():
+    codes = torch.zeros((2, 32), dtype=torch.float8_e4m3fn, requires_grad=True)
+    plain, s = codes.detach(), torch.ones((2, 1))
+    for make in (lambda c: fp8.Fp8Rows(c, s), lambda c: fp8.Fp8Weights(c[None], s[None, :1]),
+                 lambda c: fp8.Fp8Weights(plain[None], s[None, :1], up=(c[None], s[None, :1]))):
+        with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*gradient"):
+            make(codes)
+    with torch.no_grad():
+        assert fp8.Fp8Rows(codes, s).rows == 2
+
+
 # ---------------------------------------------------------------------------
 # Quantisation
 # ---------------------------------------------------------------------------

@@ -58,7 +58,7 @@ class Fp8Rows:
         if scales.dtype != torch.float32 or scales.shape != (self.rows, _blocks(self.cols)):
             raise invalid(f"scales: float32 {(self.rows, _blocks(self.cols))}, not {scales.dtype} "
                           f"{tuple(scales.shape)}")
-        if wants_grad(scales):
+        if wants_grad(codes, scales):
             refuse_grad()
         same_device(codes, scales=scales)
         self._buf = self._codes_view = codes
@@ -193,7 +193,7 @@ class Fp8Weights:
             want = (self.entries, _blocks(self.n), _blocks(self.k))
             if s.dtype != torch.float32 or s.shape != want or not s.is_contiguous():
                 raise invalid(f"weight scales: contiguous float32 {want}")
-            if wants_grad(s):
+            if wants_grad(c, s):
                 refuse_grad()
             same_device(codes, codes=c, scales=s)
             self._keep.append((c, s))
