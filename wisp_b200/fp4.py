@@ -149,6 +149,10 @@ class Fp4Rows:
         q._ts = None if tensor_scale is None else tensor_scale.data_ptr()
         return q
 
+    def __reduce__(self):
+        # (copies and pickles are made anew from their own tensors: the addresses are of these)
+        return Fp4Rows, (self.fmt, self.codes, self.scales, self.tensor_scale)
+
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """As torch.Tensor.record_stream: the rows are in use on `stream` too."""
         for t in (self._buf, *(self._views or ()), self.tensor_scale):

@@ -81,6 +81,10 @@ class Fp8Rows:
         q.rows, q.cols = rows, cols
         return q
 
+    def __reduce__(self):
+        # (copies and pickles are made anew from their own tensors: the addresses are of these)
+        return Fp8Rows, (self.codes.view(torch.uint8), self.scales)
+
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """As torch.Tensor.record_stream: the rows are in use on `stream` too."""
         for t in (self._buf, self._codes_view, self._scales_view):
