@@ -117,6 +117,16 @@ def test_product_refuses(kw, match):
              C.byref(x), a["segs"], a["n_segs"], a["out"], a["ld"], None, None, match=match)
 
 
+def test_products_refuse_an_error_word_off_its_alignment():
+    m8, m4 = abi.WispFp8Mats(P, P), abi.WispFp4Mats(P, P, None)
+    for flag in (P + 1, P + 2):
+        _refused("wisp_b200_fp8_product", C.byref(abi.WispFp8Config(2, 64, 64, 0, 1)), C.byref(m8), None,
+                 C.byref(abi.WispFp8Rows(P, P, 1, 4, 3)), P, 2, P, 64, flag, None, match="aligned")
+        _refused("wisp_b200_fp4_product",
+                 C.byref(abi.WispFp4Config(abi.WISP_FP4_MX, 2, 64, 64, 0, 1)), C.byref(m4), None,
+                 C.byref(abi.WispFp4Rows(P, P, None, 3)), P, 2, P, 64, flag, None, match="aligned")
+
+
 def test_moe_refusals():
     cfg = abi.WispMoeConfig()
     cfg.tokens, cfg.hidden, cfg.inter, cfg.n_experts, cfg.top_k = 4, 256, 128, 8, 2

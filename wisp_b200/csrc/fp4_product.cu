@@ -824,9 +824,11 @@ extern "C" WispError wisp_b200_fp4_product(const WispFp4Config* cfg, const WispF
   if (!x->codes || !x->scales || !d_out)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: null pointer argument (rows, out)");
   if (((uintptr_t)x->codes & 15) || ((uintptr_t)x->tensor_scale & 3) ||
-      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3))
+      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3) ||
+      ((uintptr_t)d_error_flag & 3))
     return WB_FAIL(WISP_ERR_INVALID_ARG,
-                   "fp4_product: row codes must be 16-byte aligned, out to its type");
+                   "fp4_product: row codes must be 16-byte aligned, segments and error word 4-byte, "
+                   "out to its type");
   const bool nv = cfg->format == WISP_FP4_NV;
   if (!nv && x->tensor_scale)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp4_product: MX rows have no tensor scale");

@@ -953,9 +953,11 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   if (!x->codes || !x->scales || !d_out)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: null pointer argument (rows, out)");
   if (((uintptr_t)x->codes & 15) || ((uintptr_t)x->scales & 3) ||
-      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3))
+      ((uintptr_t)d_out % dt_size(cfg->out_type)) || ((uintptr_t)d_segs & 3) ||
+      ((uintptr_t)d_error_flag & 3))
     return WB_FAIL(WISP_ERR_INVALID_ARG,
-                   "fp8_product: row codes must be 16-byte aligned, scales and out to their types");
+                   "fp8_product: row codes must be 16-byte aligned, segments and error word 4-byte, "
+                   "scales and out to their types");
   int dev = 0, sms = 0;
   WB_CUDA_CHECK(wb::device_sms(&dev, &sms));
   auto tiles_of = [&](int rows_per_tile) {     // an upper bound: at most one per row, and
