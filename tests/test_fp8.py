@@ -157,6 +157,41 @@ def test_moe_refusals():
     call(need, match="2\\^31")
 
 
+@pytest.mark.parametrize("kw,match", [
+    (dict(router_bias=P + 2), "router_bias"), (dict(score_bias=P + 1), "score_bias"),
+    (dict(idx=P + 2), "topk_idx"), (dict(wt=P + 1), "topk_w"), (dict(flag=P + 2), "error word"),
+    (dict(gate=(None, P)), "null pointer argument \\(gate"), (dict(up=(P, None)), "null.*\\(up"),
+    (dict(down=(None, None)), "null.*\\(down"), (dict(gate=(P + 8, P)), "gate codes.*aligned"),
+    (dict(up=(P, P + 2)), "up codes.*aligned"), (dict(down=(P + 4, P)), "down codes.*aligned"),
+])
+def test_moe_refuses_before_it_launches(kw, match):
+    """What one of the layer's later steps would refuse, or a kernel would stumble over."""
+    a = dict(router_bias=None, score_bias=None, idx=None, wt=None, flag=None, gate=(P, P), up=(P, P),
+             down=(P, P))
+    a.update(kw)
+    cfg = abi.WispMoeConfig()
+    cfg.tokens, cfg.hidden, cfg.inter, cfg.n_experts, cfg.top_k = 4, 256, 128, 8, 2
+    r = routing.policy()
+    w = abi.WispFp8MoeWeights()
+    w.router_w, w.router_bias, w.score_bias = P, a["router_bias"], a["score_bias"]
+    for name in ("gate", "up", "down"):
+        setattr(w, name, abi.WispFp8Mats(*a[name]))
+    _refused("wisp_b200_fp8_moe_forward", C.byref(cfg), C.byref(r), C.byref(w), P, P, a["idx"], a["wt"],
+             P, 1 << 40, a["flag"], None, match=match)
+
+
+def test_moe_workspace_of_sizes_past_the_products():
+    cfg = abi.WispMoeConfig()
+    cfg.tokens, cfg.n_experts, cfg.top_k = 1, 8, 2
+    size = lambda: abi.lib().wisp_b200_fp8_moe_workspace_bytes(C.byref(cfg), None)
+    for h, i, ok in ((1 << 27, 128, True), ((1 << 27) + 128, 128, False), (128, (1 << 27) + 128, False),
+                     (1 << 26, 1 << 20, True)):
+        cfg.hidden, cfg.inter = h, i
+        assert (size() > 0) == ok
+    cfg.n_experts, cfg.hidden, cfg.inter = 1024, 128, 1 << 21     # 2^31 rows of gate
+    assert size() == 0
+
+
 def test_python_refusals():
     x = torch.zeros(2, 64)
     with pytest.raises(RuntimeError, match="no CPU path"):

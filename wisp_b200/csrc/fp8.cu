@@ -606,6 +606,16 @@ WispError wb::fp8_validate(const WispFp8Config* c, const char* who, WispErrCtx* 
   return WISP_OK;
 }
 
+WispError wb::fp8_check_mats(const WispFp8Mats* m, const char* who, const char* what,
+                             WispErrCtx* err) {
+  if (!m || !m->codes || !m->scales)
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: null pointer argument (%s)", who, what);
+  if (((uintptr_t)m->codes & 15) || ((uintptr_t)m->scales & 3))
+    return WB_FAIL(WISP_ERR_INVALID_ARG, "%s: %s codes must be 16-byte, scales 4-byte aligned", who,
+                   what);
+  return WISP_OK;
+}
+
 extern "C" WispError wisp_b200_fp8_quantize_weights(const void* d_w, int w_type, int n_entries,
                                                     int n, int k, uint8_t* d_codes,
                                                     float* d_scales, cudaStream_t stream,

@@ -920,15 +920,6 @@ WispError cluster_room(int dev, int size, int* room, WispErrCtx* err) {
   return WISP_OK;
 }
 
-WispError check_mats(const WispFp8Mats* m, const char* what, WispErrCtx* err) {
-  if (!m || !m->codes || !m->scales)
-    return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: null pointer argument (%s)", what);
-  if (((uintptr_t)m->codes & 15) || ((uintptr_t)m->scales & 3))
-    return WB_FAIL(WISP_ERR_INVALID_ARG,
-                   "fp8_product: %s codes must be 16-byte, scales 4-byte aligned", what);
-  return WISP_OK;
-}
-
 }  // namespace
 
 extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispFp8Mats* w,
@@ -938,8 +929,9 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
                                            WispErrCtx* err) {
   WispError e = wb::fp8_validate(cfg, "fp8_product", err);
   if (e != WISP_OK) return e;
-  if ((e = check_mats(w, "weights", err)) != WISP_OK) return e;
-  if (cfg->swiglu && (e = check_mats(up, "up weights", err)) != WISP_OK) return e;
+  if ((e = wb::fp8_check_mats(w, "fp8_product", "weights", err)) != WISP_OK) return e;
+  if (cfg->swiglu && (e = wb::fp8_check_mats(up, "fp8_product", "up weights", err)) != WISP_OK)
+    return e;
   if (!cfg->swiglu && up)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_product: up weights without swiglu");
   if (!x || x->rows < 0 || x->rows > wb::kMaxRows)

@@ -103,6 +103,7 @@ WispError fp4_validate(const WispFp4Config* c, const char* who, WispErrCtx* err)
 
 // The same for fp8 (fp8.cu) and for a routing (select.cu).
 WispError fp8_validate(const WispFp8Config* c, const char* who, WispErrCtx* err);
+WispError fp8_check_mats(const WispFp8Mats* m, const char* who, const char* what, WispErrCtx* err);
 WispError routing_validate(const WispRouting* r, int tokens, int n_experts, int top_k,
                            const char* who, WispErrCtx* err);
 

@@ -714,6 +714,12 @@ WispError validate_fp8(const WispMoeConfig* c, const WispRouting* r, WispErrCtx*
   if (r) v.scoring = WISP_SCORE_SOFTMAX;
   WispError e = validate(&v, err);
   if (e != WISP_OK) return e;
+  // the products' limits
+  const int V = c->n_experts + (c->has_shared ? 1 : 0);
+  const WispFp8Config gu = {V, c->inter, c->hidden, 1, WISP_DT_BF16};
+  const WispFp8Config dn = {V, c->hidden, c->inter, 0, WISP_DT_BF16};
+  if ((e = wb::fp8_validate(&gu, "fp8_moe", err)) != WISP_OK) return e;
+  if ((e = wb::fp8_validate(&dn, "fp8_moe", err)) != WISP_OK) return e;
   // rows are counted in 32 bits
   if ((int64_t)c->tokens * (c->top_k + (c->has_shared ? 1 : 0)) > 0x7fffff00LL)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe: %d tokens of %d experts are more than 2^31 - 256 "
@@ -750,6 +756,15 @@ extern "C" WispError wisp_b200_fp8_moe_forward(const WispMoeConfig* cfg, const W
   if (workspace_bytes < ws.bytes)
     return WB_FAIL(WISP_ERR_INVALID_ARG, "fp8_moe_forward: workspace %zu < required %zu",
                    workspace_bytes, ws.bytes);
+  // (all that the steps below would refuse, before the first of them is launched)
+  if (((uintptr_t)w->router_bias | (uintptr_t)w->score_bias | (uintptr_t)d_topk_idx |
+       (uintptr_t)d_topk_w | (uintptr_t)d_error_flag) & 3)
+    return WB_FAIL(WISP_ERR_INVALID_ARG,
+                   "fp8_moe_forward: router_bias, score_bias, topk_idx, topk_w and the error word must "
+                   "be 4-byte aligned");
+  if ((e = wb::fp8_check_mats(&w->gate, "fp8_moe_forward", "gate", err)) != WISP_OK) return e;
+  if ((e = wb::fp8_check_mats(&w->up, "fp8_moe_forward", "up", err)) != WISP_OK) return e;
+  if ((e = wb::fp8_check_mats(&w->down, "fp8_moe_forward", "down", err)) != WISP_OK) return e;
   const Workspace& b = ws.base;
   const int T = cfg->tokens, M = cfg->hidden, I = cfg->inter;
   const int V = cfg->n_experts + (cfg->has_shared ? 1 : 0);
