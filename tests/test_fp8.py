@@ -192,6 +192,27 @@ def test_moe_workspace_of_sizes_past_the_products():
     assert size() == 0
 
 
+def test_moe_workspace_holds_copied_tokens_only_where_rows_are_copied():
+    """A layer that quantises every row has no use for its tokens' codes, however many rows it has."""
+    cfg = abi.WispMoeConfig()
+    cfg.hidden, cfg.inter, cfg.n_experts = 2048, 128, 8
+
+    def size(tokens):
+        cfg.tokens = tokens
+        return abi.lib().wisp_b200_fp8_moe_workspace_bytes(C.byref(cfg), None)
+
+    # one token more: what it needs, and slack for parts that are rounded up to 256 bytes and for
+    # the plan's counters; its codes and those of all before it would be 4 MB and more
+    for top_k, shared in ((1, 0), (2, 0), (1, 1), (2, 1)):
+        cfg.top_k, cfg.has_shared = top_k, shared
+        for tokens in (1023, 2047, 4095, 8191):
+            assert size(tokens + 1) - size(tokens) < 1 << 20
+    cfg.top_k, cfg.has_shared = 4, 0               # 2^23 values of four rows a token: from 1024 on
+    assert size(1024) - size(1023) > 1024 * 2048
+    cfg.top_k, cfg.has_shared = 3, 1
+    assert size(1024) - size(1023) > 1024 * 2048
+
+
 def test_python_refusals():
     x = torch.zeros(2, 64)
     with pytest.raises(RuntimeError, match="no CPU path"):
@@ -1162,6 +1183,31 @@ def test_moe_layer_of_several_k_stages(tokens):
     layer.check()
     _check_layer(layer, x, out)
     assert torch.equal(layer.forward(x), out)
+
+
+@pytest.mark.gpu
+@POW2
+@pytest.mark.parametrize("shared", [False, True], ids=["routed", "shared"])
+@pytest.mark.parametrize("hidden,tokens,top_k", [
+    (512, 3277, 5), (512, 3276, 4), (1024, 2049, 4), (2048, 1023, 4), (2048, 3277, 5), (2048, 2060, 3),
+    (2048, 2060, 1),
+])
+def test_moe_layer_rows_quantised_singly_and_copied(hidden, tokens, top_k, shared, pow2):
+    """Both sides of where the layer copies its tokens' codes instead of quantising every row, for
+    either kind of scale, with tokens of NaN, which have no rows."""
+    spec = synth.MoeSpec("copy", hidden, 128, 16, top_k, has_shared=shared)
+    layer = _layer(spec, tokens, pow2=pow2, routing=routing.policy(**V3))
+    layer.workspace.fill_(0x7f)
+    x = torch.randn((tokens, hidden), device=DEV).to(torch.bfloat16)
+    bad = torch.zeros(tokens, dtype=torch.bool, device=DEV)
+    bad[2::97] = True
+    x[bad] = float("nan")
+    out = layer.forward(x)
+    layer.check()
+    assert (layer.idx[bad] == -1).all() and (layer.idx[~bad] >= 0).all()
+    _check_layer(layer, x, out, ~bad)
+    assert out[bad].isnan().all() if shared else (out[bad] == 0).all()
+    assert torch.equal(layer.forward(x)[~bad], out[~bad])
 
 
 @pytest.mark.gpu

@@ -529,7 +529,7 @@ struct Fp4Ws {
   Workspace base;      // routing, plan, token lists
   float* part;
   uint16_t* y;         // bf16 expert outputs
-  uint8_t* tc;         // the tokens' codes and scales (kGatherRows)
+  uint8_t* tc;         // the tokens' codes and scales (copy_fp8_rows)
   uint8_t* ts;
   uint8_t* xc;
   uint8_t* xs;
@@ -658,11 +658,24 @@ extern "C" WispError wisp_b200_fp4_moe_forward(const WispMoeConfig* cfg, const W
 
 namespace {
 
+// Whether the layer quantises its tokens once and copies codes and scales to their rows,
+// instead of quantising every row: one launch more and the codes read and written again,
+// against the reading and the arithmetic of rows wanted `lanes` times. Powers of two need
+// little arithmetic, so that copying them pays later. us, every row / copied, 7168 columns:
+// one lane of 2048 tokens 12.2 / 17.3 (powers of two 7.7 / 12.9), two 20.7 / 21.1 (11.6 /
+// 17.6), three 28.7 / 23.1 (16.0 / 18.9), four 37.2 / 27.2 (21.4 / 23.8), five 45.6 / 30.3
+// (26.1 / 27.2), nine 79.1 / 42.4 (45.0 / 40.4); nine of 512 22.5 / 15.5 (12.6 / 14.0).
+// 2048 columns: three lanes of 2048 11.3 / 10.4 (6.7 / 8.5), of 1024 6.7 / 7.4, five of 512
+// 6.2 / 6.5, of 1024 10.0 / 8.2 (6.1 / 7.5), of 4096 27.0 / 18.0 (15.6 / 15.2).
+bool copy_fp8_rows(int tokens, int lanes, int cols, bool pow2) {
+  return lanes >= (pow2 ? 5 : 4) && (int64_t)tokens * lanes * cols >= (pow2 ? 1 << 25 : 1 << 23);
+}
+
 struct Fp8Ws {
   Workspace base;      // routing, plan, token lists
   float* part;
   uint16_t* y;         // bf16 expert outputs
-  uint8_t* tc;         // the tokens' codes and scales (kGatherRows)
+  uint8_t* tc;         // the tokens' codes and scales (copy_fp8_rows)
   float* ts;
   uint8_t* xc;
   float* xs;
@@ -693,7 +706,8 @@ Fp8Ws carve_fp8(const WispMoeConfig* c, void* base) {
   ws.y = cv.take<uint16_t>(base, (size_t)b.rows * M);
   b.tok_cnt = cv.take<int>(base, T);
   b.tok_list = cv.take<int>(base, (size_t)T * b.lanes);
-  const size_t tokens = b.rows >= kGatherRows ? T : 0;
+  // (what the scales are is not known here; of the two, copying powers of two pays later)
+  const size_t tokens = copy_fp8_rows(T, b.lanes, M, false) ? T : 0;
   ws.tc = cv.take<uint8_t>(base, tokens * M);
   ws.ts = cv.take<float>(base, tokens * (M / 128));
   ws.xc = cv.take<uint8_t>(base, (size_t)b.rows * M);
@@ -784,7 +798,7 @@ extern "C" WispError wisp_b200_fp8_moe_forward(const WispMoeConfig* cfg, const W
   e = wb::launch_plan(cfg, idx, wt, b.counts, b.segs, b.row_token, b.row_weight, stream, err,
                       b.plan_scratch);
   if (e != WISP_OK) return e;
-  if (b.rows >= kGatherRows) {
+  if (copy_fp8_rows(T, b.lanes, M, w->pow2)) {
     e = wisp_b200_fp8_quantize(d_x, WISP_DT_BF16, M, T, nullptr, T, M, w->pow2, ws.tc, ws.ts, 1, T,
                                stream, err);
     if (e != WISP_OK) return e;
