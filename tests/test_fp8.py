@@ -737,6 +737,18 @@ def test_product_split_over_k_by_any_number(swiglu, n, k, counts):
 
 
 @pytest.mark.gpu
+@SWIGLU
+@pytest.mark.parametrize("counts", [[65], [140], [193], [66, 193, 130]])
+def test_product_split_over_k_by_cut_segments(swiglu, counts):
+    """Segments cut into tiles of 48 rows (65: and 17; 140: and 44; 130: and 34; 66: and 18) and of
+    64 (193: and one)."""
+    for dtype in DT.values():
+        q, w, mats, segs, dev, out = _run_product(swiglu, dtype, 121, 4608, counts)
+        assert torch.equal(fp8.product(q, w, dev, dtype=dtype), out)
+        w.check()
+
+
+@pytest.mark.gpu
 def test_product_many_segments_same_expert():
     """1025 segments, experts out of order and repeated."""
     counts = [(i * 7) % 4 for i in range(1025)]
@@ -1183,6 +1195,154 @@ def test_moe_layer_of_several_k_stages(tokens):
     layer.check()
     _check_layer(layer, x, out)
     assert torch.equal(layer.forward(x), out)
+
+
+def _check_choice(layer, x):
+    """Every token's experts and weights against intervals of the 64-bit scores. A logit is a sum of
+    products that are exact in fp32 (8 + 8 or 8 + 11 bits): at most `hidden` roundings and a few for
+    the parts and the bias, each by 2^-23 of the terms' magnitudes (twice a rounding to nearest).
+    With logits off by at most d, a sigmoid is off by at most d / 4 and a softmax by a factor
+    e^(2 d). A choice is wrong where no scores within their intervals make it."""
+    r, spec = layer.routing, layer.spec
+    router, lbias, sbias = layer._keep
+    w = router.double()
+    l, mag = x.double() @ w.T, x.double().abs() @ w.T.abs()
+    if lbias is not None:
+        l, mag = l + lbias.double(), mag + lbias.double().abs()
+    d = (spec.hidden + 16) * 2.0 ** -23 * mag
+    if r.scoring == abi.WISP_ROUTE_SOFTMAX:
+        s, f = torch.softmax(l, 1), torch.exp(2 * d.amax(1, keepdim=True))
+        lo, hi = s / f, s * f
+    else:
+        s = torch.sigmoid(l)
+        lo, hi = s - d / 4, s + d / 4
+    b = torch.zeros_like(l) if sbias is None else sbias.double().expand_as(l)
+    clo, chi = (lo + b - 1e-12).cpu(), (hi + b + 1e-12).cpu()
+    lo, hi, idx, wt = lo.cpu(), hi.cpu(), layer.idx.cpu().long(), layer.wt.double().cpu()
+    k, G, per = spec.top_k, r.n_groups, spec.n_experts // r.n_groups
+    top = min(r.group_top, per)
+    glo, ghi = (c.view(-1, G, per).topk(top, 2)[0].sum(2) for c in (clo, chi))
+    for t in range(x.shape[0]):
+        e = idx[t].tolist()
+        assert len(set(e)) == k and min(e) >= 0 and max(e) < spec.n_experts
+        assert all(chi[t, p] >= clo[t, q] for p, q in zip(e, e[1:])), (t, "order")
+        used = {p // per for p in e}
+        assert len(used) <= r.topk_groups
+        for g in used:          # not surely behind as many groups as are kept
+            assert sum((glo[t] > ghi[t, g]).tolist()) < r.topk_groups, (t, "group", g)
+        for g in range(G):      # nothing is surely better and left out
+            left = [p for p in range(g * per, (g + 1) * per) if p not in e and clo[t, p] > chi[t, e[-1]]]
+            if left:
+                assert g not in used, (t, "left out", left)
+                others = sum(bool(ghi[t, h] >= glo[t, g]) for h in range(G) if h != g)
+                assert others >= r.topk_groups, (t, "group left out", g)
+        # the weights of these experts, whose scores carry no score bias
+        a, z = lo[t, e].clamp(min=0), hi[t, e]
+        if r.renormalize:
+            a, z = a / (z.sum() - z + a), z / (a.sum() - a + z)
+        eps = 2.0 ** -23
+        assert (wt[t] >= a * r.scaling * (1 - eps)).all() and (wt[t] <= z * r.scaling * (1 + eps)).all(), t
+
+
+CHOICES = {
+    "sigmoid": dict(scoring=abi.WISP_ROUTE_SIGMOID, n_groups=4, topk_groups=2, scaling=2.5),
+    "softmax": dict(scoring=abi.WISP_ROUTE_SOFTMAX, n_groups=8, topk_groups=3, group_top=1),
+    "softmax as it is": dict(scoring=abi.WISP_ROUTE_SOFTMAX, renormalize=False),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 4, 5, 64, 700])    # logits of a few tokens, by parts of K
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("policy", list(CHOICES))
+def test_moe_layer_router_with_both_biases(policy, dtype, tokens):
+    """One bias before the scores, one for the choice alone; either kind of router."""
+    spec = synth.MoeSpec("biases", 1536, 128, 32, 4)
+    g = torch.Generator(device=DEV).manual_seed(31)
+    lbias = torch.randn(32, generator=g, device=DEV) * 0.7
+    base = _layer(spec, tokens, routing=routing.policy(**CHOICES[policy]))
+    router, _, sbias = base._keep
+    x = torch.randn((tokens, spec.hidden), generator=g, device=DEV).to(torch.bfloat16)
+    for lb, sb in ((lbias, sbias), (lbias, None), (None, sbias)):
+        layer = fp8.Fp8MoeLayer(spec, router.to(DT[dtype]), lb, base.gate_up, base.down, tokens,
+                                routing=base.routing, score_bias=sb)
+        out = layer.forward(x)
+        layer.check()
+        _check_choice(layer, x)
+        _check_layer(layer, x, out)
+    if tokens >= 64:                   # the check tells the two biases apart
+        layer._keep = (router, sbias, None)
+        with pytest.raises(AssertionError):
+            _check_choice(layer, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 4, 64, 700])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_moe_layer_without_a_routing_routes_as_the_other_layers(dtype, tokens):
+    """The logits' bias and the router's type reach the routing that the layers share."""
+    g = torch.Generator(device=DEV).manual_seed(32)
+    lbias = torch.randn(32, generator=g, device=DEV) * 0.7
+    for spec in (synth.MoeSpec("soft", 1536, 128, 32, 4),
+                 synth.MoeSpec("sig", 1536, 128, 32, 4, scoring=abi.WISP_SCORE_SIGMOID_GROUPED, n_groups=4,
+                               topk_groups=2, routed_scaling=2.5)):
+        base = _layer(spec, tokens)
+        router = base._keep[0].to(DT[dtype])
+        layer = fp8.Fp8MoeLayer(spec, router, lbias, base.gate_up, base.down, tokens)
+        x = torch.randn((tokens, spec.hidden), generator=g, device=DEV).to(torch.bfloat16)
+        out = layer.forward(x)
+        layer.check()
+        _check_layer(layer, x, out)
+        w = abi.WispMoeWeights(router.data_ptr(), lbias.data_ptr(), None, None)
+        nbytes = abi.lib().wisp_b200_route_workspace_bytes(C.byref(layer.cfg))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        idx, wt = torch.empty_like(layer.idx), torch.empty_like(layer.wt)
+        abi.call("wisp_b200_route_ws", C.byref(layer.cfg), C.byref(w), x.data_ptr(), None, idx.data_ptr(),
+                 wt.data_ptr(), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(layer.idx, idx) and torch.equal(layer.wt, wt)
+        base.forward(x)
+        assert tokens < 64 or not torch.equal(base.idx, idx)
+
+
+@pytest.mark.gpu
+@POW2
+@pytest.mark.parametrize("tokens", [1, 24])
+def test_moe_layer_of_256_experts(pow2, tokens):
+    """The shape whose times the documents give: 256 experts of 2 x 2048 x 7168 and a shared one,
+    four of eight groups, eight experts a token. Every product against 64 bits, and the layer against
+    these stages."""
+    spec = synth.MoeSpec("large", 7168, 2048, 256, 8, has_shared=True)
+    V = spec.n_virtual
+    g = torch.Generator(device=DEV).manual_seed(41)
+
+    def mats(n, k):
+        codes = torch.randint(0, 256, (V, n, k), generator=g, device=DEV, dtype=torch.uint8)
+        codes &= 0xBF                   # magnitudes below 2, none of them NaN
+        scales = torch.rand((V, n // 128, k // 128), generator=g, device=DEV) * 2 / k ** 0.5
+        return codes, scales
+
+    sets = [mats(2048, 7168), mats(2048, 7168), mats(7168, 2048)]
+    gate_up, down = fp8.Fp8Weights(*sets[0], up=sets[1]), fp8.Fp8Weights(*sets[2])
+    router = (torch.randn((256, 7168), generator=g, device=DEV) * 0.02).to(torch.bfloat16)
+    sbias = torch.randn(256, generator=g, device=DEV) * 0.05
+    layer = fp8.Fp8MoeLayer(spec, router, None, gate_up, down, tokens, pow2=pow2, score_bias=sbias,
+                            routing=routing.policy(n_groups=8, topk_groups=4, scaling=2.5))
+    x = torch.randn((tokens, 7168), generator=g, device=DEV).to(torch.bfloat16)
+    out = layer.forward(x)
+    layer.check()
+    assert torch.equal(layer.forward(x), out)
+    _check_choice(layer, x)
+    _check_layer(layer, x, out)
+    # the stages that _check_layer goes through
+    idx = layer.idx.cpu()
+    rows = [[t for t in range(tokens) if e in idx[t].tolist()] for e in range(256)] + [list(range(tokens))]
+    segs, dev = _segs([len(r) for r in rows])
+    tok = torch.tensor([t for r in rows for t in r], dtype=torch.int32, device=DEV)
+    q = _check_quantize(x, pow2, rows=tok, src=x[tok.long()])
+    h = fp8.product(q, gate_up, dev, dtype=torch.bfloat16)
+    _check(h, q, sets[:2], segs, 7168)
+    q = _check_quantize(h, pow2)
+    _check(fp8.product(q, down, dev, dtype=torch.bfloat16), q, sets[2:], segs, 2048)
 
 
 @pytest.mark.gpu
