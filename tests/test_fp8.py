@@ -12,7 +12,7 @@ import torch
 
 import fp4_ref
 import fp8_ref as ref
-from wisp_b200 import abi, fp8, norm, routing, synth
+from wisp_b200 import abi, fp4, fp8, norm, routing, synth
 
 P = 1 << 20   # a non-null aligned stand-in pointer; never dereferenced here
 DEV = "cuda"
@@ -1057,6 +1057,27 @@ def test_product_of_the_most_rows():
         part = fp8.Fp8Rows(codes[r0:r0 + 50], scales[r0:r0 + 50])
         _check(out[r0:r0 + 50], part, [mats], [(0, 0, 50)], 16)
     assert int((out != 0).sum()) <= 150
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [4, 8])
+def test_weights_made_in_inference_mode_are_checked_outside(bits):
+    """What check reports it clears, wherever the weights were made."""
+    g = torch.Generator(device=DEV).manual_seed(10)
+    values = torch.randn((2, 64, 64), generator=g, device=DEV)
+    x = torch.randn((5, 64), generator=g, device=DEV)
+    with torch.inference_mode():
+        w = fp8.Fp8Weights.from_values(values) if bits == 8 else \
+            fp4.Fp4Weights.from_values(abi.WISP_FP4_MX, values)
+    q, product = (fp8.quantize(x), fp8.product) if bits == 8 else \
+        (fp4.quantize(x, abi.WISP_FP4_MX), fp4.product)
+    segs = torch.tensor([[7, 0, 2, 0], [1, 2, 3, 0]], dtype=torch.int32, device=DEV)     # no matrix 7
+    for mode in (torch.no_grad, torch.inference_mode, torch.enable_grad):
+        with mode():
+            product(q, w, segs)
+            with pytest.raises(RuntimeError, match=r"wisp engine error \[4\].*skipped"):
+                w.check()
+            w.check()
 
 
 @pytest.mark.gpu

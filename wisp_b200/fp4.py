@@ -277,7 +277,8 @@ class Fp4Weights:
                          prepared.data_ptr(), nbytes, stream_of(codes))
                 self._keep.append((c, prepared, ts))
                 structs.append(abi.WispFp4Mats(c.data_ptr(), prepared.data_ptr(), ptr(ts)))
-            self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
+            with torch.inference_mode(False):        # (check clears it in either mode)
+                self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
             # laid out once: any stream may use the object from here on
             torch.cuda.current_stream(codes.device).synchronize()
         self.mats = structs[0]

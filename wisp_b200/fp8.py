@@ -204,7 +204,8 @@ class Fp8Weights:
             self._keep.append((c, s))
             structs.append(abi.WispFp8Mats(c.data_ptr(), s.data_ptr()))
         with elsewhere(codes) or contextlib.nullcontext():
-            self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
+            with torch.inference_mode(False):        # (check clears it in either mode)
+                self.error_word = torch.zeros(1, dtype=torch.int32, device=codes.device)
             # any stream may use the object from here on
             torch.cuda.current_stream(codes.device).synchronize()
         self.mats = structs[0]
