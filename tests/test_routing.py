@@ -162,6 +162,24 @@ def test_groups_of_large_biases_that_cancel(scoring, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("below", [3.0, 5.44, 9.0])
+def test_softmax_of_many_logits_below_the_largest(below):
+    """1023 logits about 5.4 below the largest are where a sum of quick exponentials is off the
+    most; the bias brings choices as close as that, and closer."""
+    g = torch.Generator(device=DEV).manual_seed(14)
+    e = 1024
+    x = -below + torch.randn((1, e), generator=g, device=DEV).repeat(2, 1) * 2.0 ** -12
+    x[:, 17] = 0.0
+    score = torch.softmax(x[0].double(), 0)
+    for step in range(17, 27):
+        i = torch.randint(-3, 4, (e,), generator=g, device=DEV).double()
+        bias = (score.max() * (2.0 + i * 2.0 ** -step) - score).float()
+        for groups, kept, top in ((1, 1, 1), (16, 3, 2), (16, 3, 1)):
+            _check(x, 8, abi.WISP_ROUTE_SOFTMAX, bias, n_groups=groups, topk_groups=kept,
+                   group_top=top)
+
+
+@pytest.mark.gpu
 @SCORING
 def test_values_that_cannot_be_chosen(scoring):
     """-infinite logits and biases, NaN, infinities, extreme logits, rows with too few experts left

@@ -260,11 +260,16 @@ WB_DEV uint32_t take_best(uint32_t (&key)[PER], int lane, uint32_t& expert) {
 // One warp per token; lane l holds experts l + 32 j, j < PER.
 //
 // The result is that of 64-bit scores and choices (route_exact), found in 32 bits
-// where that decides it. The quick exponential of x is off by 2 + 1.2 |x| ulp, which
-// makes at most 1.5 * 2^-23 of a sigmoid s (s (1 - s) |x| < 0.23) and, with a sum and
-// the quick reciprocal, 7 * 2^-24: 2^-21 covers it. A softmax score is off by 9 * 2^-24 of
-// the largest score (e^-x x < 0.37) and by the sum's error of at most 43 * 2^-24 of itself:
-// 2^-18 of the largest. Adding the bias rounds by 2^-24 of the choice, the sum of two choices
+// where that decides it. With u = 2^-24, half a step of fp32 at most: the quick exponential
+// of x is off by 2 + 1.2 |x| steps, (4 + 2.4 |x|) u of itself. A sigmoid s takes s (1 - s) of
+// that, at most 1.3 u (at |x| = 0.8), and with the sum in its divisor (1 u) and
+// the quick reciprocal (2 u) it is off by less than 5 u: 2^-21 covers it. A softmax, d
+// below the largest logit, has an exponential off by (4 + 3.4 d) u of itself, d u of it
+// from rounding the argument: e^-d times that is at most 4 u of the largest. Their sum is
+// off by their errors' mean, at most 20 u of it (1023 of them at d = 5.4 beside the
+// largest: 19.1), by 36 roundings (31 in a lane, 5 across) and the reciprocal's 2 u: 58 u.
+// With the last product's rounding a score is off by at most 4 + 58 + 1 = 63 u of the
+// largest score: 2^-18. Adding the bias rounds by u of the choice, the sum of two choices
 // by as much, and the comparison again: 2^-22 of each choice. Without a bias the scores
 // are in the logits' order, which needs no scores at all: equal logits are ties, and
 // those 2^-20 apart have different 64-bit scores as long as these are not near 1 (logits above
