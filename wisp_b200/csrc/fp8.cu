@@ -33,6 +33,8 @@ constexpr float kTop = 448.f;
 constexpr float kTiny = 1e-30f, kRaise = 1.2676506002282294e30f;     // 2^100
 constexpr float kBelow = 1.f - 4.76837158203125e-7f, kAbove = 1.f + 4.76837158203125e-7f;  // 2^-21
 
+constexpr int kSms = 148;      // a B200's; layouts depend on it, results do not
+
 // How `rows` rows of `cols` values lie over the grid, at R rows per thread: a row's
 // threads over equal CTAs of at most 256, or, of short rows, several in one CTA as long as
 // that leaves four CTAs an SM (100,000 bf16 rows of 64, us: quantise 23.6 -> 9.6, back 27.3 ->
@@ -43,7 +45,7 @@ struct Layout {
 Layout layout_rows(int rows, int cols, int R) {
   const int units = (cols + kBlock - 1) / kBlock * kLanes;
   for (int k = 256 / units; k > 1; k--)
-    if (units * k % 32 == 0 && rows >= (int64_t)148 * 4 * R * k)
+    if (units * k % 32 == 0 && rows >= (int64_t)kSms * 4 * R * k)
       return {dim3(((int64_t)rows + R * k - 1) / (R * k)), dim3(units, k)};
   const int parts = (units + 255) / 256;
   const int threads = ((units + parts - 1) / parts + 31) / 32 * 32;
@@ -51,7 +53,7 @@ Layout layout_rows(int rows, int cols, int R) {
 }
 // Several rows per thread once there are enough to fill the GPU all the same.
 bool many_rows(int rows, int cols, int R) {
-  return (int64_t)rows * layout_rows(1, cols, 1).grid.y >= 148 * 8 * R;
+  return (int64_t)rows * layout_rows(1, cols, 1).grid.y >= kSms * 8 * R;
 }
 
 // 16 values of one thread as they lie in memory.

@@ -30,11 +30,12 @@
 // added.
 //
 // Measured (us; L2 flushed by writes, whose way back to memory costs ~20): 64 experts of
-// 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows each 297 / 308 / 344 / 455, where the
-// weights take 287 at the copy rate; 64 of 7168 x 2048 175 / 195 / 225 / 282 (143): bound
-// by HBM up to ~100 rows. 8192 x 8192 x 7168 375 = 2.57 PFLOP/s; without a pause between
-// calls 470, as the power limit lowers the clock. A block of a wide tile takes 0.44 (0.27
-// at the MMAs' nominal rate), a change of tiles 2.5 more.
+// 2 x 2048 x 7168 with 1 / 64 / 128 / 256 rows each 289 / 302 / 334 / 444, where the
+// weights take 287 at the copy rate (on another B200 297 / 308 / 344 / 455); 64 of 7168 x
+// 2048, fp32 outputs, 171 / 192 / 233 / 281 (143): bound by HBM up to ~100 rows. 8192 x 8192 x
+// 7168 373 = 2.58 PFLOP/s; without a pause between calls 470, as the power limit lowers
+// the clock. A block of a wide tile takes 0.44 (0.27 at the MMAs' nominal rate), a change of
+// tiles 2.5 more.
 //
 // Warps of a persistent CTA: 0 issues the TMA copies (128 k per stage, 128-byte
 // swizzle), 1 the MMAs, 2 hands out the tiles, 3 multiplies the scales, 4-11 are the
@@ -661,7 +662,7 @@ fp8_product_kernel(const __grid_constant__ Params p) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     cluster_wait();
     // warp % 4 is the lane quadrant; the two warps of a quadrant take alternate
-    // groups of 16 rows of a narrow tile, a half of each 128 features of a wide one
+    // groups of 32 rows of a narrow tile, a half of each 128 features of a wide one
     const Warp me = {lane, warp & 3, (warp - kEpiWarp) >> 2, rank};
     Reduce<SWIGLU> red;
     red.buf = reinterpret_cast<float*>(smem + kRingBytes - kRedBytes);
@@ -965,7 +966,10 @@ extern "C" WispError wisp_b200_fp8_product(const WispFp8Config* cfg, const WispF
   // 7168 x 7168 21.1 / 14.2 (by two); by half as many or fewer / so: 2048 x 7168 10.2 / 9.5
   // (six), 4096 x 7168 14.0 / 10.7 (four), 7168 x 2048 10.1 / 8.8 (two). 100 rows as pairs / as
   // tiles of 64: 256 x 7168 23.7 / 12.8, 2048 x 7168 24.1 / 14.9, gate/up 1536 x 2048 15.9 /
-  // 13.8; 3000 rows of 128 x 7168 23.9 / 19.0. (Where many segments make the bound on tiles
+  // 13.8; 3000 rows of 128 x 7168 23.9 / 19.0. From 16 blocks on: of 8 to 15 one row gains
+  // and 32 to 128 lose, whose join costs more than the blocks (n 2048, one row / 64 / 128, as
+  // it is 7.3 / 8.1 / 9.3 with k 1024, 9.5 / 10.4 / 11.5 with k 1920; by two or three 7.2 / 10.1 /
+  // 11.3, 7.8 / 11.2 / 12.6). (Where many segments make the bound on tiles
   // too large it may be too few: 8 of 512 x 2048 with 64 rows 11.0 as pairs, 11.8 by two.)
   int split = 1;
   if (nk >= 16) {

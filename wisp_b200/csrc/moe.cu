@@ -423,7 +423,10 @@ namespace {
 // fixed order of combine_ordered_kernel over bf16 rows. (fp32 rows would double
 // the traffic of the down product's output and of this sum, 2.1 GB of 2.9 at
 // 4096 tokens; one rounding of 2^-9 per expert's output is a fiftieth of what
-// its 4-bit operands cost.) One block per token and 2048 columns, 8 per thread.
+// its 4-bit operands cost. Of 8-bit ones it is a 26th: normal values through an
+// expert of 2 x 2048 x 7168 are 4.3 % off by quantising both its inputs to e4m3, 0.17 %
+// by the rounding; with the SwiGLU rows in bf16 too 4.33 % in place of 4.32.)
+// One block per token and 2048 columns, 8 per thread.
 // SCAN: the token's rows are found by reading all of row_token, else they come
 // from token_rows_kernel.
 constexpr int kScanRows = 1024;
