@@ -677,7 +677,8 @@ WispError wisp_b200_select_experts(const WispRouting* routing, const void* d_log
  * score_bias as its bias, and cfg's scoring, n_groups, topk_groups and
  * routed_scaling are ignored, as group_size and deterministic always are (every run
  * gives the same bits). d_x, router_w and d_out 16-byte aligned, the workspace
- * 256-byte. One call at a time per workspace. */
+ * 256-byte, the other arrays to their types: what the layer refuses, it refuses before it
+ * launches anything. One call at a time per workspace. */
 typedef struct {
     const uint16_t* router_w;   /* as in WispMoeWeights */
     const float* router_bias;   /* added to the logits; may be NULL */
